@@ -46,6 +46,12 @@ SOURCES = [
     ("metadata.cpp", ["-ffp-contract=off"]),
     ("lbfgs.cpp", ["-ffp-contract=off"]),
     ("gpm.cpp", ["-ffp-contract=off"]),
+    ("attn_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=0"], "attn_kernel_f32"),
+    ("attn_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=1"], "attn_kernel_bf16"),
+    ("attn_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=2"], "attn_kernel_f16"),
+    ("rotary_kernel.hip", ["-ffp-contract=fast"]),
+    ("norm_kernel.hip", ["-ffp-contract=fast"]),
+    ("ops_api.cpp", ["-ffp-contract=off"]),
 ]
 
 

@@ -1,0 +1,941 @@
+// Differential attention (mtpx_diff_attention, _backward, _cache): two
+// softmax maps over the same values,
+//
+//   out = (P_0 - lambda P_1) V,   P_m = softmax(scale Q_m K_m^T).
+//
+//   attn_forward_kernel   out, and lse and P_1 V for the backward pass
+//   attn_dq_kernel        dq, and per row D_m = sum_j P_m dP (for the next)
+//   attn_dkv_kernel       dk, dv; the group of query heads that share them
+//                         is summed in registers
+//   dlambda_kernel        sums the partials of dlambda in a fixed order
+//   attn_cache_kernel     one row per sequence, keys split over workgroups
+//   attn_cache_join       joins their partial results
+//
+// Compiled once per element type (MTPX_OPS_TYPE).
+#include "ops_device.hpp"
+
+namespace mtpx {
+
+namespace {
+
+#if MTPX_OPS_TYPE == 0
+typedef float Type;
+#define MTPX_OPS_NAME(f) f##_f32
+#elif MTPX_OPS_TYPE == 1
+typedef __bf16 Type;
+#define MTPX_OPS_NAME(f) f##_bf16
+#else
+typedef _Float16 Type;
+#define MTPX_OPS_NAME(f) f##_f16
+#endif
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+
+// Keys k0 .. k0 + 63 of a sequence of nk that are there and not masked.
+__device__ inline unsigned long long seen_keys(const unsigned char *mask, int k0, int nk, int lane)
+{
+    const int k = k0 + lane;
+    return __ballot(k < nk && (!mask || mask[k]));
+}
+
+// Rounds per-lane column results 16 t + 4 (l / 16) + r, of width 2 D, to the
+// row that lane l % 16 stands for.
+template <class T, int D>
+__device__ inline void store_columns(T *row, int64_t map, int dim, int t, int lane, f32x4 v, int vec)
+{
+    const int m = t * 16 / D, c = t * 16 % D + 4 * (lane >> 4);
+    store4(row + m * map, c, dim, v, vec);
+}
+
+// Forward.  A workgroup takes kWaves * QT * 16 query rows of one head, each
+// wave QT * 16 of them; the keys and values come in tiles of KB rows through
+// LDS.  S^T = K Q^T leaves a query per lane column: its running maximum and
+// sum are per lane, and exp(S^T) is operand B of O^T += V^T P^T as it stands.
+// The two maps keep their own maximum, sum and product, since their
+// normalisers are known only at the end; each V fragment read from LDS serves
+// both.  P is rounded to T for the product (its 32-bit sum is the
+// normaliser), as V is in T already.
+template <class T, int D, int QT, int KB>
+__global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, int table, int ntiles)
+{
+    using TL = Tile<T, D>;
+    constexpr int kTile = KB * TL::kRowBytes;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int head = id / ntiles, kv = head / (a.heads / a.kv_heads);
+    const SeqTile st = a.tiles.q[table][id % ntiles];
+    const Seq sq = a.seq[st.seq];
+    const int shift = sq.nk - sq.nq;
+    const float c = a.scale * kLog2e, lambda = a.lambda[head];
+
+    const T *kp = (const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row;
+    const T *vp = (const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row;
+    const unsigned char *mask = a.mask ? a.mask + sq.k0 : nullptr;
+
+    const int w0 = st.start + wave * QT * 16;  // first row of the wave
+    Frag<T> qf[2][QT][D / 32];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = w0 + t * 16 + (lane & 15);
+        const T *qp = (const T *)a.q.data + head * a.q.head + (sq.q0 + row) * a.q.row;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk)
+                qf[m][t][kk] = load_frag(qp + m * a.q.map, kk * 32 + 8 * g, a.dim, row < sq.nq, a.vec);
+    }
+    f32x4 acc[2][QT][D / 8];
+    float top[2][QT], sum[2][QT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            top[m][t] = -INFINITY;
+            sum[m][t] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                acc[m][t][i] = f32x4{0, 0, 0, 0};
+        }
+
+    // keys that the last row of the workgroup sees
+    int nk = sq.nk;
+    if (a.causal)
+        nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
+    Stage<T, D, KB, kThreads> sk, sv;
+    unsigned long long bits = 0;
+    if (nk > 0) {
+        bits = seen_keys(mask, 0, nk, lane);
+        sk.load(kp, a.k, a.dim, 0, bits, tid, a.vec);
+        sv.load(vp, a.v, a.dim, 0, bits, tid, a.vec);
+    }
+    for (int k0 = 0; k0 < nk; k0 += KB) {
+        __syncthreads();
+        sk.store(smem, tid);
+        sv.store(smem + kTile, tid);
+        __syncthreads();
+        unsigned long long now = bits;
+        if constexpr (KB < 64)
+            now &= (1ull << KB) - 1;
+        if (k0 + KB < nk) {
+            bits = seen_keys(mask, k0 + KB, nk, lane);
+            sk.load(kp, a.k, a.dim, k0 + KB, bits, tid, a.vec);
+            sv.load(vp, a.v, a.dim, k0 + KB, bits, tid, a.vec);
+        }
+        if (now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift))
+            continue;
+
+        f32x4 s[2][KB / 16][QT];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kt = 0; kt < KB / 16; ++kt) {
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+                    s[m][kt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int kk = 0; kk < D / 32; ++kk) {
+                    const Frag<T> kf = TL::row_frag(smem, kt * 16, m * D + kk * 32, lane);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        s[m][kt][t] = mma(kf, qf[m][t][kk], s[m][kt][t]);
+                }
+            }
+        const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
+        if (now != full || (a.causal && k0 + KB - 1 > w0 + shift)) {
+            const unsigned long long mine = now >> (4 * g);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const int last = a.causal ? w0 + t * 16 + (lane & 15) + shift - k0 - 4 * g : KB;
+#pragma unroll
+                for (int kt = 0; kt < KB / 16; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool on = (mine >> (16 * kt + r) & 1) && 16 * kt + r <= last;
+                        s[0][kt][t][r] = on ? s[0][kt][t][r] : -INFINITY;
+                        s[1][kt][t][r] = on ? s[1][kt][t][r] : -INFINITY;
+                    }
+            }
+        }
+        Frag<T> pf[2][KB / 32][QT];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                float hi = s[m][0][t][0];
+#pragma unroll
+                for (int kt = 0; kt < KB / 16; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        hi = fmaxf(hi, s[m][kt][t][r]);
+                hi = fmaxf(top[m][t], column_max(hi));
+                if (__any(hi > top[m][t])) {
+                    // rows that have seen no key yet have nothing to rescale
+                    const float f = top[m][t] == -INFINITY ? 0.f : exp2_fast((top[m][t] - hi) * c);
+                    top[m][t] = hi;
+                    sum[m][t] *= f;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        acc[m][t][i] *= f;
+                }
+                const float base = hi == -INFINITY ? 0.f : hi * c;
+                float part = 0.f;
+#pragma unroll
+                for (int kt = 0; kt < KB / 16; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = exp2_fast(fmaf(s[m][kt][t][r], c, -base));
+                        s[m][kt][t][r] = p;
+                        part += p;
+                    }
+                sum[m][t] += part;
+#pragma unroll
+                for (int b = 0; b < KB / 32; ++b)
+                    pf[m][b][t] = pack<T>(s[m][2 * b][t], s[m][2 * b + 1][t]);
+            }
+#pragma unroll
+        for (int b = 0; b < KB / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const Frag<T> vf = TL::column_frag(smem + kTile, b * 32, i * 16, lane);
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        acc[m][t][i] = mma(vf, pf[m][b][t], acc[m][t][i]);
+            }
+    }
+
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = w0 + t * 16 + (lane & 15);
+        float inv[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float total = column_sum(sum[m][t]);
+            inv[m] = total > 0.f || total != total ? 1.f / total : 0.f;
+            if (a.lse && row < sq.nq && g == 0)
+                a.lse[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] =
+                    total == 0.f ? -INFINITY : fmaf(top[m][t], a.scale, __logf(total));
+        }
+        if (row >= sq.nq)
+            continue;
+        T *op = (T *)a.out.data + head * a.out.head + (sq.q0 + row) * a.out.row;
+        T *o1 = (T *)a.out1 + ((sq.q0 + row) * a.heads + head) * 2 * a.dim;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const f32x4 second = acc[1][t][i] * inv[1];
+            store_columns<T, D>(op, a.out.map, a.dim, i, lane, acc[0][t][i] * inv[0] - lambda * second, a.vec);
+            if (a.out1)
+                store_columns<T, D>(o1, a.dim, a.dim, i, lane, second, a.vec);
+        }
+    }
+}
+
+// Gradient of the queries.  Work split, tiles and fragments as in the forward
+// pass: S^T and dP^T = V dO^T come out with a query per lane column, so
+// dS_m^T = P_m (dP - D_m) is operand B of dQ_m^T += K_m^T dS_m^T.  The rows'
+// D_m = dO . O_m are formed here from out and out1 (O_0 = out + lambda O_1)
+// and left for the key pass.  dlambda is -sum D_1; since the sum of
+// P_1 (dP - D_1) over a row is what the rounded out1 took from D_1, adding it
+// gives D_1 from 32-bit values.
+template <class T, int D, int QT, int KB>
+__global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int table, int ntiles)
+{
+    using TL = Tile<T, D>;
+    constexpr int kTile = KB * TL::kRowBytes;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int head = id / ntiles, kv = head / (a.heads / a.kv_heads);
+    const SeqTile st = a.tiles.q[table][id % ntiles];
+    const Seq sq = a.seq[st.seq];
+    const int shift = sq.nk - sq.nq;
+    const float c = a.scale * kLog2e, lambda = a.lambda[head];
+
+    const T *kp = (const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row;
+    const T *vp = (const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row;
+    const unsigned char *mask = a.mask ? a.mask + sq.k0 : nullptr;
+
+    const int w0 = st.start + wave * QT * 16;
+    Frag<T> qf[2][QT][D / 32], df[2][QT][D / 32];
+    float base[2][QT], delta[2][QT], dlam = 0.f;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = w0 + t * 16 + (lane & 15);
+        const bool live = row < sq.nq;
+        const T *qp = (const T *)a.q.data + head * a.q.head + (sq.q0 + row) * a.q.row;
+        const T *dp = (const T *)a.dout.data + head * a.dout.head + (sq.q0 + row) * a.dout.row;
+        const T *op = (const T *)a.out.data + head * a.out.head + (sq.q0 + row) * a.out.row;
+        const T *o1 = (const T *)a.out1 + ((sq.q0 + row) * a.heads + head) * 2 * a.dim;
+        float dot = 0.f, dot1 = 0.f;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk) {
+                const int col = kk * 32 + 8 * g;
+                qf[m][t][kk] = load_frag(qp + m * a.q.map, col, a.dim, live, a.vec);
+                df[m][t][kk] = load_frag(dp + m * a.dout.map, col, a.dim, live, a.vec);
+                const Frag<T> of = load_frag(op + m * a.out.map, col, a.dim, live, a.vec);
+                const Frag<T> o1f = load_frag(o1 + m * a.dim, col, a.dim, live, a.vec);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    dot = fmaf((float)df[m][t][kk][j], (float)of[j], dot);
+                    dot1 = fmaf((float)df[m][t][kk][j], (float)o1f[j], dot1);
+                }
+            }
+        delta[1][t] = column_sum(dot1);
+        delta[0][t] = fmaf(lambda, delta[1][t], column_sum(dot));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int64_t at = ((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row;
+            const float lse = live ? a.lse[at] : -INFINITY;
+            // a row without a key: exp2(s c - inf) is 0
+            base[m][t] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            if (live && g == 0)
+                a.delta[at] = delta[m][t];
+        }
+        if (g == 0)
+            dlam += delta[1][t];
+    }
+    f32x4 acc[2][QT][D / 16];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                acc[m][t][i] = f32x4{0, 0, 0, 0};
+
+    int nk = sq.nk;
+    if (a.causal)
+        nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
+    Stage<T, D, KB, kThreads> sk, sv;
+    unsigned long long bits = 0;
+    if (nk > 0) {
+        bits = seen_keys(mask, 0, nk, lane);
+        sk.load(kp, a.k, a.dim, 0, bits, tid, a.vec);
+        sv.load(vp, a.v, a.dim, 0, bits, tid, a.vec);
+    }
+    for (int k0 = 0; k0 < nk; k0 += KB) {
+        __syncthreads();
+        sk.store(smem, tid);
+        sv.store(smem + kTile, tid);
+        __syncthreads();
+        unsigned long long now = bits;
+        if constexpr (KB < 64)
+            now &= (1ull << KB) - 1;
+        if (k0 + KB < nk) {
+            bits = seen_keys(mask, k0 + KB, nk, lane);
+            sk.load(kp, a.k, a.dim, k0 + KB, bits, tid, a.vec);
+            sv.load(vp, a.v, a.dim, k0 + KB, bits, tid, a.vec);
+        }
+        if (now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift))
+            continue;
+        const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
+        const bool partly = now != full || (a.causal && k0 + KB - 1 > w0 + shift);
+#pragma unroll
+        for (int b = 0; b < KB / 32; ++b) {
+            f32x4 s[2][2][QT], dp[2][QT];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r0 = b * 32 + u * 16;
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    s[0][u][t] = s[1][u][t] = dp[u][t] = f32x4{0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int kk = 0; kk < D / 32; ++kk) {
+                        const Frag<T> kf = TL::row_frag(smem, r0, m * D + kk * 32, lane);
+                        const Frag<T> vf = TL::row_frag(smem + kTile, r0, m * D + kk * 32, lane);
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) {
+                            s[m][u][t] = mma(kf, qf[m][t][kk], s[m][u][t]);
+                            dp[u][t] = mma(vf, df[m][t][kk], dp[u][t]);
+                        }
+                    }
+            }
+            if (partly) {
+                const unsigned mine = (unsigned)(now >> (32 * b + 4 * g));
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    const int last = a.causal ? w0 + t * 16 + (lane & 15) + shift - k0 - 32 * b - 4 * g : 32;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool on = (mine >> (16 * u + r) & 1) && 16 * u + r <= last;
+                            s[0][u][t][r] = on ? s[0][u][t][r] : -INFINITY;
+                            s[1][u][t][r] = on ? s[1][u][t][r] : -INFINITY;
+                        }
+                }
+            }
+            Frag<T> sf[2][QT];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = exp2_fast(fmaf(s[m][u][t][r], c, -base[m][t]));
+                            s[m][u][t][r] = p * (dp[u][t][r] - delta[m][t]);
+                            if (m == 1)
+                                dlam += s[m][u][t][r];
+                        }
+                    sf[m][t] = pack<T>(s[m][0][t], s[m][1][t]);
+                }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const Frag<T> kf = TL::column_frag(smem, b * 32, m * D + i * 16, lane);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        acc[m][t][i] = mma(kf, sf[m][t], acc[m][t][i]);
+                }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = w0 + t * 16 + (lane & 15);
+        if (row >= sq.nq)
+            continue;
+        T *qp = (T *)a.dq.data + head * a.dq.head + (sq.q0 + row) * a.dq.row;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                store4(qp + m * a.dq.map, i * 16 + 4 * g, a.dim,
+                       acc[m][t][i] * (m ? -lambda * a.scale : a.scale), a.vec);
+    }
+    // this workgroup's share of dlambda
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        dlam += __shfl_xor(dlam, o);
+    __syncthreads();
+    float *red = reinterpret_cast<float *>(smem);
+    if (lane == 0)
+        red[wave] = dlam;
+    __syncthreads();
+    if (tid == 0) {
+        float total = 0.f;
+        for (int w = 0; w < kWaves; ++w)
+            total += red[w];
+        a.dlam_part[(int64_t)head * ntiles + id % ntiles] = -total;
+    }
+}
+
+// Gradient of the keys and values.  The mirror image of attn_dq_kernel: a
+// workgroup takes kWaves * KT * 16 keys of one key head, each wave KT * 16;
+// the rows' q, dO and statistics come in tiles of QB rows through LDS.  S and
+// dP come out with a key per lane column: P_0 - lambda P_1 and dS_m are
+// operand B of dV^T += dO^T (P_0 - lambda P_1) and dK_m^T += Q_m^T dS_m.  The
+// query heads that share the key head follow one another, so their sum stays
+// in registers.
+template <class T, int D, int KT, int QB>
+__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
+{
+    using TL = Tile<T, D>;
+    constexpr int kTile = QB * TL::kRowBytes;
+    extern __shared__ __align__(16) char smem[];
+    float *stat = reinterpret_cast<float *>(smem + 2 * kTile);  // [4][QB]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int kv = id / ntiles, group = a.heads / a.kv_heads;
+    const SeqTile st = a.tiles.k[table][id % ntiles];
+    const Seq sq = a.seq[st.seq];
+    const int shift = sq.nk - sq.nq;
+    const float c = a.scale * kLog2e;
+
+    const int w0 = st.start + wave * KT * 16;  // first key of the wave
+    Frag<T> kf[2][KT][D / 32], vf[2][KT][D / 32];
+    bool live[KT];
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const int key = w0 + t * 16 + (lane & 15);
+        live[t] = key < sq.nk && (!a.mask || a.mask[sq.k0 + key]);
+        any |= live[t];
+        const T *kp = (const T *)a.k.data + kv * a.k.head + (sq.k0 + key) * a.k.row;
+        const T *vp = (const T *)a.v.data + kv * a.v.head + (sq.k0 + key) * a.v.row;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk) {
+                kf[m][t][kk] = load_frag(kp + m * a.k.map, kk * 32 + 8 * g, a.dim, live[t], a.vec);
+                vf[m][t][kk] = load_frag(vp + m * a.v.map, kk * 32 + 8 * g, a.dim, live[t], a.vec);
+            }
+    }
+    const bool busy = __any(any);
+    f32x4 dk[2][KT][D / 16], dv[KT][D / 8];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            dk[0][t][i] = dk[1][t][i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+            dv[t][i] = f32x4{0, 0, 0, 0};
+    }
+
+    // rows before the first that sees a key of this workgroup are left out
+    const int first = a.causal ? max(0, st.start - shift) / QB * QB : 0;
+    const int per = sq.nq > first ? (sq.nq - first + QB - 1) / QB : 0;
+    const int steps = per * group;
+    Stage<T, D, QB, kThreads> sq_, sd;
+    float st_reg = 0.f;
+    auto fetch = [&](int step) {
+        const int head = kv * group + step / per, q0 = first + step % per * QB;
+        const int there = sq.nq - q0;
+        const unsigned long long bits = there >= 64 ? ~0ull : (1ull << there) - 1;
+        sq_.load((const T *)a.q.data + head * a.q.head + sq.q0 * a.q.row, a.q, a.dim, q0, bits, tid, a.vec);
+        sd.load((const T *)a.dout.data + head * a.dout.head + sq.q0 * a.dout.row, a.dout, a.dim, q0, bits, tid,
+                a.vec);
+        if (tid < 4 * QB) {
+            const int which = tid / QB, row = q0 + tid % QB;
+            const float *src = which < 2 ? a.lse : a.delta;
+            st_reg = which < 2 ? -INFINITY : 0.f;
+            if (row < sq.nq)
+                st_reg = src[((int64_t)(which & 1) * a.heads + head) * a.total_q + sq.q0 + row];
+            if (which < 2)
+                st_reg = st_reg == -INFINITY ? INFINITY : st_reg * kLog2e;
+        }
+    };
+    if (steps > 0)
+        fetch(0);
+    for (int step = 0; step < steps; ++step) {
+        __syncthreads();
+        sq_.store(smem, tid);
+        sd.store(smem + kTile, tid);
+        if (tid < 4 * QB)
+            stat[tid] = st_reg;
+        __syncthreads();
+        const float lambda = a.lambda[kv * group + step / per];
+        const int q0 = first + step % per * QB;
+        if (step + 1 < steps)
+            fetch(step + 1);
+        if (!busy || (a.causal && q0 + QB - 1 + shift < w0))
+            continue;
+        const bool partly = a.causal && q0 + shift < w0 + KT * 16 - 1;
+#pragma unroll
+        for (int b = 0; b < QB / 32; ++b) {
+            f32x4 s[2][2][KT], dp[2][KT];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r0 = b * 32 + u * 16;
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+                    s[0][u][t] = s[1][u][t] = dp[u][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int kk = 0; kk < D / 32; ++kk) {
+                        const Frag<T> qf = TL::row_frag(smem, r0, m * D + kk * 32, lane);
+                        const Frag<T> df = TL::row_frag(smem + kTile, r0, m * D + kk * 32, lane);
+#pragma unroll
+                        for (int t = 0; t < KT; ++t) {
+                            s[m][u][t] = mma(qf, kf[m][t][kk], s[m][u][t]);
+                            dp[u][t] = mma(df, vf[m][t][kk], dp[u][t]);
+                        }
+                    }
+            }
+            Frag<T> pf[KT], sf[2][KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                // the first row of this block that sees the lane's key
+                const int from = a.causal ? w0 + t * 16 + (lane & 15) - shift - q0 - 32 * b - 4 * g : -1;
+                f32x4 both[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r0 = b * 32 + u * 16 + 4 * g;
+                    const f32x4 l0 = *reinterpret_cast<const f32x4 *>(stat + r0);
+                    const f32x4 l1 = *reinterpret_cast<const f32x4 *>(stat + QB + r0);
+                    const f32x4 d0 = *reinterpret_cast<const f32x4 *>(stat + 2 * QB + r0);
+                    const f32x4 d1 = *reinterpret_cast<const f32x4 *>(stat + 3 * QB + r0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float p0 = exp2_fast(fmaf(s[0][u][t][r], c, -l0[r]));
+                        float p1 = exp2_fast(fmaf(s[1][u][t][r], c, -l1[r]));
+                        if (partly && 16 * u + r < from)
+                            p0 = p1 = 0.f;
+                        p1 *= -lambda;
+                        both[u][r] = p0 + p1;
+                        s[0][u][t][r] = p0 * (dp[u][t][r] - d0[r]);
+                        s[1][u][t][r] = p1 * (dp[u][t][r] - d1[r]);
+                    }
+                }
+                pf[t] = pack<T>(both[0], both[1]);
+                sf[0][t] = pack<T>(s[0][0][t], s[0][1][t]);
+                sf[1][t] = pack<T>(s[1][0][t], s[1][1][t]);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const Frag<T> df = TL::column_frag(smem + kTile, b * 32, i * 16, lane);
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+                    dv[t][i] = mma(df, pf[t], dv[t][i]);
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const Frag<T> qf = TL::column_frag(smem, b * 32, m * D + i * 16, lane);
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+                        dk[m][t][i] = mma(qf, sf[m][t], dk[m][t][i]);
+                }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const int key = w0 + t * 16 + (lane & 15);
+        if (key >= sq.nk)
+            continue;
+        // a masked key's gradients are 0, whatever its column holds
+        const f32x4 none = {0, 0, 0, 0};
+        T *kp = (T *)a.dk.data + kv * a.dk.head + (sq.k0 + key) * a.dk.row;
+        T *vp = (T *)a.dv.data + kv * a.dv.head + (sq.k0 + key) * a.dv.row;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                store4(kp + m * a.dk.map, i * 16 + 4 * g, a.dim, live[t] ? dk[m][t][i] * a.scale : none, a.vec);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+            store_columns<T, D>(vp, a.dv.map, a.dim, i, lane, live[t] ? dv[t][i] : none, a.vec);
+    }
+}
+
+#if MTPX_OPS_TYPE == 0
+// Sums the query tiles' shares of dlambda, one workgroup per head.
+__global__ __launch_bounds__(kThreads) void dlambda_kernel(const float *part, float *dlambda, int n)
+{
+    __shared__ float red[kThreads];
+    const int tid = threadIdx.x;
+    float v = 0.f;
+    for (int i = tid; i < n; i += kThreads)
+        v += part[(int64_t)blockIdx.x * n + i];
+    red[tid] = v;
+    __syncthreads();
+    for (int o = kThreads / 2; o > 0; o >>= 1) {
+        if (tid < o)
+            red[tid] += red[tid + o];
+        __syncthreads();
+    }
+    if (tid == 0)
+        dlambda[blockIdx.x] = red[0];
+}
+#endif
+
+// One query row per sequence.  A workgroup takes one key head of one sequence
+// and one of `splits` runs of its keys, for up to 16 of the query heads that
+// share the key head (the columns of S^T; fewer leave columns empty, which
+// costs nothing, as the reads of the cache bound the kernel).  Its waves take
+// steps of 32 keys in turn, each with its own maxima and sums: no wave waits
+// for another until the end.  A wave reads K as operand A straight from
+// memory; V goes through LDS of its own to be read by columns.  The waves'
+// results are joined through LDS, the workgroups' by attn_cache_join, from
+// [split][head][2][2 + 2 D] floats (maximum, sum, product).
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
+{
+    using TL = Tile<T, D>;
+    constexpr int kTile = 32 * TL::kRowBytes;
+    constexpr int kPart = 2 + 2 * D;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int group = a.heads / a.kv_heads, blocks = (group + 15) / 16;
+    const int split = blockIdx.x, kv = blockIdx.y / blocks, seq = blockIdx.z;
+    const int head0 = kv * group + blockIdx.y % blocks * 16;
+    const int count = min(16, (kv + 1) * group - head0);
+    const float c = a.scale * kLog2e;
+    char *tile = smem + wave * kTile;
+
+    int64_t len = a.lengths[seq];
+    len = len < 0 ? 0 : len > a.capacity ? a.capacity : len;
+    // whole steps, split as evenly as they go
+    const int64_t nsteps = (len + 31) / 32;
+    const int64_t s0 = nsteps * split / a.splits, s1 = nsteps * (split + 1) / a.splits;
+
+    const T *kp = (const T *)a.k.data + seq * a.k_sequence + kv * a.k.head;
+    const T *vp = (const T *)a.v.data + seq * a.v_sequence + kv * a.v.head;
+
+    const int col = lane & 15;
+    const T *qp = (const T *)a.q.data + seq * a.q.row + (head0 + col) * a.q.head;
+    Frag<T> qf[2][D / 32];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk)
+            qf[m][kk] = load_frag(qp + m * a.q.map, kk * 32 + 8 * g, a.dim, col < count, a.vec);
+
+    f32x4 acc[2][D / 8];
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+        acc[0][i] = acc[1][i] = f32x4{0, 0, 0, 0};
+
+    Stage<T, D, 32, kWave> sv;
+    Frag<T> kf[2][2][D / 32];
+    auto fetch = [&](int64_t step) {
+        const int64_t k0 = step * 32;
+        const int there = (int)min((int64_t)32, len - k0);
+        const unsigned long long bits = (1ull << there) - 1;
+        sv.load(vp, a.v, a.dim, k0, bits, lane, a.vec);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = 16 * u + (lane & 15);
+            const T *p = kp + (k0 + r) * a.k.row;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int kk = 0; kk < D / 32; ++kk)
+                    kf[u][m][kk] = load_frag(p + m * a.k.map, kk * 32 + 8 * g, a.dim, r < there, a.vec);
+        }
+    };
+    if (s0 + wave < s1)
+        fetch(s0 + wave);
+    for (int64_t step = s0 + wave; step < s1; step += kWaves) {
+        const int there = (int)min((int64_t)32, len - step * 32);
+        f32x4 s[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                s[m][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int kk = 0; kk < D / 32; ++kk)
+                    s[m][u] = mma(kf[u][m][kk], qf[m][kk], s[m][u]);
+            }
+        // the wave's own reads of the last step's values are done before these
+        // writes: both go through the LDS in program order
+        sv.store(tile, lane);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (step + kWaves < s1)
+            fetch(step + kWaves);
+        if (there < 32) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * u + 4 * g + r >= there)
+                        s[0][u][r] = s[1][u][r] = -INFINITY;
+        }
+        Frag<T> pf[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float hi = s[m][0][0];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    hi = fmaxf(hi, s[m][u][r]);
+            hi = fmaxf(top[m], column_max(hi));
+            if (__any(hi > top[m])) {
+                const float f = top[m] == -INFINITY ? 0.f : exp2_fast((top[m] - hi) * c);
+                top[m] = hi;
+                sum[m] *= f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    acc[m][i] *= f;
+            }
+            const float base = hi == -INFINITY ? 0.f : hi * c;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = exp2_fast(fmaf(s[m][u][r], c, -base));
+                    s[m][u][r] = p;
+                    sum[m] += p;
+                }
+            pf[m] = pack<T>(s[m][0], s[m][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const Frag<T> vf = TL::column_frag(tile, 0, i * 16, lane);
+            acc[0][i] = mma(vf, pf[0], acc[0][i]);
+            acc[1][i] = mma(vf, pf[1], acc[1][i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // Join the waves, one map at a time: column-major products in LDS.
+    float *red = reinterpret_cast<float *>(smem);  // [kWaves][16][kPart]
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const float total = column_sum(sum[m]);
+        __syncthreads();
+        float *mine = red + (wave * 16 + col) * kPart;
+        if (g == 0) {
+            mine[0] = top[m];
+            mine[1] = total;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                mine[2 + i * 16 + 4 * g + r] = acc[m][i][r];
+        __syncthreads();
+        for (int e = tid; e < count * kPart; e += kThreads) {
+            const int h = e / kPart, x = e % kPart;
+            float hi = -INFINITY;
+            for (int w = 0; w < kWaves; ++w)
+                hi = fmaxf(hi, red[(w * 16 + h) * kPart]);
+            float v = 0.f;
+            for (int w = 0; w < kWaves; ++w) {
+                const float *o = red + (w * 16 + h) * kPart;
+                const float f = o[0] == -INFINITY ? 0.f : exp2_fast((o[0] - hi) * c);
+                v += f * o[x ? x : 1];
+            }
+            a.part[((((int64_t)seq * a.heads + head0 + h) * 2 + m) * a.splits + split) * kPart + x] = x ? v : hi;
+        }
+    }
+}
+
+// Joins the splits of one sequence and head: one workgroup, a thread per
+// column of the two products.
+template <class T, int D>
+__global__ __launch_bounds__(2 * D) void attn_cache_join(CacheArgs a)
+{
+    constexpr int kPart = 2 + 2 * D;
+    const int x = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
+    const float c = a.scale * kLog2e;
+    float o[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const float *p = a.part + (((int64_t)seq * a.heads + head) * 2 + m) * a.splits * kPart;
+        float hi = -INFINITY;
+        for (int i = 0; i < a.splits; ++i)
+            hi = fmaxf(hi, p[i * kPart]);
+        float total = 0.f, v = 0.f;
+        for (int i = 0; i < a.splits; ++i) {
+            const float f = p[i * kPart] == -INFINITY ? 0.f : exp2_fast((p[i * kPart] - hi) * c);
+            total += f * p[i * kPart + 1];
+            v += f * p[i * kPart + 2 + x];
+        }
+        o[m] = total == 0.f ? 0.f : v / total;
+    }
+    const int m = x / D, col = x % D;
+    if (col < a.dim)
+        ((T *)a.out.data)[seq * a.out.row + head * a.out.head + m * a.out.map + col] =
+            (T)(o[0] - a.lambda[head] * o[1]);
+}
+
+// Tile shapes by head width: rows of a wave (16 QT), rows of a tile in LDS.
+template <class T, int D>
+struct Shape {
+    static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
+    static constexpr int kWide = (D <= 64 && sizeof(T) == 2) || D == 32 ? 2 : 1;
+    static constexpr int kTable = kWide == 2 ? 1 : 0;  // kTileRows
+    static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
+};
+
+template <int D>
+hipError_t forward(const AttnArgs &a, hipStream_t s)
+{
+    using S = Shape<Type, D>;
+    const int n = a.tiles.nq[S::kTable];
+    attn_forward_kernel<Type, D, S::kWide, S::kRows>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kLds, s>>>(a, S::kTable, n);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t backward(const AttnArgs &a, hipStream_t s)
+{
+    using S = Shape<Type, D>;
+    const int nq = a.tiles.nq[S::kTable], nk = a.tiles.nk[S::kTable];
+    if (nq > 0) {
+        attn_dq_kernel<Type, D, S::kWide, S::kRows>
+            <<<dim3((unsigned)((int64_t)nq * a.heads)), dim3(kThreads), S::kLds, s>>>(a, S::kTable, nq);
+        if (hipError_t e = hipGetLastError())
+            return e;
+    }
+    if (nk > 0) {
+        attn_dkv_kernel<Type, D, S::kWide, S::kRows>
+            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(kThreads),
+               S::kLds + 4 * S::kRows * sizeof(float), s>>>(a, S::kTable, nk);
+    }
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t cache(const CacheArgs &a, hipStream_t s)
+{
+    const int group = a.heads / a.kv_heads;
+    const size_t tiles = (size_t)kWaves * 32 * 2 * D * sizeof(Type);
+    const size_t join = (size_t)kWaves * 16 * (2 + 2 * D) * sizeof(float);
+    attn_cache_kernel<Type, D><<<dim3(a.splits, a.kv_heads * ((group + 15) / 16), a.sequences),
+                                 dim3(kThreads), tiles > join ? tiles : join, s>>>(a);
+    if (hipError_t e = hipGetLastError())
+        return e;
+    attn_cache_join<Type, D><<<dim3(a.heads, a.sequences), dim3(2 * D), 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t MTPX_OPS_NAME(attn_forward)(const AttnArgs &a, hipStream_t s)
+{
+    return a.dim <= 32 ? forward<32>(a, s) : a.dim <= 64 ? forward<64>(a, s) : forward<128>(a, s);
+}
+hipError_t MTPX_OPS_NAME(attn_backward)(const AttnArgs &a, hipStream_t s)
+{
+    return a.dim <= 32 ? backward<32>(a, s) : a.dim <= 64 ? backward<64>(a, s) : backward<128>(a, s);
+}
+hipError_t MTPX_OPS_NAME(attn_cache)(const CacheArgs &a, hipStream_t s)
+{
+    return a.dim <= 32 ? cache<32>(a, s) : a.dim <= 64 ? cache<64>(a, s) : cache<128>(a, s);
+}
+int MTPX_OPS_NAME(attn_tiles)(int dim, const TileTable &t)
+{
+    return t.nq[dim <= 32 ? Shape<Type, 32>::kTable
+                          : dim <= 64 ? Shape<Type, 64>::kTable : Shape<Type, 128>::kTable];
+}
+
+#if MTPX_OPS_TYPE == 0
+hipError_t attn_forward_bf16(const AttnArgs &, hipStream_t);
+hipError_t attn_forward_f16(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_bf16(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_f16(const AttnArgs &, hipStream_t);
+hipError_t attn_cache_bf16(const CacheArgs &, hipStream_t);
+hipError_t attn_cache_f16(const CacheArgs &, hipStream_t);
+int attn_tiles_bf16(int, const TileTable &);
+int attn_tiles_f16(int, const TileTable &);
+
+int attn_backward_tiles(int dtype, int dim, const TileTable &t)
+{
+    return dtype == MTPX_F32 ? attn_tiles_f32(dim, t)
+                             : dtype == MTPX_BF16 ? attn_tiles_bf16(dim, t) : attn_tiles_f16(dim, t);
+}
+hipError_t launch_attn_forward(int dtype, const AttnArgs &a, hipStream_t s)
+{
+    return dtype == MTPX_F32 ? attn_forward_f32(a, s)
+                             : dtype == MTPX_BF16 ? attn_forward_bf16(a, s) : attn_forward_f16(a, s);
+}
+hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s)
+{
+    const hipError_t e = dtype == MTPX_F32 ? attn_backward_f32(a, s)
+                         : dtype == MTPX_BF16 ? attn_backward_bf16(a, s) : attn_backward_f16(a, s);
+    if (e != hipSuccess)
+        return e;
+    dlambda_kernel<<<dim3(a.heads), dim3(kThreads), 0, s>>>(a.dlam_part, a.dlambda,
+                                                            attn_backward_tiles(dtype, a.dim, a.tiles));
+    return hipGetLastError();
+}
+hipError_t launch_attn_cache(int dtype, const CacheArgs &a, hipStream_t s)
+{
+    return dtype == MTPX_F32 ? attn_cache_f32(a, s)
+                             : dtype == MTPX_BF16 ? attn_cache_bf16(a, s) : attn_cache_f16(a, s);
+}
+#endif
+
+}  // namespace mtpx

@@ -1,0 +1,555 @@
+// C ABI of the operators on device tensors (include/mtpx.h): argument checks,
+// workspaces, launches on the caller's stream.
+#include "context.hpp"
+#include "ops_internal.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <new>
+
+struct mtpx_sequences {
+    int device = 0, n = 0;
+    int64_t total_q = 0, total_k = 0;
+    DBuf seq, tiles;
+    TileTable table{};
+    ~mtpx_sequences()
+    {
+        seq.release();
+        tiles.release();
+    }
+};
+
+namespace mtpx {
+namespace {
+
+constexpr int64_t kMaxLength = int64_t(1) << 30;  // rows of one sequence
+constexpr int64_t kMaxGrid = INT32_MAX;
+constexpr int kMaxSplits = 128;
+
+int invalid(mtpx_context *ctx, const std::string &msg) { return set_error(ctx, MTPX_E_INVALID, msg); }
+
+size_t dtype_bytes(int dtype) { return dtype == MTPX_F32 ? 4 : 2; }
+bool is_dtype(int d) { return d == MTPX_F32 || d == MTPX_BF16 || d == MTPX_F16; }
+bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// A tensor of rows: present, element-aligned, strides that count forward.
+int check_rows(mtpx_context *ctx, const mtpx_rows &r, int dtype, const char *name)
+{
+    if (!r.data)
+        return invalid(ctx, std::string("null ") + name);
+    if (!aligned(r.data, dtype_bytes(dtype)))
+        return invalid(ctx, std::string(name) + " is not aligned to its elements");
+    if (r.row < 0 || r.head < 0 || r.map < 0)
+        return invalid(ctx, std::string(name) + " has a negative stride");
+    return MTPX_OK;
+}
+int check_flat(mtpx_context *ctx, const void *p, size_t align, const char *name)
+{
+    if (!p)
+        return invalid(ctx, std::string("null ") + name);
+    if (!aligned(p, align))
+        return invalid(ctx, std::string(name) + " is not aligned to its elements");
+    return MTPX_OK;
+}
+
+bool whole_pieces(const mtpx_rows &r, size_t size)
+{
+    return aligned(r.data, 16) && r.row * size % 16 == 0 && r.head * size % 16 == 0 &&
+           r.map * size % 16 == 0;
+}
+
+#define MTPX_TRY(expr)                                                                     \
+    do {                                                                                   \
+        if (int rc_ = (expr))                                                              \
+            return rc_;                                                                    \
+    } while (0)
+
+int check_heads(mtpx_context *ctx, int dtype, int heads, int kv_heads, int dim, float scale)
+{
+    if (!is_dtype(dtype))
+        return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
+        return invalid(ctx, "heads must be a positive multiple of kv_heads");
+    if (dim < 1)
+        return invalid(ctx, "dim must be positive");
+    if (dim > 128)
+        return set_error(ctx, MTPX_E_CAPACITY, "dim beyond 128");
+    if (!(scale > 0.f) || !std::isfinite(scale))
+        return invalid(ctx, "scale must be positive and finite");
+    return MTPX_OK;
+}
+
+struct AttnSizes {
+    size_t delta, part, total;
+};
+AttnSizes attn_workspace(const mtpx_diff_attention_request &r)
+{
+    const mtpx_sequences &q = *r.sequences;
+    auto pad = [](size_t n) { return (n + 15) / 16 * 16; };
+    AttnSizes s;
+    s.delta = pad(sizeof(float) * 2 * (size_t)r.heads * (size_t)q.total_q);
+    s.part = pad(sizeof(float) * (size_t)r.heads *
+                 (size_t)attn_backward_tiles(r.dtype, r.dim, q.table));
+    s.total = std::max<size_t>(s.delta + s.part, 16);
+    return s;
+}
+
+// Checks of both passes and the launch arguments they share.
+int attn_args(mtpx_context *ctx, const mtpx_diff_attention_request &r, bool back, AttnArgs &a)
+{
+    MTPX_TRY(check_heads(ctx, r.dtype, r.heads, r.kv_heads, r.dim, r.scale));
+    if (!r.sequences)
+        return invalid(ctx, "null sequences");
+    const mtpx_sequences &sq = *r.sequences;
+    if (sq.device != ctx->device)
+        return invalid(ctx, "the sequences belong to another device");
+    for (int i = 0; i < 2; ++i)
+        if ((int64_t)std::max(sq.table.nq[i], sq.table.nk[i]) * r.heads > kMaxGrid)
+            return set_error(ctx, MTPX_E_CAPACITY, "too many rows and heads for one launch");
+    const size_t size = dtype_bytes(r.dtype);
+    const bool q = sq.total_q > 0, k = sq.total_k > 0;
+    if (q) {
+        MTPX_TRY(check_rows(ctx, r.q, r.dtype, "q"));
+        MTPX_TRY(check_rows(ctx, r.out, r.dtype, "out"));
+    }
+    if (k) {
+        MTPX_TRY(check_rows(ctx, r.k, r.dtype, "k"));
+        MTPX_TRY(check_rows(ctx, r.v, r.dtype, "v"));
+    }
+    MTPX_TRY(check_flat(ctx, r.lambda, 4, "lambda"));
+    if ((r.lse != nullptr) != (r.out1 != nullptr))
+        return invalid(ctx, "lse and out1 are kept together");
+    if (r.lse) {
+        MTPX_TRY(check_flat(ctx, r.lse, 4, "lse"));
+        MTPX_TRY(check_flat(ctx, r.out1, size, "out1"));
+    }
+    bool vec = r.dim * size % 16 == 0 && (!r.out1 || aligned(r.out1, 16));
+    auto also = [&](const mtpx_rows &t) { vec = vec && (!t.data || whole_pieces(t, size)); };
+    for (const mtpx_rows *t : {&r.q, &r.k, &r.v, &r.out})
+        also(*t);
+    if (back) {
+        if (q) {
+            MTPX_TRY(check_rows(ctx, r.dout, r.dtype, "dout"));
+            MTPX_TRY(check_rows(ctx, r.dq, r.dtype, "dq"));
+            if (!r.lse)
+                return invalid(ctx, "null lse and out1");
+        }
+        if (k) {
+            MTPX_TRY(check_rows(ctx, r.dk, r.dtype, "dk"));
+            MTPX_TRY(check_rows(ctx, r.dv, r.dtype, "dv"));
+        }
+        MTPX_TRY(check_flat(ctx, r.dlambda, 4, "dlambda"));
+        for (const mtpx_rows *t : {&r.dout, &r.dq, &r.dk, &r.dv})
+            also(*t);
+    }
+    a.seq = sq.seq.as<Seq>();
+    a.tiles = sq.table;
+    a.heads = r.heads;
+    a.kv_heads = r.kv_heads;
+    a.dim = r.dim;
+    a.causal = r.causal != 0;
+    a.total_q = sq.total_q;
+    a.scale = r.scale;
+    a.q = r.q;
+    a.k = r.k;
+    a.v = r.v;
+    a.out = r.out;
+    a.dout = r.dout;
+    a.dq = r.dq;
+    a.dk = r.dk;
+    a.dv = r.dv;
+    a.mask = r.key_mask;
+    a.lambda = r.lambda;
+    a.out1 = r.out1;
+    a.lse = r.lse;
+    a.delta = a.dlam_part = nullptr;
+    a.dlambda = r.dlambda;
+    a.vec = vec;
+    return MTPX_OK;
+}
+
+// Workgroups that share one sequence's keys: enough to fill the device, each
+// with a step of 32 keys per wave at least.
+int cache_splits(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
+{
+    const int group = r.heads / r.kv_heads;
+    const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * ((group + 15) / 16), 1);
+    const int64_t most = std::max<int64_t>((r.capacity + 127) / 128, 1);
+    const int64_t want = (4 * (int64_t)ctx->num_cus + base - 1) / base;
+    return (int)std::min<int64_t>({want, most, (int64_t)kMaxSplits});
+}
+
+int check_cache(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
+{
+    MTPX_TRY(check_heads(ctx, r.dtype, r.heads, r.kv_heads, r.dim, r.scale));
+    if (r.sequences < 0 || r.capacity < 0)
+        return invalid(ctx, "negative count");
+    if (r.sequences > 65535 || r.heads > 65535)
+        return set_error(ctx, MTPX_E_CAPACITY, "more than 65535 sequences or heads");
+    return MTPX_OK;
+}
+size_t cache_bytes(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
+{
+    const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128;
+    return std::max<size_t>(sizeof(float) * 2 * (size_t)r.sequences * r.heads *
+                                cache_splits(ctx, r) * (2 + 2 * width),
+                            16);
+}
+
+int check_norm(mtpx_context *ctx, const mtpx_norm_block_request &r)
+{
+    if (!is_dtype(r.dtype))
+        return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
+    if (r.rows < 0 || r.width < 1)
+        return invalid(ctx, "rows must not be negative and width positive");
+    if (r.width > 16384 || r.rows > kMaxGrid)
+        return set_error(ctx, MTPX_E_CAPACITY, "width beyond 16384 or too many rows");
+    if (r.kind != MTPX_NORM_RMS && r.kind != MTPX_NORM_LAYER)
+        return invalid(ctx, "unknown norm kind");
+    if (r.gate_act < MTPX_GATE_NONE || r.gate_act > MTPX_GATE_TANH)
+        return invalid(ctx, "unknown gate activation");
+    if (!(r.eps >= 0.f) || !std::isfinite(r.residual_scale) || !std::isfinite(r.block_scale))
+        return invalid(ctx, "eps must not be negative and the scales finite");
+    for (int64_t s : {r.x_row, r.y_row, r.gate_row, r.s_row, r.n_row, r.ds_row, r.dn_row, r.dx_row,
+                      r.dy_row, r.dgate_row})
+        if (s < 0)
+            return invalid(ctx, "negative row stride");
+    return MTPX_OK;
+}
+
+int norm_args(mtpx_context *ctx, const mtpx_norm_block_request &r, bool back, NormArgs &a)
+{
+    MTPX_TRY(check_norm(ctx, r));
+    const size_t size = dtype_bytes(r.dtype);
+    bool vec = r.width * size % 16 == 0;
+    auto tensor = [&](const void *p, int64_t row, bool need, const char *name) -> int {
+        if (!p)
+            return need ? invalid(ctx, std::string("null ") + name) : MTPX_OK;
+        if (!aligned(p, size))
+            return invalid(ctx, std::string(name) + " is not aligned to its elements");
+        vec = vec && aligned(p, 16) && row * size % 16 == 0;
+        return MTPX_OK;
+    };
+    const bool rows = r.rows > 0;
+    MTPX_TRY(tensor(r.x, r.x_row, false, "x"));
+    MTPX_TRY(tensor(r.y, r.y_row, rows, "y"));
+    MTPX_TRY(tensor(r.gate, r.gate_row, false, "gate"));
+    MTPX_TRY(tensor(r.post_weight, 0, false, "post_weight"));
+    MTPX_TRY(tensor(r.pre_weight, 0, false, "pre_weight"));
+    if (r.stats && !aligned(r.stats, 16))
+        return invalid(ctx, "stats are not aligned to 16 bytes");
+    if (!back) {
+        MTPX_TRY(tensor(r.s, r.s_row, rows, "s"));
+        MTPX_TRY(tensor(r.n, r.n_row, false, "n"));
+    } else {
+        if (rows && !r.stats)
+            return invalid(ctx, "null stats");
+        if (r.dgate && !r.gate)
+            return invalid(ctx, "dgate without a gate");
+        if (r.dx && !r.x)
+            return invalid(ctx, "dx without x");
+        if (r.dpost_weight && !r.post_weight)
+            return invalid(ctx, "dpost_weight without post_weight");
+        if (r.dpre_weight && !r.pre_weight)
+            return invalid(ctx, "dpre_weight without pre_weight");
+        MTPX_TRY(tensor(r.ds, r.ds_row, false, "ds"));
+        MTPX_TRY(tensor(r.dn, r.dn_row, false, "dn"));
+        MTPX_TRY(tensor(r.dx, r.dx_row, false, "dx"));
+        MTPX_TRY(tensor(r.dy, r.dy_row, false, "dy"));
+        MTPX_TRY(tensor(r.dgate, r.dgate_row, false, "dgate"));
+        for (const void *p : {r.dpost_weight, r.dpre_weight})
+            if (!aligned(p, size))
+                return invalid(ctx, "a weight gradient is not aligned to its elements");
+    }
+    a = NormArgs{r.rows, r.width, r.kind, r.gate_act, r.residual_scale, r.block_scale, r.eps,
+                 r.x, r.y, r.gate, r.post_weight, r.pre_weight, r.x_row, r.y_row, r.gate_row,
+                 r.s, r.n, r.s_row, r.n_row, r.stats, r.ds, r.dn, r.ds_row, r.dn_row,
+                 r.dx, r.dy, r.dgate, r.dpost_weight, r.dpre_weight, r.dx_row, r.dy_row,
+                 r.dgate_row, nullptr, norm_backward_parts(r.rows, r.width), vec};
+    return MTPX_OK;
+}
+
+size_t norm_bytes(const mtpx_norm_block_request &r)
+{
+    return std::max<size_t>(sizeof(float) * 3 * (size_t)norm_backward_parts(r.rows, r.width) * r.width, 16);
+}
+
+int check_workspace(mtpx_context *ctx, const void *p, size_t have, size_t need)
+{
+    if (have < need || !p)
+        return invalid(ctx, "the workspace holds " + std::to_string(p ? have : 0) + " bytes, " +
+                                std::to_string(need) + " are needed");
+    if (!aligned(p, 16))
+        return invalid(ctx, "the workspace is not aligned to 16 bytes");
+    return MTPX_OK;
+}
+
+}  // namespace
+}  // namespace mtpx
+
+extern "C" {
+
+int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    const mtpx_rotary_request &r = *req;
+    if (!is_dtype(r.dtype))
+        return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
+    if (r.rows < 0 || r.heads < 1 || r.dim < 1)
+        return invalid(ctx, "rows must not be negative, heads and dim positive");
+    if (r.dim > 1024 || r.rows > kMaxGrid)
+        return set_error(ctx, MTPX_E_CAPACITY, "dim beyond 1024 or too many rows");
+    if (r.rotated < 0 || r.rotated > r.dim || r.rotated % 2 != 0)
+        return invalid(ctx, "rotated must be even and at most dim");
+    if (r.axes < 1 || r.axes > 8)
+        return invalid(ctx, "axes must be 1 to 8");
+    if (r.position_dtype != MTPX_F32 && r.position_dtype != MTPX_F64 &&
+        r.position_dtype != MTPX_I32 && r.position_dtype != MTPX_I64)
+        return invalid(ctx, "unknown position_dtype");
+    if (r.position_row < 0 || r.position_axis < 0)
+        return invalid(ctx, "negative position stride");
+    const size_t psize = r.position_dtype == MTPX_F32 || r.position_dtype == MTPX_I32 ? 4 : 8;
+    if (r.dpositions) {
+        if (!r.inverse)
+            return invalid(ctx, "dpositions needs inverse");
+        if (r.position_dtype != MTPX_F32 && r.position_dtype != MTPX_F64)
+            return invalid(ctx, "integer positions have no gradient");
+    }
+    if (r.rows == 0)
+        return MTPX_OK;
+    MTPX_TRY(check_rows(ctx, r.x, r.dtype, "x"));
+    MTPX_TRY(check_rows(ctx, r.y, r.dtype, "y"));
+    MTPX_TRY(check_flat(ctx, r.positions, psize, "positions"));
+    if (r.rotated > 0) {
+        MTPX_TRY(check_flat(ctx, r.freq, 4, "freq"));
+        MTPX_TRY(check_flat(ctx, r.axis, 4, "axis"));
+    }
+    if (r.dpositions) {
+        MTPX_TRY(check_rows(ctx, r.forward, r.dtype, "forward"));
+        MTPX_TRY(check_flat(ctx, r.dpositions, psize, "dpositions"));
+    }
+    if (r.y.data == r.x.data && (r.y.row != r.x.row || r.y.head != r.x.head))
+        return invalid(ctx, "y in the place of x needs its strides");
+    // the widest access that every piece of a row allows
+    const int64_t size = (int64_t)dtype_bytes(r.dtype), half = r.rotated / 2;
+    int width = (int)(16 / size);
+    auto fits = [&](const mtpx_rows &t) {
+        return aligned(t.data, width * size) && t.row % width == 0 && t.head % width == 0;
+    };
+    while (width > 1 && !((r.interleaved ? r.rotated : half) % width == 0 &&
+                          (r.dim - r.rotated) % width == 0 && fits(r.x) && fits(r.y) &&
+                          (!r.dpositions || fits(r.forward))))
+        width /= 2;
+    RotaryArgs a{r.rows, r.heads, r.dim, r.rotated, r.interleaved != 0, r.inverse != 0, r.axes,
+                 r.position_dtype, r.x, r.y, r.forward, r.positions, r.position_row,
+                 r.position_axis, r.freq, r.axis, r.dpositions, width};
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_rotary(r.dtype, a, (hipStream_t)r.stream), "launch rotary");
+    return MTPX_OK;
+}
+
+int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
+                          const int64_t *k_offsets, mtpx_sequences **out)
+{
+    if (!ctx || !out)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    *out = nullptr;
+    if (n < 0 || !q_offsets)
+        return invalid(ctx, "sequences need a count and offsets");
+    const int64_t *ko = k_offsets ? k_offsets : q_offsets;
+    if (q_offsets[0] != 0 || ko[0] != 0)
+        return invalid(ctx, "offsets start at 0");
+    for (int i = 0; i < n; ++i) {
+        if (q_offsets[i + 1] < q_offsets[i] || ko[i + 1] < ko[i])
+            return invalid(ctx, "offsets must ascend");
+        if (q_offsets[i + 1] - q_offsets[i] > kMaxLength || ko[i + 1] - ko[i] > kMaxLength)
+            return set_error(ctx, MTPX_E_CAPACITY, "a sequence of more than 2^30 rows");
+    }
+    mtpx_sequences *sq = nullptr;
+    try {
+        sq = new mtpx_sequences;
+        sq->device = ctx->device;
+        sq->n = n;
+        sq->total_q = q_offsets[n];
+        sq->total_k = ko[n];
+        std::vector<Seq> seqs((size_t)n);
+        for (int i = 0; i < n; ++i)
+            seqs[i] = Seq{q_offsets[i], ko[i], (int)(q_offsets[i + 1] - q_offsets[i]),
+                          (int)(ko[i + 1] - ko[i])};
+        // the tiles with the most work first: they start while there is other
+        // work to fill the device's last round with
+        std::vector<SeqTile> all;
+        size_t first[4], count[4];
+        for (int side = 0; side < 2; ++side)
+            for (int j = 0; j < 2; ++j) {
+                std::vector<SeqTile> t;
+                for (int i = 0; i < n; ++i) {
+                    const int rows = side ? seqs[i].nk : seqs[i].nq;
+                    for (int64_t s = 0; s < rows; s += kTileRows[j])
+                        t.push_back(SeqTile{i, (int)s});
+                }
+                std::stable_sort(t.begin(), t.end(), [&](const SeqTile &a, const SeqTile &b) {
+                    const int la = side ? seqs[a.seq].nq : seqs[a.seq].nk;
+                    const int lb = side ? seqs[b.seq].nq : seqs[b.seq].nk;
+                    // with causal rows the last queries and the first keys have the most
+                    return la != lb ? la > lb : side ? a.start < b.start : a.start > b.start;
+                });
+                if (t.size() > (size_t)kMaxGrid) {
+                    delete sq;
+                    return set_error(ctx, MTPX_E_CAPACITY, "too many rows for one launch");
+                }
+                first[2 * side + j] = all.size();
+                count[2 * side + j] = t.size();
+                all.insert(all.end(), t.begin(), t.end());
+            }
+        (void)hipSetDevice(ctx->device);
+        hipError_t e = upload(sq->seq, seqs, ctx->stream);
+        if (e == hipSuccess)
+            e = upload(sq->tiles, all, ctx->stream);
+        if (e == hipSuccess)
+            e = hipStreamSynchronize(ctx->stream);
+        if (e != hipSuccess) {
+            delete sq;
+            return hip_fail(ctx, e, "upload sequences");
+        }
+        for (int j = 0; j < 2; ++j) {
+            sq->table.q[j] = sq->tiles.as<SeqTile>() + first[j];
+            sq->table.k[j] = sq->tiles.as<SeqTile>() + first[2 + j];
+            sq->table.nq[j] = (int)count[j];
+            sq->table.nk[j] = (int)count[2 + j];
+        }
+    } catch (const std::exception &) {
+        delete sq;
+        return set_error(ctx, MTPX_E_ALLOC, "out of host memory");
+    }
+    *out = sq;
+    return MTPX_OK;
+}
+
+void mtpx_sequences_destroy(mtpx_sequences *seqs)
+{
+    if (!seqs)
+        return;
+    (void)hipSetDevice(seqs->device);
+    delete seqs;
+}
+
+int mtpx_diff_attention(mtpx_context *ctx, const mtpx_diff_attention_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    AttnArgs a{};
+    MTPX_TRY(attn_args(ctx, *req, false, a));
+    if (a.total_q == 0)
+        return MTPX_OK;
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_attn_forward(req->dtype, a, (hipStream_t)req->stream), "launch attention");
+    return MTPX_OK;
+}
+
+int mtpx_diff_attention_workspace(mtpx_context *ctx, const mtpx_diff_attention_request *req,
+                                  size_t *bytes)
+{
+    if (!ctx || !req || !bytes)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    MTPX_TRY(check_heads(ctx, req->dtype, req->heads, req->kv_heads, req->dim, 1.f));
+    if (!req->sequences)
+        return invalid(ctx, "null sequences");
+    *bytes = attn_workspace(*req).total;
+    return MTPX_OK;
+}
+
+int mtpx_diff_attention_backward(mtpx_context *ctx, const mtpx_diff_attention_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    AttnArgs a{};
+    MTPX_TRY(attn_args(ctx, *req, true, a));
+    const AttnSizes w = attn_workspace(*req);
+    MTPX_TRY(check_workspace(ctx, req->workspace, req->workspace_bytes, w.total));
+    a.delta = static_cast<float *>(req->workspace);
+    a.dlam_part = a.delta + w.delta / sizeof(float);
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_attn_backward(req->dtype, a, (hipStream_t)req->stream), "launch attention gradient");
+    return MTPX_OK;
+}
+
+int mtpx_diff_attention_cache_workspace(mtpx_context *ctx,
+                                        const mtpx_diff_attention_cache_request *req, size_t *bytes)
+{
+    if (!ctx || !req || !bytes)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    mtpx_diff_attention_cache_request r = *req;
+    r.scale = 1.f;
+    MTPX_TRY(check_cache(ctx, r));
+    *bytes = cache_bytes(ctx, r);
+    return MTPX_OK;
+}
+
+int mtpx_diff_attention_cache(mtpx_context *ctx, const mtpx_diff_attention_cache_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    const mtpx_diff_attention_cache_request &r = *req;
+    MTPX_TRY(check_cache(ctx, r));
+    if (r.sequences == 0)
+        return MTPX_OK;
+    MTPX_TRY(check_rows(ctx, r.q, r.dtype, "q"));
+    MTPX_TRY(check_rows(ctx, r.out, r.dtype, "out"));
+    if (r.capacity > 0) {
+        MTPX_TRY(check_rows(ctx, r.k, r.dtype, "k"));
+        MTPX_TRY(check_rows(ctx, r.v, r.dtype, "v"));
+        if (r.k_sequence < 0 || r.v_sequence < 0)
+            return invalid(ctx, "negative sequence stride");
+    }
+    MTPX_TRY(check_flat(ctx, r.lengths, 4, "lengths"));
+    MTPX_TRY(check_flat(ctx, r.lambda, 4, "lambda"));
+    MTPX_TRY(check_workspace(ctx, r.workspace, r.workspace_bytes, cache_bytes(ctx, r)));
+    const size_t size = dtype_bytes(r.dtype);
+    const bool vec = r.dim * size % 16 == 0 && whole_pieces(r.q, size) && whole_pieces(r.k, size) &&
+                     whole_pieces(r.v, size) && r.k_sequence * size % 16 == 0 &&
+                     r.v_sequence * size % 16 == 0;
+    CacheArgs a{r.sequences, r.heads, r.kv_heads, r.dim, cache_splits(ctx, r), r.capacity,
+                r.k_sequence, r.v_sequence, r.scale, r.q, r.k, r.v, r.out, r.lengths, r.lambda,
+                static_cast<float *>(r.workspace), vec};
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_attn_cache(r.dtype, a, (hipStream_t)r.stream), "launch cache attention");
+    return MTPX_OK;
+}
+
+int mtpx_norm_block(mtpx_context *ctx, const mtpx_norm_block_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    NormArgs a;
+    MTPX_TRY(norm_args(ctx, *req, false, a));
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_norm_forward(req->dtype, a, (hipStream_t)req->stream), "launch norm block");
+    return MTPX_OK;
+}
+
+int mtpx_norm_block_workspace(mtpx_context *ctx, const mtpx_norm_block_request *req, size_t *bytes)
+{
+    if (!ctx || !req || !bytes)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    MTPX_TRY(check_norm(ctx, *req));
+    *bytes = norm_bytes(*req);
+    return MTPX_OK;
+}
+
+int mtpx_norm_block_backward(mtpx_context *ctx, const mtpx_norm_block_request *req)
+{
+    if (!ctx || !req)
+        return set_error(ctx, MTPX_E_INVALID, "null argument");
+    NormArgs a;
+    MTPX_TRY(norm_args(ctx, *req, true, a));
+    MTPX_TRY(check_workspace(ctx, req->workspace, req->workspace_bytes, norm_bytes(*req)));
+    a.part = static_cast<float *>(req->workspace);
+    (void)hipSetDevice(ctx->device);
+    HIP_TRY(launch_norm_backward(req->dtype, a, (hipStream_t)req->stream), "launch norm block gradient");
+    return MTPX_OK;
+}
+
+}  // extern "C"

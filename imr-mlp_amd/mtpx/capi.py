@@ -438,6 +438,7 @@ class Context:
         if rc != OK:
             raise MtpxError(rc, "mtpx_create(%d)" % device)
         self.h = h
+        self.device = device
 
     def close(self):
         if getattr(self, "h", None):

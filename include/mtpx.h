@@ -584,6 +584,190 @@ int mtpx_orthogonalize(mtpx_context *ctx);
  * {whole call, components kernel, Gram kernel, rows}. */
 int mtpx_last_linear_timings(const mtpx_context *ctx, double out[4]);
 
+/* ---- operators on device tensors --------------------------------------
+ * The parts of a trained block over all atoms of a structure (or all tokens
+ * of a sequence), next to the short-ranged descriptors: rotary positions
+ * with several axes, differential attention, and the norms around a block
+ * with its gate and residual scale.  No counterpart in the reference.
+ *
+ * These calls take device pointers on the context's device.  They check
+ * their arguments, queue kernels on the caller's stream and return without
+ * waiting: no host memory is read after the return, nothing is allocated
+ * (scratch memory is the caller's workspace), so a call can be recorded into
+ * a HIP graph.  A tensor used on another stream is the caller's to order.
+ * `stream` is a hipStream_t; NULL is the device's default stream, not the
+ * context's own.
+ *
+ * Tensors hold MTPX_BF16, MTPX_F16 or MTPX_F32; one call has one such type
+ * for all its tensors unless a field says otherwise.  Sums, statistics and
+ * exponentials are 32-bit floats whatever the type, results are rounded once
+ * when they are written, and no result depends on the order in which
+ * workgroups run.  Every tensor's last dimension is contiguous; the other
+ * strides are counted in elements and may be any non-negative value (0
+ * broadcasts an input; outputs must not overlap).  Addresses need the
+ * alignment of one element; rows at multiples of 16 bytes are read faster. */
+#define MTPX_F32 0
+#define MTPX_BF16 1
+#define MTPX_F16 2
+#define MTPX_F64 3 /* positions and their gradient only */
+#define MTPX_I32 4 /* positions only */
+#define MTPX_I64 5 /* positions only */
+
+/* Rows of heads: element e of map m of head h of row r is at
+ * data[r * row + h * head + m * map + e]. */
+typedef struct mtpx_rows {
+    void *data;
+    int64_t row, head, map;
+} mtpx_rows;
+
+/* Rotary positions on several axes.  Pair p < rotated / 2 of every head of
+ * row r turns by theta = positions[r][axis[p]] * freq[p]:
+ *   y1 = x1 cos(theta) - x2 sin(theta),  y2 = x1 sin(theta) + x2 cos(theta).
+ * The pair is (p, p + rotated / 2), or (2p, 2p + 1) with `interleaved`;
+ * elements from `rotated` on are copied.  theta is reduced in 64 bits, so
+ * large positions keep their phase.  `inverse` turns by -theta: the backward
+ * pass, x being the gradient of y and y the gradient of x.  With
+ * dpositions (needs inverse, and `forward`, the x of the forward pass) the
+ * gradient of the positions is written as well: f64 for f64 positions, f32
+ * for f32 ones; integer positions have none.  y may be x itself (same
+ * strides). */
+typedef struct mtpx_rotary_request {
+    void *stream;
+    int dtype;
+    int64_t rows;
+    int heads, dim, rotated; /* rotated even, at most dim; dim <= 1024 */
+    int interleaved, inverse;
+    mtpx_rows x, y;          /* map unused */
+    const void *positions;   /* [rows][axes]; MTPX_F32, F64, I32 or I64 */
+    int position_dtype;
+    int64_t position_row, position_axis;
+    int axes;                /* 1 to 8 */
+    const float *freq;       /* [rotated / 2], radians per unit */
+    const int *axis;         /* [rotated / 2], each in [0, axes); others are read as axis 0 */
+    mtpx_rows forward;
+    void *dpositions;        /* [rows][axes], contiguous */
+} mtpx_rotary_request;
+int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *request);
+
+/* Sequences of a ragged batch: sequence i holds the query rows
+ * [q_offsets[i], q_offsets[i + 1]) and the key rows [k_offsets[i],
+ * k_offsets[i + 1]) (host arrays of n + 1, ascending from 0; k_offsets NULL:
+ * the same).  Empty sequences are allowed.  Built once per batch; waits for
+ * its upload.  Destroy it after the work that uses it has finished. */
+typedef struct mtpx_sequences mtpx_sequences;
+int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
+                          const int64_t *k_offsets, mtpx_sequences **out);
+void mtpx_sequences_destroy(mtpx_sequences *seqs);
+
+/* Differential attention over a ragged batch:
+ *   P_m = softmax(scale q_m k_m^T),  m = 0, 1
+ *   out = (P_0 - lambda[head] P_1) v
+ * per sequence and head; head h reads the keys and values of head
+ * h / (heads / kv_heads).  q and k hold two maps of `dim` elements, v and
+ * out 2 dim elements (two "maps" of dim, contiguous or not).  A key is seen
+ * by a row if key_mask is NULL or nonzero for it, and, with `causal`, if it
+ * is not after the row (the last row of a sequence sees its last key).  A
+ * row without a key gives 0, its gradient is 0 and its lse -inf.  What q, k,
+ * v hold at masked keys does not matter, NaN included; keys and values that
+ * only later rows of a causal sequence see must be finite.
+ *
+ * Forward: out; with lse (f32 [2][heads][q rows], natural logarithm) and
+ * out1 ([q rows][heads][2 dim], contiguous: P_1 v) what the backward pass
+ * needs is kept; both or neither.
+ * Backward: reads q, k, v, lambda, out, out1, lse and dout; writes dq, dk,
+ * dv (every element of every row) and dlambda [heads].  Shared heads' and
+ * all rows' gradients are summed in a fixed order. */
+typedef struct mtpx_diff_attention_request {
+    void *stream;
+    int dtype;
+    const mtpx_sequences *sequences;
+    int heads, kv_heads, dim; /* dim 1 to 128 */
+    int causal;
+    float scale;              /* positive */
+    mtpx_rows q, k, v;
+    const unsigned char *key_mask; /* [k rows] or NULL */
+    const float *lambda;      /* [heads] */
+    mtpx_rows out;
+    void *out1;
+    float *lse;
+    mtpx_rows dout, dq, dk, dv;    /* backward only */
+    float *dlambda;
+    void *workspace;          /* backward only, 16-byte aligned */
+    size_t workspace_bytes;
+} mtpx_diff_attention_request;
+int mtpx_diff_attention(mtpx_context *ctx, const mtpx_diff_attention_request *request);
+int mtpx_diff_attention_backward(mtpx_context *ctx, const mtpx_diff_attention_request *request);
+/* Workspace of mtpx_diff_attention_backward for these sequences and heads. */
+int mtpx_diff_attention_workspace(mtpx_context *ctx, const mtpx_diff_attention_request *request,
+                                  size_t *bytes);
+
+/* One query row per sequence against a cache: row b sees the first
+ * lengths[b] of the `capacity` rows of cache b (device array; values beyond
+ * [0, capacity] are clamped; 0 gives 0).  What the cache holds beyond a
+ * length does not matter.  A sequence's keys are split over workgroups whose
+ * partial results the workspace holds. */
+typedef struct mtpx_diff_attention_cache_request {
+    void *stream;
+    int dtype;
+    int sequences, heads, kv_heads, dim;
+    int64_t capacity;
+    float scale;
+    mtpx_rows q, k, v;        /* q.row, k.row, v.row: stride of the sequence for q, of a cached row for k, v */
+    int64_t k_sequence, v_sequence;
+    const int *lengths;
+    const float *lambda;
+    mtpx_rows out;
+    void *workspace;
+    size_t workspace_bytes;
+} mtpx_diff_attention_cache_request;
+int mtpx_diff_attention_cache(mtpx_context *ctx, const mtpx_diff_attention_cache_request *request);
+int mtpx_diff_attention_cache_workspace(mtpx_context *ctx,
+                                        const mtpx_diff_attention_cache_request *request,
+                                        size_t *bytes);
+
+/* The norms around a block, its gate and the residual: with y the block's
+ * output and x the residual stream
+ *   u = norm(y),  s = residual_scale x + block_scale act(gate) (u post_weight)
+ *   n = norm(s) pre_weight
+ * norm(t) = t / sqrt(mean(t^2) + eps) (MTPX_NORM_RMS) or the same of
+ * t - mean(t) (MTPX_NORM_LAYER); n is taken of the unrounded s.  x NULL: no
+ * residual; gate NULL: 1; weights NULL: 1; n NULL: s only.  gate_row 0 is a
+ * gate shared by all rows.  stats (f32 [rows][4]) is what the backward pass
+ * needs.
+ * Backward: reads x, y, gate, the weights, stats, ds and dn (gradients of s
+ * and n; either may be NULL: zero); writes dx, dy, dgate ([rows][width], or
+ * [width] for a shared gate), dpost_weight and dpre_weight [width], each
+ * unless NULL. */
+#define MTPX_NORM_RMS 0
+#define MTPX_NORM_LAYER 1
+#define MTPX_GATE_NONE 0
+#define MTPX_GATE_SIGMOID 1
+#define MTPX_GATE_TANH 2
+typedef struct mtpx_norm_block_request {
+    void *stream;
+    int dtype;
+    int64_t rows;
+    int width;                /* 1 to 16384 */
+    int kind, gate_act;
+    float residual_scale, block_scale, eps;
+    const void *x, *y, *gate, *post_weight, *pre_weight;
+    int64_t x_row, y_row, gate_row;
+    void *s, *n;
+    int64_t s_row, n_row;
+    float *stats;
+    const void *ds, *dn;      /* backward only */
+    int64_t ds_row, dn_row;
+    void *dx, *dy, *dgate, *dpost_weight, *dpre_weight;
+    int64_t dx_row, dy_row, dgate_row;
+    void *workspace;
+    size_t workspace_bytes;
+} mtpx_norm_block_request;
+int mtpx_norm_block(mtpx_context *ctx, const mtpx_norm_block_request *request);
+int mtpx_norm_block_backward(mtpx_context *ctx, const mtpx_norm_block_request *request);
+/* Workspace of mtpx_norm_block_backward. */
+int mtpx_norm_block_workspace(mtpx_context *ctx, const mtpx_norm_block_request *request,
+                              size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif
