@@ -17,31 +17,40 @@ constexpr int kMaxBlock = 1024;
 // that are read at once (V 1 where rows are not whole 16-byte pieces).
 template <class T, int NT, int E, int V>
 struct Row {
-    static constexpr int kBlock = NT < 256 ? 256 : NT;
+    static constexpr int kBlock = NT == kWave ? 256 : NT;
     static constexpr int kPerBlock = kBlock / NT;  // rows of a workgroup
     static constexpr int kPieces = E / V;
     static __device__ inline int column(int i, int t) { return (i * NT + t) * V; }
 
-    // Columns beyond width are `beyond`.
-    static __device__ inline void load(const T *p, int width, int t, float beyond, float (&v)[E])
+    // A row as it lies in memory: read ahead, widened when it is needed.
+    // Columns beyond width are 0.
+    struct alignas(V * sizeof(T)) Piece {
+        T e[V];
+    };
+    struct Raw {
+        Piece p[kPieces];
+    };
+    static __device__ inline void fetch(const T *p, int width, int t, Raw &r)
     {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int c = column(i, t);
-            if constexpr (V == 1) {
-                v[i] = c < width ? (float)p[c] : beyond;
-            } else {
-                union {
-                    u32x4 v;
-                    T e[V];
-                } u;
-                if (c < width)
-                    u.v = *reinterpret_cast<const u32x4 *>(p + c);
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    v[i * V + j] = c < width ? (float)u.e[j] : beyond;
-            }
+            r.p[i] = Piece{};
+            if (c < width)
+                r.p[i] = *reinterpret_cast<const Piece *>(p + c);
         }
+    }
+    static __device__ inline void widen(const Raw &r, float (&v)[E])
+    {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            v[e] = (float)r.p[e / V].e[e % V];
+    }
+    static __device__ inline void load(const T *p, int width, int t, float (&v)[E])
+    {
+        Raw r;
+        fetch(p, width, t, r);
+        widen(r, v);
     }
     static __device__ inline void store(T *p, int width, int t, const float (&v)[E])
     {
@@ -50,18 +59,11 @@ struct Row {
             const int c = column(i, t);
             if (c >= width)
                 continue;
-            if constexpr (V == 1) {
-                p[c] = (T)v[i];
-            } else {
-                union {
-                    u32x4 v;
-                    T e[V];
-                } u;
+            Piece u;
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    u.e[j] = (T)v[i * V + j];
-                *reinterpret_cast<u32x4 *>(p + c) = u.v;
-            }
+            for (int j = 0; j < V; ++j)
+                u.e[j] = (T)v[i * V + j];
+            *reinterpret_cast<Piece *>(p + c) = u;
         }
     }
     static __device__ inline bool inside(int e, int t, int width)
@@ -71,9 +73,7 @@ struct Row {
     // Sum over the row's threads, in a fixed order.
     static __device__ inline float sum(float v, float *red)
     {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            v += __shfl_xor(v, o);
+        v = wave_sum(v);
         if constexpr (NT > kWave) {
             constexpr int kWavesRow = NT / kWave;
             const int wave = threadIdx.x / kWave;
@@ -90,12 +90,20 @@ struct Row {
     }
 };
 
+// 1 / (1 + e^-g) and tanh(g) from one exponential and one reciprocal (a unit
+// in the last place each); tanh near 0, where 1 - e cancels, from its series,
+// whose first term left out is 9e-9 of it at 1/4.
 __device__ inline float act(int kind, float g)
 {
     if (kind == MTPX_GATE_SIGMOID)
-        return 1.f / (1.f + __expf(-g));
-    if (kind == MTPX_GATE_TANH)
-        return tanhf(g);
+        return __builtin_amdgcn_rcpf(1.f + exp2_fast(-g * kLog2e));
+    if (kind == MTPX_GATE_TANH) {
+        const float e = exp2_fast(-2.f * kLog2e * fabsf(g));
+        const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), g);
+        const float q = g * g;
+        const float near = g + g * q * fmaf(q, fmaf(q, fmaf(q, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3);
+        return fabsf(g) < 0.25f ? near : far;
+    }
     return g;
 }
 // Derivative from the activation's value.
@@ -127,95 +135,155 @@ __device__ inline void normalise(float (&v)[E], int kind, int width, float eps, 
     inv = 1.f / sqrtf(R::sum(q, red) / width + eps);
 }
 
+// A group of NT threads takes rows part, part + groups, ...: the weights and a
+// gate shared by all rows stay in registers, and a row's inputs are read while
+// the row before is worked on.
 template <class T, int NT, int E, int V>
 __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_forward_kernel(NormArgs a)
 {
     using R = Row<T, NT, E, V>;
     __shared__ float red[kMaxBlock / kWave];
     const int t = threadIdx.x % NT;
-    const int64_t row = (int64_t)blockIdx.x * R::kPerBlock + threadIdx.x / NT;
-    if (row >= a.rows)  // whole waves: a row's threads leave together
+    const int64_t part = (int64_t)blockIdx.x * R::kPerBlock + threadIdx.x / NT;
+    const int64_t groups = (int64_t)gridDim.x * R::kPerBlock;
+    const bool own_gate = a.gate && a.gate_row != 0;
+    if (part >= a.rows)  // whole waves: a row's threads leave together
         return;
-    float v[E], w[E], x[E];
-    R::load((const T *)a.y + row * a.y_row, a.width, t, 0.f, v);
-    if (a.x)
-        R::load((const T *)a.x + row * a.x_row, a.width, t, 0.f, x);
-    if (a.gate)
-        R::load((const T *)a.gate + row * a.gate_row, a.width, t, 0.f, w);
-    float mean, inv;
-    normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
-    if (a.stats && t == 0) {
-        a.stats[4 * row] = mean;
-        a.stats[4 * row + 1] = inv;
-    }
-    const float b = a.block_scale * inv;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        v[e] *= a.gate ? b * act(a.act, w[e]) : b;
-    }
-    if (a.post) {
-        R::load((const T *)a.post, a.width, t, 0.f, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            v[e] *= w[e];
-    }
-    if (a.x) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            v[e] = fmaf(a.residual_scale, x[e], v[e]);
-    }
-    R::store((T *)a.s + row * a.s_row, a.width, t, v);
-    if (!a.n)
-        return;
-    normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
-    if (a.stats && t == 0) {
-        a.stats[4 * row + 2] = mean;
-        a.stats[4 * row + 3] = inv;
-    }
-    if (a.pre)
-        R::load((const T *)a.pre, a.width, t, 0.f, w);
+    float post[E], pre[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-        v[e] *= a.pre ? inv * w[e] : inv;
-    R::store((T *)a.n + row * a.n_row, a.width, t, v);
+        post[e] = pre[e] = 1.f;
+    if (a.post)
+        R::load((const T *)a.post, a.width, t, post);
+    if (a.pre)
+        R::load((const T *)a.pre, a.width, t, pre);
+    if (a.gate && !own_gate) {
+        float g[E];
+        R::load((const T *)a.gate, a.width, t, g);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            post[e] *= act(a.act, g[e]);
+    }
+    typename R::Raw ry, rx, rg;
+    auto ahead = [&](int64_t row) {
+        if (row >= a.rows)
+            return;
+        R::fetch((const T *)a.y + row * a.y_row, a.width, t, ry);
+        if (a.x)
+            R::fetch((const T *)a.x + row * a.x_row, a.width, t, rx);
+        if (own_gate)
+            R::fetch((const T *)a.gate + row * a.gate_row, a.width, t, rg);
+    };
+    ahead(part);
+    for (int64_t row = part; row < a.rows; row += groups) {
+        float v[E], x[E], g[E];
+        R::widen(ry, v);
+        R::widen(rx, x);
+        R::widen(rg, g);
+        ahead(row + groups);
+        float mean, inv;
+        normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
+        if (a.stats && t == 0) {
+            a.stats[4 * row] = mean;
+            a.stats[4 * row + 1] = inv;
+        }
+        const float b = a.block_scale * inv;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            v[e] *= b * post[e];
+        if (own_gate) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                v[e] *= act(a.act, g[e]);
+        }
+        if (a.x) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                v[e] = fmaf(a.residual_scale, x[e], v[e]);
+        }
+        R::store((T *)a.s + row * a.s_row, a.width, t, v);
+        if (!a.n)
+            continue;
+        normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
+        if (a.stats && t == 0) {
+            a.stats[4 * row + 2] = mean;
+            a.stats[4 * row + 3] = inv;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            v[e] *= inv * pre[e];
+        R::store((T *)a.n + row * a.n_row, a.width, t, v);
+    }
 }
 
 // With v = (s - mean) r:  ds = ds_in + r (dv - [mean dv] - v mean(dv v)),
 // dv = dn w2; the same again through the first norm.  s is formed again from
 // x, y and the gate (the bytes of reading it back, without its rounding).
-// A group of NT threads takes rows part, part + parts, ... and keeps its
-// share of the weights' gradients in registers.
+// A group of NT threads takes rows part, part + groups, ... and keeps its
+// share of the weights' gradients in registers; a.parts workgroups leave one
+// partial row of each.
 template <class T, int NT, int E, int V>
-__global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_backward_kernel(NormArgs a)
+__global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void norm_backward_kernel(NormArgs a)
 {
     using R = Row<T, NT, E, V>;
     __shared__ float red[kMaxBlock / kWave];
     const int t = threadIdx.x % NT;
-    const int part = blockIdx.x * R::kPerBlock + threadIdx.x / NT;
-    if (part >= a.parts)
-        return;
+    // (a group without a row stays for the sums at the end)
+    const int64_t part = (int64_t)blockIdx.x * R::kPerBlock + threadIdx.x / NT;
+    const int64_t groups = (int64_t)gridDim.x * R::kPerBlock;
     const bool layer = a.kind == MTPX_NORM_LAYER;
     const float scale = 1.f / a.width;
     float dw1[E], dw2[E], dgs[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
         dw1[e] = dw2[e] = dgs[e] = 0.f;
-    for (int64_t row = part; row < a.rows; row += a.parts) {
-        const f32x4 st = *reinterpret_cast<const f32x4 *>(a.stats + 4 * row);
-        float u[E], v[E], g[E], w[E], ds[E];
-        R::load((const T *)a.y + row * a.y_row, a.width, t, 0.f, u);
+    const bool own_gate = a.gate && a.gate_row != 0;
+    float g[E];
+    if (a.gate && !own_gate) {
+        R::load((const T *)a.gate, a.width, t, g);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            g[e] = act(a.act, g[e]);
+    }
+    // what a row starts with is read one row ahead
+    typename R::Raw ry, rx, rdn, rds, rpost, rpre;
+    if (a.post)
+        R::fetch((const T *)a.post, a.width, t, rpost);
+    if (a.pre)
+        R::fetch((const T *)a.pre, a.width, t, rpre);
+    f32x4 rst;
+    auto ahead = [&](int64_t row) {
+        if (row >= a.rows)
+            return;
+        R::fetch((const T *)a.y + row * a.y_row, a.width, t, ry);
         if (a.x)
-            R::load((const T *)a.x + row * a.x_row, a.width, t, 0.f, v);
-        if (a.gate)
-            R::load((const T *)a.gate + row * a.gate_row, a.width, t, 0.f, g);
+            R::fetch((const T *)a.x + row * a.x_row, a.width, t, rx);
         if (a.dn)
-            R::load((const T *)a.dn + row * a.dn_row, a.width, t, 0.f, ds);
+            R::fetch((const T *)a.dn + row * a.dn_row, a.width, t, rdn);
+        if (a.ds)
+            R::fetch((const T *)a.ds + row * a.ds_row, a.width, t, rds);
+        rst = *reinterpret_cast<const f32x4 *>(a.stats + 4 * row);
+    };
+    ahead(part);
+    for (int64_t row = part; row < a.rows; row += groups) {
+        const f32x4 st = rst;
+        float u[E], v[E], w[E], ds[E];
+        R::widen(ry, u);
+        R::widen(rx, v);
+        R::widen(rdn, ds);
+        const typename R::Raw into = rds;
+        if (own_gate)
+            R::load((const T *)a.gate + row * a.gate_row, a.width, t, g);
         if (a.post)
-            R::load((const T *)a.post, a.width, t, 0.f, w);
+            R::widen(rpost, w);
+        ahead(row + groups);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             u[e] = R::inside(e, t, a.width) ? (u[e] - st[0]) * st[1] : 0.f;
-            g[e] = a.gate ? act(a.act, g[e]) : 1.f;
+            if (!a.gate)
+                g[e] = 1.f;
+            else if (own_gate)
+                g[e] = act(a.act, g[e]);
             if (!a.post)
                 w[e] = 1.f;
             const float z = a.block_scale * g[e] * u[e] * w[e];
@@ -224,7 +292,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_backward_kern
         if (a.dn) {
             float w2[E], s0 = 0.f, s1 = 0.f;
             if (a.pre)
-                R::load((const T *)a.pre, a.width, t, 0.f, w2);
+                R::widen(rpre, w2);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 v[e] = R::inside(e, t, a.width) ? (v[e] - st[2]) * st[3] : 0.f;
@@ -245,7 +313,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_backward_kern
                 ds[e] = 0.f;
         }
         if (a.ds) {
-            R::load((const T *)a.ds + row * a.ds_row, a.width, t, 0.f, v);
+            R::widen(into, v);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 ds[e] += v[e];
@@ -280,12 +348,29 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_backward_kern
             R::store((T *)a.dy + row * a.dy_row, a.width, t, ds);
         }
     }
+    // The rows of a workgroup are summed through LDS, in their order.
     auto leave = [&](int which, const float (&d)[E]) {
-        float *p = a.part + ((int64_t)which * a.parts + part) * a.width;
+        float *p = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.width;
+        if constexpr (R::kPerBlock == 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (R::inside(e, t, a.width))
-                p[R::column(e / V, t) + e % V] = d[e];
+            for (int e = 0; e < E; ++e)
+                if (R::inside(e, t, a.width))
+                    p[R::column(e / V, t) + e % V] = d[e];
+        } else {
+            __shared__ float sums[R::kPerBlock][NT * E];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                sums[threadIdx.x / NT][R::column(e / V, t) + e % V] = d[e];
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.width; c += R::kBlock) {
+                float s = 0.f;
+#pragma unroll
+                for (int r = 0; r < R::kPerBlock; ++r)
+                    s += sums[r][c];
+                p[c] = s;
+            }
+        }
     };
     if (a.dpost)
         leave(0, dw1);
@@ -308,9 +393,11 @@ __global__ __launch_bounds__(kMaxBlock) void norm_parts_kernel(NormArgs a)
         return;
     const int c = blockIdx.x * kWave + lane;
     float v = 0.f;
-    if (c < a.width)
+    if (c < a.width) {
+#pragma unroll 8
         for (int p = run; p < a.parts; p += kRuns)
             v += a.part[((int64_t)which * a.parts + p) * a.width + c];
+    }
     red[run][lane] = v;
     __syncthreads();
     if (run == 0 && c < a.width) {
@@ -324,8 +411,10 @@ template <class T, int NT, int E, int V>
 hipError_t run(const NormArgs &a, bool back, hipStream_t s)
 {
     using R = Row<T, NT, E, V>;
-    const int64_t groups = back ? a.parts : a.rows;
-    const dim3 grid((unsigned)((groups + R::kPerBlock - 1) / R::kPerBlock)), block(R::kBlock);
+    // the forward pass: what its registers let in at once, four waves per SIMD
+    const int64_t need = (a.rows + R::kPerBlock - 1) / R::kPerBlock;
+    const int64_t most = 256 * 16 * kWave / R::kBlock;
+    const dim3 grid((unsigned)(back ? a.parts : need < most ? need : most)), block(R::kBlock);
     if (back)
         norm_backward_kernel<T, NT, E, V><<<grid, block, 0, s>>>(a);
     else
@@ -333,17 +422,26 @@ hipError_t run(const NormArgs &a, bool back, hipStream_t s)
     return hipGetLastError();
 }
 
-// The fewest threads that hold a row with 8 or 16 elements each.
+// The fewest threads that hold a row with 8 elements each (16 beyond 8,192
+// columns): more elements leave the backward pass fewer waves per SIMD to
+// hide its reads (160,000 rows of 1,024: 611 us with 16 elements a thread).
+int row_threads(int width)
+{
+    int n = kWave;
+    while (n < kMaxBlock && width > 8 * n)
+        n *= 2;
+    return n;
+}
 template <class T, int V>
 hipError_t by_width(const NormArgs &a, bool back, hipStream_t s)
 {
-    if (a.width <= 512)
-        return run<T, 64, 8, V>(a, back, s);
-    if (a.width <= 1024)
-        return run<T, 64, 16, V>(a, back, s);
-    if (a.width <= 4096)
-        return run<T, 256, 16, V>(a, back, s);
-    return run<T, 1024, 16, V>(a, back, s);
+    switch (row_threads(a.width)) {
+    case 64: return run<T, 64, 8, V>(a, back, s);
+    case 128: return run<T, 128, 8, V>(a, back, s);
+    case 256: return run<T, 256, 8, V>(a, back, s);
+    case 512: return run<T, 512, 8, V>(a, back, s);
+    default: return a.width <= 8192 ? run<T, 1024, 8, V>(a, back, s) : run<T, 1024, 16, V>(a, back, s);
+    }
 }
 
 template <class T>
@@ -364,12 +462,15 @@ hipError_t by_type(int dtype, const NormArgs &a, bool back, hipStream_t s)
 
 }  // namespace
 
-// Rows are spread over as many groups as fill the chip a few times over;
-// each leaves one partial row per weight gradient.
+// Workgroups of the backward pass: as many as the chip holds at once (three
+// waves per SIMD by their registers), so that a weight gradient takes the
+// fewest partial rows; rows of one wave come four to a workgroup.
 int norm_backward_parts(int64_t rows, int width)
 {
-    const int most = width <= 1024 ? 4096 : width <= 4096 ? 1024 : 512;
-    return (int)(rows < most ? rows : most);
+    const int n = row_threads(width);
+    const int64_t need = n == kWave ? (rows + 3) / 4 : rows;
+    const int64_t most = 256 * 12 * kWave / (n == kWave ? 256 : n);
+    return (int)(need < most ? need : most);
 }
 hipError_t launch_norm_forward(int dtype, const NormArgs &a, hipStream_t s)
 {

@@ -64,12 +64,23 @@ __device__ inline f32x4 mma(f32x8 a, f32x8 b, f32x4 c)
     return c;
 }
 
-// Two results below one another as operand B, rounded to T once.
+// Results below one another as operand B, rounded to T once.
+template <class T>
+using Half = T __attribute__((ext_vector_type(4)));
+template <class T>
+__device__ inline Half<T> round4(f32x4 a)
+{
+    return __builtin_convertvector(a, Half<T>);
+}
+template <class T>
+__device__ inline Frag<T> join(Half<T> a, Half<T> b)
+{
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 template <class T>
 __device__ inline Frag<T> pack(f32x4 a, f32x4 b)
 {
-    const f32x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_convertvector(v, Frag<T>);
+    return join<T>(round4<T>(a), round4<T>(b));
 }
 
 // 16 bytes (E elements) of a row, of which `valid` exist; the others are 0.
@@ -139,26 +150,61 @@ struct Tile {
     {
         return row * kRowBytes + ((piece ^ (row & 7)) << 4);
     }
-    // Operand A: row r0 + l % 16, columns c0 + 8 (l / 16) + j.
-    static __device__ inline Frag<T> row_frag(const char *tile, int r0, int c0, int lane)
-    {
-        constexpr int N = 8 / E;
-        const int row = r0 + (lane & 15), piece = c0 / E + (lane >> 4) * N;
-        union {
-            u32x4 v[N];
-            Frag<T> f;
-        } u;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            u.v[i] = *reinterpret_cast<const u32x4 *>(tile + at(row, piece + i));
-        return u.f;
-    }
-    // Operand A of the transposed tile: column c0 + l % 16, contraction over
-    // rows r0 + 16 t + 4 (l / 16) + r at j = 4 t + r.
-    static __device__ inline Frag<T> column_frag(const char *tile, int r0, int c0, int lane)
+};
+
+// A lane's byte offsets of its fragments in a tile.  The permutation touches
+// only the low three bits of a piece's number, so the places of all pieces
+// follow from a few, to which whole constants are added.
+template <class T, int D>
+struct Reader {
+    using TL = Tile<T, D>;
+    static constexpr int E = TL::E, RB = TL::kRowBytes;
+    static constexpr bool kHalf = sizeof(T) == 2;
+    int row[2];   // row_frag: the pieces whose bit 2 is clear, set (32 bits: first, second)
+    int col[kHalf ? 4 : 8];
+
+    __device__ inline void init(int lane)
     {
         const int g = lane >> 4, i = lane & 15;
-        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            row[h] = TL::at(i, kHalf ? 4 * h + g : 2 * g + h);
+        if constexpr (kHalf) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+                col[h] = TL::at(4 * g + (i >> 2), 2 * h + ((i & 3) >> 1)) + ((i & 1) << 3);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 8; ++h)
+                col[h] = TL::at(4 * g + (h & 3), (h & 4) + (i >> 2)) + (i & 3) * 4;
+        }
+    }
+    // Operand A: row r0 + l % 16, columns c0 + 8 (l / 16) + j; r0 a multiple
+    // of 8, c0 a constant multiple of 32.
+    __device__ inline Frag<T> row_frag(const char *tile, int r0, int c0) const
+    {
+        union {
+            u32x4 v[8 / E];
+            Frag<T> f;
+        } u;
+        if constexpr (kHalf) {
+            const int piece = c0 / E;
+            u.v[0] = *reinterpret_cast<const u32x4 *>(tile + row[piece >> 2 & 1] +
+                                                      (r0 * RB + (piece & ~7) * 16));
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                u.v[h] = *reinterpret_cast<const u32x4 *>(tile + row[h] + (r0 * RB + c0 / E * 16));
+        }
+        return u.f;
+    }
+    // Operand A of the transposed tile: column c0 + l % 16 (c0 a constant
+    // multiple of 16), contraction over rows r0 + 16 t + 4 (l / 16) + r at
+    // j = 4 t + r.
+    __device__ inline Frag<T> column_frag(const char *tile, int r0, int c0) const
+    {
+        const int piece = c0 / E;
+        if constexpr (kHalf) {
             // ds_read_b64_tr_b16: of 16 lanes that read 4 rows of 16 elements
             // (lane i: row i / 4, elements 4 (i % 4) ...), lane i gets column i
             union {
@@ -166,36 +212,31 @@ struct Tile {
                 Frag<T> f;
             } u;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int row = r0 + 16 * t + 4 * g + (i >> 2);
-                const char *p = tile + at(row, c0 / E + ((i & 3) >> 1)) + ((i & 1) << 3);
+            for (int t = 0; t < 2; ++t)
                 u.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)p);
-            }
+                    (__attribute__((address_space(3))) s16x4 *)(tile + col[piece >> 1 & 3] +
+                                                                ((r0 + 16 * t) * RB + (piece & ~7) * 16)));
             return u.f;
         } else {
             Frag<T> f;
-            const int c = c0 + i;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int row = r0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                f[j] = *reinterpret_cast<const T *>(tile + at(row, c / E) + (c % E) * sizeof(T));
-            }
+            for (int j = 0; j < 8; ++j)
+                f[j] = *reinterpret_cast<const T *>(tile + col[(piece & 4) + (j & 3)] +
+                                                    ((r0 + 16 * (j >> 2)) * RB + (piece & ~7) * 16));
             return f;
         }
     }
 };
 
-// The way of a tile from global memory through registers into LDS, by a
-// workgroup of NT threads: thread t moves piece t % kPieces of rows
-// t / kPieces, + NT / kPieces, ...
+// The way of a tile from global memory through registers into LDS, by one
+// wave: lane l moves piece l % kPieces of rows l / kPieces, + 64 / kPieces, ...
 template <class T, int D, int ROWS, int NT>
 struct Stage {
     using TL = Tile<T, D>;
     static constexpr int kStep = NT / TL::kPieces;
     static constexpr int N = ROWS / kStep;
     static_assert(ROWS % kStep == 0, "rows of a tile");
-    u32x4 r[N];
+    u32x4 r[N ? N : 1];
 
     // Rows first, first + 1, ... of head-shifted `base`; a row whose bit in
     // `live` is not set, and columns beyond dim of either map, are 0.
@@ -220,15 +261,108 @@ struct Stage {
     }
 };
 
-// Consecutive workgroups go to the 8 XCDs in turn; this order gives each XCD
-// a contiguous run of work items, so that neighbours share its L2.
-__device__ inline int xcd_order(int b, int n)
+// 16 bytes of zeros that a load takes in the place of a row that is not there.
+__device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
+
+// 16 bytes per lane from global memory straight into LDS, at byte `offset`
+// (the same in every lane) + 16 lane of the workgroup's LDS.  They are there
+// after wait_loads().
+__device__ inline void load_to_lds(const void *p, unsigned offset)
 {
-    const int per = n / 8, rest = n % 8, x = b % 8;
-    return x * per + (x < rest ? x : rest) + b / 8;
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(offset), "v"(p)
+                 : "memory", "m0");
+}
+// (After the reads of what lay there: wait_reads() or a barrier.)
+__device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A tile's way from global memory straight into LDS, by a workgroup of WAVES
+// waves, without passing through registers.  A wave's instruction fills 1 KiB
+// of the tile: kGroup rows; lane l fills the piece that lies at place
+// l % kPieces of its row and so reads the one that the permutation puts there.
+template <class T, int D, int ROWS, int WAVES>
+struct Loader {
+    using TL = Tile<T, D>;
+    static constexpr int kGroup = 1024 / TL::kRowBytes;
+    static constexpr int N = ROWS / (kGroup * WAVES);
+    static_assert(N * kGroup * WAVES == ROWS, "rows of a tile");
+    const T *base;   // of the head, row 0 of the sequence
+    int64_t row, map;
+    int dim, vec, lane, wave;
+
+    __device__ inline void init(const T *b, const mtpx_rows &s, int d, int v, int tid)
+    {
+        base = b;
+        row = s.row;
+        map = s.map;
+        dim = d;
+        vec = v;
+        lane = tid & 63;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    }
+    // Rows first, ... into the tile at byte `tile` of the workgroup's LDS
+    // (`smem` its start); a row whose bit in `live` is not set, and columns
+    // beyond dim of either map, become 0.
+    __device__ inline void load(char *smem, int tile, int64_t first, unsigned long long live) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r0 = (i * WAVES + wave) * kGroup, r = r0 + lane / TL::kPieces;
+            const int col = ((lane % TL::kPieces) ^ (r & 7)) * TL::E, c = col % D;
+            const T *p = base + (first + r) * row + (col / D) * map + c;
+            const bool on = (live >> r & 1) && c < dim;
+            if (vec)
+                load_to_lds(on ? (const void *)p : (const void *)&kZeroPiece, tile + r0 * TL::kRowBytes);
+            else
+                *reinterpret_cast<u32x4 *>(smem + tile + r0 * TL::kRowBytes + lane * 16) =
+                    load16(p, on ? dim - c : 0, 0);
+        }
+    }
+};
+
+// The tile and head of workgroup b.  Consecutive workgroups go to the 8 XCDs
+// in turn, each with an L2 of its own: a head's tiles stay on one XCD where
+// the heads go round evenly (then head by head), and on as few as there are
+// heads to go round otherwise.  Tiles come with the most work first.
+struct Work {
+    int tile, head;
+};
+__device__ inline Work work_item(int b, int ntiles, int heads)
+{
+    if (heads % 8 != 0)
+        return {b / heads, b % heads};
+    const int y = b / 8;
+    return {y % ntiles, y / ntiles * 8 + b % 8};
 }
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest of three, without the quieting of NaNs that fmaxf comes with.
+__device__ inline float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// Sum over a wave, in a fixed order, in every lane: shifts within rows of 16
+// lanes, then from row to row, by data-parallel moves that need no LDS.
+template <int CONTROL, int ROWS>
+__device__ inline float moved(float v)
+{
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, ROWS, 0xf, false));
+}
+__device__ inline float wave_sum(float v)
+{
+    v += moved<0x111, 0xf>(v);  // row_shr:1
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // row_bcast:15
+    v += moved<0x143, 0xc>(v);  // row_bcast:31
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 
 // Maximum and sum over the four lanes that hold one column of a result.
 __device__ inline float column_max(float v)
