@@ -29,6 +29,17 @@ typedef _Float16 Type;
 #define MTPX_OPS_NAME(f) f##_f16
 #endif
 
+#ifndef FW
+#define FW 4
+#endif
+#ifndef FO
+#define FO S::kWaves
+#endif
+#ifdef PRIO
+#define MTPX_PRIO(x) __builtin_amdgcn_s_setprio(x)
+#else
+#define MTPX_PRIO(x)
+#endif
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
 // Keys k0 .. k0 + 63 of a sequence of nk that are there and not masked.
@@ -47,31 +58,44 @@ __device__ inline void store_columns(T *row, int64_t map, int dim, int t, int la
     store4(row + m * map, c, dim, v, vec);
 }
 
+// A row's exponentials are taken relative to a level (in powers of two) that
+// is renewed, and the row's products rescaled, only when a score passes it by
+// this much: exp2 then stays below 2^8, within every type's range, and most
+// steps need no comparison between lanes.  kNoLevel, the level of a row that
+// has seen no key, is passed by every finite score.
+constexpr float kSlack = 8.f, kNoLevel = -3.0e38f;
+
 // Forward.  A workgroup takes kWaves * QT * 16 query rows of one head, each
-// wave QT * 16 of them; the keys and values come in tiles of KB rows through
-// LDS.  S^T = K Q^T leaves a query per lane column: its running maximum and
-// sum are per lane, and exp(S^T) is operand B of O^T += V^T P^T as it stands.
-// The two maps keep their own maximum, sum and product, since their
-// normalisers are known only at the end; each V fragment read from LDS serves
-// both.  P is rounded to T for the product (its 32-bit sum is the
-// normaliser), as V is in T already.
-template <class T, int D, int QT, int KB>
-__global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, int table, int ntiles)
+// wave QT * 16 of them; the keys and values come in tiles of KB rows straight
+// into LDS, the next tile while the present one is worked on (BUF 2).
+// S^T = K Q^T leaves a query per lane column: its running maximum and sum are
+// per lane, and exp(S^T) is operand B of O^T += V^T P^T as it stands.  The two
+// maps keep their own maximum, sum and product, since their normalisers are
+// known only at the end; each V fragment read from LDS serves both.  P is
+// rounded to T for the product (its 32-bit sum is the normaliser), as V is in
+// T already.
+template <class T, int D, int W, int QT, int KB, int BUF, int OCC>
+__global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a, int table, int ntiles)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = KB * TL::kRowBytes;
     extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int head = id / ntiles, kv = head / (a.heads / a.kv_heads);
-    const SeqTile st = a.tiles.q[table][id % ntiles];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Work wk = work_item(blockIdx.x, ntiles, a.heads);
+    const int head = wk.head, kv = head / (a.heads / a.kv_heads);
+    const SeqTile st = a.tiles.q[table][wk.tile];
     const Seq sq = a.seq[st.seq];
     const int shift = sq.nk - sq.nq;
-    const float c = a.scale * kLog2e, lambda = a.lambda[head];
+    const float lambda = a.lambda[head];
+    const float c = a.scale * kLog2e;
 
-    const T *kp = (const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row;
-    const T *vp = (const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row;
+    Reader<T, D> rd;
+    rd.init(lane);
     const unsigned char *mask = a.mask ? a.mask + sq.k0 : nullptr;
+    Loader<T, D, KB, W> lk, lv;
+    lk.init((const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row, a.k, a.dim, a.vec, tid);
+    lv.init((const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row, a.v, a.dim, a.vec, tid);
 
     const int w0 = st.start + wave * QT * 16;  // first row of the wave
     Frag<T> qf[2][QT][D / 32];
@@ -86,12 +110,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, i
                 qf[m][t][kk] = load_frag(qp + m * a.q.map, kk * 32 + 8 * g, a.dim, row < sq.nq, a.vec);
     }
     f32x4 acc[2][QT][D / 8];
-    float top[2][QT], sum[2][QT];
+    float level[2][QT], sum[2][QT];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            top[m][t] = -INFINITY;
+            level[m][t] = kNoLevel;
             sum[m][t] = 0.f;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
@@ -101,109 +125,139 @@ __global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, i
     // keys that the last row of the workgroup sees
     int nk = sq.nk;
     if (a.causal)
-        nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
-    Stage<T, D, KB, kThreads> sk, sv;
+        nk = min(nk, min(st.start + W * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
     if (nk > 0) {
         bits = seen_keys(mask, 0, nk, lane);
-        sk.load(kp, a.k, a.dim, 0, bits, tid, a.vec);
-        sv.load(vp, a.v, a.dim, 0, bits, tid, a.vec);
+        lk.load(smem, 0, 0, bits);
+        lv.load(smem, kTile, 0, bits);
     }
+    int buf = 0;
     for (int k0 = 0; k0 < nk; k0 += KB) {
-        __syncthreads();
-        sk.store(smem, tid);
-        sv.store(smem + kTile, tid);
+        wait_loads();
         __syncthreads();
         unsigned long long now = bits;
         if constexpr (KB < 64)
             now &= (1ull << KB) - 1;
-        if (k0 + KB < nk) {
-            bits = seen_keys(mask, k0 + KB, nk, lane);
-            sk.load(kp, a.k, a.dim, k0 + KB, bits, tid, a.vec);
-            sv.load(vp, a.v, a.dim, k0 + KB, bits, tid, a.vec);
-        }
-        if (now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift))
-            continue;
-
-        f32x4 s[2][KB / 16][QT];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int kt = 0; kt < KB / 16; ++kt) {
-#pragma unroll
-                for (int t = 0; t < QT; ++t)
-                    s[m][kt][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int kk = 0; kk < D / 32; ++kk) {
-                    const Frag<T> kf = TL::row_frag(smem, kt * 16, m * D + kk * 32, lane);
-#pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        s[m][kt][t] = mma(kf, qf[m][t][kk], s[m][kt][t]);
-                }
+        const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
+        auto next = [&] {
+            if (k0 + KB < nk) {
+                buf = BUF - 1 - buf;
+                bits = seen_keys(mask, k0 + KB, nk, lane);
+                lk.load(smem, buf * 2 * kTile, k0 + KB, bits);
+                lv.load(smem, buf * 2 * kTile + kTile, k0 + KB, bits);
             }
+        };
+        if constexpr (BUF == 2)
+            next();
+        const bool idle = now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift);
         const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
-        if (now != full || (a.causal && k0 + KB - 1 > w0 + shift)) {
-            const unsigned long long mine = now >> (4 * g);
+        const bool partly = now != full || (a.causal && k0 + KB - 1 > w0 + shift);
+        if (!idle) {
+#pragma unroll 1
+            for (int b = 0; b < KB / 32; ++b) {
+                f32x4 s[2][2][QT];
+                {
+                    // u, then map, then columns: one K fragment ahead
+                    constexpr int kSteps = 2 * 2 * (D / 32);
+                    Frag<T> kf = rd.row_frag(kt, b * 32, 0);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                const int last = a.causal ? w0 + t * 16 + (lane & 15) + shift - k0 - 4 * g : KB;
+                    for (int x = 0; x < kSteps; ++x) {
+                        const int u = x / (D / 16), m = x / (D / 32) % 2, kk = x % (D / 32);
+                        Frag<T> ahead;
+                        if (x + 1 < kSteps) {
+                            const int y = x + 1, mc = y / (D / 32) % 2 * D + y % (D / 32) * 32;
+                            ahead = rd.row_frag(kt, b * 32 + y / (D / 16) * 16, mc);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int kt = 0; kt < KB / 16; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool on = (mine >> (16 * kt + r) & 1) && 16 * kt + r <= last;
-                        s[0][kt][t][r] = on ? s[0][kt][t][r] : -INFINITY;
-                        s[1][kt][t][r] = on ? s[1][kt][t][r] : -INFINITY;
+                        for (int t = 0; t < QT; ++t)
+                            s[m][u][t] = mma(kf, qf[m][t][kk], kk ? s[m][u][t] : f32x4{0, 0, 0, 0});
+                        __builtin_amdgcn_sched_barrier(0);
+                        kf = ahead;
                     }
-            }
-        }
-        Frag<T> pf[2][KB / 32][QT];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                float hi = s[m][0][t][0];
-#pragma unroll
-                for (int kt = 0; kt < KB / 16; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        hi = fmaxf(hi, s[m][kt][t][r]);
-                hi = fmaxf(top[m][t], column_max(hi));
-                if (__any(hi > top[m][t])) {
-                    // rows that have seen no key yet have nothing to rescale
-                    const float f = top[m][t] == -INFINITY ? 0.f : exp2_fast((top[m][t] - hi) * c);
-                    top[m][t] = hi;
-                    sum[m][t] *= f;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        acc[m][t][i] *= f;
                 }
-                const float base = hi == -INFINITY ? 0.f : hi * c;
-                float part = 0.f;
+                if (partly) {
+                    const unsigned mine = (unsigned)(now >> (32 * b + 4 * g));
 #pragma unroll
-                for (int kt = 0; kt < KB / 16; ++kt)
+                    for (int t = 0; t < QT; ++t) {
+                        const int last =
+                            a.causal ? w0 + t * 16 + (lane & 15) + shift - k0 - 32 * b - 4 * g : 32;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = exp2_fast(fmaf(s[m][kt][t][r], c, -base));
-                        s[m][kt][t][r] = p;
-                        part += p;
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const bool on = (mine >> (16 * u + r) & 1) && 16 * u + r <= last;
+                                s[0][u][t][r] = on ? s[0][u][t][r] : -INFINITY;
+                                s[1][u][t][r] = on ? s[1][u][t][r] : -INFINITY;
+                            }
                     }
-                sum[m][t] += part;
-#pragma unroll
-                for (int b = 0; b < KB / 32; ++b)
-                    pf[m][b][t] = pack<T>(s[m][2 * b][t], s[m][2 * b + 1][t]);
-            }
-#pragma unroll
-        for (int b = 0; b < KB / 32; ++b)
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const Frag<T> vf = TL::column_frag(smem + kTile, b * 32, i * 16, lane);
+                }
+                float hi[2][QT];
+                bool passed = false;
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        acc[m][t][i] = mma(vf, pf[m][b][t], acc[m][t][i]);
+                    for (int t = 0; t < QT; ++t) {
+                        const f32x4 x = s[m][0][t], y = s[m][1][t];
+                        hi[m][t] = max3(max3(x[0], x[1], x[2]), max3(x[3], y[0], y[1]), max3(y[2], y[3], y[3]));
+                        passed |= fmaf(hi[m][t], c, -level[m][t]) > kSlack;
+                    }
+                if (__any(passed)) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) {
+                            const float up = fmaxf(level[m][t], column_max(hi[m][t]) * c);
+                            const float f = exp2_fast(level[m][t] - up);
+                            level[m][t] = up;
+                            sum[m][t] *= f;
+#pragma unroll
+                            for (int i = 0; i < D / 8; ++i)
+                                acc[m][t][i] *= f;
+                        }
+                }
+                Frag<T> pf[2][QT];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        float part[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float p = exp2_fast(fmaf(s[m][u][t][r], c, -level[m][t]));
+                                s[m][u][t][r] = p;
+                                part[u] = r ? part[u] + p : p;
+                            }
+                        sum[m][t] += part[0] + part[1];
+                        pf[m][t] = pack<T>(s[m][0][t], s[m][1][t]);
+                    }
+                // one V fragment ahead of the products, so that none waits for LDS
+                MTPX_PRIO(1);
+                Frag<T> vf = rd.column_frag(vt, b * 32, 0);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    Frag<T> ahead;
+                    if (i + 1 < D / 8)
+                        ahead = rd.column_frag(vt, b * 32, (i + 1) * 16);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t)
+                            acc[m][t][i] = mma(vf, pf[m][t], acc[m][t][i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    vf = ahead;
+                }
+                MTPX_PRIO(0);
             }
+        }
+        if constexpr (BUF == 1) {
+            __syncthreads();
+            next();
+        }
     }
 
 #pragma unroll
@@ -216,7 +270,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, i
             inv[m] = total > 0.f || total != total ? 1.f / total : 0.f;
             if (a.lse && row < sq.nq && g == 0)
                 a.lse[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] =
-                    total == 0.f ? -INFINITY : fmaf(top[m][t], a.scale, __logf(total));
+                    total == 0.f ? -INFINITY : fmaf(level[m][t], kLn2, __logf(total));
         }
         if (row >= sq.nq)
             continue;
@@ -239,23 +293,27 @@ __global__ __launch_bounds__(kThreads, 1) void attn_forward_kernel(AttnArgs a, i
 // and left for the key pass.  dlambda is -sum D_1; since the sum of
 // P_1 (dP - D_1) over a row is what the rounded out1 took from D_1, adding it
 // gives D_1 from 32-bit values.
-template <class T, int D, int QT, int KB>
-__global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int table, int ntiles)
+template <class T, int D, int QT, int KB, int BUF, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int table, int ntiles)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = KB * TL::kRowBytes;
     extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int head = id / ntiles, kv = head / (a.heads / a.kv_heads);
-    const SeqTile st = a.tiles.q[table][id % ntiles];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Work wk = work_item(blockIdx.x, ntiles, a.heads);
+    const int head = wk.head, kv = head / (a.heads / a.kv_heads);
+    const SeqTile st = a.tiles.q[table][wk.tile];
     const Seq sq = a.seq[st.seq];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e, lambda = a.lambda[head];
 
-    const T *kp = (const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row;
-    const T *vp = (const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row;
+    Loader<T, D, KB, kWaves> lk, lv;
+    lk.init((const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row, a.k, a.dim, a.vec, tid);
+    lv.init((const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row, a.v, a.dim, a.vec, tid);
     const unsigned char *mask = a.mask ? a.mask + sq.k0 : nullptr;
+    Reader<T, D> rd;
+    rd.init(lane);
 
     const int w0 = st.start + wave * QT * 16;
     Frag<T> qf[2][QT][D / 32], df[2][QT][D / 32];
@@ -310,31 +368,35 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int ta
     int nk = sq.nk;
     if (a.causal)
         nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
-    Stage<T, D, KB, kThreads> sk, sv;
     unsigned long long bits = 0;
     if (nk > 0) {
         bits = seen_keys(mask, 0, nk, lane);
-        sk.load(kp, a.k, a.dim, 0, bits, tid, a.vec);
-        sv.load(vp, a.v, a.dim, 0, bits, tid, a.vec);
+        lk.load(smem, 0, 0, bits);
+        lv.load(smem, kTile, 0, bits);
     }
+    int buf = 0;
     for (int k0 = 0; k0 < nk; k0 += KB) {
-        __syncthreads();
-        sk.store(smem, tid);
-        sv.store(smem + kTile, tid);
+        wait_loads();
         __syncthreads();
         unsigned long long now = bits;
         if constexpr (KB < 64)
             now &= (1ull << KB) - 1;
-        if (k0 + KB < nk) {
-            bits = seen_keys(mask, k0 + KB, nk, lane);
-            sk.load(kp, a.k, a.dim, k0 + KB, bits, tid, a.vec);
-            sv.load(vp, a.v, a.dim, k0 + KB, bits, tid, a.vec);
-        }
-        if (now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift))
-            continue;
+        const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
+        auto next = [&] {
+            if (k0 + KB < nk) {
+                buf = BUF - 1 - buf;
+                bits = seen_keys(mask, k0 + KB, nk, lane);
+                lk.load(smem, buf * 2 * kTile, k0 + KB, bits);
+                lv.load(smem, buf * 2 * kTile + kTile, k0 + KB, bits);
+            }
+        };
+        if constexpr (BUF == 2)
+            next();
+        const bool idle = now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift);
         const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
         const bool partly = now != full || (a.causal && k0 + KB - 1 > w0 + shift);
-#pragma unroll
+        if (!idle) {
+#pragma unroll 1
         for (int b = 0; b < KB / 32; ++b) {
             f32x4 s[2][2][QT], dp[2][QT];
 #pragma unroll
@@ -348,8 +410,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int ta
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int kk = 0; kk < D / 32; ++kk) {
-                        const Frag<T> kf = TL::row_frag(smem, r0, m * D + kk * 32, lane);
-                        const Frag<T> vf = TL::row_frag(smem + kTile, r0, m * D + kk * 32, lane);
+                        const Frag<T> kf = rd.row_frag(kt, r0, m * D + kk * 32);
+                        const Frag<T> vf = rd.row_frag(vt, r0, m * D + kk * 32);
 #pragma unroll
                         for (int t = 0; t < QT; ++t) {
                             s[m][u][t] = mma(kf, qf[m][t][kk], s[m][u][t]);
@@ -392,11 +454,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int ta
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const Frag<T> kf = TL::column_frag(smem, b * 32, m * D + i * 16, lane);
+                    const Frag<T> kf = rd.column_frag(kt, b * 32, m * D + i * 16);
 #pragma unroll
                     for (int t = 0; t < QT; ++t)
                         acc[m][t][i] = mma(kf, sf[m][t], acc[m][t][i]);
                 }
+        }
+        }
+        if constexpr (BUF == 1) {
+            __syncthreads();
+            next();
         }
     }
 
@@ -426,7 +493,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int ta
         float total = 0.f;
         for (int w = 0; w < kWaves; ++w)
             total += red[w];
-        a.dlam_part[(int64_t)head * ntiles + id % ntiles] = -total;
+        a.dlam_part[(int64_t)head * ntiles + wk.tile] = -total;
     }
 }
 
@@ -437,21 +504,24 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(AttnArgs a, int ta
 // operand B of dV^T += dO^T (P_0 - lambda P_1) and dK_m^T += Q_m^T dS_m.  The
 // query heads that share the key head follow one another, so their sum stays
 // in registers.
-template <class T, int D, int KT, int QB>
-__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
+template <class T, int D, int KT, int QB, int BUF, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = QB * TL::kRowBytes;
     extern __shared__ __align__(16) char smem[];
-    float *stat = reinterpret_cast<float *>(smem + 2 * kTile);  // [4][QB]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int kv = id / ntiles, group = a.heads / a.kv_heads;
-    const SeqTile st = a.tiles.k[table][id % ntiles];
+    float *stats = reinterpret_cast<float *>(smem + BUF * 2 * kTile);  // [BUF][4][QB]
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Work wk = work_item(blockIdx.x, ntiles, a.kv_heads);
+    const int kv = wk.head, group = a.heads / a.kv_heads;
+    const SeqTile st = a.tiles.k[table][wk.tile];
     const Seq sq = a.seq[st.seq];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e;
 
+    Reader<T, D> rd;
+    rd.init(lane);
     const int w0 = st.start + wave * KT * 16;  // first key of the wave
     Frag<T> kf[2][KT][D / 32], vf[2][KT][D / 32];
     bool live[KT];
@@ -487,108 +557,127 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(AttnArgs a, int t
     const int first = a.causal ? max(0, st.start - shift) / QB * QB : 0;
     const int per = sq.nq > first ? (sq.nq - first + QB - 1) / QB : 0;
     const int steps = per * group;
-    Stage<T, D, QB, kThreads> sq_, sd;
+    Loader<T, D, QB, kWaves> lq, ld;
+    lq.init((const T *)a.q.data + sq.q0 * a.q.row, a.q, a.dim, a.vec, tid);
+    ld.init((const T *)a.dout.data + sq.q0 * a.dout.row, a.dout, a.dim, a.vec, tid);
+    const T *q_base = lq.base, *d_base = ld.base;
+    // A step's tiles go into buffer `to`; its statistics come into a register
+    // and from there into LDS once no wave reads the buffer any more.
     float st_reg = 0.f;
-    auto fetch = [&](int step) {
+    auto fetch = [&](int step, int to) {
         const int head = kv * group + step / per, q0 = first + step % per * QB;
         const int there = sq.nq - q0;
         const unsigned long long bits = there >= 64 ? ~0ull : (1ull << there) - 1;
-        sq_.load((const T *)a.q.data + head * a.q.head + sq.q0 * a.q.row, a.q, a.dim, q0, bits, tid, a.vec);
-        sd.load((const T *)a.dout.data + head * a.dout.head + sq.q0 * a.dout.row, a.dout, a.dim, q0, bits, tid,
-                a.vec);
+        lq.base = q_base + head * a.q.head;
+        ld.base = d_base + head * a.dout.head;
         if (tid < 4 * QB) {
             const int which = tid / QB, row = q0 + tid % QB;
             const float *src = which < 2 ? a.lse : a.delta;
             st_reg = which < 2 ? -INFINITY : 0.f;
             if (row < sq.nq)
                 st_reg = src[((int64_t)(which & 1) * a.heads + head) * a.total_q + sq.q0 + row];
-            if (which < 2)
-                st_reg = st_reg == -INFINITY ? INFINITY : st_reg * kLog2e;
         }
+        lq.load(smem, to * 2 * kTile, q0, bits);
+        ld.load(smem, to * 2 * kTile + kTile, q0, bits);
     };
-    if (steps > 0)
-        fetch(0);
-    for (int step = 0; step < steps; ++step) {
-        __syncthreads();
-        sq_.store(smem, tid);
-        sd.store(smem + kTile, tid);
+    auto keep = [&](int to) {
         if (tid < 4 * QB)
-            stat[tid] = st_reg;
+            stats[to * 4 * QB + tid] =
+                tid >= 2 * QB ? st_reg : st_reg == -INFINITY ? INFINITY : st_reg * kLog2e;
+    };
+    if (steps > 0) {
+        fetch(0, 0);
+        keep(0);
+    }
+    int buf = 0;
+    for (int step = 0; step < steps; ++step) {
+        wait_loads();
         __syncthreads();
+        const char *qt = smem + buf * 2 * kTile, *dt = qt + kTile;
+        const float *stat = stats + buf * 4 * QB;
         const float lambda = a.lambda[kv * group + step / per];
         const int q0 = first + step % per * QB;
-        if (step + 1 < steps)
-            fetch(step + 1);
-        if (!busy || (a.causal && q0 + QB - 1 + shift < w0))
-            continue;
+        if constexpr (BUF == 2) {
+            buf ^= 1;
+            if (step + 1 < steps)
+                fetch(step + 1, buf);
+        }
+        const bool idle = !busy || (a.causal && q0 + QB - 1 + shift < w0);
         const bool partly = a.causal && q0 + shift < w0 + KT * 16 - 1;
-#pragma unroll
+        if (!idle) {
+#pragma unroll 1
         for (int b = 0; b < QB / 32; ++b) {
-            f32x4 s[2][2][KT], dp[2][KT];
+            // 16 rows at a time, so that their scores are gone before the next
+            Half<T> ph[KT][2], sh[2][KT][2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int r0 = b * 32 + u * 16;
+                f32x4 s[2][KT], dp[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
-                    s[0][u][t] = s[1][u][t] = dp[u][t] = f32x4{0, 0, 0, 0};
+                    s[0][t] = s[1][t] = dp[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int kk = 0; kk < D / 32; ++kk) {
-                        const Frag<T> qf = TL::row_frag(smem, r0, m * D + kk * 32, lane);
-                        const Frag<T> df = TL::row_frag(smem + kTile, r0, m * D + kk * 32, lane);
+                        const Frag<T> qf = rd.row_frag(qt, r0, m * D + kk * 32);
+                        const Frag<T> df = rd.row_frag(dt, r0, m * D + kk * 32);
 #pragma unroll
                         for (int t = 0; t < KT; ++t) {
-                            s[m][u][t] = mma(qf, kf[m][t][kk], s[m][u][t]);
-                            dp[u][t] = mma(df, vf[m][t][kk], dp[u][t]);
+                            s[m][t] = mma(qf, kf[m][t][kk], s[m][t]);
+                            dp[t] = mma(df, vf[m][t][kk], dp[t]);
                         }
                     }
-            }
-            Frag<T> pf[KT], sf[2][KT];
+                const f32x4 l0 = *reinterpret_cast<const f32x4 *>(stat + r0 + 4 * g);
+                const f32x4 l1 = *reinterpret_cast<const f32x4 *>(stat + QB + r0 + 4 * g);
+                const f32x4 d0 = *reinterpret_cast<const f32x4 *>(stat + 2 * QB + r0 + 4 * g);
+                const f32x4 d1 = *reinterpret_cast<const f32x4 *>(stat + 3 * QB + r0 + 4 * g);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                // the first row of this block that sees the lane's key
-                const int from = a.causal ? w0 + t * 16 + (lane & 15) - shift - q0 - 32 * b - 4 * g : -1;
-                f32x4 both[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int r0 = b * 32 + u * 16 + 4 * g;
-                    const f32x4 l0 = *reinterpret_cast<const f32x4 *>(stat + r0);
-                    const f32x4 l1 = *reinterpret_cast<const f32x4 *>(stat + QB + r0);
-                    const f32x4 d0 = *reinterpret_cast<const f32x4 *>(stat + 2 * QB + r0);
-                    const f32x4 d1 = *reinterpret_cast<const f32x4 *>(stat + 3 * QB + r0);
+                for (int t = 0; t < KT; ++t) {
+                    // the first row of this block that sees the lane's key
+                    const int from = a.causal ? w0 + t * 16 + (lane & 15) - shift - q0 - r0 - 4 * g : -1;
+                    f32x4 both;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float p0 = exp2_fast(fmaf(s[0][u][t][r], c, -l0[r]));
-                        float p1 = exp2_fast(fmaf(s[1][u][t][r], c, -l1[r]));
-                        if (partly && 16 * u + r < from)
+                        float p0 = exp2_fast(fmaf(s[0][t][r], c, -l0[r]));
+                        float p1 = exp2_fast(fmaf(s[1][t][r], c, -l1[r]));
+                        if (partly && r < from)
                             p0 = p1 = 0.f;
                         p1 *= -lambda;
-                        both[u][r] = p0 + p1;
-                        s[0][u][t][r] = p0 * (dp[u][t][r] - d0[r]);
-                        s[1][u][t][r] = p1 * (dp[u][t][r] - d1[r]);
+                        both[r] = p0 + p1;
+                        s[0][t][r] = p0 * (dp[t][r] - d0[r]);
+                        s[1][t][r] = p1 * (dp[t][r] - d1[r]);
                     }
+                    ph[t][u] = round4<T>(both);
+                    sh[0][t][u] = round4<T>(s[0][t]);
+                    sh[1][t][u] = round4<T>(s[1][t]);
                 }
-                pf[t] = pack<T>(both[0], both[1]);
-                sf[0][t] = pack<T>(s[0][0][t], s[0][1][t]);
-                sf[1][t] = pack<T>(s[1][0][t], s[1][1][t]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-                const Frag<T> df = TL::column_frag(smem + kTile, b * 32, i * 16, lane);
+                const Frag<T> df = rd.column_frag(dt, b * 32, i * 16);
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
-                    dv[t][i] = mma(df, pf[t], dv[t][i]);
+                    dv[t][i] = mma(df, join<T>(ph[t][0], ph[t][1]), dv[t][i]);
             }
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const Frag<T> qf = TL::column_frag(smem, b * 32, m * D + i * 16, lane);
+                    const Frag<T> qf = rd.column_frag(qt, b * 32, m * D + i * 16);
 #pragma unroll
                     for (int t = 0; t < KT; ++t)
-                        dk[m][t][i] = mma(qf, sf[m][t], dk[m][t][i]);
+                        dk[m][t][i] = mma(qf, join<T>(sh[m][t][0], sh[m][t][1]), dk[m][t][i]);
                 }
+        }
+        }
+        if constexpr (BUF == 1)
+            __syncthreads();
+        if (step + 1 < steps) {
+            if constexpr (BUF == 1)
+                fetch(step + 1, 0);
+            keep(buf);
         }
     }
 
@@ -640,22 +729,26 @@ __global__ __launch_bounds__(kThreads) void dlambda_kernel(const float *part, fl
 // steps of 32 keys in turn, each with its own maxima and sums: no wave waits
 // for another until the end.  A wave reads K as operand A straight from
 // memory; V goes through LDS of its own to be read by columns.  The waves'
-// results are joined through LDS, the workgroups' by attn_cache_join, from
-// [split][head][2][2 + 2 D] floats (maximum, sum, product).
-template <class T, int D>
-__global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
+// results are joined through LDS.  With one split they are the result; the
+// workgroups' are joined by attn_cache_join otherwise, from
+// [sequence][head][map][split][2 + 2 D] floats (maximum, sum, product).
+template <class T, int D, int W, int OCC>
+__global__ __launch_bounds__(W * kWave, OCC) void attn_cache_kernel(CacheArgs a)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = 32 * TL::kRowBytes;
     constexpr int kPart = 2 + 2 * D;
     extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = a.heads / a.kv_heads, blocks = (group + 15) / 16;
     const int split = blockIdx.x, kv = blockIdx.y / blocks, seq = blockIdx.z;
     const int head0 = kv * group + blockIdx.y % blocks * 16;
     const int count = min(16, (kv + 1) * group - head0);
     const float c = a.scale * kLog2e;
     char *tile = smem + wave * kTile;
+    Reader<T, D> rd;
+    rd.init(lane);
 
     int64_t len = a.lengths[seq];
     len = len < 0 ? 0 : len > a.capacity ? a.capacity : len;
@@ -681,13 +774,21 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
     for (int i = 0; i < D / 8; ++i)
         acc[0][i] = acc[1][i] = f32x4{0, 0, 0, 0};
 
-    Stage<T, D, 32, kWave> sv;
+    // Rows of 256 bytes a map and more leave no registers to read a step ahead:
+    // there the values go straight into LDS, and other waves hide the wait.
+    constexpr bool kAhead = D * sizeof(T) < 256;
+    Stage<T, D, kAhead ? 32 : 0, kWave> sv;
+    Loader<T, D, 32, 1> lv;
+    lv.init(vp, a.v, a.dim, a.vec, lane);
     Frag<T> kf[2][2][D / 32];
     auto fetch = [&](int64_t step) {
         const int64_t k0 = step * 32;
         const int there = (int)min((int64_t)32, len - k0);
         const unsigned long long bits = (1ull << there) - 1;
-        sv.load(vp, a.v, a.dim, k0, bits, lane, a.vec);
+        if constexpr (kAhead)
+            sv.load(vp, a.v, a.dim, k0, bits, lane, a.vec);
+        else
+            lv.load(smem, wave * kTile, k0, bits);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int r = 16 * u + (lane & 15);
@@ -699,10 +800,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
                     kf[u][m][kk] = load_frag(p + m * a.k.map, kk * 32 + 8 * g, a.dim, r < there, a.vec);
         }
     };
-    if (s0 + wave < s1)
+    if (kAhead && s0 + wave < s1)
         fetch(s0 + wave);
-    for (int64_t step = s0 + wave; step < s1; step += kWaves) {
+    for (int64_t step = s0 + wave; step < s1; step += W) {
         const int there = (int)min((int64_t)32, len - step * 32);
+        if constexpr (!kAhead) {
+            wait_reads();
+            fetch(step);
+        }
         f32x4 s[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -713,13 +818,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
                 for (int kk = 0; kk < D / 32; ++kk)
                     s[m][u] = mma(kf[u][m][kk], qf[m][kk], s[m][u]);
             }
-        // the wave's own reads of the last step's values are done before these
-        // writes: both go through the LDS in program order
-        sv.store(tile, lane);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (step + kWaves < s1)
-            fetch(step + kWaves);
+        if constexpr (kAhead) {
+            // the wave's own reads of the last step's values are done before
+            // these writes: both go through the LDS in program order
+            sv.store(tile, lane);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (step + W < s1)
+                fetch(step + W);
+        } else {
+            wait_loads();
+        }
         if (there < 32) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -759,7 +868,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
         }
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-            const Frag<T> vf = TL::column_frag(tile, 0, i * 16, lane);
+            const Frag<T> vf = rd.column_frag(tile, 0, i * 16);
             acc[0][i] = mma(vf, pf[0], acc[0][i]);
             acc[1][i] = mma(vf, pf[1], acc[1][i]);
         }
@@ -767,8 +876,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
         __builtin_amdgcn_wave_barrier();
     }
 
-    // Join the waves, one map at a time: column-major products in LDS.
-    float *red = reinterpret_cast<float *>(smem);  // [kWaves][16][kPart]
+    // Join the waves, one map at a time: column-major products in LDS, and the
+    // first map's result beside them while the second's are joined.
+    float *red = reinterpret_cast<float *>(smem);  // [W][16][kPart], [16][2 D]
+    float *first = red + W * 16 * kPart;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const float total = column_sum(sum[m]);
@@ -784,49 +895,74 @@ __global__ __launch_bounds__(kThreads, 1) void attn_cache_kernel(CacheArgs a)
             for (int r = 0; r < 4; ++r)
                 mine[2 + i * 16 + 4 * g + r] = acc[m][i][r];
         __syncthreads();
-        for (int e = tid; e < count * kPart; e += kThreads) {
-            const int h = e / kPart, x = e % kPart;
+        for (int e = tid; e < count * 2 * D; e += W * kWave) {
+            const int h = e / (2 * D), x = e % (2 * D);
             float hi = -INFINITY;
-            for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+            for (int w = 0; w < W; ++w)
                 hi = fmaxf(hi, red[(w * 16 + h) * kPart]);
-            float v = 0.f;
-            for (int w = 0; w < kWaves; ++w) {
+            float v = 0.f, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
                 const float *o = red + (w * 16 + h) * kPart;
                 const float f = o[0] == -INFINITY ? 0.f : exp2_fast((o[0] - hi) * c);
-                v += f * o[x ? x : 1];
+                v = fmaf(f, o[2 + x], v);
+                l = fmaf(f, o[1], l);
             }
-            a.part[((((int64_t)seq * a.heads + head0 + h) * 2 + m) * a.splits + split) * kPart + x] = x ? v : hi;
+            if (a.splits > 1) {
+                float *p = a.part + ((((int64_t)seq * a.heads + head0 + h) * 2 + m) * a.splits + split) * kPart;
+                if (x == 0) {
+                    p[0] = hi;
+                    p[1] = l;
+                }
+                p[2 + x] = v;
+                continue;
+            }
+            v = l == 0.f ? 0.f : v / l;
+            if (m == 0) {
+                first[e] = v;
+            } else if (x % D < a.dim) {
+                ((T *)a.out.data)[seq * a.out.row + (head0 + h) * a.out.head + x / D * a.out.map + x % D] =
+                    (T)(first[e] - a.lambda[head0 + h] * v);
+            }
         }
     }
 }
 
-// Joins the splits of one sequence and head: one workgroup, a thread per
-// column of the two products.
+// Joins the splits of one sequence and head: a thread per map and column,
+// the splits' weights in LDS.
 template <class T, int D>
-__global__ __launch_bounds__(2 * D) void attn_cache_join(CacheArgs a)
+__global__ __launch_bounds__(4 * D) void attn_cache_join(CacheArgs a)
 {
     constexpr int kPart = 2 + 2 * D;
-    const int x = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
+    __shared__ float weight[2][kMaxSplits], joined[2 * D];
+    const int tid = threadIdx.x, m = tid / (2 * D), x = tid % (2 * D), head = blockIdx.x, seq = blockIdx.y;
     const float c = a.scale * kLog2e;
-    float o[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const float *p = a.part + (((int64_t)seq * a.heads + head) * 2 + m) * a.splits * kPart;
-        float hi = -INFINITY;
-        for (int i = 0; i < a.splits; ++i)
-            hi = fmaxf(hi, p[i * kPart]);
-        float total = 0.f, v = 0.f;
-        for (int i = 0; i < a.splits; ++i) {
-            const float f = p[i * kPart] == -INFINITY ? 0.f : exp2_fast((p[i * kPart] - hi) * c);
-            total += f * p[i * kPart + 1];
-            v += f * p[i * kPart + 2 + x];
-        }
-        o[m] = total == 0.f ? 0.f : v / total;
+    const float *p = a.part + (((int64_t)seq * a.heads + head) * 2 + m) * a.splits * kPart;
+    // maxima, then weights, of this map's splits (a map has 2 D >= 64 threads)
+    for (int i = x; i < a.splits; i += 2 * D)
+        weight[m][i] = p[i * kPart];
+    __syncthreads();
+    float hi = -INFINITY;
+    for (int i = 0; i < a.splits; ++i)
+        hi = fmaxf(hi, weight[m][i]);
+    __syncthreads();
+    for (int i = x; i < a.splits; i += 2 * D)
+        weight[m][i] = weight[m][i] == -INFINITY ? 0.f : exp2_fast((weight[m][i] - hi) * c);
+    __syncthreads();
+    float total = 0.f, v = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < a.splits; ++i) {
+        total = fmaf(weight[m][i], p[i * kPart + 1], total);
+        v = fmaf(weight[m][i], p[i * kPart + 2 + x], v);
     }
-    const int m = x / D, col = x % D;
-    if (col < a.dim)
-        ((T *)a.out.data)[seq * a.out.row + head * a.out.head + m * a.out.map + col] =
-            (T)(o[0] - a.lambda[head] * o[1]);
+    v = total == 0.f ? 0.f : v / total;
+    if (m == 1)
+        joined[x] = v;
+    __syncthreads();
+    if (m == 0 && x % D < a.dim)
+        ((T *)a.out.data)[seq * a.out.row + head * a.out.head + x / D * a.out.map + x % D] =
+            (T)(v - a.lambda[head] * joined[x]);
 }
 
 // Tile shapes by head width: rows of a wave (16 QT), rows of a tile in LDS.
@@ -835,7 +971,13 @@ struct Shape {
     static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
     static constexpr int kWide = (D <= 64 && sizeof(T) == 2) || D == 32 ? 2 : 1;
     static constexpr int kTable = kWide == 2 ? 1 : 0;  // kTileRows
+    // the gradients of keys and values take most of a wave's registers at 16 keys
+    static constexpr int kKeyWide = 1, kKeyTable = 0;
     static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
+    // two buffers of both tiles within the 64 KiB that loads into LDS address
+    static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
+    static constexpr int kWaves = kLds <= 32768 ? 2 : 1;  // waves per SIMD: registers of one
+    static constexpr int kKeyWaves = D == 128 ? 1 : kWaves;
 };
 
 template <int D>
@@ -843,8 +985,9 @@ hipError_t forward(const AttnArgs &a, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[S::kTable];
-    attn_forward_kernel<Type, D, S::kWide, S::kRows>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kLds, s>>>(a, S::kTable, n);
+    attn_forward_kernel<Type, D, FW, 4 * S::kWide / FW, S::kRows, S::kBuffers, FO>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(FW * kWave), S::kBuffers * S::kLds, s>>>(
+            a, S::kTable, n);
     return hipGetLastError();
 }
 
@@ -852,32 +995,46 @@ template <int D>
 hipError_t backward(const AttnArgs &a, hipStream_t s)
 {
     using S = Shape<Type, D>;
-    const int nq = a.tiles.nq[S::kTable], nk = a.tiles.nk[S::kTable];
+    const int nq = a.tiles.nq[S::kTable], nk = a.tiles.nk[S::kKeyTable];
     if (nq > 0) {
-        attn_dq_kernel<Type, D, S::kWide, S::kRows>
-            <<<dim3((unsigned)((int64_t)nq * a.heads)), dim3(kThreads), S::kLds, s>>>(a, S::kTable, nq);
+        attn_dq_kernel<Type, D, S::kWide, S::kRows, S::kBuffers, S::kWaves>
+            <<<dim3((unsigned)((int64_t)nq * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(
+                a, S::kTable, nq);
         if (hipError_t e = hipGetLastError())
             return e;
     }
     if (nk > 0) {
-        attn_dkv_kernel<Type, D, S::kWide, S::kRows>
+        attn_dkv_kernel<Type, D, S::kKeyWide, S::kRows, S::kBuffers, S::kKeyWaves>
             <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(kThreads),
-               S::kLds + 4 * S::kRows * sizeof(float), s>>>(a, S::kTable, nk);
+               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)), s>>>(a, S::kKeyTable, nk);
     }
     return hipGetLastError();
 }
 
+template <int D, int W>
+hipError_t cache_waves(const CacheArgs &a, hipStream_t s)
+{
+    const int group = a.heads / a.kv_heads;
+    constexpr size_t tiles = (size_t)W * 32 * 2 * D * sizeof(Type);
+    static_assert(tiles <= 65536, "what loads into LDS address");
+    constexpr size_t join = ((size_t)W * 16 * (2 + 2 * D) + 16 * 2 * D) * sizeof(float);
+    constexpr int occ = D * sizeof(Type) < 256 ? 2 : 1;
+    attn_cache_kernel<Type, D, W, occ><<<dim3(a.splits, a.kv_heads * ((group + 15) / 16), a.sequences),
+                                         dim3(W * kWave), tiles > join ? tiles : join, s>>>(a);
+    return hipGetLastError();
+}
+// Eight waves where one workgroup takes a whole cache, four where splits
+// share it, fewer where their tiles would not fit.
 template <int D>
 hipError_t cache(const CacheArgs &a, hipStream_t s)
 {
-    const int group = a.heads / a.kv_heads;
-    const size_t tiles = (size_t)kWaves * 32 * 2 * D * sizeof(Type);
-    const size_t join = (size_t)kWaves * 16 * (2 + 2 * D) * sizeof(float);
-    attn_cache_kernel<Type, D><<<dim3(a.splits, a.kv_heads * ((group + 15) / 16), a.sequences),
-                                 dim3(kThreads), tiles > join ? tiles : join, s>>>(a);
-    if (hipError_t e = hipGetLastError())
+    constexpr int most = 1024 / (D * (int)sizeof(Type));
+    if (a.splits == 1)
+        return cache_waves<D, most < 8 ? most : 8>(a, s);
+    const hipError_t e = cache_waves<D, most < 4 ? most : 4>(a, s);
+    if (e != hipSuccess)
         return e;
-    attn_cache_join<Type, D><<<dim3(a.heads, a.sequences), dim3(2 * D), 0, s>>>(a);
+    attn_cache_join<Type, D><<<dim3(a.heads, a.sequences), dim3(4 * D), 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -25,7 +25,6 @@ namespace {
 
 constexpr int64_t kMaxLength = int64_t(1) << 30;  // rows of one sequence
 constexpr int64_t kMaxGrid = INT32_MAX;
-constexpr int kMaxSplits = 128;
 
 int invalid(mtpx_context *ctx, const std::string &msg) { return set_error(ctx, MTPX_E_INVALID, msg); }
 
@@ -169,13 +168,16 @@ int attn_args(mtpx_context *ctx, const mtpx_diff_attention_request &r, bool back
     return MTPX_OK;
 }
 
-// Workgroups that share one sequence's keys: enough to fill the device, each
-// with a step of 32 keys per wave at least.
+// Workgroups that share one sequence's keys: one where its eight waves have no
+// more than four steps of 32 keys each (a second launch costs as much), else
+// enough to fill the device, each with a step per wave at least.
 int cache_splits(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
 {
+    if (r.capacity <= 8 * 4 * 32)
+        return 1;
     const int group = r.heads / r.kv_heads;
     const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * ((group + 15) / 16), 1);
-    const int64_t most = std::max<int64_t>((r.capacity + 127) / 128, 1);
+    const int64_t most = (r.capacity + 127) / 128;
     const int64_t want = (4 * (int64_t)ctx->num_cus + base - 1) / base;
     return (int)std::min<int64_t>({want, most, (int64_t)kMaxSplits});
 }
@@ -191,10 +193,8 @@ int check_cache(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
 }
 size_t cache_bytes(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
 {
-    const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128;
-    return std::max<size_t>(sizeof(float) * 2 * (size_t)r.sequences * r.heads *
-                                cache_splits(ctx, r) * (2 + 2 * width),
-                            16);
+    const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128, splits = cache_splits(ctx, r);
+    return splits == 1 ? 0 : sizeof(float) * 2 * (size_t)r.sequences * r.heads * splits * (2 + 2 * width);
 }
 
 int check_norm(mtpx_context *ctx, const mtpx_norm_block_request &r)
@@ -277,6 +277,8 @@ size_t norm_bytes(const mtpx_norm_block_request &r)
 
 int check_workspace(mtpx_context *ctx, const void *p, size_t have, size_t need)
 {
+    if (need == 0)
+        return MTPX_OK;
     if (have < need || !p)
         return invalid(ctx, "the workspace holds " + std::to_string(p ? have : 0) + " bytes, " +
                                 std::to_string(need) + " are needed");

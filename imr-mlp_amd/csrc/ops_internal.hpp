@@ -41,6 +41,8 @@ struct AttnArgs {
     int vec;  // every row is a whole number of 16-byte pieces at a 16-byte address
 };
 
+constexpr int kMaxSplits = 128;  // of one sequence's cache
+
 struct CacheArgs {
     int sequences, heads, kv_heads, dim, splits;
     int64_t capacity, k_sequence, v_sequence;
