@@ -439,6 +439,7 @@ class Context:
             raise MtpxError(rc, "mtpx_create(%d)" % device)
         self.h = h
         self.device = device
+        self.workspaces = {}  # sizes that mtpx.ops has asked for
 
     def close(self):
         if getattr(self, "h", None):

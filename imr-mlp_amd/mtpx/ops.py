@@ -15,6 +15,7 @@ or a refused argument raises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -74,6 +75,20 @@ class NormRequest(C.Structure):
                 ("dgate_row", _l), ("workspace", _p), ("workspace_bytes", C.c_size_t)]
 
 
+def _packer(cls):
+    """The C layout of a request as one flat list of its fields: packing it
+    takes a third of the time that filling the ctypes structure does, which
+    counts in calls of a few microseconds."""
+    codes = {_p: "P", _i: "i", _l: "q", _f: "f", C.c_size_t: "N"}
+    fmt = "".join("Pqqq" if f is Rows else codes[f] for _, f in cls._fields_)
+    # (a structure's size is a multiple of its strictest alignment)
+    s = struct.Struct("@" + fmt + "0P")
+    assert s.size == C.sizeof(cls)
+    return s.pack
+
+
+_pack_rotary, _pack_cache, _pack_norm = (_packer(c) for c in (RotaryRequest, CacheRequest, NormRequest))
+
 _lib = None
 
 
@@ -83,16 +98,16 @@ def _ops():
     if _lib is None:
         L = capi.lib()
         ctx, size = C.c_void_p, C.POINTER(C.c_size_t)
-        L.mtpx_rotary.argtypes = [ctx, C.POINTER(RotaryRequest)]
+        L.mtpx_rotary.argtypes = [ctx, _p]
         L.mtpx_sequences_create.argtypes = [ctx, _i, C.POINTER(_l), C.POINTER(_l), C.POINTER(_p)]
         L.mtpx_sequences_destroy.argtypes = [_p]
         L.mtpx_sequences_destroy.restype = None
-        for name, req in (("diff_attention", AttentionRequest),
-                          ("diff_attention_cache", CacheRequest), ("norm_block", NormRequest)):
-            getattr(L, "mtpx_" + name).argtypes = [ctx, C.POINTER(req)]
-            getattr(L, "mtpx_%s_workspace" % name).argtypes = [ctx, C.POINTER(req), size]
+        for name, req in (("diff_attention", C.POINTER(AttentionRequest)),
+                          ("diff_attention_cache", _p), ("norm_block", _p)):
+            getattr(L, "mtpx_" + name).argtypes = [ctx, req]
+            getattr(L, "mtpx_%s_workspace" % name).argtypes = [ctx, req, size]
         L.mtpx_diff_attention_backward.argtypes = [ctx, C.POINTER(AttentionRequest)]
-        L.mtpx_norm_block_backward.argtypes = [ctx, C.POINTER(NormRequest)]
+        L.mtpx_norm_block_backward.argtypes = [ctx, _p]
         _lib = L
     return _lib
 
@@ -103,14 +118,22 @@ def _fail(what):
 
 def _tensor(ctx, t, name, shape=None, dtype=None):
     """Checks a device tensor (None in shape: any size) and returns it."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != ctx.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
         _fail("%s is not a tensor on the context's device" % name)
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         _fail("%s is %s, not %s" % (name, t.dtype, dtype))
-    if shape is not None and (t.dim() != len(shape) or
-                              any(w is not None and w != n for w, n in zip(shape, t.shape))):
-        _fail("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    if shape is not None and t.shape != shape:
+        if t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+            _fail("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     return t
+
+
+def _strides(ctx, t, name, shape, dtype=None):
+    """Strides of a checked tensor whose last dimension is contiguous."""
+    s = _tensor(ctx, t, name, shape, dtype).stride()
+    if s[-1] != 1 and t.shape[-1] > 1:
+        _fail("the last dimension of %s is not contiguous" % name)
+    return s
 
 
 def _inner(t, name):
@@ -127,12 +150,11 @@ def _typed(ctx, t, name):
 
 
 def _stream(ctx):
-    return torch.cuda.current_stream(ctx.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(ctx.device)
 
 
-def _heads(t):
-    """[rows][heads][dim]"""
-    return Rows(t.data_ptr(), t.stride(0), t.stride(1), 0)
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _maps(t):
@@ -145,12 +167,18 @@ def _wide(t):
     return Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[2] // 2)
 
 
-def _workspace(ctx, query, req):
-    n = C.c_size_t()
-    ctx._check(query(ctx.h, C.byref(req), C.byref(n)), "workspace")
-    w = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
-    req.workspace, req.workspace_bytes = w.data_ptr(), n.value
-    return w
+def _bytes(ctx, query, request, **sizes):
+    """Workspace that a call of these sizes needs: asked for once per context."""
+    key = (request, *sizes.values())
+    if key not in ctx.workspaces:
+        n = C.c_size_t()
+        ctx._check(query(ctx.h, C.byref(request(**sizes)), C.byref(n)), "workspace")
+        ctx.workspaces[key] = n.value
+    return ctx.workspaces[key]
+
+
+def _workspace(ctx, size):
+    return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
 
 
 # ---- rotary positions ----------------------------------------------------------
@@ -158,27 +186,26 @@ def _workspace(ctx, query, req):
 
 def _rotary(ctx, x, positions, freq, axis, interleaved, inverse, out, forward, dpositions):
     dtype = _typed(ctx, x, "x")
-    rows, heads, dim = _tensor(ctx, x, "x", (None, None, None)).shape
-    _inner(x, "x")
-    _tensor(ctx, positions, "positions", (rows, None))
+    sx = _strides(ctx, x, "x", (None, None, None))
+    rows, heads, dim = shape = x.shape
+    sp = _tensor(ctx, positions, "positions", (rows, None)).stride()
     if positions.dtype not in POSITION_DTYPES:
         _fail("positions are %s, not float32, float64, int32 or int64" % positions.dtype)
     _tensor(ctx, freq, "freq", (None,), torch.float32)
-    _tensor(ctx, axis, "axis", tuple(freq.shape), torch.int32)
+    _tensor(ctx, axis, "axis", freq.shape, torch.int32)
     if not freq.is_contiguous() or not axis.is_contiguous():
         _fail("freq and axis must be contiguous")
-    y = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device) if out is None else out
-    if out is not None:
-        _inner(_tensor(ctx, out, "out", (rows, heads, dim), x.dtype), "out")
-    req = RotaryRequest(_stream(ctx), dtype, rows, heads, dim, 2 * freq.shape[0],
-                        int(interleaved), int(inverse), _heads(x), _heads(y),
-                        positions.data_ptr(), POSITION_DTYPES[positions.dtype],
-                        positions.stride(0), positions.stride(1), positions.shape[1],
-                        freq.data_ptr(), axis.data_ptr())
+    y = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
+    sy = _strides(ctx, y, "out", shape, x.dtype)
+    f, sf = None, (0, 0)
     if dpositions is not None:
-        _inner(_tensor(ctx, forward, "x", (rows, heads, dim), x.dtype), "x")
-        req.forward, req.dpositions = _heads(forward), dpositions.data_ptr()
-    ctx._check(_ops().mtpx_rotary(ctx.h, C.byref(req)), "rotary")
+        sf, f = _strides(ctx, forward, "x", shape, x.dtype), forward.data_ptr()
+    req = _pack_rotary(
+        _stream(ctx), dtype, rows, heads, dim, 2 * freq.shape[0], interleaved, inverse,
+        x.data_ptr(), sx[0], sx[1], 0, y.data_ptr(), sy[0], sy[1], 0, positions.data_ptr(),
+        POSITION_DTYPES[positions.dtype], sp[0], sp[1], positions.shape[1], freq.data_ptr(),
+        axis.data_ptr(), f or 0, sf[0], sf[1], 0, 0 if dpositions is None else dpositions.data_ptr())
+    ctx._check(_ops().mtpx_rotary(ctx.h, req), "rotary")
     return y
 
 
@@ -296,7 +323,11 @@ def diff_attention_backward(ctx, dout, q, k, v, lam, seqs, out, saved, *, causal
     dlam = torch.empty(heads, dtype=torch.float32, device=q.device)
     req.out, req.dout, req.out1, req.lse = _wide(out), _wide(dout), out1.data_ptr(), lse.data_ptr()
     req.dq, req.dk, req.dv, req.dlambda = _maps(dq), _maps(dk), _wide(dv), dlam.data_ptr()
-    w = _workspace(ctx, _ops().mtpx_diff_attention_workspace, req)  # noqa: F841 -- kept until queued
+    n = C.c_size_t()
+    ctx._check(_ops().mtpx_diff_attention_workspace(ctx.h, C.byref(req), C.byref(n)), "workspace")
+    req.workspace_bytes = n.value
+    w = _workspace(ctx, req.workspace_bytes)  # held until the kernels are queued
+    req.workspace = w.data_ptr()
     ctx._check(_ops().mtpx_diff_attention_backward(ctx.h, C.byref(req)), "diff_attention_backward")
     return dq, dk, dv, dlam
 
@@ -307,63 +338,64 @@ def diff_attention_cache(ctx, q, k, v, lam, lengths, *, scale=None, out=None):
     heads, 2 dim], lengths [sequences] int32 on the device.  Returns
     [sequences, heads, 2 dim]."""
     dtype = _typed(ctx, q, "q")
-    n, heads, _, dim = _tensor(ctx, q, "q", (None, None, 2, None)).shape
-    cap, kv = _tensor(ctx, k, "k", (n, None, None, 2, dim), q.dtype).shape[1:3]
-    _tensor(ctx, v, "v", (n, cap, kv, 2 * dim), q.dtype)
+    sq = _strides(ctx, q, "q", (None, None, 2, None))
+    n, heads, _, dim = q.shape
+    sk = _strides(ctx, k, "k", (n, None, None, 2, dim), q.dtype)
+    cap, kv = k.shape[1:3]
+    sv = _strides(ctx, v, "v", (n, cap, kv, 2 * dim), q.dtype)
     _tensor(ctx, lengths, "lengths", (n,), torch.int32)
     _tensor(ctx, lam, "lam", (heads,), torch.float32)
     if not lam.is_contiguous() or not lengths.is_contiguous():
         _fail("lam and lengths must be contiguous")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _inner(t, name)
+    shape = (n, heads, 2 * dim)
     if out is None:
-        out = torch.empty((n, heads, 2 * dim), dtype=q.dtype, device=q.device)
-    else:
-        _inner(_tensor(ctx, out, "out", (n, heads, 2 * dim), q.dtype), "out")
-    req = CacheRequest(_stream(ctx), dtype, n, heads, kv, dim, cap,
-                       dim ** -0.5 if scale is None else scale, _maps(q),
-                       Rows(k.data_ptr(), k.stride(1), k.stride(2), k.stride(3)),
-                       Rows(v.data_ptr(), v.stride(1), v.stride(2), dim), k.stride(0),
-                       v.stride(0), lengths.data_ptr(), lam.data_ptr(), _wide(out))
-    w = _workspace(ctx, _ops().mtpx_diff_attention_cache_workspace, req)  # noqa: F841
-    ctx._check(_ops().mtpx_diff_attention_cache(ctx.h, C.byref(req)), "diff_attention_cache")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    so = _strides(ctx, out, "out", shape, q.dtype)
+    size = _bytes(ctx, _ops().mtpx_diff_attention_cache_workspace, CacheRequest, dtype=dtype,
+                  sequences=n, heads=heads, kv_heads=kv, dim=dim, capacity=cap)
+    w = _workspace(ctx, size) if size else None  # held until the kernels are queued
+    req = _pack_cache(
+        _stream(ctx), dtype, n, heads, kv, dim, cap, dim ** -0.5 if scale is None else scale,
+        q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[1], sk[2], sk[3], v.data_ptr(), sv[1],
+        sv[2], dim, sk[0], sv[0], lengths.data_ptr(), lam.data_ptr(), out.data_ptr(), so[0], so[1],
+        dim, _ptr(w), size)
+    ctx._check(_ops().mtpx_diff_attention_cache(ctx.h, req), "diff_attention_cache")
     return out
 
 
 # ---- norms around a block ----------------------------------------------------------
 
 
-def _row(t):
-    return (None, 0) if t is None else (t.data_ptr(), t.stride(0))
-
-
 def _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_scale, block_scale,
-          eps):
+          eps, s, n, stats, ds=None, dn=None, dx=None, dy=None, dgate=None, dpost=None, dpre=None,
+          work=None, work_bytes=0):
+    """The checked and packed request of either pass; results are contiguous."""
     dtype = _typed(ctx, y, "y")
-    rows, width = _tensor(ctx, y, "y", (None, None)).shape
-    _inner(y, "y")
+    sy = _strides(ctx, y, "y", (None, None))
+    shape = rows, width = y.shape
     if kind not in NORMS or gate_act not in GATES:
         _fail("kind is one of %s, gate_act of %s" % (tuple(NORMS), tuple(GATES)))
-    if x is not None:
-        _inner(_tensor(ctx, x, "x", (rows, width), y.dtype), "x")
+    sx = (0,) if x is None else _strides(ctx, x, "x", shape, y.dtype)
     gate_row = 0
     if gate is not None:
-        _inner(_tensor(ctx, gate, "gate", (width,) if gate.dim() == 1 else (rows, width), y.dtype),
-               "gate")
-        if gate.dim() == 2:
-            gate_row = gate.stride(0)
+        one = gate.dim() == 1
+        sg = _strides(ctx, gate, "gate", (width,) if one else shape, y.dtype)
+        if not one:
+            gate_row = sg[0]
             if gate_row == 0:
                 _fail("a gate shared by all rows is [width]")
-    for w, name in ((post_weight, "post_weight"), (pre_weight, "pre_weight")):
-        if w is not None:
-            _inner(_tensor(ctx, w, name, (width,), y.dtype), name)
-    px, sx = _row(x)
-    return NormRequest(_stream(ctx), dtype, rows, width, NORMS[kind], GATES[gate_act],
-                       residual_scale, block_scale, eps, px, y.data_ptr(),
-                       None if gate is None else gate.data_ptr(),
-                       None if post_weight is None else post_weight.data_ptr(),
-                       None if pre_weight is None else pre_weight.data_ptr(), sx, y.stride(0),
-                       gate_row)
+    if post_weight is not None:
+        _strides(ctx, post_weight, "post_weight", (width,), y.dtype)
+    if pre_weight is not None:
+        _strides(ctx, pre_weight, "pre_weight", (width,), y.dtype)
+    sds = (0,) if ds is None else _strides(ctx, ds, "ds", shape, y.dtype)
+    sdn = (0,) if dn is None else _strides(ctx, dn, "dn", shape, y.dtype)
+    return _pack_norm(
+        _stream(ctx), dtype, rows, width, NORMS[kind], GATES[gate_act], residual_scale, block_scale,
+        eps, _ptr(x), y.data_ptr(), _ptr(gate), _ptr(post_weight), _ptr(pre_weight), sx[0], sy[0],
+        gate_row, _ptr(s), _ptr(n), width, width, _ptr(stats), _ptr(ds), _ptr(dn), sds[0], sdn[0],
+        _ptr(dx), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), width, width,
+        width if gate_row else 0, _ptr(work), work_bytes)
 
 
 def norm_block(ctx, x, y, gate=None, post_weight=None, pre_weight=None, *, kind="rms",
@@ -374,16 +406,13 @@ def norm_block(ctx, x, y, gate=None, post_weight=None, pre_weight=None, *, kind=
     width] (x None: no residual; gate [rows, width], [width] or None; weights
     [width] or None).  Returns (s, n), with save (s, n, stats); without
     next_norm n is None."""
+    shape = _tensor(ctx, y, "y", (None, None)).shape
+    s = torch.empty(shape, dtype=y.dtype, device=y.device)
+    n = torch.empty(shape, dtype=y.dtype, device=y.device) if next_norm else None
+    stats = torch.empty((shape[0], 4), dtype=torch.float32, device=y.device) if save else None
     req = _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_scale,
-                block_scale, eps)
-    s = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    n = torch.empty_like(s) if next_norm else None
-    (req.s, req.s_row), (req.n, req.n_row) = _row(s), _row(n)
-    stats = None
-    if save:
-        stats = torch.empty((y.shape[0], 4), dtype=torch.float32, device=y.device)
-        req.stats = stats.data_ptr()
-    ctx._check(_ops().mtpx_norm_block(ctx.h, C.byref(req)), "norm_block")
+                block_scale, eps, s, n, stats)
+    ctx._check(_ops().mtpx_norm_block(ctx.h, req), "norm_block")
     return (s, n, stats) if save else (s, n)
 
 
@@ -392,30 +421,22 @@ def norm_block_backward(ctx, ds, dn, x, y, gate, post_weight, pre_weight, stats,
     """(dx, dy, dgate, dpost_weight, dpre_weight) from the gradients of s and n
     (either may be None) and the forward pass's inputs and stats; None in the
     place of an input that was not given."""
-    req = _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_scale,
-                block_scale, eps)
-    _tensor(ctx, stats, "stats", (y.shape[0], 4), torch.float32)
+    dtype = _typed(ctx, y, "y")
+    rows, width = _tensor(ctx, y, "y", (None, None)).shape
+    _tensor(ctx, stats, "stats", (rows, 4), torch.float32)
     if not stats.is_contiguous():
         _fail("stats must be contiguous")
-    for t, name in ((ds, "ds"), (dn, "dn")):
-        if t is not None:
-            _inner(_tensor(ctx, t, name, y.shape, y.dtype), name)
-    req.stats = stats.data_ptr()
-    (req.ds, req.ds_row), (req.dn, req.dn_row) = _row(ds), _row(dn)
 
     def like(t):
         return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
     dx, dy, dgate, dpost, dpre = like(x), like(y), like(gate), like(post_weight), like(pre_weight)
-    (req.dx, req.dx_row), (req.dy, req.dy_row) = _row(dx), _row(dy)
-    if dgate is not None:
-        req.dgate, req.dgate_row = dgate.data_ptr(), dgate.stride(0) if dgate.dim() == 2 else 0
-    if dpost is not None:
-        req.dpost_weight = dpost.data_ptr()
-    if dpre is not None:
-        req.dpre_weight = dpre.data_ptr()
-    w = _workspace(ctx, _ops().mtpx_norm_block_workspace, req)  # noqa: F841
-    ctx._check(_ops().mtpx_norm_block_backward(ctx.h, C.byref(req)), "norm_block_backward")
+    size = _bytes(ctx, _ops().mtpx_norm_block_workspace, NormRequest, dtype=dtype, rows=rows,
+                  width=width)
+    w = _workspace(ctx, size)  # held until the kernels are queued
+    req = _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_scale,
+                block_scale, eps, None, None, stats, ds, dn, dx, dy, dgate, dpost, dpre, w, size)
+    ctx._check(_ops().mtpx_norm_block_backward(ctx.h, req), "norm_block_backward")
     return dx, dy, dgate, dpost, dpre
 
 
