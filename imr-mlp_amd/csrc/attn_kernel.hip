@@ -45,8 +45,12 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 // Keys k0 .. k0 + 63 of a sequence of nk that are there and not masked.
 __device__ inline unsigned long long seen_keys(const unsigned char *mask, int k0, int nk, int lane)
 {
+    if (!mask) {
+        const int there = nk - k0;
+        return there >= 64 ? ~0ull : (1ull << there) - 1;
+    }
     const int k = k0 + lane;
-    return __ballot(k < nk && (!mask || mask[k]));
+    return __ballot(k < nk && mask[k]);
 }
 
 // Rounds per-lane column results 16 t + 4 (l / 16) + r, of width 2 D, to the
@@ -79,6 +83,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
 {
     using TL = Tile<T, D>;
     constexpr int kTile = KB * TL::kRowBytes;
+    constexpr unsigned long long kFull = ~0ull >> (64 - KB);
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -128,31 +133,30 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
         nk = min(nk, min(st.start + W * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
     if (nk > 0) {
-        bits = seen_keys(mask, 0, nk, lane);
-        lk.load(smem, 0, 0, bits);
-        lv.load(smem, kTile, 0, bits);
+        bits = seen_keys(mask, 0, nk, lane) & kFull;
+        lk.load(smem, 0, bits, bits == kFull);
+        lv.load(smem, kTile, bits, bits == kFull);
     }
     int buf = 0;
     for (int k0 = 0; k0 < nk; k0 += KB) {
         wait_loads();
         __syncthreads();
-        unsigned long long now = bits;
-        if constexpr (KB < 64)
-            now &= (1ull << KB) - 1;
+        const unsigned long long now = bits;
         const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
         auto next = [&] {
             if (k0 + KB < nk) {
                 buf = BUF - 1 - buf;
-                bits = seen_keys(mask, k0 + KB, nk, lane);
-                lk.load(smem, buf * 2 * kTile, k0 + KB, bits);
-                lv.load(smem, buf * 2 * kTile + kTile, k0 + KB, bits);
+                bits = seen_keys(mask, k0 + KB, nk, lane) & kFull;
+                lk.next();
+                lv.next();
+                lk.load(smem, buf * 2 * kTile, bits, bits == kFull);
+                lv.load(smem, buf * 2 * kTile + kTile, bits, bits == kFull);
             }
         };
         if constexpr (BUF == 2)
             next();
         const bool idle = now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift);
-        const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
-        const bool partly = now != full || (a.causal && k0 + KB - 1 > w0 + shift);
+        const bool partly = now != kFull || (a.causal && k0 + KB - 1 > w0 + shift);
         if (!idle) {
 #pragma unroll 1
             for (int b = 0; b < KB / 32; ++b) {
@@ -298,6 +302,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
 {
     using TL = Tile<T, D>;
     constexpr int kTile = KB * TL::kRowBytes;
+    constexpr unsigned long long kFull = ~0ull >> (64 - KB);
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -370,31 +375,30 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
         nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
     if (nk > 0) {
-        bits = seen_keys(mask, 0, nk, lane);
-        lk.load(smem, 0, 0, bits);
-        lv.load(smem, kTile, 0, bits);
+        bits = seen_keys(mask, 0, nk, lane) & kFull;
+        lk.load(smem, 0, bits, bits == kFull);
+        lv.load(smem, kTile, bits, bits == kFull);
     }
     int buf = 0;
     for (int k0 = 0; k0 < nk; k0 += KB) {
         wait_loads();
         __syncthreads();
-        unsigned long long now = bits;
-        if constexpr (KB < 64)
-            now &= (1ull << KB) - 1;
+        const unsigned long long now = bits;
         const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
         auto next = [&] {
             if (k0 + KB < nk) {
                 buf = BUF - 1 - buf;
-                bits = seen_keys(mask, k0 + KB, nk, lane);
-                lk.load(smem, buf * 2 * kTile, k0 + KB, bits);
-                lv.load(smem, buf * 2 * kTile + kTile, k0 + KB, bits);
+                bits = seen_keys(mask, k0 + KB, nk, lane) & kFull;
+                lk.next();
+                lv.next();
+                lk.load(smem, buf * 2 * kTile, bits, bits == kFull);
+                lv.load(smem, buf * 2 * kTile + kTile, bits, bits == kFull);
             }
         };
         if constexpr (BUF == 2)
             next();
         const bool idle = now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift);
-        const unsigned long long full = KB < 64 ? (1ull << (KB & 63)) - 1 : ~0ull;
-        const bool partly = now != full || (a.causal && k0 + KB - 1 > w0 + shift);
+        const bool partly = now != kFull || (a.causal && k0 + KB - 1 > w0 + shift);
         if (!idle) {
 #pragma unroll 1
         for (int b = 0; b < KB / 32; ++b) {
@@ -497,15 +501,19 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     }
 }
 
-// Gradient of the keys and values.  The mirror image of attn_dq_kernel: a
-// workgroup takes kWaves * KT * 16 keys of one key head, each wave KT * 16;
-// the rows' q, dO and statistics come in tiles of QB rows through LDS.  S and
-// dP come out with a key per lane column: P_0 - lambda P_1 and dS_m are
-// operand B of dV^T += dO^T (P_0 - lambda P_1) and dK_m^T += Q_m^T dS_m.  The
-// query heads that share the key head follow one another, so their sum stays
-// in registers.
-template <class T, int D, int KT, int QB, int BUF, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
+// Gradient of the keys and values.  A workgroup takes W * KT * 8 keys of one
+// key head; the rows' q, dO and statistics come in tiles of QB rows through
+// LDS.  S and dP come out with a key per lane column: P = P_0 - lambda P_1 and
+// dS_m are operand B of dV^T += dO^T P and dK_m^T += Q_m^T dS_m.
+//
+// Two waves share KT * 16 keys.  Of 32 rows, each forms the scores of 16; the
+// first then hands its dS to the second, which sums dK, and gets P for the
+// rest, as it sums dV.  One wave alone would hold both sums and could afford
+// half as many keys, at twice the reads of the tiles from LDS, which bound it
+// (8,192 causal rows: 1,750 us).  The query heads that share the key head
+// follow one another, so their sum stays in registers.
+template <class T, int D, int W, int KT, int QB, int BUF, int OCC>
+__global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = QB * TL::kRowBytes;
@@ -513,16 +521,19 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int
     float *stats = reinterpret_cast<float *>(smem + BUF * 2 * kTile);  // [BUF][4][QB]
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pair = wave >> 1, half = wave & 1;
+    // what one wave of a pair hands to the other: [2][3][KT][lane], in turn
+    Half<T> *given = reinterpret_cast<Half<T> *>(stats + BUF * 4 * QB) + pair * (2 * 3 * KT * kWave) + lane;
     const Work wk = work_item(blockIdx.x, ntiles, a.kv_heads);
     const int kv = wk.head, group = a.heads / a.kv_heads;
     const SeqTile st = a.tiles.k[table][wk.tile];
     const Seq sq = a.seq[st.seq];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e;
-
     Reader<T, D> rd;
     rd.init(lane);
-    const int w0 = st.start + wave * KT * 16;  // first key of the wave
+
+    const int w0 = st.start + pair * KT * 16;  // first key of the pair
     Frag<T> kf[2][KT][D / 32], vf[2][KT][D / 32];
     bool live[KT];
     bool any = false;
@@ -542,51 +553,67 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int
             }
     }
     const bool busy = __any(any);
-    f32x4 dk[2][KT][D / 16], dv[KT][D / 8];
+    // dV of the first wave, dK_0 and dK_1 side by side of the second
+    f32x4 acc[KT][D / 8];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-            dk[0][t][i] = dk[1][t][i] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
-            dv[t][i] = f32x4{0, 0, 0, 0};
-    }
+            acc[t][i] = f32x4{0, 0, 0, 0};
 
     // rows before the first that sees a key of this workgroup are left out
     const int first = a.causal ? max(0, st.start - shift) / QB * QB : 0;
     const int per = sq.nq > first ? (sq.nq - first + QB - 1) / QB : 0;
     const int steps = per * group;
-    Loader<T, D, QB, kWaves> lq, ld;
+    Loader<T, D, QB, W> lq, ld;
     lq.init((const T *)a.q.data + sq.q0 * a.q.row, a.q, a.dim, a.vec, tid);
     ld.init((const T *)a.dout.data + sq.q0 * a.dout.row, a.dout, a.dim, a.vec, tid);
-    const T *q_base = lq.base, *d_base = ld.base;
-    // A step's tiles go into buffer `to`; its statistics come into a register
-    // and from there into LDS once no wave reads the buffer any more.
-    float st_reg = 0.f;
-    auto fetch = [&](int step, int to) {
-        const int head = kv * group + step / per, q0 = first + step % per * QB;
-        const int there = sq.nq - q0;
+    lq.move(kv * group * a.q.head + first * a.q.row);
+    ld.move(kv * group * a.dout.head + first * a.dout.row);
+    // The tiles go round the rows once per query head.
+    int to_head = kv * group, to_q0 = first, head = to_head, q0 = first;
+    auto onward = [&](int &h, int &q) {
+        q += QB;
+        if (q >= sq.nq) {
+            q = first;
+            ++h;
+            return true;
+        }
+        return false;
+    };
+    // A step's tiles go into buffer `to`; its statistics and lambda come into
+    // registers, and the statistics from there into LDS once no wave reads the
+    // buffer any more.
+    float st_reg = 0.f, lambda = 0.f, lambda_to = 0.f;
+    auto fetch = [&](int to) {
+        const int there = sq.nq - to_q0;
         const unsigned long long bits = there >= 64 ? ~0ull : (1ull << there) - 1;
-        lq.base = q_base + head * a.q.head;
-        ld.base = d_base + head * a.dout.head;
         if (tid < 4 * QB) {
-            const int which = tid / QB, row = q0 + tid % QB;
+            const int which = tid / QB, row = to_q0 + tid % QB;
             const float *src = which < 2 ? a.lse : a.delta;
             st_reg = which < 2 ? -INFINITY : 0.f;
             if (row < sq.nq)
-                st_reg = src[((int64_t)(which & 1) * a.heads + head) * a.total_q + sq.q0 + row];
+                st_reg = src[((int64_t)(which & 1) * a.heads + to_head) * a.total_q + sq.q0 + row];
         }
-        lq.load(smem, to * 2 * kTile, q0, bits);
-        ld.load(smem, to * 2 * kTile + kTile, q0, bits);
+        lambda_to = a.lambda[to_head];
+        lq.load(smem, to * 2 * kTile, bits, there >= QB);
+        ld.load(smem, to * 2 * kTile + kTile, bits, there >= QB);
+        lq.next();
+        ld.next();
+        if (onward(to_head, to_q0)) {
+            lq.move(a.q.head - (int64_t)per * QB * a.q.row);
+            ld.move(a.dout.head - (int64_t)per * QB * a.dout.row);
+        }
     };
     auto keep = [&](int to) {
         if (tid < 4 * QB)
             stats[to * 4 * QB + tid] =
                 tid >= 2 * QB ? st_reg : st_reg == -INFINITY ? INFINITY : st_reg * kLog2e;
+        lambda = lambda_to;
     };
+    static_assert(4 * QB <= W * kWave, "a thread per statistic");
     if (steps > 0) {
-        fetch(0, 0);
+        fetch(0);
         keep(0);
     }
     int buf = 0;
@@ -595,23 +622,19 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int
         __syncthreads();
         const char *qt = smem + buf * 2 * kTile, *dt = qt + kTile;
         const float *stat = stats + buf * 4 * QB;
-        const float lambda = a.lambda[kv * group + step / per];
-        const int q0 = first + step % per * QB;
         if constexpr (BUF == 2) {
             buf ^= 1;
             if (step + 1 < steps)
-                fetch(step + 1, buf);
+                fetch(buf);
         }
         const bool idle = !busy || (a.causal && q0 + QB - 1 + shift < w0);
         const bool partly = a.causal && q0 + shift < w0 + KT * 16 - 1;
-        if (!idle) {
 #pragma unroll 1
         for (int b = 0; b < QB / 32; ++b) {
-            // 16 rows at a time, so that their scores are gone before the next
-            Half<T> ph[KT][2], sh[2][KT][2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r0 = b * 32 + u * 16;
+            Half<T> *turn = given + (b & 1) * (3 * KT * kWave);
+            Half<T> ph[KT], sh[2][KT];
+            if (!idle) {
+                const int r0 = b * 32 + half * 16;
                 f32x4 s[2][KT], dp[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
@@ -634,7 +657,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int
                 const f32x4 d1 = *reinterpret_cast<const f32x4 *>(stat + 3 * QB + r0 + 4 * g);
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
-                    // the first row of this block that sees the lane's key
+                    // the first row of these that sees the lane's key
                     const int from = a.causal ? w0 + t * 16 + (lane & 15) - shift - q0 - r0 - 4 * g : -1;
                     f32x4 both;
 #pragma unroll
@@ -648,56 +671,69 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dkv_kernel(AttnArgs a, int
                         s[0][t][r] = p0 * (dp[t][r] - d0[r]);
                         s[1][t][r] = p1 * (dp[t][r] - d1[r]);
                     }
-                    ph[t][u] = round4<T>(both);
-                    sh[0][t][u] = round4<T>(s[0][t]);
-                    sh[1][t][u] = round4<T>(s[1][t]);
+                    ph[t] = round4<T>(both);
+                    sh[0][t] = round4<T>(s[0][t]);
+                    sh[1][t] = round4<T>(s[1][t]);
+                    if (half) {
+                        turn[t * kWave] = ph[t];
+                    } else {
+                        turn[(KT + t) * kWave] = sh[0][t];
+                        turn[(2 * KT + t) * kWave] = sh[1][t];
+                    }
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+            __syncthreads();
+            if (idle)
+                continue;
+            // operand B of the wave's products: P twice, or dS_0 and dS_1
+            Frag<T> bf[2][KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                if (half) {
+                    bf[0][t] = join<T>(turn[(KT + t) * kWave], sh[0][t]);
+                    bf[1][t] = join<T>(turn[(2 * KT + t) * kWave], sh[1][t]);
+                } else {
+                    bf[0][t] = bf[1][t] = join<T>(ph[t], turn[t * kWave]);
+                }
+            }
+            const char *tile = half ? qt : dt;
+            Frag<T> xf = rd.column_frag(tile, b * 32, 0);
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-                const Frag<T> df = rd.column_frag(dt, b * 32, i * 16);
+                Frag<T> ahead;
+                if (i + 1 < D / 8)
+                    ahead = rd.column_frag(tile, b * 32, (i + 1) * 16);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
-                    dv[t][i] = mma(df, join<T>(ph[t][0], ph[t][1]), dv[t][i]);
+                    acc[t][i] = mma(xf, bf[i / (D / 16)][t], acc[t][i]);
+                __builtin_amdgcn_sched_barrier(0);
+                xf = ahead;
             }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const Frag<T> qf = rd.column_frag(qt, b * 32, m * D + i * 16);
-#pragma unroll
-                    for (int t = 0; t < KT; ++t)
-                        dk[m][t][i] = mma(qf, join<T>(sh[m][t][0], sh[m][t][1]), dk[m][t][i]);
-                }
-        }
         }
         if constexpr (BUF == 1)
             __syncthreads();
         if (step + 1 < steps) {
             if constexpr (BUF == 1)
-                fetch(step + 1, 0);
+                fetch(0);
             keep(buf);
         }
+        onward(head, q0);
     }
 
+    const mtpx_rows &to = half ? a.dk : a.dv;
+    const float factor = half ? a.scale : 1.f;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
         const int key = w0 + t * 16 + (lane & 15);
         if (key >= sq.nk)
             continue;
+        T *p = (T *)to.data + kv * to.head + (sq.k0 + key) * to.row;
         // a masked key's gradients are 0, whatever its column holds
         const f32x4 none = {0, 0, 0, 0};
-        T *kp = (T *)a.dk.data + kv * a.dk.head + (sq.k0 + key) * a.dk.row;
-        T *vp = (T *)a.dv.data + kv * a.dv.head + (sq.k0 + key) * a.dv.row;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                store4(kp + m * a.dk.map, i * 16 + 4 * g, a.dim, live[t] ? dk[m][t][i] * a.scale : none, a.vec);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
-            store_columns<T, D>(vp, a.dv.map, a.dim, i, lane, live[t] ? dv[t][i] : none, a.vec);
+            store_columns<T, D>(p, to.map, a.dim, i, lane, live[t] ? acc[t][i] * factor : none, a.vec);
     }
 }
 
@@ -778,8 +814,6 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_cache_kernel(CacheArgs a)
     // there the values go straight into LDS, and other waves hide the wait.
     constexpr bool kAhead = D * sizeof(T) < 256;
     Stage<T, D, kAhead ? 32 : 0, kWave> sv;
-    Loader<T, D, 32, 1> lv;
-    lv.init(vp, a.v, a.dim, a.vec, lane);
     Frag<T> kf[2][2][D / 32];
     auto fetch = [&](int64_t step) {
         const int64_t k0 = step * 32;
@@ -787,8 +821,12 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_cache_kernel(CacheArgs a)
         const unsigned long long bits = (1ull << there) - 1;
         if constexpr (kAhead)
             sv.load(vp, a.v, a.dim, k0, bits, lane, a.vec);
-        else
-            lv.load(smem, wave * kTile, k0, bits);
+        else {
+            Loader<T, D, 32, 1> lv;
+            lv.init(vp, a.v, a.dim, a.vec, lane);
+            lv.move(k0 * a.v.row);
+            lv.load(smem, wave * kTile, bits, there == 32);
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int r = 16 * u + (lane & 15);
@@ -971,13 +1009,15 @@ struct Shape {
     static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
     static constexpr int kWide = (D <= 64 && sizeof(T) == 2) || D == 32 ? 2 : 1;
     static constexpr int kTable = kWide == 2 ? 1 : 0;  // kTileRows
-    // the gradients of keys and values take most of a wave's registers at 16 keys
-    static constexpr int kKeyWide = 1, kKeyTable = 0;
+        // 64 keys: two pairs of waves that share 32 keys where a wave's registers
+    // hold those (and two workgroups' LDS a CU), four pairs that share 16 else
+    static constexpr int kKeyWide = D <= 64 && sizeof(T) == 2 ? 2 : 1, kKeyTable = 0;
+    static constexpr int kKeyWaves = 8 / kKeyWide;
+    static constexpr size_t kGiven = kKeyWaves / 2 * 2 * 3 * kKeyWide * kWave * 4 * sizeof(T);
     static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
     // two buffers of both tiles within the 64 KiB that loads into LDS address
     static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
     static constexpr int kWaves = kLds <= 32768 ? 2 : 1;  // waves per SIMD: registers of one
-    static constexpr int kKeyWaves = D == 128 ? 1 : kWaves;
 };
 
 template <int D>
@@ -1004,9 +1044,10 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
             return e;
     }
     if (nk > 0) {
-        attn_dkv_kernel<Type, D, S::kKeyWide, S::kRows, S::kBuffers, S::kKeyWaves>
-            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(kThreads),
-               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)), s>>>(a, S::kKeyTable, nk);
+        attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kRows, S::kBuffers, 2>
+            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave),
+               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)) + S::kGiven, s>>>(
+                a, S::kKeyTable, nk);
     }
     return hipGetLastError();
 }

@@ -274,48 +274,74 @@ __device__ inline void load_to_lds(const void *p, unsigned offset)
 }
 // (After the reads of what lay there: wait_reads() or a barrier.)
 __device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for them and all other loads.  (The instruction itself, not assembly
+// text: the compiler then knows that its own loads have come too and does not
+// wait for those again, and so for the loads into LDS, where they are used.)
+__device__ inline void wait_loads()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
 
-// A tile's way from global memory straight into LDS, by a workgroup of WAVES
+// A tile's way from global memory straight into LDS, by a workgroup of W
 // waves, without passing through registers.  A wave's instruction fills 1 KiB
 // of the tile: kGroup rows; lane l fills the piece that lies at place
 // l % kPieces of its row and so reads the one that the permutation puts there.
-template <class T, int D, int ROWS, int WAVES>
+// The lane's address moves from tile to tile by whole strides.
+template <class T, int D, int ROWS, int W>
 struct Loader {
     using TL = Tile<T, D>;
     static constexpr int kGroup = 1024 / TL::kRowBytes;
-    static constexpr int N = ROWS / (kGroup * WAVES);
-    static_assert(N * kGroup * WAVES == ROWS, "rows of a tile");
-    const T *base;   // of the head, row 0 of the sequence
+    static constexpr int N = ROWS / (kGroup * W);
+    static_assert(N * kGroup * W == ROWS, "rows of a tile");
+    // the permutation is the same in all of a lane's rows, or changes
+    static constexpr bool kSame = W * kGroup % 8 == 0;
+    const T *at;  // the lane's row of the next tile
     int64_t row, map;
     int dim, vec, lane, wave;
 
-    __device__ inline void init(const T *b, const mtpx_rows &s, int d, int v, int tid)
+    __device__ inline int column(int i) const
     {
-        base = b;
+        const int r = (kSame ? 0 : i * W * kGroup) + wave * kGroup + lane / TL::kPieces;
+        return ((lane % TL::kPieces) ^ (r & 7)) * TL::E;
+    }
+    // From row 0 of the sequence (`base`, of the head) on.
+    __device__ inline void init(const T *base, const mtpx_rows &s, int d, int v, int tid)
+    {
         row = s.row;
         map = s.map;
         dim = d;
         vec = v;
         lane = tid & 63;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        at = base + (wave * kGroup + lane / TL::kPieces) * row;
+        if constexpr (kSame)
+            at += column(0) / D * map + column(0) % D;
     }
-    // Rows first, ... into the tile at byte `tile` of the workgroup's LDS
-    // (`smem` its start); a row whose bit in `live` is not set, and columns
-    // beyond dim of either map, become 0.
-    __device__ inline void load(char *smem, int tile, int64_t first, unsigned long long live) const
+    __device__ inline void move(int64_t elements) { at += elements; }
+    __device__ inline void next() { at += ROWS * row; }
+    // The tile at `at` to byte `tile` of the workgroup's LDS (`smem` its
+    // start); a row whose bit in `live` is not set (`all`: every bit is), and
+    // columns beyond dim of either map, become 0.
+    __device__ inline void load(char *smem, int tile, unsigned long long live, bool all) const
     {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r0 = (i * WAVES + wave) * kGroup, r = r0 + lane / TL::kPieces;
-            const int col = ((lane % TL::kPieces) ^ (r & 7)) * TL::E, c = col % D;
-            const T *p = base + (first + r) * row + (col / D) * map + c;
-            const bool on = (live >> r & 1) && c < dim;
+            const int to = tile + (i * W + wave) * 1024;
+            const T *p = at + i * (W * kGroup * row);
+            if constexpr (!kSame)
+                p += column(i) / D * map + column(i) % D;
+            if (vec && all && dim == D) {
+                load_to_lds(p, to);
+                continue;
+            }
+            const int c = column(i) % D;
+            const bool on = (live >> ((i * W + wave) * kGroup + lane / TL::kPieces) & 1) && c < dim;
             if (vec)
-                load_to_lds(on ? (const void *)p : (const void *)&kZeroPiece, tile + r0 * TL::kRowBytes);
+                load_to_lds(on ? (const void *)p : (const void *)&kZeroPiece, to);
             else
-                *reinterpret_cast<u32x4 *>(smem + tile + r0 * TL::kRowBytes + lane * 16) =
-                    load16(p, on ? dim - c : 0, 0);
+                *reinterpret_cast<u32x4 *>(smem + to + lane * 16) = load16(p, on ? dim - c : 0, 0);
         }
     }
 };
