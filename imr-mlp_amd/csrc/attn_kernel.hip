@@ -522,8 +522,9 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pair = wave >> 1, half = wave & 1;
-    // what one wave of a pair hands to the other: [2][3][KT][lane], in turn
-    Half<T> *given = reinterpret_cast<Half<T> *>(stats + BUF * 4 * QB) + pair * (2 * 3 * KT * kWave) + lane;
+    // what one wave of a pair hands to the other: [3][U][KT][lane]
+    constexpr int U = QB / 32;
+    Half<T> *given = reinterpret_cast<Half<T> *>(stats + BUF * 4 * QB) + pair * (3 * U * KT * kWave) + lane;
     const Work wk = work_item(blockIdx.x, ntiles, a.kv_heads);
     const int kv = wk.head, group = a.heads / a.kv_heads;
     const SeqTile st = a.tiles.k[table][wk.tile];
@@ -629,12 +630,13 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
         }
         const bool idle = !busy || (a.causal && q0 + QB - 1 + shift < w0);
         const bool partly = a.causal && q0 + shift < w0 + KT * 16 - 1;
-#pragma unroll 1
-        for (int b = 0; b < QB / 32; ++b) {
-            Half<T> *turn = given + (b & 1) * (3 * KT * kWave);
-            Half<T> ph[KT], sh[2][KT];
-            if (!idle) {
-                const int r0 = b * 32 + half * 16;
+        // Of each 32 rows whose products follow, a wave forms the scores of 16
+        // (QB 32), or all of every other 32.
+        Half<T> ph[U][KT], sh[2][U][KT];
+        if (!idle) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r0 = (half * U + u) * 16;
                 f32x4 s[2][KT], dp[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
@@ -658,7 +660,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
                     // the first row of these that sees the lane's key
-                    const int from = a.causal ? w0 + t * 16 + (lane & 15) - shift - q0 - r0 - 4 * g : -1;
+                    const int from = partly ? w0 + t * 16 + (lane & 15) - shift - q0 - r0 - 4 * g : -1;
                     f32x4 both;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -671,38 +673,48 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
                         s[0][t][r] = p0 * (dp[t][r] - d0[r]);
                         s[1][t][r] = p1 * (dp[t][r] - d1[r]);
                     }
-                    ph[t] = round4<T>(both);
-                    sh[0][t] = round4<T>(s[0][t]);
-                    sh[1][t] = round4<T>(s[1][t]);
+                    ph[u][t] = round4<T>(both);
+                    sh[0][u][t] = round4<T>(s[0][t]);
+                    sh[1][u][t] = round4<T>(s[1][t]);
                     if (half) {
-                        turn[t * kWave] = ph[t];
+                        given[(u * KT + t) * kWave] = ph[u][t];
                     } else {
-                        turn[(KT + t) * kWave] = sh[0][t];
-                        turn[(2 * KT + t) * kWave] = sh[1][t];
+                        given[((U + u) * KT + t) * kWave] = sh[0][u][t];
+                        given[((2 * U + u) * KT + t) * kWave] = sh[1][u][t];
                     }
                 }
             }
-            __syncthreads();
-            if (idle)
-                continue;
+        }
+        __syncthreads();
+        if (!idle) {
             // operand B of the wave's products: P twice, or dS_0 and dS_1
-            Frag<T> bf[2][KT];
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                if (half) {
-                    bf[0][t] = join<T>(turn[(KT + t) * kWave], sh[0][t]);
-                    bf[1][t] = join<T>(turn[(2 * KT + t) * kWave], sh[1][t]);
-                } else {
-                    bf[0][t] = bf[1][t] = join<T>(ph[t], turn[t * kWave]);
-                }
-            }
+            auto mine = [&](int m, int u, int t) { return half ? sh[m][u][t] : ph[u][t]; };
+            auto other = [&](int m, int u, int t) {
+                return given[((half ? (1 + m) * U : 0) + u) * KT * kWave + t * kWave];
+            };
             const char *tile = half ? qt : dt;
-            Frag<T> xf = rd.column_frag(tile, b * 32, 0);
+            constexpr int kSteps = U * (D / 8);
+            Frag<T> xf = rd.column_frag(tile, 0, 0), bf[2][KT];
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
+            for (int x = 0; x < kSteps; ++x) {
+                const int b = x / (D / 8), i = x % (D / 8);
+                if (i == 0) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int t = 0; t < KT; ++t) {
+                            if constexpr (U == 1) {
+                                const Half<T> o = other(m, 0, t), w = mine(m, 0, t);
+                                bf[m][t] = half ? join<T>(o, w) : join<T>(w, o);
+                            } else {
+                                bf[m][t] = b == half ? join<T>(mine(m, 0, t), mine(m, 1, t))
+                                                     : join<T>(other(m, 0, t), other(m, 1, t));
+                            }
+                        }
+                }
                 Frag<T> ahead;
-                if (i + 1 < D / 8)
-                    ahead = rd.column_frag(tile, b * 32, (i + 1) * 16);
+                if (x + 1 < kSteps)
+                    ahead = rd.column_frag(tile, (x + 1) / (D / 8) * 32, (x + 1) % (D / 8) * 16);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
@@ -1013,7 +1025,7 @@ struct Shape {
     // hold those (and two workgroups' LDS a CU), four pairs that share 16 else
     static constexpr int kKeyWide = D <= 64 && sizeof(T) == 2 ? 2 : 1, kKeyTable = 0;
     static constexpr int kKeyWaves = 8 / kKeyWide;
-    static constexpr size_t kGiven = kKeyWaves / 2 * 2 * 3 * kKeyWide * kWave * 4 * sizeof(T);
+    static constexpr size_t kGiven = kKeyWaves / 2 * 3 * (kRows / 32) * kKeyWide * kWave * 4 * sizeof(T);
     static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
     // two buffers of both tiles within the 64 KiB that loads into LDS address
     static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
