@@ -53,6 +53,12 @@ __device__ inline unsigned long long seen_keys(const unsigned char *mask, int k0
     return __ballot(k < nk && mask[k]);
 }
 
+// Whether no row up to `last` sees any of the 32 keys from k0 + 32 b on.
+__device__ inline bool empty_block(unsigned long long seen, int b, int causal, int k0, int last)
+{
+    return (unsigned)(seen >> (32 * b)) == 0 || (causal && k0 + 32 * b > last);
+}
+
 // Rounds per-lane column results 16 t + 4 (l / 16) + r, of width 2 D, to the
 // row that lane l % 16 stands for.
 template <class T, int D>
@@ -160,6 +166,8 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
         if (!idle) {
 #pragma unroll 1
             for (int b = 0; b < KB / 32; ++b) {
+                if (empty_block(now, b, a.causal, k0, w0 + QT * 16 - 1 + shift))
+                    continue;
                 f32x4 s[2][2][QT];
                 {
                     // u, then map, then columns: one K fragment ahead
@@ -402,6 +410,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
         if (!idle) {
 #pragma unroll 1
         for (int b = 0; b < KB / 32; ++b) {
+            if (empty_block(now, b, a.causal, k0, w0 + QT * 16 - 1 + shift))
+                continue;
             f32x4 s[2][2][QT], dp[2][QT];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
