@@ -29,17 +29,6 @@ typedef _Float16 Type;
 #define MTPX_OPS_NAME(f) f##_f16
 #endif
 
-#ifndef FW
-#define FW 4
-#endif
-#ifndef FO
-#define FO S::kWaves
-#endif
-#ifdef PRIO
-#define MTPX_PRIO(x) __builtin_amdgcn_s_setprio(x)
-#else
-#define MTPX_PRIO(x)
-#endif
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
 // Keys k0 .. k0 + 63 of a sequence of nk that are there and not masked.
@@ -95,8 +84,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Work wk = work_item(blockIdx.x, ntiles, a.heads);
     const int head = wk.head, kv = head / (a.heads / a.kv_heads);
-    const SeqTile st = a.tiles.q[table][wk.tile];
-    const Seq sq = a.seq[st.seq];
+    const SeqTile sq = a.tiles.q[table][wk.tile];
     const int shift = sq.nk - sq.nq;
     const float lambda = a.lambda[head];
     const float c = a.scale * kLog2e;
@@ -108,7 +96,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
     lk.init((const T *)a.k.data + kv * a.k.head + sq.k0 * a.k.row, a.k, a.dim, a.vec, tid);
     lv.init((const T *)a.v.data + kv * a.v.head + sq.k0 * a.v.row, a.v, a.dim, a.vec, tid);
 
-    const int w0 = st.start + wave * QT * 16;  // first row of the wave
+    const int w0 = sq.start + wave * QT * 16;  // first row of the wave
     Frag<T> qf[2][QT][D / 32];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -136,7 +124,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
     // keys that the last row of the workgroup sees
     int nk = sq.nk;
     if (a.causal)
-        nk = min(nk, min(st.start + W * QT * 16, sq.nq) + shift);
+        nk = min(nk, min(sq.start + W * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
     if (nk > 0) {
         bits = seen_keys(mask, 0, nk, lane) & kFull;
@@ -247,7 +235,6 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
                         pf[m][t] = pack<T>(s[m][0][t], s[m][1][t]);
                     }
                 // one V fragment ahead of the products, so that none waits for LDS
-                MTPX_PRIO(1);
                 Frag<T> vf = rd.column_frag(vt, b * 32, 0);
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
@@ -263,7 +250,6 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
                     __builtin_amdgcn_sched_barrier(0);
                     vf = ahead;
                 }
-                MTPX_PRIO(0);
             }
         }
         if constexpr (BUF == 1) {
@@ -316,8 +302,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Work wk = work_item(blockIdx.x, ntiles, a.heads);
     const int head = wk.head, kv = head / (a.heads / a.kv_heads);
-    const SeqTile st = a.tiles.q[table][wk.tile];
-    const Seq sq = a.seq[st.seq];
+    const SeqTile sq = a.tiles.q[table][wk.tile];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e, lambda = a.lambda[head];
 
@@ -328,7 +313,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     Reader<T, D> rd;
     rd.init(lane);
 
-    const int w0 = st.start + wave * QT * 16;
+    const int w0 = sq.start + wave * QT * 16;
     Frag<T> qf[2][QT][D / 32], df[2][QT][D / 32];
     float base[2][QT], delta[2][QT], dlam = 0.f;
 #pragma unroll
@@ -380,7 +365,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
 
     int nk = sq.nk;
     if (a.causal)
-        nk = min(nk, min(st.start + kWaves * QT * 16, sq.nq) + shift);
+        nk = min(nk, min(sq.start + kWaves * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
     if (nk > 0) {
         bits = seen_keys(mask, 0, nk, lane) & kFull;
@@ -537,14 +522,13 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
     Half<T> *given = reinterpret_cast<Half<T> *>(stats + BUF * 4 * QB) + pair * (3 * U * KT * kWave) + lane;
     const Work wk = work_item(blockIdx.x, ntiles, a.kv_heads);
     const int kv = wk.head, group = a.heads / a.kv_heads;
-    const SeqTile st = a.tiles.k[table][wk.tile];
-    const Seq sq = a.seq[st.seq];
+    const SeqTile sq = a.tiles.k[table][wk.tile];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e;
     Reader<T, D> rd;
     rd.init(lane);
 
-    const int w0 = st.start + pair * KT * 16;  // first key of the pair
+    const int w0 = sq.start + pair * KT * 16;  // first key of the pair
     Frag<T> kf[2][KT][D / 32], vf[2][KT][D / 32];
     bool live[KT];
     bool any = false;
@@ -573,7 +557,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
             acc[t][i] = f32x4{0, 0, 0, 0};
 
     // rows before the first that sees a key of this workgroup are left out
-    const int first = a.causal ? max(0, st.start - shift) / QB * QB : 0;
+    const int first = a.causal ? max(0, sq.start - shift) / QB * QB : 0;
     const int per = sq.nq > first ? (sq.nq - first + QB - 1) / QB : 0;
     const int steps = per * group;
     Loader<T, D, QB, W> lq, ld;
@@ -1029,47 +1013,72 @@ __global__ __launch_bounds__(4 * D) void attn_cache_join(CacheArgs a)
 template <class T, int D>
 struct Shape {
     static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
+    // most 16-row groups a wave's registers hold
     static constexpr int kWide = (D <= 64 && sizeof(T) == 2) || D == 32 ? 2 : 1;
-    static constexpr int kTable = kWide == 2 ? 1 : 0;  // kTileRows
-        // 64 keys: two pairs of waves that share 32 keys where a wave's registers
+    // 64 keys: two pairs of waves that share 32 keys where a wave's registers
     // hold those (and two workgroups' LDS a CU), four pairs that share 16 else
-    static constexpr int kKeyWide = D <= 64 && sizeof(T) == 2 ? 2 : 1, kKeyTable = 0;
+    static constexpr int kKeyWide = D <= 64 && sizeof(T) == 2 ? 2 : 1;
     static constexpr int kKeyWaves = 8 / kKeyWide;
     static constexpr size_t kGiven = kKeyWaves / 2 * 3 * (kRows / 32) * kKeyWide * kWave * 4 * sizeof(T);
     static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
     // two buffers of both tiles within the 64 KiB that loads into LDS address
     static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
-    static constexpr int kWaves = kLds <= 32768 ? 2 : 1;  // waves per SIMD: registers of one
+    static constexpr int kOccupancy = kLds <= 32768 ? 2 : 1;  // waves per SIMD: registers of one
 };
 
+// Tables of 64 and 128 rows.
+constexpr int kNarrow = 0, kBroad = 1;
+
+// 32 rows a wave halve the reads from LDS per product and are right for work
+// that fills the device (32,000 rows of 8 heads, 64 wide: 5.8 ms, 6.9 ms with
+// 16 rows a wave); where tiles of 128 rows are fewer than two workgroups a CU,
+// tiles of 64 spread the work further (997 rows of 8 heads: 41 us and 26 us).
+template <int D>
+int query_table(const TileTable &t, int heads)
+{
+    return Shape<Type, D>::kWide == 2 && (int64_t)t.nq[kBroad] * heads >= 512 ? kBroad : kNarrow;
+}
+
+template <int D, int QT>
+hipError_t forward_rows(const AttnArgs &a, int table, hipStream_t s)
+{
+    using S = Shape<Type, D>;
+    const int n = a.tiles.nq[table];
+    attn_forward_kernel<Type, D, 4, QT, S::kRows, S::kBuffers, S::kOccupancy>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(a, table, n);
+    return hipGetLastError();
+}
 template <int D>
 hipError_t forward(const AttnArgs &a, hipStream_t s)
 {
-    using S = Shape<Type, D>;
-    const int n = a.tiles.nq[S::kTable];
-    attn_forward_kernel<Type, D, FW, 4 * S::kWide / FW, S::kRows, S::kBuffers, FO>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(FW * kWave), S::kBuffers * S::kLds, s>>>(
-            a, S::kTable, n);
-    return hipGetLastError();
+    if (query_table<D>(a.tiles, a.heads) == kBroad)
+        return forward_rows<D, Shape<Type, D>::kWide>(a, kBroad, s);
+    return forward_rows<D, 1>(a, kNarrow, s);
 }
 
+template <int D, int QT>
+hipError_t dq_rows(const AttnArgs &a, int table, hipStream_t s)
+{
+    using S = Shape<Type, D>;
+    const int n = a.tiles.nq[table];
+    attn_dq_kernel<Type, D, QT, S::kRows, S::kBuffers, S::kOccupancy>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(a, table, n);
+    return hipGetLastError();
+}
 template <int D>
 hipError_t backward(const AttnArgs &a, hipStream_t s)
 {
     using S = Shape<Type, D>;
-    const int nq = a.tiles.nq[S::kTable], nk = a.tiles.nk[S::kKeyTable];
-    if (nq > 0) {
-        attn_dq_kernel<Type, D, S::kWide, S::kRows, S::kBuffers, S::kWaves>
-            <<<dim3((unsigned)((int64_t)nq * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(
-                a, S::kTable, nq);
-        if (hipError_t e = hipGetLastError())
+    if (a.tiles.nq[kNarrow] > 0) {
+        const bool broad = query_table<D>(a.tiles, a.heads) == kBroad;
+        if (hipError_t e = broad ? dq_rows<D, S::kWide>(a, kBroad, s) : dq_rows<D, 1>(a, kNarrow, s))
             return e;
     }
+    const int nk = a.tiles.nk[kNarrow];
     if (nk > 0) {
         attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kRows, S::kBuffers, 2>
             <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave),
-               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)) + S::kGiven, s>>>(
-                a, S::kKeyTable, nk);
+               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)) + S::kGiven, s>>>(a, kNarrow, nk);
     }
     return hipGetLastError();
 }
@@ -1115,10 +1124,10 @@ hipError_t MTPX_OPS_NAME(attn_cache)(const CacheArgs &a, hipStream_t s)
 {
     return a.dim <= 32 ? cache<32>(a, s) : a.dim <= 64 ? cache<64>(a, s) : cache<128>(a, s);
 }
-int MTPX_OPS_NAME(attn_tiles)(int dim, const TileTable &t)
+int MTPX_OPS_NAME(attn_tiles)(int dim, int heads, const TileTable &t)
 {
-    return t.nq[dim <= 32 ? Shape<Type, 32>::kTable
-                          : dim <= 64 ? Shape<Type, 64>::kTable : Shape<Type, 128>::kTable];
+    return t.nq[dim <= 32 ? query_table<32>(t, heads)
+                          : dim <= 64 ? query_table<64>(t, heads) : query_table<128>(t, heads)];
 }
 
 #if MTPX_OPS_TYPE == 0
@@ -1128,13 +1137,14 @@ hipError_t attn_backward_bf16(const AttnArgs &, hipStream_t);
 hipError_t attn_backward_f16(const AttnArgs &, hipStream_t);
 hipError_t attn_cache_bf16(const CacheArgs &, hipStream_t);
 hipError_t attn_cache_f16(const CacheArgs &, hipStream_t);
-int attn_tiles_bf16(int, const TileTable &);
-int attn_tiles_f16(int, const TileTable &);
+int attn_tiles_bf16(int, int, const TileTable &);
+int attn_tiles_f16(int, int, const TileTable &);
 
-int attn_backward_tiles(int dtype, int dim, const TileTable &t)
+int attn_backward_tiles(int dtype, int dim, int heads, const TileTable &t)
 {
-    return dtype == MTPX_F32 ? attn_tiles_f32(dim, t)
-                             : dtype == MTPX_BF16 ? attn_tiles_bf16(dim, t) : attn_tiles_f16(dim, t);
+    return dtype == MTPX_F32    ? attn_tiles_f32(dim, heads, t)
+           : dtype == MTPX_BF16 ? attn_tiles_bf16(dim, heads, t)
+                                : attn_tiles_f16(dim, heads, t);
 }
 hipError_t launch_attn_forward(int dtype, const AttnArgs &a, hipStream_t s)
 {
@@ -1148,7 +1158,7 @@ hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s)
     if (e != hipSuccess)
         return e;
     dlambda_kernel<<<dim3(a.heads), dim3(kThreads), 0, s>>>(a.dlam_part, a.dlambda,
-                                                            attn_backward_tiles(dtype, a.dim, a.tiles));
+                                                            attn_backward_tiles(dtype, a.dim, a.heads, a.tiles));
     return hipGetLastError();
 }
 hipError_t launch_attn_cache(int dtype, const CacheArgs &a, hipStream_t s)

@@ -17,8 +17,9 @@ constexpr int kMaxBlock = 1024;
 // that are read at once (V 1 where rows are not whole 16-byte pieces).
 template <class T, int NT, int E, int V>
 struct Row {
-    static constexpr int kBlock = NT == kWave ? 256 : NT;
-    static constexpr int kPerBlock = kBlock / NT;  // rows of a workgroup
+    static constexpr int kBlock = NT <= kWave ? 256 : NT;
+    static constexpr int kPerBlock = kBlock / NT;                    // rows of a workgroup
+    static constexpr int kPerWave = NT < kWave ? kWave / NT : 1;      // and of a wave
     static constexpr int kPieces = E / V;
     static __device__ inline int column(int i, int t) { return (i * NT + t) * V; }
 
@@ -73,6 +74,10 @@ struct Row {
     // Sum over the row's threads, in a fixed order.
     static __device__ inline float sum(float v, float *red)
     {
+        if constexpr (NT < kWave) {
+            v = row16_sum(v);
+            return NT == 32 ? v + __shfl_xor(v, 16) : v;
+        }
         v = wave_sum(v);
         if constexpr (NT > kWave) {
             constexpr int kWavesRow = NT / kWave;
@@ -147,7 +152,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_forward_kerne
     const int64_t part = (int64_t)blockIdx.x * R::kPerBlock + threadIdx.x / NT;
     const int64_t groups = (int64_t)gridDim.x * R::kPerBlock;
     const bool own_gate = a.gate && a.gate_row != 0;
-    if (part >= a.rows)  // whole waves: a row's threads leave together
+    if (NT >= kWave && part >= a.rows)  // a row's threads leave together
         return;
     float post[E], pre[E];
 #pragma unroll
@@ -175,7 +180,10 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_forward_kerne
             R::fetch((const T *)a.gate + row * a.gate_row, a.width, t, rg);
     };
     ahead(part);
-    for (int64_t row = part; row < a.rows; row += groups) {
+    // (a wave's rows end together: one beyond the last is worked on unseen)
+    for (int64_t row0 = part - part % R::kPerWave; row0 < a.rows; row0 += groups) {
+        const int64_t row = row0 + part % R::kPerWave;
+        const bool there = row < a.rows;
         float v[E], x[E], g[E];
         R::widen(ry, v);
         R::widen(rx, x);
@@ -183,7 +191,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_forward_kerne
         ahead(row + groups);
         float mean, inv;
         normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
-        if (a.stats && t == 0) {
+        if (a.stats && t == 0 && there) {
             a.stats[4 * row] = mean;
             a.stats[4 * row + 1] = inv;
         }
@@ -201,18 +209,18 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock)) void norm_forward_kerne
             for (int e = 0; e < E; ++e)
                 v[e] = fmaf(a.residual_scale, x[e], v[e]);
         }
-        R::store((T *)a.s + row * a.s_row, a.width, t, v);
+        R::store((T *)a.s + row * a.s_row, there ? a.width : 0, t, v);
         if (!a.n)
             continue;
         normalise<R>(v, a.kind, a.width, a.eps, t, red, mean, inv);
-        if (a.stats && t == 0) {
+        if (a.stats && t == 0 && there) {
             a.stats[4 * row + 2] = mean;
             a.stats[4 * row + 3] = inv;
         }
 #pragma unroll
         for (int e = 0; e < E; ++e)
             v[e] *= inv * pre[e];
-        R::store((T *)a.n + row * a.n_row, a.width, t, v);
+        R::store((T *)a.n + row * a.n_row, there ? a.width : 0, t, v);
     }
 }
 
@@ -253,8 +261,12 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void
         R::fetch((const T *)a.pre, a.width, t, rpre);
     f32x4 rst;
     auto ahead = [&](int64_t row) {
-        if (row >= a.rows)
+        if (row >= a.rows) {
+            // zeros take part in the sums of a wave's other rows
+            rst = f32x4{0, 0, 0, 0};
+            ry = rx = rdn = rds = typename R::Raw{};
             return;
+        }
         R::fetch((const T *)a.y + row * a.y_row, a.width, t, ry);
         if (a.x)
             R::fetch((const T *)a.x + row * a.x_row, a.width, t, rx);
@@ -265,7 +277,9 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void
         rst = *reinterpret_cast<const f32x4 *>(a.stats + 4 * row);
     };
     ahead(part);
-    for (int64_t row = part; row < a.rows; row += groups) {
+    for (int64_t row0 = part - part % R::kPerWave; row0 < a.rows; row0 += groups) {
+        const int64_t row = row0 + part % R::kPerWave;
+        const bool there = row < a.rows;
         const f32x4 st = rst;
         float u[E], v[E], w[E], ds[E];
         R::widen(ry, u);
@@ -273,7 +287,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void
         R::widen(rdn, ds);
         const typename R::Raw into = rds;
         if (own_gate)
-            R::load((const T *)a.gate + row * a.gate_row, a.width, t, g);
+            R::load((const T *)a.gate + row * a.gate_row, there ? a.width : 0, t, g);
         if (a.post)
             R::widen(rpost, w);
         ahead(row + groups);
@@ -322,7 +336,7 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 v[e] = a.residual_scale * ds[e];
-            R::store((T *)a.dx + row * a.dx_row, a.width, t, v);
+            R::store((T *)a.dx + row * a.dx_row, there ? a.width : 0, t, v);
         }
         // through the gate and the first norm
         float s0 = 0.f, s1 = 0.f;
@@ -338,14 +352,14 @@ __global__ __launch_bounds__((Row<T, NT, E, V>::kBlock), NT < 1024 ? 3 : 4) void
             s1 = fmaf(ds[e], u[e], s1);
         }
         if (a.dgate && a.gate_row != 0)
-            R::store((T *)a.dgate + row * a.dgate_row, a.width, t, v);
+            R::store((T *)a.dgate + row * a.dgate_row, there ? a.width : 0, t, v);
         if (a.dy) {
             s0 = layer ? R::sum(s0, red) * scale : 0.f;
             s1 = R::sum(s1, red) * scale;
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 ds[e] = st[1] * (ds[e] - s0 - u[e] * s1);
-            R::store((T *)a.dy + row * a.dy_row, a.width, t, ds);
+            R::store((T *)a.dy + row * a.dy_row, there ? a.width : 0, t, ds);
         }
     }
     // The rows of a workgroup are summed through LDS, in their order.
@@ -423,11 +437,11 @@ hipError_t run(const NormArgs &a, bool back, hipStream_t s)
 }
 
 // The fewest threads that hold a row with 8 elements each (16 beyond 8,192
-// columns): more elements leave the backward pass fewer waves per SIMD to
+// columns), a power of two from 16 on: more elements leave the backward pass fewer waves per SIMD to
 // hide its reads (160,000 rows of 1,024: 611 us with 16 elements a thread).
 int row_threads(int width)
 {
-    int n = kWave;
+    int n = 16;
     while (n < kMaxBlock && width > 8 * n)
         n *= 2;
     return n;
@@ -436,6 +450,8 @@ template <class T, int V>
 hipError_t by_width(const NormArgs &a, bool back, hipStream_t s)
 {
     switch (row_threads(a.width)) {
+    case 16: return run<T, 16, 8, V>(a, back, s);
+    case 32: return run<T, 32, 8, V>(a, back, s);
     case 64: return run<T, 64, 8, V>(a, back, s);
     case 128: return run<T, 128, 8, V>(a, back, s);
     case 256: return run<T, 256, 8, V>(a, back, s);
@@ -464,12 +480,12 @@ hipError_t by_type(int dtype, const NormArgs &a, bool back, hipStream_t s)
 
 // Workgroups of the backward pass: as many as the chip holds at once (three
 // waves per SIMD by their registers), so that a weight gradient takes the
-// fewest partial rows; rows of one wave come four to a workgroup.
+// fewest partial rows; rows of one wave and less share a workgroup.
 int norm_backward_parts(int64_t rows, int width)
 {
     const int n = row_threads(width);
-    const int64_t need = n == kWave ? (rows + 3) / 4 : rows;
-    const int64_t most = 256 * 12 * kWave / (n == kWave ? 256 : n);
+    const int block = n <= kWave ? 256 : n, together = block / n;
+    const int64_t need = (rows + together - 1) / together, most = 256 * 12 * kWave / block;
     return (int)(need < most ? need : most);
 }
 hipError_t launch_norm_forward(int dtype, const NormArgs &a, hipStream_t s)

@@ -11,13 +11,9 @@
 struct mtpx_sequences {
     int device = 0, n = 0;
     int64_t total_q = 0, total_k = 0;
-    DBuf seq, tiles;
+    DBuf tiles;
     TileTable table{};
-    ~mtpx_sequences()
-    {
-        seq.release();
-        tiles.release();
-    }
+    ~mtpx_sequences() { tiles.release(); }
 };
 
 namespace mtpx {
@@ -89,7 +85,7 @@ AttnSizes attn_workspace(const mtpx_diff_attention_request &r)
     AttnSizes s;
     s.delta = pad(sizeof(float) * 2 * (size_t)r.heads * (size_t)q.total_q);
     s.part = pad(sizeof(float) * (size_t)r.heads *
-                 (size_t)attn_backward_tiles(r.dtype, r.dim, q.table));
+                 (size_t)attn_backward_tiles(r.dtype, r.dim, r.heads, q.table));
     s.total = std::max<size_t>(s.delta + s.part, 16);
     return s;
 }
@@ -142,7 +138,6 @@ int attn_args(mtpx_context *ctx, const mtpx_diff_attention_request &r, bool back
         for (const mtpx_rows *t : {&r.dout, &r.dq, &r.dk, &r.dv})
             also(*t);
     }
-    a.seq = sq.seq.as<Seq>();
     a.tiles = sq.table;
     a.heads = r.heads;
     a.kv_heads = r.kv_heads;
@@ -346,7 +341,13 @@ int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *req)
         width /= 2;
     RotaryArgs a{r.rows, r.heads, r.dim, r.rotated, r.interleaved != 0, r.inverse != 0, r.axes,
                  r.position_dtype, r.x, r.y, r.forward, r.positions, r.position_row,
-                 r.position_axis, r.freq, r.axis, r.dpositions, width};
+                 r.position_axis, r.freq, r.axis, r.dpositions, width, 0};
+    // a row gets a lane per piece, or as few as its pairs' table allows
+    const int64_t unit = r.interleaved && width > 1 ? width / 2 : width;
+    const int64_t pieces = (half / unit + (r.dim - r.rotated) / width) * r.heads;
+    a.lanes = 64;
+    while (a.lanes > 4 && a.lanes / 2 >= pieces && half * (128 / a.lanes) <= 512)
+        a.lanes /= 2;
     (void)hipSetDevice(ctx->device);
     HIP_TRY(launch_rotary(r.dtype, a, (hipStream_t)r.stream), "launch rotary");
     return MTPX_OK;
@@ -376,10 +377,6 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
         sq->n = n;
         sq->total_q = q_offsets[n];
         sq->total_k = ko[n];
-        std::vector<Seq> seqs((size_t)n);
-        for (int i = 0; i < n; ++i)
-            seqs[i] = Seq{q_offsets[i], ko[i], (int)(q_offsets[i + 1] - q_offsets[i]),
-                          (int)(ko[i + 1] - ko[i])};
         // the tiles with the most work first: they start while there is other
         // work to fill the device's last round with
         std::vector<SeqTile> all;
@@ -388,13 +385,12 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
             for (int j = 0; j < 2; ++j) {
                 std::vector<SeqTile> t;
                 for (int i = 0; i < n; ++i) {
-                    const int rows = side ? seqs[i].nk : seqs[i].nq;
-                    for (int64_t s = 0; s < rows; s += kTileRows[j])
-                        t.push_back(SeqTile{i, (int)s});
+                    const int nq = (int)(q_offsets[i + 1] - q_offsets[i]), nk = (int)(ko[i + 1] - ko[i]);
+                    for (int64_t s = 0; s < (side ? nk : nq); s += kTileRows[j])
+                        t.push_back(SeqTile{q_offsets[i], ko[i], nq, nk, (int)s});
                 }
                 std::stable_sort(t.begin(), t.end(), [&](const SeqTile &a, const SeqTile &b) {
-                    const int la = side ? seqs[a.seq].nq : seqs[a.seq].nk;
-                    const int lb = side ? seqs[b.seq].nq : seqs[b.seq].nk;
+                    const int la = side ? a.nq : a.nk, lb = side ? b.nq : b.nk;
                     // with causal rows the last queries and the first keys have the most
                     return la != lb ? la > lb : side ? a.start < b.start : a.start > b.start;
                 });
@@ -407,9 +403,7 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                 all.insert(all.end(), t.begin(), t.end());
             }
         (void)hipSetDevice(ctx->device);
-        hipError_t e = upload(sq->seq, seqs, ctx->stream);
-        if (e == hipSuccess)
-            e = upload(sq->tiles, all, ctx->stream);
+        hipError_t e = upload(sq->tiles, all, ctx->stream);
         if (e == hipSuccess)
             e = hipStreamSynchronize(ctx->stream);
         if (e != hipSuccess) {

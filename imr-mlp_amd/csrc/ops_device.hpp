@@ -267,10 +267,13 @@ __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
 // 16 bytes per lane from global memory straight into LDS, at byte `offset`
 // (the same in every lane) + 16 lane of the workgroup's LDS.  They are there
 // after wait_loads().
+// (As assembly text, since the compiler would wait for such loads before any
+// read of the LDS that it cannot tell from their target.  It has no output
+// register, and what it writes is waited for in wait_loads().  A write of m0
+// takes one wait state to reach it.)
 __device__ inline void load_to_lds(const void *p, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(offset), "v"(p)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(offset) : "memory");
 }
 // (After the reads of what lay there: wait_reads() or a barrier.)
 __device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -371,13 +374,21 @@ __device__ inline float max3(float a, float b, float c)
     return r;
 }
 
-// Sum over a wave, in a fixed order, in every lane: shifts within rows of 16
-// lanes, then from row to row, by data-parallel moves that need no LDS.
+// Sum over 16 lanes or a wave, in a fixed order, in every lane: rotations or
+// shifts within rows of 16 lanes, then from row to row, by data-parallel moves
+// that need no LDS.
 template <int CONTROL, int ROWS>
 __device__ inline float moved(float v)
 {
     return __builtin_bit_cast(
         float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, ROWS, 0xf, false));
+}
+__device__ inline float row16_sum(float v)
+{
+    v += moved<0x128, 0xf>(v);  // row_ror:8
+    v += moved<0x124, 0xf>(v);
+    v += moved<0x122, 0xf>(v);
+    return v + moved<0x121, 0xf>(v);
 }
 __device__ inline float wave_sum(float v)
 {

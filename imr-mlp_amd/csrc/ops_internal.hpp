@@ -10,13 +10,11 @@
 
 namespace mtpx {
 
-// One sequence of a ragged batch, and a run of its rows that one workgroup takes.
-struct Seq {
-    int64_t q0, k0;
-    int nq, nk;
-};
+// A run of rows of one sequence of a ragged batch that one workgroup takes:
+// queries or keys start .. start + tile rows - 1, with the sequence's place.
 struct SeqTile {
-    int seq, start;
+    int64_t q0, k0;
+    int nq, nk, start;
 };
 
 // Row counts of the tile tables a sequence handle keeps.
@@ -28,7 +26,6 @@ struct TileTable {
 };
 
 struct AttnArgs {
-    const Seq *seq;
     TileTable tiles;
     int heads, kv_heads, dim, causal;
     int64_t total_q;
@@ -64,6 +61,7 @@ struct RotaryArgs {
     const int *axis;
     void *dpositions;
     int width;  // elements of one access
+    int lanes;  // of a row: a power of two up to 64
 };
 
 struct NormArgs {
@@ -88,7 +86,7 @@ struct NormArgs {
 hipError_t launch_attn_forward(int dtype, const AttnArgs &a, hipStream_t s);
 hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s);
 // Query tiles of the backward pass, each of which leaves one partial of dlambda per head.
-int attn_backward_tiles(int dtype, int dim, const TileTable &t);
+int attn_backward_tiles(int dtype, int dim, int heads, const TileTable &t);
 hipError_t launch_attn_cache(int dtype, const CacheArgs &a, hipStream_t s);
 hipError_t launch_rotary(int dtype, const RotaryArgs &a, hipStream_t s);
 hipError_t launch_norm_forward(int dtype, const NormArgs &a, hipStream_t s);
