@@ -1,0 +1,170 @@
+"""A trained block over all atoms of a structure, on top of a short-ranged potential.
+
+    python examples/global_block.py [--structures 40] [--steps 120]
+
+A moment tensor potential sees an atom's neighbours within its cutoff.  This
+program adds what lies beyond: a block in which every atom attends to all atoms
+of its structure.  Its positions enter by rotation with whole numbers of turns
+over the cell, so that scores depend on differences of positions only and the
+cell's periodic images are the same atom.  The block is
+
+    x -> norm -> q, k, v -> rotary (x, y, z) -> differential attention
+      -> projection -> norm, gate, residual, norm -> energies
+
+with the library's operators for everything but the plain matrix products.  It
+learns, over a ragged batch of structures, an energy of long waves between two
+kinds of charge that no descriptor within the cutoff holds.  Afterwards the
+forces of the correction are taken through the rotation's gradient of the
+positions and compared with differences, and one atom is moved: its row alone
+is computed, against the keys and values kept for the others.
+"""
+import argparse
+import os
+import sys
+
+import numpy as np
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "imr-mlp_amd"))
+
+from mtpx import capi, ops, synth  # noqa: E402
+
+HEADS, DIM, WIDTH, CUTOFF = 2, 24, 64, 5.0
+LAMBDA_INIT = 0.2
+
+
+def structures(count, seed=7):
+    """FCC cells of several sizes, strained and displaced, with random species."""
+    out = []
+    for i in range(count):
+        rng = synth.rng_for(seed, i)
+        s = synth.lattice("fcc", (2 + i % 3, 2, 2 + i % 2), 3.9)
+        s = synth.displace(synth.strain(s, rng, 0.02), rng, 0.1)
+        s.types = (synth.uniform(rng, s.n) * 2).astype(np.int32)
+        out.append(s)
+    return out
+
+
+def long_range_energy(s):
+    """Charges of the two species meeting in the cell's longest waves."""
+    frac = s.pos @ np.linalg.inv(s.cell)
+    charge = np.where(s.types == 0, 1.0, -1.0)
+    return sum(abs((charge * np.exp(2j * np.pi * frac[:, a])).sum()) ** 2 for a in range(3)) / s.n ** 2
+
+
+class Block(torch.nn.Module):
+    def __init__(self, ctx, device):
+        super().__init__()
+        self.ctx = ctx
+        inner = HEADS * 2 * DIM
+
+        def weight(*shape):
+            return torch.nn.Parameter(torch.randn(shape, device=device) / shape[0] ** 0.5)
+
+        def ones(n, value=1.0):
+            return torch.nn.Parameter(torch.full((n,), value, device=device))
+
+        self.embed, self.qkv, self.back, self.read = weight(3, WIDTH), weight(WIDTH, 3 * inner), weight(inner, WIDTH), weight(WIDTH, 1)
+        self.first, self.post, self.pre, self.gate = ones(WIDTH), ones(WIDTH), ones(WIDTH), ones(WIDTH, 0.5)
+        # lambda = exp(a . b) - exp(c . d) + its initial value, per head
+        self.parts = torch.nn.Parameter(0.1 * torch.randn((4, HEADS, DIM), device=device))
+        pair = torch.arange(DIM // 2, device=device)
+        self.register_buffer("axis", (pair % 3).int())
+        self.register_buffer("freq", 2 * torch.pi * (1 + pair // 3).float())
+
+    def lam(self):
+        a, b, c, d = self.parts
+        return ((a * b).sum(1).exp() - (c * d).sum(1).exp() + LAMBDA_INIT).contiguous()
+
+    def project(self, atoms, frac):
+        """Residual stream and rotated q, k, and v of every atom."""
+        x = atoms @ self.embed
+        n = ops.NormBlockFn.apply(self.ctx, None, x, None, self.first, None, dict(next_norm=False))[0]
+        p = n @ self.qkv
+        inner = HEADS * 2 * DIM
+        qk = p[:, :2 * inner].unflatten(1, (4 * HEADS, DIM))  # q and k turn together
+        qk = ops.RotaryFn.apply(self.ctx, qk, frac, self.freq, self.axis)
+        q, k = qk[:, :2 * HEADS].unflatten(1, (HEADS, 2)), qk[:, 2 * HEADS:].unflatten(1, (HEADS, 2))
+        return x, q, k, p[:, 2 * inner:].unflatten(1, (HEADS, 2 * DIM))
+
+    def energies(self, x, attended):
+        y = attended.flatten(1) @ self.back
+        _, n = ops.NormBlockFn.apply(self.ctx, x, y, self.gate, self.post, self.pre, dict(gate_act="tanh"))
+        return (n @ self.read)[:, 0]
+
+    def forward(self, atoms, frac, seqs):
+        x, q, k, v = self.project(atoms, frac)
+        return self.energies(x, ops.DiffAttentionFn.apply(self.ctx, q, k, v, self.lam(), seqs))
+
+
+def run(count=40, steps=120, log=print):
+    torch.manual_seed(0)
+    device = torch.device("cuda", 0)
+    ctx = capi.Context(0)
+    batch = structures(count)
+    for s in batch:
+        s.pos = capi.wrap(s.cell, s.pbc, s.pos)
+
+    # the short-ranged part: energies per atom from the potential
+    ctx.load_model_text(synth.random_model("shapeev-10.mtp", 2, 8, 2.0, CUTOFF, -0.05, 0.05, synth.rng_for(3)))
+    offsets = np.asarray(ctx.set_structures(batch, CUTOFF), np.int64)
+    site = np.asarray(ctx.compute_batch()[3]).ravel()
+    types = np.concatenate([s.types for s in batch])
+    atoms = np.stack([types == 0, types == 1, (site - site.mean()) / site.std()], 1)
+    frac = np.concatenate([s.pos @ np.linalg.inv(s.cell) for s in batch])
+    target = np.array([long_range_energy(s) for s in batch])
+
+    atoms, frac, target = (torch.tensor(t, dtype=torch.float32, device=device) for t in (atoms, frac, (target - target.mean()) / target.std()))
+    seqs = ops.Sequences(ctx, offsets)
+    which = torch.repeat_interleave(torch.arange(count, device=device), torch.tensor(np.diff(offsets), device=device))
+    size = torch.tensor(np.diff(offsets), device=device).float()
+
+    def per_structure(e):
+        return torch.zeros(count, device=device).index_add(0, which, e) / size
+
+    block = Block(ctx, device)
+    adam = torch.optim.Adam(block.parameters(), lr=3e-3)
+    losses = []
+    for step in range(steps):
+        adam.zero_grad()
+        loss = (per_structure(block(atoms, frac, seqs)) - target).square().mean()
+        loss.backward()
+        adam.step()
+        losses.append(float(loss.detach()))
+        if step % 20 == 0 or step == steps - 1:
+            log("step %4d  loss %.5f" % (step, losses[-1]))
+
+    # forces of the correction, through the gradient of the positions
+    at = frac.clone().requires_grad_(True)
+    block(atoms, at, seqs).sum().backward()
+    toward = torch.randn(frac.shape, generator=torch.Generator().manual_seed(1)).to(device)
+    toward /= toward.norm()
+    h = 3e-3
+    with torch.no_grad():
+        up, down = (block(atoms, frac + s * h * toward, seqs).double().sum() for s in (1, -1))
+    slope, expected = float((at.grad * toward).sum()), float(up - down) / (2 * h)
+    log("slope of the energy along a displacement %.5f, from differences %.5f" % (slope, expected))
+
+    # one atom of the largest structure moves: its row against the kept rows
+    i = int(np.argmax(np.diff(offsets)))
+    rows = slice(int(offsets[i]), int(offsets[i + 1]))
+    with torch.no_grad():
+        moved = frac.clone()
+        moved[rows.start] += 0.05
+        x, q, k, v = block.project(atoms, moved)
+        length = torch.tensor([rows.stop - rows.start], dtype=torch.int32, device=device)
+        one = ops.diff_attention_cache(ctx, q[rows.start:rows.start + 1], k[None, rows], v[None, rows], block.lam(), length)
+        alone = float(block.energies(x[rows.start:rows.start + 1], one))
+        among = float(block(atoms, moved, seqs)[rows.start])
+    log("energy of the moved atom alone %.6f, with its whole batch %.6f" % (alone, among))
+    ctx.close()
+    return dict(losses=losses, slope=slope, expected=expected, alone=alone, among=among)
+
+
+if __name__ == "__main__":
+    p = argparse.ArgumentParser(description=__doc__.split("\n")[0])
+    p.add_argument("--structures", type=int, default=40)
+    p.add_argument("--steps", type=int, default=120)
+    a = p.parse_args()
+    run(a.structures, a.steps)

@@ -20,7 +20,8 @@ namespace mtpx {
 namespace {
 
 constexpr int64_t kMaxLength = int64_t(1) << 30;  // rows of one sequence
-constexpr int64_t kMaxGrid = INT32_MAX;
+// a launch's threads are counted in 32 bits: workgroups of 512, rows of 64
+constexpr int64_t kMaxGroups = UINT32_MAX / 512, kMaxRows = UINT32_MAX / 64;
 
 int invalid(mtpx_context *ctx, const std::string &msg) { return set_error(ctx, MTPX_E_INVALID, msg); }
 
@@ -100,7 +101,7 @@ int attn_args(mtpx_context *ctx, const mtpx_diff_attention_request &r, bool back
     if (sq.device != ctx->device)
         return invalid(ctx, "the sequences belong to another device");
     for (int i = 0; i < 2; ++i)
-        if ((int64_t)std::max(sq.table.nq[i], sq.table.nk[i]) * r.heads > kMaxGrid)
+        if ((int64_t)std::max(sq.table.nq[i], sq.table.nk[i]) * r.heads > kMaxGroups)
             return set_error(ctx, MTPX_E_CAPACITY, "too many rows and heads for one launch");
     const size_t size = dtype_bytes(r.dtype);
     const bool q = sq.total_q > 0, k = sq.total_k > 0;
@@ -198,7 +199,7 @@ int check_norm(mtpx_context *ctx, const mtpx_norm_block_request &r)
         return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
     if (r.rows < 0 || r.width < 1)
         return invalid(ctx, "rows must not be negative and width positive");
-    if (r.width > 16384 || r.rows > kMaxGrid)
+    if (r.width > 16384 || r.rows > kMaxRows)
         return set_error(ctx, MTPX_E_CAPACITY, "width beyond 16384 or too many rows");
     if (r.kind != MTPX_NORM_RMS && r.kind != MTPX_NORM_LAYER)
         return invalid(ctx, "unknown norm kind");
@@ -296,7 +297,7 @@ int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *req)
         return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
     if (r.rows < 0 || r.heads < 1 || r.dim < 1)
         return invalid(ctx, "rows must not be negative, heads and dim positive");
-    if (r.dim > 1024 || r.rows > kMaxGrid)
+    if (r.dim > 1024 || r.rows > kMaxRows)
         return set_error(ctx, MTPX_E_CAPACITY, "dim beyond 1024 or too many rows");
     if (r.rotated < 0 || r.rotated > r.dim || r.rotated % 2 != 0)
         return invalid(ctx, "rotated must be even and at most dim");
@@ -394,7 +395,7 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                     // with causal rows the last queries and the first keys have the most
                     return la != lb ? la > lb : side ? a.start < b.start : a.start > b.start;
                 });
-                if (t.size() > (size_t)kMaxGrid) {
+                if (t.size() > (size_t)kMaxGroups) {
                     delete sq;
                     return set_error(ctx, MTPX_E_CAPACITY, "too many rows for one launch");
                 }

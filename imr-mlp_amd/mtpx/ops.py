@@ -488,12 +488,12 @@ class DiffAttentionFn(torch.autograd.Function):
 
 class NormBlockFn(torch.autograd.Function):
     """NormBlockFn.apply(ctx, x, y, gate, post_weight, pre_weight, options):
-    norm_block with the keyword arguments in the dict options."""
+    (s, n) of norm_block with the keyword arguments in the dict options."""
 
     @staticmethod
     def forward(fn, ctx, x, y, gate, post_weight, pre_weight, options):
         s, n, stats = norm_block(ctx, x, y, gate, post_weight, pre_weight, save=True, **options)
-        fn.ctx, fn.options = ctx, options
+        fn.ctx, fn.options = ctx, {k: v for k, v in options.items() if k != "next_norm"}
         fn.save_for_backward(x, y, gate, post_weight, pre_weight, stats)
         fn.set_materialize_grads(False)
         return s, n

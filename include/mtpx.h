@@ -634,7 +634,7 @@ typedef struct mtpx_rows {
 typedef struct mtpx_rotary_request {
     void *stream;
     int dtype;
-    int64_t rows;
+    int64_t rows;            /* below 2^26 */
     int heads, dim, rotated; /* rotated even, at most dim; dim <= 1024 */
     int interleaved, inverse;
     mtpx_rows x, y;          /* map unused */
@@ -746,7 +746,7 @@ int mtpx_diff_attention_cache_workspace(mtpx_context *ctx,
 typedef struct mtpx_norm_block_request {
     void *stream;
     int dtype;
-    int64_t rows;
+    int64_t rows;             /* below 2^26 */
     int width;                /* 1 to 16384 */
     int kind, gate_act;
     float residual_scale, block_scale, eps;
