@@ -1018,17 +1018,27 @@ __global__ __launch_bounds__(4 * D) void attn_cache_join(CacheArgs a)
 template <class T, int D>
 struct Shape {
     static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
-    // most 16-row groups a wave's registers hold
-    static constexpr int kWide = (D <= 64 && sizeof(T) == 2) || D == 32 ? 2 : 1;
+    // 16-row groups of a wave: two share the reads from LDS that bound 16-bit
+    // products; 32-bit products take so long that more waves serve them better
+    static constexpr int kWide = D <= 64 && sizeof(T) == 2 ? 2 : 1;
     // 64 keys: two pairs of waves that share 32 keys where a wave's registers
     // hold those (and two workgroups' LDS a CU), four pairs that share 16 else
     static constexpr int kKeyWide = D <= 64 && sizeof(T) == 2 ? 2 : 1;
     static constexpr int kKeyWaves = 8 / kKeyWide;
-    static constexpr size_t kGiven = kKeyWaves / 2 * 3 * (kRows / 32) * kKeyWide * kWave * 4 * sizeof(T);
     static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
     // two buffers of both tiles within the 64 KiB that loads into LDS address
     static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
-    static constexpr int kOccupancy = kLds <= 32768 ? 2 : 1;  // waves per SIMD: registers of one
+    // waves per SIMD that the registers of one let in
+    static constexpr int kOccupancy = kLds > 32768 ? 1 : D == 32 && sizeof(T) == 2 ? 3 : 2;
+    // narrow 32-bit heads: three and four, to which one buffer leaves the LDS
+    // (200 structures of 84 atoms: forward 103 us with two buffers and two
+    // waves, 92 us so; key pass 164 us with 64 rows twice, 122 us with 32 once)
+    static constexpr bool kMore = D == 32 && sizeof(T) == 4;
+    static constexpr int kQueryBuffers = kMore ? 1 : kBuffers, kQueryOccupancy = kMore ? 3 : kOccupancy;
+    static constexpr int kKeyRows = kMore ? 32 : kRows, kKeyBuffers = kMore ? 1 : kBuffers;
+    static constexpr int kKeyOccupancy = kMore ? 4 : kOccupancy > 2 ? 3 : 2;
+    static constexpr size_t kKeyLds = kKeyBuffers * (4 * (size_t)kKeyRows * D * sizeof(T) + 4 * kKeyRows * sizeof(float)) +
+                                      kKeyWaves / 2 * 3 * (kKeyRows / 32) * kKeyWide * kWave * 4 * sizeof(T);
 };
 
 // Tables of 64 and 128 rows.
@@ -1049,8 +1059,8 @@ hipError_t forward_rows(const AttnArgs &a, int table, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[table];
-    attn_forward_kernel<Type, D, 4, QT, S::kRows, S::kBuffers, S::kOccupancy>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(a, table, n);
+    attn_forward_kernel<Type, D, 4, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s>>>(a, table, n);
     return hipGetLastError();
 }
 template <int D>
@@ -1066,8 +1076,8 @@ hipError_t dq_rows(const AttnArgs &a, int table, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[table];
-    attn_dq_kernel<Type, D, QT, S::kRows, S::kBuffers, S::kOccupancy>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kBuffers * S::kLds, s>>>(a, table, n);
+    attn_dq_kernel<Type, D, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy>
+        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s>>>(a, table, n);
     return hipGetLastError();
 }
 template <int D>
@@ -1081,9 +1091,9 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
     }
     const int nk = a.tiles.nk[kNarrow];
     if (nk > 0) {
-        attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kRows, S::kBuffers, 2>
-            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave),
-               S::kBuffers * (S::kLds + 4 * S::kRows * sizeof(float)) + S::kGiven, s>>>(a, kNarrow, nk);
+        attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kKeyRows, S::kKeyBuffers, S::kKeyOccupancy>
+            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave), S::kKeyLds, s>>>(
+                a, kNarrow, nk);
     }
     return hipGetLastError();
 }
