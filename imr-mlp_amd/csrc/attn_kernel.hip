@@ -31,16 +31,31 @@ typedef _Float16 Type;
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
-// Keys k0 .. k0 + 63 of a sequence of nk that are there and not masked.
-__device__ inline unsigned long long seen_keys(const unsigned char *mask, int k0, int nk, int lane)
-{
-    if (!mask) {
-        const int there = nk - k0;
-        return there >= 64 ? ~0ull : (1ull << there) - 1;
+// Which of the keys k0 .. k0 + 63 of a sequence of nk are there and not
+// masked; the mask is read `step` keys ahead, so that no step waits for it.
+struct SeenKeys {
+    const unsigned char *mask;
+    int nk, lane;
+    unsigned char ahead = 0;
+
+    __device__ inline SeenKeys(const unsigned char *m, int n, int l) : mask(m), nk(n), lane(l)
+    {
+        if (mask && lane < nk)
+            ahead = mask[lane];
     }
-    const int k = k0 + lane;
-    return __ballot(k < nk && mask[k]);
-}
+    __device__ inline unsigned long long at(int k0, int step)
+    {
+        if (!mask) {
+            const int there = nk - k0;
+            return there >= 64 ? ~0ull : (1ull << there) - 1;
+        }
+        const int k = k0 + lane;
+        const unsigned long long bits = __ballot(k < nk && ahead);
+        if (k + step < nk)
+            ahead = mask[k + step];
+        return bits;
+    }
+};
 
 // Whether no row up to `last` sees any of the 32 keys from k0 + 32 b on.
 __device__ inline bool empty_block(unsigned long long seen, int b, int causal, int k0, int last)
@@ -126,8 +141,9 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
     if (a.causal)
         nk = min(nk, min(sq.start + W * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
+    SeenKeys seen(mask, nk, lane);
     if (nk > 0) {
-        bits = seen_keys(mask, 0, nk, lane) & kFull;
+        bits = seen.at(0, KB) & kFull;
         lk.load(smem, 0, bits, bits == kFull);
         lv.load(smem, kTile, bits, bits == kFull);
     }
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
         auto next = [&] {
             if (k0 + KB < nk) {
                 buf = BUF - 1 - buf;
-                bits = seen_keys(mask, k0 + KB, nk, lane) & kFull;
+                bits = seen.at(k0 + KB, KB) & kFull;
                 lk.next();
                 lv.next();
                 lk.load(smem, buf * 2 * kTile, bits, bits == kFull);
@@ -370,8 +386,9 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     if (a.causal)
         nk = min(nk, min(sq.start + kWaves * QT * 16, sq.nq) + shift);
     unsigned long long bits = 0;
+    SeenKeys seen(mask, nk, lane);
     if (nk > 0) {
-        bits = seen_keys(mask, 0, nk, lane) & kFull;
+        bits = seen.at(0, KB) & kFull;
         lk.load(smem, 0, bits, bits == kFull);
         lv.load(smem, kTile, bits, bits == kFull);
     }
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
         auto next = [&] {
             if (k0 + KB < nk) {
                 buf = BUF - 1 - buf;
-                bits = seen_keys(mask, k0 + KB, nk, lane) & kFull;
+                bits = seen.at(k0 + KB, KB) & kFull;
                 lk.next();
                 lv.next();
                 lk.load(smem, buf * 2 * kTile, bits, bits == kFull);
