@@ -174,7 +174,7 @@ int cache_splits(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
     const int group = r.heads / r.kv_heads;
     const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * ((group + 15) / 16), 1);
     const int64_t most = (r.capacity + 127) / 128;
-    const int64_t want = (4 * (int64_t)ctx->num_cus + base - 1) / base;
+    const int64_t want = (8 * (int64_t)ctx->num_cus + base - 1) / base;
     return (int)std::min<int64_t>({want, most, (int64_t)kMaxSplits});
 }
 
