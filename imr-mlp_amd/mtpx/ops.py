@@ -128,9 +128,13 @@ def _tensor(ctx, t, name, shape=None, dtype=None):
     return t
 
 
-def _strides(ctx, t, name, shape, dtype=None):
-    """Strides of a checked tensor whose last dimension is contiguous."""
-    s = _tensor(ctx, t, name, shape, dtype).stride()
+def _strides(ctx, t, name, shape, dtype):
+    """Strides of a tensor of this shape and type on the context's device whose
+    last dimension is contiguous."""
+    if (not isinstance(t, torch.Tensor) or t.get_device() != ctx.device or t.dtype is not dtype or
+            t.shape != shape):
+        _tensor(ctx, t, name, shape, dtype)  # says which
+    s = t.stride()
     if s[-1] != 1 and t.shape[-1] > 1:
         _fail("the last dimension of %s is not contiguous" % name)
     return s
@@ -142,11 +146,16 @@ def _inner(t, name):
     return t
 
 
-def _typed(ctx, t, name):
-    _tensor(ctx, t, name)
-    if t.dtype not in DTYPES:
+def _typed(ctx, t, name, dims):
+    """The type code of a tensor of so many dimensions on the context's device."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
+        _fail("%s is not a tensor on the context's device" % name)
+    code = DTYPES.get(t.dtype)
+    if code is None:
         _fail("%s is %s, not float32, bfloat16 or float16" % (name, t.dtype))
-    return DTYPES[t.dtype]
+    if t.dim() != dims:
+        _fail("%s has %d dimensions, not %d" % (name, t.dim(), dims))
+    return code
 
 
 def _stream(ctx):
@@ -185,25 +194,28 @@ def _workspace(ctx, size):
 
 
 def _rotary(ctx, x, positions, freq, axis, interleaved, inverse, out, forward, dpositions):
-    dtype = _typed(ctx, x, "x")
-    sx = _strides(ctx, x, "x", (None, None, None))
-    rows, heads, dim = shape = x.shape
+    dtype = _typed(ctx, x, "x", 3)
+    shape = x.shape
+    sx = _strides(ctx, x, "x", shape, x.dtype)
+    rows, heads, dim = shape
     sp = _tensor(ctx, positions, "positions", (rows, None)).stride()
-    if positions.dtype not in POSITION_DTYPES:
+    ptype = POSITION_DTYPES.get(positions.dtype)
+    if ptype is None:
         _fail("positions are %s, not float32, float64, int32 or int64" % positions.dtype)
-    _tensor(ctx, freq, "freq", (None,), torch.float32)
-    _tensor(ctx, axis, "axis", freq.shape, torch.int32)
-    if not freq.is_contiguous() or not axis.is_contiguous():
-        _fail("freq and axis must be contiguous")
-    y = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
-    sy = _strides(ctx, y, "out", shape, x.dtype)
+    pairs = (freq.numel(),) if isinstance(freq, torch.Tensor) else (None,)
+    _strides(ctx, freq, "freq", pairs, torch.float32)
+    _strides(ctx, axis, "axis", pairs, torch.int32)
+    if out is None:
+        y, sy = x.new_empty(shape), (heads * dim, dim)
+    else:
+        y, sy = out, _strides(ctx, out, "out", shape, x.dtype)
     f, sf = None, (0, 0)
     if dpositions is not None:
         sf, f = _strides(ctx, forward, "x", shape, x.dtype), forward.data_ptr()
     req = _pack_rotary(
-        _stream(ctx), dtype, rows, heads, dim, 2 * freq.shape[0], interleaved, inverse,
+        _stream(ctx), dtype, rows, heads, dim, 2 * pairs[0], interleaved, inverse,
         x.data_ptr(), sx[0], sx[1], 0, y.data_ptr(), sy[0], sy[1], 0, positions.data_ptr(),
-        POSITION_DTYPES[positions.dtype], sp[0], sp[1], positions.shape[1], freq.data_ptr(),
+        ptype, sp[0], sp[1], positions.shape[1], freq.data_ptr(),
         axis.data_ptr(), f or 0, sf[0], sf[1], 0, 0 if dpositions is None else dpositions.data_ptr())
     ctx._check(_ops().mtpx_rotary(ctx.h, req), "rotary")
     return y
@@ -259,7 +271,7 @@ class Sequences:
 
 
 def _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask):
-    dtype = _typed(ctx, q, "q")
+    dtype = _typed(ctx, q, "q", 4)
     heads, dim = _tensor(ctx, q, "q", (None, None, 2, None)).shape[1::2]
     kv = _tensor(ctx, k, "k", (None, None, 2, dim), q.dtype).shape[1]
     _tensor(ctx, v, "v", (k.shape[0], kv, 2 * dim), q.dtype)
@@ -337,20 +349,22 @@ def diff_attention_cache(ctx, q, k, v, lam, lengths, *, scale=None, out=None):
     k [sequences, capacity, kv heads, 2, dim], v [sequences, capacity, kv
     heads, 2 dim], lengths [sequences] int32 on the device.  Returns
     [sequences, heads, 2 dim]."""
-    dtype = _typed(ctx, q, "q")
-    sq = _strides(ctx, q, "q", (None, None, 2, None))
+    dtype = _typed(ctx, q, "q", 4)
+    of = q.dtype
     n, heads, _, dim = q.shape
-    sk = _strides(ctx, k, "k", (n, None, None, 2, dim), q.dtype)
-    cap, kv = k.shape[1:3]
-    sv = _strides(ctx, v, "v", (n, cap, kv, 2 * dim), q.dtype)
-    _tensor(ctx, lengths, "lengths", (n,), torch.int32)
-    _tensor(ctx, lam, "lam", (heads,), torch.float32)
-    if not lam.is_contiguous() or not lengths.is_contiguous():
-        _fail("lam and lengths must be contiguous")
+    sq = _strides(ctx, q, "q", (n, heads, 2, dim), of)
+    if not isinstance(k, torch.Tensor) or k.dim() != 5:
+        _fail("k is not [sequences, capacity, kv heads, 2, dim]")
+    _, cap, kv, _, _ = k.shape
+    sk = _strides(ctx, k, "k", (n, cap, kv, 2, dim), of)
+    sv = _strides(ctx, v, "v", (n, cap, kv, 2 * dim), of)
+    _strides(ctx, lengths, "lengths", (n,), torch.int32)
+    _strides(ctx, lam, "lam", (heads,), torch.float32)
     shape = (n, heads, 2 * dim)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    so = _strides(ctx, out, "out", shape, q.dtype)
+        out, so = q.new_empty(shape), (heads * 2 * dim, 2 * dim)
+    else:
+        so = _strides(ctx, out, "out", shape, of)
     size = _bytes(ctx, _ops().mtpx_diff_attention_cache_workspace, CacheRequest, dtype=dtype,
                   sequences=n, heads=heads, kv_heads=kv, dim=dim, capacity=cap)
     w = _workspace(ctx, size) if size else None  # held until the kernels are queued
@@ -370,26 +384,27 @@ def _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_sca
           eps, s, n, stats, ds=None, dn=None, dx=None, dy=None, dgate=None, dpost=None, dpre=None,
           work=None, work_bytes=0):
     """The checked and packed request of either pass; results are contiguous."""
-    dtype = _typed(ctx, y, "y")
-    sy = _strides(ctx, y, "y", (None, None))
-    shape = rows, width = y.shape
+    dtype, of = _typed(ctx, y, "y", 2), y.dtype
+    shape = y.shape
+    rows, width = shape
+    sy = _strides(ctx, y, "y", shape, of)
     if kind not in NORMS or gate_act not in GATES:
         _fail("kind is one of %s, gate_act of %s" % (tuple(NORMS), tuple(GATES)))
-    sx = (0,) if x is None else _strides(ctx, x, "x", shape, y.dtype)
+    sx = (0,) if x is None else _strides(ctx, x, "x", shape, of)
     gate_row = 0
     if gate is not None:
         one = gate.dim() == 1
-        sg = _strides(ctx, gate, "gate", (width,) if one else shape, y.dtype)
+        sg = _strides(ctx, gate, "gate", (width,) if one else shape, of)
         if not one:
             gate_row = sg[0]
             if gate_row == 0:
                 _fail("a gate shared by all rows is [width]")
     if post_weight is not None:
-        _strides(ctx, post_weight, "post_weight", (width,), y.dtype)
+        _strides(ctx, post_weight, "post_weight", (width,), of)
     if pre_weight is not None:
-        _strides(ctx, pre_weight, "pre_weight", (width,), y.dtype)
-    sds = (0,) if ds is None else _strides(ctx, ds, "ds", shape, y.dtype)
-    sdn = (0,) if dn is None else _strides(ctx, dn, "dn", shape, y.dtype)
+        _strides(ctx, pre_weight, "pre_weight", (width,), of)
+    sds = (0,) if ds is None else _strides(ctx, ds, "ds", shape, of)
+    sdn = (0,) if dn is None else _strides(ctx, dn, "dn", shape, of)
     return _pack_norm(
         _stream(ctx), dtype, rows, width, NORMS[kind], GATES[gate_act], residual_scale, block_scale,
         eps, _ptr(x), y.data_ptr(), _ptr(gate), _ptr(post_weight), _ptr(pre_weight), sx[0], sy[0],
@@ -406,10 +421,11 @@ def norm_block(ctx, x, y, gate=None, post_weight=None, pre_weight=None, *, kind=
     width] (x None: no residual; gate [rows, width], [width] or None; weights
     [width] or None).  Returns (s, n), with save (s, n, stats); without
     next_norm n is None."""
-    shape = _tensor(ctx, y, "y", (None, None)).shape
-    s = torch.empty(shape, dtype=y.dtype, device=y.device)
-    n = torch.empty(shape, dtype=y.dtype, device=y.device) if next_norm else None
-    stats = torch.empty((shape[0], 4), dtype=torch.float32, device=y.device) if save else None
+    if not isinstance(y, torch.Tensor):
+        _fail("y is not a tensor")
+    s = y.new_empty(y.shape)
+    n = y.new_empty(y.shape) if next_norm else None
+    stats = y.new_empty((len(y), 4), dtype=torch.float32) if save else None
     req = _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_scale,
                 block_scale, eps, s, n, stats)
     ctx._check(_ops().mtpx_norm_block(ctx.h, req), "norm_block")
@@ -421,14 +437,14 @@ def norm_block_backward(ctx, ds, dn, x, y, gate, post_weight, pre_weight, stats,
     """(dx, dy, dgate, dpost_weight, dpre_weight) from the gradients of s and n
     (either may be None) and the forward pass's inputs and stats; None in the
     place of an input that was not given."""
-    dtype = _typed(ctx, y, "y")
-    rows, width = _tensor(ctx, y, "y", (None, None)).shape
+    dtype = _typed(ctx, y, "y", 2)
+    rows, width = y.shape
     _tensor(ctx, stats, "stats", (rows, 4), torch.float32)
     if not stats.is_contiguous():
         _fail("stats must be contiguous")
 
     def like(t):
-        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        return None if t is None else t.new_empty(t.shape)
 
     dx, dy, dgate, dpost, dpre = like(x), like(y), like(gate), like(post_weight), like(pre_weight)
     size = _bytes(ctx, _ops().mtpx_norm_block_workspace, NormRequest, dtype=dtype, rows=rows,
