@@ -10,18 +10,28 @@ Functions with gradients come twice: as a pair (f, f_backward) on plain
 tensors, and as an autograd function (RotaryFn, DiffAttentionFn, NormBlockFn).
 Tensors are float32, bfloat16 or float16; their last dimension has to be
 contiguous, other strides are free.  There is no fallback: a missing library
-or a refused argument raises.
+or a refused argument raises.  torch and the library share one HIP runtime if
+this module or torch is imported before the library is first used; the other
+order is refused.
 """
 from __future__ import annotations
 
 import ctypes as C
 import struct
+import sys
 
 import numpy as np
-import torch
 
 from . import capi
 from .capi import MtpxError  # noqa: F401 -- what the calls raise
+
+if capi._lib is not None and "torch" not in sys.modules:
+    # the library has brought its own HIP runtime, and a process's second one
+    # finds no device
+    raise ImportError("import torch or mtpx.ops before the first call of mtpx.capi: "
+                      "the library then uses torch's HIP runtime")
+
+import torch  # noqa: E402
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POSITION_DTYPES = {torch.float32: 0, torch.float64: 3, torch.int32: 4, torch.int64: 5}

@@ -2,6 +2,7 @@ import os
 import sys
 
 import pytest
+import torch  # noqa: F401 -- before libmtpx.so, so that both use torch's HIP runtime (mtpx.ops)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 for p in (os.path.join(ROOT, "imr-mlp_amd"), os.path.join(ROOT, "oracle"), ROOT):

@@ -5,6 +5,7 @@ import ctypes as C
 import math
 import os
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -48,6 +49,16 @@ def test_null_arguments_are_refused():
         assert getattr(L, "mtpx_%s_workspace" % f)(None, C.byref(r()), C.byref(n)) == -1
     assert L.mtpx_sequences_create(None, 0, None, None, C.byref(h)) == -1 and not h.value
     L.mtpx_sequences_destroy(None)
+
+
+def test_torch_comes_before_the_library():
+    """In a process of its own: the library used first, then mtpx.ops."""
+    code = "import sys; sys.path.insert(0, %r); from mtpx import capi; capi.lib(); from mtpx import ops"
+    code = code % os.path.join(capi.ROOT, "imr-mlp_amd")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode != 0 and "before the first call of mtpx.capi" in r.stderr
+    ok = subprocess.run([sys.executable, "-c", code.replace("import sys;", "import sys, torch;")], capture_output=True)
+    assert ok.returncode == 0
 
 
 class _Ctx:
