@@ -411,6 +411,8 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
             delete sq;
             return hip_fail(ctx, e, "upload sequences");
         }
+        for (int i = 0; i < n; ++i)
+            sq->table.longest_k = std::max(sq->table.longest_k, (int)(ko[i + 1] - ko[i]));
         for (int j = 0; j < 2; ++j) {
             sq->table.q[j] = sq->tiles.as<SeqTile>() + first[j];
             sq->table.k[j] = sq->tiles.as<SeqTile>() + first[2 + j];

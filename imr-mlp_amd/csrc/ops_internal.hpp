@@ -23,6 +23,7 @@ constexpr int kTileRows[2] = {64, 128};
 struct TileTable {
     const SeqTile *q[2], *k[2];  // by kTileRows
     int nq[2], nk[2];
+    int longest_k;  // most keys of a sequence
 };
 
 struct AttnArgs {

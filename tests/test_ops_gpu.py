@@ -180,6 +180,39 @@ def test_attention_masks(ctx, dtype, causal, dim):
 
 
 @dtypes
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 32), (2, 2, 64), (2, 1, 128)])
+def test_attention_single_keys(ctx, dtype, heads, kv, dim):
+    """Sequences of one key: its probability is 1, so the scores have no
+    gradient, exactly; values and lambda have theirs."""
+    c = attention_case(dim, dtype, [1, 3, 1, 0, 2] * 9, [1, 1, 1, 1, 1] * 9, heads, kv, dim)
+    for causal in (False, True):
+        check_attention(ctx, c, causal)
+        dev = [c[n].cuda() for n in ("q", "k", "v", "lam")]
+        seqs = ops.Sequences(ctx, c["q_off"], c["k_off"])
+        out, saved = ops.diff_attention(ctx, *dev, seqs, causal=causal, save=True)
+        dq, dk, dv, _ = ops.diff_attention_backward(ctx, c["dout"].cuda(), *dev, seqs, out, saved, causal=causal)
+        assert float(dq.abs().max()) == 0.0 and float(dk.abs().max()) == 0.0 and float(dv.abs().max()) > 0.0
+
+
+@dtypes
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_attention_few_keys(ctx, dtype, dim):
+    """Sequences of two to four rows, where dS is a small difference: two
+    roundings (of dS and of the result), each at most u and u / sqrt(3) in the
+    mean over many elements, and nothing of the roundings of the saved results."""
+    n = [2, 3, 4] * 30
+    c = attention_case(dim + 1, dtype, n, n, 4, 4, dim)
+    dev = [c[t].cuda() for t in ("q", "k", "v", "lam")]
+    seqs = ops.Sequences(ctx, c["q_off"], c["k_off"])
+    out, saved = ops.diff_attention(ctx, *dev, seqs, save=True)
+    grads = ops.diff_attention_backward(ctx, c["dout"].cuda(), *dev, seqs, out, saved)
+    r = OO.attention(*(c[t].double() for t in ("q", "k", "v", "lam")), dim ** -0.5, c["q_off"], c["k_off"], dout=c["dout"].double())
+    for got, name in zip(grads, ("dq", "dk")):
+        off = float((got.double().cpu() - r[name]).norm() / r[name].norm())
+        assert off < math.sqrt(2 / 3) * OO.UNIT[dtype] * 1.1 + OO.F32 * (16 + 4 * dim + 4 * r["scores"])
+
+
+@dtypes
 def test_attention_large_scores(ctx, dtype):
     """Scores of several hundred: one key takes a row, exponentials of the others vanish."""
     c = attention_case(3, dtype, [100], [100], 2, 2, 32)
