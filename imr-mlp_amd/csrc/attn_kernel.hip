@@ -6,8 +6,8 @@
 //   attn_forward_kernel   out, and lse and P_1 V for the backward pass
 //   attn_dq_kernel        dq, and per row D_m = sum_j P_m dP (for the next)
 //   attn_dkv_kernel       dk, dv; the group of query heads that share them
-//                         is summed in registers
-//   dlambda_kernel        sums the partials of dlambda in a fixed order
+//                         is summed in registers; dlambda from its shares
+//   dlambda_kernel        the same where there are no keys
 //   attn_cache_kernel     one row per sequence, keys split over workgroups
 //   attn_cache_join       joins their partial results
 //
@@ -561,6 +561,34 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     }
 }
 
+// dlambda of one head from the query tiles' shares, by one workgroup.
+template <int THREADS>
+__device__ inline void sum_shares(const float *part, int n, float *dlambda, float *red, int tid)
+{
+    float v = 0.f;
+    for (int i = tid; i < n; i += THREADS)
+        v += part[i];
+    v = wave_sum(v);
+    __syncthreads();
+    if (tid % kWave == 0)
+        red[tid / kWave] = v;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < THREADS / kWave; ++w)
+            v += red[w];
+        *dlambda = v;
+    }
+}
+
+#if MTPX_OPS_TYPE == 0
+// The same where no key pass runs (its first workgroups do it otherwise).
+__global__ __launch_bounds__(kThreads) void dlambda_kernel(const float *part, float *dlambda, int n)
+{
+    __shared__ float red[kWaves];
+    sum_shares<kThreads>(part + (int64_t)blockIdx.x * n, n, dlambda + blockIdx.x, red, threadIdx.x);
+}
+#endif
+
 // Gradient of the keys and values.  A workgroup takes W * KT * 8 keys of one
 // key head; the rows' q, dO and statistics come in tiles of QB rows through
 // LDS.  S and dP come out with a key per lane column: P = P_0 - lambda P_1 and
@@ -574,7 +602,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
 // heads that share the key head follow one another, so their sum stays in
 // registers.  What bounds it now are the waits at its two barriers a tile.
 template <class T, int D, int W, int KT, int QB, int BUF, int OCC>
-__global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, int table, int ntiles)
+__global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, int table, int ntiles, int shares)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = QB * TL::kRowBytes;
@@ -792,6 +820,12 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
         onward(head, q0);
     }
 
+    // the last tile has the least work: it sums its heads' shares of dlambda
+    if (wk.tile == ntiles - 1)
+        for (int h = kv * group; h < (kv + 1) * group; ++h)
+            sum_shares<W * kWave>(a.dlam_part + (int64_t)h * shares, shares, a.dlambda + h,
+                                  reinterpret_cast<float *>(smem), tid);
+
     const mtpx_rows &to = half ? a.dk : a.dv;
     const float factor = half ? a.scale : 1.f;
 #pragma unroll
@@ -809,27 +843,6 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
             store_columns<T, D>(p, to.map, a.dim, i, lane, some ? acc[t][i] * factor : none, a.vec);
     }
 }
-
-#if MTPX_OPS_TYPE == 0
-// Sums the query tiles' shares of dlambda, one workgroup per head.
-__global__ __launch_bounds__(kThreads) void dlambda_kernel(const float *part, float *dlambda, int n)
-{
-    __shared__ float red[kThreads];
-    const int tid = threadIdx.x;
-    float v = 0.f;
-    for (int i = tid; i < n; i += kThreads)
-        v += part[(int64_t)blockIdx.x * n + i];
-    red[tid] = v;
-    __syncthreads();
-    for (int o = kThreads / 2; o > 0; o >>= 1) {
-        if (tid < o)
-            red[tid] += red[tid + o];
-        __syncthreads();
-    }
-    if (tid == 0)
-        dlambda[blockIdx.x] = red[0];
-}
-#endif
 
 // One query row per sequence.  A workgroup takes one key head of one sequence
 // and one of `splits` runs of its keys, for up to 16 of the query heads that
@@ -1166,7 +1179,7 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
     if (nk > 0) {
         attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kKeyRows, S::kKeyBuffers, S::kKeyOccupancy>
             <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave), S::kKeyLds, s>>>(
-                a, kNarrow, nk);
+                a, kNarrow, nk, a.tiles.nq[query_table<D>(a.tiles, a.heads)]);
     }
     return hipGetLastError();
 }
@@ -1243,7 +1256,7 @@ hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s)
 {
     const hipError_t e = dtype == MTPX_F32 ? attn_backward_f32(a, s)
                          : dtype == MTPX_BF16 ? attn_backward_bf16(a, s) : attn_backward_f16(a, s);
-    if (e != hipSuccess)
+    if (e != hipSuccess || a.tiles.nk[kNarrow] > 0)
         return e;
     dlambda_kernel<<<dim3(a.heads), dim3(kThreads), 0, s>>>(a.dlam_part, a.dlambda,
                                                             attn_backward_tiles(dtype, a.dim, a.heads, a.tiles));
