@@ -97,7 +97,8 @@ def _packer(cls):
     return s.pack
 
 
-_pack_rotary, _pack_cache, _pack_norm = (_packer(c) for c in (RotaryRequest, CacheRequest, NormRequest))
+_pack_rotary, _pack_attention, _pack_cache, _pack_norm = (
+    _packer(c) for c in (RotaryRequest, AttentionRequest, CacheRequest, NormRequest))
 
 _lib = None
 
@@ -150,12 +151,6 @@ def _strides(ctx, t, name, shape, dtype):
     return s
 
 
-def _inner(t, name):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        _fail("the last dimension of %s is not contiguous" % name)
-    return t
-
-
 def _typed(ctx, t, name, dims):
     """The type code of a tensor of so many dimensions on the context's device."""
     if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
@@ -176,20 +171,12 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _maps(t):
-    """[rows][heads][2][dim]"""
-    return Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
-
-
-def _wide(t):
-    """[rows][heads][2 dim] as two maps side by side"""
-    return Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[2] // 2)
-
-
 def _bytes(ctx, query, request, **sizes):
     """Workspace that a call of these sizes needs: asked for once per context."""
     key = (request, *sizes.values())
     if key not in ctx.workspaces:
+        if len(ctx.workspaces) > 1000:
+            ctx.workspaces.clear()
         n = C.c_size_t()
         ctx._check(query(ctx.h, C.byref(request(**sizes)), C.byref(n)), "workspace")
         ctx.workspaces[key] = n.value
@@ -280,28 +267,38 @@ class Sequences:
         self.close()
 
 
-def _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask):
-    dtype = _typed(ctx, q, "q", 4)
-    heads, dim = _tensor(ctx, q, "q", (None, None, 2, None)).shape[1::2]
-    kv = _tensor(ctx, k, "k", (None, None, 2, dim), q.dtype).shape[1]
-    _tensor(ctx, v, "v", (k.shape[0], kv, 2 * dim), q.dtype)
+_NO_ROWS = (0, 0, 0, 0)
+
+
+def _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask, out=_NO_ROWS, out1=0, lse=0,
+               dout=_NO_ROWS, dq=_NO_ROWS, dk=_NO_ROWS, dv=_NO_ROWS, dlam=0):
+    """The checked request of either pass; results as (address, row, head and
+    map stride) or addresses."""
+    dtype, of = _typed(ctx, q, "q", 4), q.dtype
+    rows, heads, _, dim = q.shape
+    sq = _strides(ctx, q, "q", (rows, heads, 2, dim), of)
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        _fail("k is not [key rows, kv heads, 2, dim]")
+    keys, kv, _, _ = k.shape
+    sk = _strides(ctx, k, "k", (keys, kv, 2, dim), of)
+    sv = _strides(ctx, v, "v", (keys, kv, 2 * dim), of)
     if seqs.h is None:
         _fail("the sequences are closed")
-    if q.shape[0] != seqs.q_rows or k.shape[0] != seqs.k_rows:
+    if rows != seqs.q_rows or keys != seqs.k_rows:
         _fail("q and k have %d and %d rows, the sequences %d and %d" %
-              (q.shape[0], k.shape[0], seqs.q_rows, seqs.k_rows))
-    _tensor(ctx, lam, "lam", (heads,), torch.float32)
-    if not lam.is_contiguous():
-        _fail("lam must be contiguous")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _inner(t, name)
+              (rows, keys, seqs.q_rows, seqs.k_rows))
+    _strides(ctx, lam, "lam", (heads,), torch.float32)
+    mask = 0
     if key_mask is not None:
-        _tensor(ctx, key_mask, "key_mask", (k.shape[0],))
+        _tensor(ctx, key_mask, "key_mask", (keys,))
         if key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous():
             _fail("key_mask must be contiguous bool or uint8")
-    return AttentionRequest(_stream(ctx), dtype, seqs.h, heads, kv, dim, int(causal),
-                            dim ** -0.5 if scale is None else scale, _maps(q), _maps(k), _wide(v),
-                            None if key_mask is None else key_mask.data_ptr(), lam.data_ptr())
+        mask = key_mask.data_ptr()
+    return AttentionRequest.from_buffer_copy(_pack_attention(
+        _stream(ctx), dtype, getattr(seqs.h, "value", seqs.h), heads, kv, dim, causal,
+        dim ** -0.5 if scale is None else scale, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(),
+        sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], dim, mask, lam.data_ptr(), *out, out1,
+        lse, *dout, *dq, *dk, *dv, dlam, 0, 0))
 
 
 def diff_attention(ctx, q, k, v, lam, seqs, *, causal=False, scale=None, key_mask=None,
@@ -311,19 +308,19 @@ def diff_attention(ctx, q, k, v, lam, seqs, *, causal=False, scale=None, key_mas
     rows, kv heads, 2 dim], lam [heads] float32; scale defaults to dim^-1/2.
     Returns out [rows, heads, 2 dim], with save (out, saved) for
     diff_attention_backward."""
-    req = _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask)
+    _typed(ctx, q, "q", 4)
     rows, heads, _, dim = q.shape
+    shape = (rows, heads, 2 * dim)
     if out is None:
-        out = torch.empty((rows, heads, 2 * dim), dtype=q.dtype, device=q.device)
+        out, so = q.new_empty(shape), (heads * 2 * dim, 2 * dim)
     else:
-        _inner(_tensor(ctx, out, "out", (rows, heads, 2 * dim), q.dtype), "out")
-    req.out = _wide(out)
+        so = _strides(ctx, out, "out", shape, q.dtype)
     saved = None
     if save:
-        saved = (torch.empty((rows, heads, 2 * dim), dtype=q.dtype, device=q.device),
-                 torch.empty((2, heads, rows), dtype=torch.float32, device=q.device))
-        req.out1, req.lse = saved[0].data_ptr(), saved[1].data_ptr()
-    ctx._check(_ops().mtpx_diff_attention(ctx.h, C.byref(req)), "diff_attention")
+        saved = q.new_empty(shape), q.new_empty((2, heads, rows), dtype=torch.float32)
+    req = _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask,
+                     (out.data_ptr(), so[0], so[1], dim), *(s.data_ptr() for s in saved or ()))
+    ctx._check(_ops().mtpx_diff_attention(ctx.h, req), "diff_attention")
     return (out, saved) if save else out
 
 
@@ -331,26 +328,31 @@ def diff_attention_backward(ctx, dout, q, k, v, lam, seqs, out, saved, *, causal
                             scale=None, key_mask=None):
     """(dq, dk, dv, dlam) from the gradient of out and what the forward call
     returned and saved."""
-    req = _attention(ctx, q, k, v, lam, seqs, causal, scale, key_mask)
+    _typed(ctx, q, "q", 4)
     rows, heads, _, dim = q.shape
-    shape = (rows, heads, 2 * dim)
-    _inner(_tensor(ctx, dout, "dout", shape, q.dtype), "dout")
-    _inner(_tensor(ctx, out, "out", shape, q.dtype), "out")
+    shape, of = (rows, heads, 2 * dim), q.dtype
+    sd = _strides(ctx, dout, "dout", shape, of)
+    so = _strides(ctx, out, "out", shape, of)
     out1, lse = saved
-    _tensor(ctx, out1, "saved[0]", shape, q.dtype)
-    _tensor(ctx, lse, "saved[1]", (2, heads, rows), torch.float32)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=q.device)
-    dv = torch.empty(v.shape, dtype=v.dtype, device=q.device)
-    dlam = torch.empty(heads, dtype=torch.float32, device=q.device)
-    req.out, req.dout, req.out1, req.lse = _wide(out), _wide(dout), out1.data_ptr(), lse.data_ptr()
-    req.dq, req.dk, req.dv, req.dlambda = _maps(dq), _maps(dk), _wide(dv), dlam.data_ptr()
+    for t, name, s, kind in ((out1, "saved[0]", shape, of),
+                             (lse, "saved[1]", (2, heads, rows), torch.float32)):
+        _strides(ctx, t, name, s, kind)
+        if not t.is_contiguous():
+            _fail("%s must be contiguous" % name)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dlam = q.new_empty(heads, dtype=torch.float32)
+    kv = k.shape[1]
+    req = _attention(
+        ctx, q, k, v, lam, seqs, causal, scale, key_mask, (out.data_ptr(), so[0], so[1], dim),
+        out1.data_ptr(), lse.data_ptr(), (dout.data_ptr(), sd[0], sd[1], dim),
+        (dq.data_ptr(), heads * 2 * dim, 2 * dim, dim), (dk.data_ptr(), kv * 2 * dim, 2 * dim, dim),
+        (dv.data_ptr(), kv * 2 * dim, 2 * dim, dim), dlam.data_ptr())
     n = C.c_size_t()
-    ctx._check(_ops().mtpx_diff_attention_workspace(ctx.h, C.byref(req), C.byref(n)), "workspace")
+    ctx._check(_ops().mtpx_diff_attention_workspace(ctx.h, req, C.byref(n)), "workspace")
     req.workspace_bytes = n.value
-    w = _workspace(ctx, req.workspace_bytes)  # held until the kernels are queued
+    w = _workspace(ctx, n.value)  # held until the kernels are queued
     req.workspace = w.data_ptr()
-    ctx._check(_ops().mtpx_diff_attention_backward(ctx.h, C.byref(req)), "diff_attention_backward")
+    ctx._check(_ops().mtpx_diff_attention_backward(ctx.h, req), "diff_attention_backward")
     return dq, dk, dv, dlam
 
 

@@ -497,9 +497,11 @@ def test_refusals(ctx):
     L = ops._ops()
     out, saved = ops.diff_attention(ctx, q, q, v, lam, seqs, save=True)
     req = ops._attention(ctx, q, q, v, lam, seqs, False, None, None)
-    req.out, req.dout = ops._wide(out), ops._wide(out)
+    wide = lambda t: ops.Rows(t.data_ptr(), t.stride(0), t.stride(1), 8)  # noqa: E731
+    maps = lambda t: ops.Rows(t.data_ptr(), *t.stride()[:3])  # noqa: E731
+    req.out, req.dout = wide(out), wide(out)
     req.out1, req.lse, req.dlambda = saved[0].data_ptr(), saved[1].data_ptr(), lam.data_ptr()
-    req.dq, req.dk, req.dv = ops._maps(q), ops._maps(q), ops._wide(v)
+    req.dq, req.dk, req.dv = maps(q), maps(q), wide(v)
     req.workspace, req.workspace_bytes = out.data_ptr(), 8
     assert L.mtpx_diff_attention_backward(ctx.h, req) == -1
     req.workspace = None
