@@ -7,7 +7,8 @@
 //   attn_dq_kernel        dq, and per row D_m = sum_j P_m dP (for the next)
 //   attn_dkv_kernel       dk, dv; the group of query heads that share them
 //                         is summed in registers; dlambda from its shares
-//   dlambda_kernel        the same where there are no keys
+//   attn_dkv_join         sums its parts where few keys leave the device idle
+//   dlambda_kernel        dlambda where there are no keys
 //   attn_cache_kernel     one row per sequence, keys split over workgroups
 //   attn_cache_join       joins their partial results
 //
@@ -614,9 +615,10 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
     // what one wave of a pair hands to the other: [3][U][KT][lane]
     constexpr int U = QB / 32;
     Half<T> *given = reinterpret_cast<Half<T> *>(stats + BUF * 4 * QB) + pair * (3 * U * KT * kWave) + lane;
-    const Work wk = work_item(blockIdx.x, ntiles, a.kv_heads);
+    const Work wk = work_item(blockIdx.x, ntiles * a.kv_parts, a.kv_heads);
     const int kv = wk.head, group = a.heads / a.kv_heads;
-    const SeqTile sq = a.tiles.k[table][wk.tile];
+    const int tile_id = wk.tile / a.kv_parts, part = wk.tile % a.kv_parts;
+    const SeqTile sq = a.tiles.k[table][tile_id];
     const int shift = sq.nk - sq.nq;
     const float c = a.scale * kLog2e;
     Reader<T, D> rd;
@@ -653,14 +655,17 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
     // rows before the first that sees a key of this workgroup are left out
     const int first = a.causal ? max(0, sq.start - shift) / QB * QB : 0;
     const int per = sq.nq > first ? (sq.nq - first + QB - 1) / QB : 0;
-    const int steps = per * group;
+    // of the walk over the rows of all its heads, this workgroup's part
+    const int step0 = (int)((int64_t)per * group * part / a.kv_parts);
+    const int steps = (int)((int64_t)per * group * (part + 1) / a.kv_parts) - step0;
+    const int head0 = kv * group + (steps ? step0 / per : 0), skip = (steps ? step0 % per : 0) * QB;
     Loader<T, D, QB, W> lq, ld;
     lq.init((const T *)a.q.data + sq.q0 * a.q.row, a.q, a.dim, a.vec, tid);
     ld.init((const T *)a.dout.data + sq.q0 * a.dout.row, a.dout, a.dim, a.vec, tid);
-    lq.move(kv * group * a.q.head + first * a.q.row);
-    ld.move(kv * group * a.dout.head + first * a.dout.row);
+    lq.move(head0 * a.q.head + (first + skip) * a.q.row);
+    ld.move(head0 * a.dout.head + (first + skip) * a.dout.row);
     // The tiles go round the rows once per query head.
-    int to_head = kv * group, to_q0 = first, head = to_head, q0 = first;
+    int to_head = head0, to_q0 = first + skip, head = to_head, q0 = to_q0;
     auto onward = [&](int &h, int &q) {
         q += QB;
         if (q >= sq.nq) {
@@ -821,7 +826,7 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
     }
 
     // the last tile has the least work: it sums its heads' shares of dlambda
-    if (wk.tile == ntiles - 1)
+    if (tile_id == ntiles - 1 && part == a.kv_parts - 1)
         for (int h = kv * group; h < (kv + 1) * group; ++h)
             sum_shares<W * kWave>(a.dlam_part + (int64_t)h * shares, shares, a.dlambda + h,
                                   reinterpret_cast<float *>(smem), tid);
@@ -834,14 +839,38 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_dkv_kernel(AttnArgs a, in
         if (key >= sq.nk)
             continue;
         T *p = (T *)to.data + kv * to.head + (sq.k0 + key) * to.row;
+        float *sums = a.kv_part + ((((int64_t)part * a.kv_heads + kv) * a.total_k + sq.k0 + key) * 2 + half) * 2 * a.dim;
         // a masked key's gradients are 0, whatever its column holds, and a
         // single key's score has none
         const f32x4 none = {0, 0, 0, 0};
         const bool some = live[t] && !(half && sq.nk == 1);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
-            store_columns<T, D>(p, to.map, a.dim, i, lane, some ? acc[t][i] * factor : none, a.vec);
+            if (a.kv_parts == 1)
+                store_columns<T, D>(p, to.map, a.dim, i, lane, some ? acc[t][i] * factor : none, a.vec);
+            else
+                store_columns<float, D>(sums, a.dim, a.dim, i, lane, some ? acc[t][i] * factor : none,
+                                        a.dim % 4 == 0);
     }
+}
+
+// Sums the parts of the key pass, in their order, and rounds them once.
+template <class T>
+__global__ __launch_bounds__(kThreads) void attn_dkv_join(AttnArgs a)
+{
+    const int width = 4 * a.dim;
+    const int64_t each = (int64_t)a.kv_heads * a.total_k * width;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= each)
+        return;
+    float v = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < a.kv_parts; ++p)
+        v += a.kv_part[p * each + i];
+    const int e = (int)(i % width), m = e / a.dim % 2, c = e % a.dim;
+    const int64_t key = i / width % a.total_k, kv = i / width / a.total_k;
+    const mtpx_rows &to = e >= 2 * a.dim ? a.dk : a.dv;
+    ((T *)to.data)[kv * to.head + key * to.row + m * to.map + c] = (T)v;
 }
 
 // One query row per sequence.  A workgroup takes one key head of one sequence
@@ -1178,8 +1207,14 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
     const int nk = a.tiles.nk[kNarrow];
     if (nk > 0) {
         attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kKeyRows, S::kKeyBuffers, S::kKeyOccupancy>
-            <<<dim3((unsigned)((int64_t)nk * a.kv_heads)), dim3(S::kKeyWaves * kWave), S::kKeyLds, s>>>(
-                a, kNarrow, nk, a.tiles.nq[query_table<D>(a.tiles, a.heads)]);
+            <<<dim3((unsigned)((int64_t)nk * a.kv_heads * a.kv_parts)), dim3(S::kKeyWaves * kWave), S::kKeyLds,
+               s>>>(a, kNarrow, nk, a.tiles.nq[query_table<D>(a.tiles, a.heads)]);
+        if (a.kv_parts > 1) {
+            if (hipError_t e = hipGetLastError())
+                return e;
+            const int64_t n = a.kv_heads * a.total_k * 4 * a.dim;
+            attn_dkv_join<Type><<<dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s>>>(a);
+        }
     }
     return hipGetLastError();
 }

@@ -23,13 +23,13 @@ constexpr int kTileRows[2] = {64, 128};
 struct TileTable {
     const SeqTile *q[2], *k[2];  // by kTileRows
     int nq[2], nk[2];
-    int longest_k;  // most keys of a sequence
+    int longest_q, longest_k;  // most rows and keys of a sequence
 };
 
 struct AttnArgs {
     TileTable tiles;
     int heads, kv_heads, dim, causal;
-    int64_t total_q;
+    int64_t total_q, total_k;
     float scale;
     mtpx_rows q, k, v, out, dout, dq, dk, dv;
     const unsigned char *mask;
@@ -37,6 +37,10 @@ struct AttnArgs {
     void *out1;
     float *lse, *delta, *dlam_part, *dlambda;
     int vec;  // every row is a whole number of 16-byte pieces at a 16-byte address
+    // the key pass's walk over the rows in so many parts, each with its sums in
+    // kv_part [part][kv head][key][dv, dk: 4 dim] (one part: none)
+    int kv_parts;
+    float *kv_part;
 };
 
 constexpr int kMaxSplits = 128;  // of one sequence's cache

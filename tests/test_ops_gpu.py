@@ -195,6 +195,17 @@ def test_attention_single_keys(ctx, dtype, heads, kv, dim):
 
 
 @dtypes
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len,k_len,heads,kv,dim", [([700], [90], 4, 1, 32), ([530, 0, 70], [530, 3, 70], 2, 2, 64),
+                                                      ([257, 400], [300, 1], 6, 2, 128), ([600], [600], 3, 1, 5),
+                                                      ([900], [40], 1, 1, 50)])
+def test_attention_shared_key_pass(ctx, dtype, causal, q_len, k_len, heads, kv, dim):
+    """Few keys and many rows: several workgroups share a tile of keys, some
+    of which have no row that sees it."""
+    check_attention(ctx, attention_case(dim, dtype, q_len, k_len, heads, kv, dim, masked=0.2), causal)
+
+
+@dtypes
 @pytest.mark.parametrize("dim", [32, 64, 128])
 def test_attention_few_keys(ctx, dtype, dim):
     """Sequences of two to four rows, where dS is a small difference: two
