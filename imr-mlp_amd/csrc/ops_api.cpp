@@ -181,15 +181,20 @@ int attn_args(mtpx_context *ctx, const mtpx_diff_attention_request &r, bool back
     return MTPX_OK;
 }
 
-// Workgroups that share one sequence's keys: one where its eight waves have no
-// more than four steps of 32 keys each (a second launch costs as much), else
-// enough to fill the device, each with a step per wave at least.
+// Workgroups that share one sequence's keys: one where its waves (eight, or as
+// many as their tiles of V leave room for) have no more than four steps of 32
+// keys each, as a second launch costs as much, or not many more and every CU
+// has two workgroups (200 caches of 1,000 rows of 8 heads, 128 wide, in 16
+// bits: 295 us so, 349 us in two splits); else enough to fill the device, each
+// with a step per wave at least (2 caches of 946 rows of 8 heads, 40 wide, in
+// 32 bits: 18 us, 59 us in one).
 int cache_splits(mtpx_context *ctx, const mtpx_diff_attention_cache_request &r)
 {
-    if (r.capacity <= 8 * 4 * 32)
-        return 1;
-    const int group = r.heads / r.kv_heads;
+    const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128, group = r.heads / r.kv_heads;
     const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * ((group + 15) / 16), 1);
+    const int waves = std::min(8, 1024 / (width * (r.dtype == MTPX_F32 ? 4 : 2)));
+    if (r.capacity <= (base >= 2 * (int64_t)ctx->num_cus ? 8 : waves) * 4 * 32)
+        return 1;
     const int64_t most = (r.capacity + 127) / 128;
     const int64_t want = (8 * (int64_t)ctx->num_cus + base - 1) / base;
     return (int)std::min<int64_t>({want, most, (int64_t)kMaxSplits});
