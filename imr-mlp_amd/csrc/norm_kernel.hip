@@ -427,7 +427,7 @@ hipError_t run(const NormArgs &a, bool back, hipStream_t s)
     using R = Row<T, NT, E, V>;
     // the forward pass: what its registers let in at once, four waves per SIMD
     const int64_t need = (a.rows + R::kPerBlock - 1) / R::kPerBlock;
-    const int64_t most = 256 * 16 * kWave / R::kBlock;
+    const int64_t most = 256 * (16 * kWave / R::kBlock);
     const dim3 grid((unsigned)(back ? a.parts : need < most ? need : most)), block(R::kBlock);
     if (back)
         norm_backward_kernel<T, NT, E, V><<<grid, block, 0, s>>>(a);
@@ -437,14 +437,17 @@ hipError_t run(const NormArgs &a, bool back, hipStream_t s)
 }
 
 // The fewest threads that hold a row with 8 elements each (16 beyond 8,192
-// columns), a power of two from 16 on: more elements leave the backward pass fewer waves per SIMD to
-// hide its reads (160,000 rows of 1,024: 611 us with 16 elements a thread).
+// columns), a power of two from 16 on or, of whole waves, 3/4 of one (forward
+// and backward of 51,198 rows of 2,352 columns in 16 bits: 887 us with 512
+// threads, 740 us with 384).  More elements leave the backward pass fewer waves
+// per SIMD to hide its reads (160,000 rows of 1,024: 611 us with 16 elements a
+// thread).
 int row_threads(int width)
 {
     int n = 16;
     while (n < kMaxBlock && width > 8 * n)
         n *= 2;
-    return n;
+    return n > 2 * kWave && width <= 6 * n ? n / 4 * 3 : n;
 }
 template <class T, int V>
 hipError_t by_width(const NormArgs &a, bool back, hipStream_t s)
@@ -454,8 +457,11 @@ hipError_t by_width(const NormArgs &a, bool back, hipStream_t s)
     case 32: return run<T, 32, 8, V>(a, back, s);
     case 64: return run<T, 64, 8, V>(a, back, s);
     case 128: return run<T, 128, 8, V>(a, back, s);
+    case 192: return run<T, 192, 8, V>(a, back, s);
     case 256: return run<T, 256, 8, V>(a, back, s);
+    case 384: return run<T, 384, 8, V>(a, back, s);
     case 512: return run<T, 512, 8, V>(a, back, s);
+    case 768: return run<T, 768, 8, V>(a, back, s);
     default: return a.width <= 8192 ? run<T, 1024, 8, V>(a, back, s) : run<T, 1024, 16, V>(a, back, s);
     }
 }

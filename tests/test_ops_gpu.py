@@ -361,6 +361,16 @@ def test_norm_block(ctx, dtype, kind, act, rows, width, gated):
     assert none is None and torch.equal(only_s, s)
 
 
+@dtypes
+@pytest.mark.parametrize("kind,act", [("rms", "sigmoid"), ("layer", "tanh")])
+@pytest.mark.parametrize("rows,width,gated", [(1100, 1024 + 8, 1), (3, 1536, 2), (3, 1537, 1), (600, 2353, 2),
+                                              (300, 4104, 1), (2, 6144, 0), (270, 6145, 2), (2, 8193, 1)])
+def test_norm_block_thread_counts(ctx, dtype, kind, act, rows, width, gated):
+    """Rows held by numbers of threads that are not powers of two, and the
+    widths beside them; several rows a workgroup."""
+    test_norm_block(ctx, dtype, kind, act, rows, width, gated)
+
+
 def test_norm_block_autograd_without_a_gradient_of_n(ctx):
     g = torch.Generator().manual_seed(2)
     x, y, gate, w1, w2 = (rand(g, *shape, dtype=torch.float32).cuda().requires_grad_(True)
