@@ -485,13 +485,13 @@ hipError_t by_type(int dtype, const NormArgs &a, bool back, hipStream_t s)
 }  // namespace
 
 // Workgroups of the backward pass: as many as the chip holds at once (three
-// waves per SIMD by their registers), so that a weight gradient takes the
+// waves per SIMD by their registers, four of the largest workgroup), so that a weight gradient takes the
 // fewest partial rows; rows of one wave and less share a workgroup.
 int norm_backward_parts(int64_t rows, int width)
 {
     const int n = row_threads(width);
     const int block = n <= kWave ? 256 : n, together = block / n;
-    const int64_t need = (rows + together - 1) / together, most = 256 * 12 * kWave / block;
+    const int64_t need = (rows + together - 1) / together, most = 256 * std::max(12 * kWave / block, 1);
     return (int)(need < most ? need : most);
 }
 hipError_t launch_norm_forward(int dtype, const NormArgs &a, hipStream_t s)
