@@ -8,6 +8,8 @@ stream of the tensors' device and returns without waiting; workspaces and
 results come from torch's allocator, so a call can be captured into a graph.
 Functions with gradients come twice: as a pair (f, f_backward) on plain
 tensors, and as an autograd function (RotaryFn, DiffAttentionFn, NormBlockFn).
+Gradients are first derivatives: differentiating one of them again (a loss of
+forces that were taken through a block) raises.
 Tensors are float32, bfloat16 or float16; their last dimension has to be
 contiguous, other strides are free.  There is no fallback: a missing library
 or a refused argument raises.  torch and the library share one HIP runtime if
@@ -17,6 +19,7 @@ order is refused.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 import sys
 
@@ -475,6 +478,40 @@ def _last_contiguous(t):
     return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+class _Refused(torch.autograd.Function):
+    """Hands gradients on; refuses to be differentiated."""
+
+    @staticmethod
+    def forward(fn, grads, *inputs):
+        fn.set_materialize_grads(False)
+        return tuple(g.detach() for g in grads)
+
+    @staticmethod
+    def backward(fn, *unused):
+        _fail("a second derivative of an operator on device tensors, which has first ones only")
+
+
+def _first_only(backward):
+    """The kernels' gradients carry no graph.  Where autograd keeps one
+    (create_graph), it would take them for constants, and a loss of them, as of
+    forces, would lose its share of every other gradient without a word: they
+    are tied to all that they depend on by a node that raises.  (torch's
+    once_differentiable does so only if an incoming gradient has a graph.)"""
+    @functools.wraps(backward)
+    def once(fn, *grads):
+        with torch.no_grad():
+            out = backward(fn, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        inputs = [t for t in (*grads, *fn.saved_tensors) if t is not None and t.requires_grad]
+        if not inputs:
+            return out
+        tied = iter(_Refused.apply([t for t in out if t is not None], *inputs))
+        return tuple(t if t is None else next(tied) for t in out)
+
+    return once
+
+
 class RotaryFn(torch.autograd.Function):
     """RotaryFn.apply(ctx, x, positions, freq, axis, interleaved): rotary with
     the gradients of x and of floating-point positions."""
@@ -487,6 +524,7 @@ class RotaryFn(torch.autograd.Function):
         return rotary(ctx, x, positions, freq, axis, interleaved=interleaved)
 
     @staticmethod
+    @_first_only
     def backward(fn, dy):
         x, positions, freq, axis = fn.saved_tensors
         dx, dpos = rotary_backward(fn.ctx, _last_contiguous(dy), positions, freq, axis,
@@ -506,6 +544,7 @@ class DiffAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_only
     def backward(fn, dout):
         q, k, v, lam, out, out1, lse, mask = fn.saved_tensors
         grads = diff_attention_backward(fn.ctx, _last_contiguous(dout), q, k, v, lam, fn.seqs,
@@ -527,6 +566,7 @@ class NormBlockFn(torch.autograd.Function):
         return s, n
 
     @staticmethod
+    @_first_only
     def backward(fn, ds, dn):
         x, y, gate, post_weight, pre_weight, stats = fn.saved_tensors
         grads = norm_block_backward(fn.ctx, _last_contiguous(ds), _last_contiguous(dn), x, y,
