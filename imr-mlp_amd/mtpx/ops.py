@@ -491,6 +491,12 @@ class _Refused(torch.autograd.Function):
         _fail("a second derivative of an operator on device tensors, which has first ones only")
 
 
+def _learned(**values):
+    """The names of arguments without a gradient that are asked for one:
+    refused in the backward pass, as None in its place would say zero."""
+    return [n for n, t in values.items() if isinstance(t, torch.Tensor) and t.requires_grad]
+
+
 def _first_only(backward):
     """The kernels' gradients carry no graph.  Where autograd keeps one
     (create_graph), it would take them for constants, and a loss of them, as of
@@ -499,6 +505,8 @@ def _first_only(backward):
     once_differentiable does so only if an incoming gradient has a graph.)"""
     @functools.wraps(backward)
     def once(fn, *grads):
+        if fn.learned:
+            _fail("%s requires a gradient and has none" % " and ".join(fn.learned))
         with torch.no_grad():
             out = backward(fn, *grads)
         if not torch.is_grad_enabled():
@@ -514,11 +522,12 @@ def _first_only(backward):
 
 class RotaryFn(torch.autograd.Function):
     """RotaryFn.apply(ctx, x, positions, freq, axis, interleaved): rotary with
-    the gradients of x and of floating-point positions."""
+    the gradients of x and of floating-point positions.  freq has none: one
+    that requires it raises in the backward pass."""
 
     @staticmethod
     def forward(fn, ctx, x, positions, freq, axis, interleaved=False):
-        fn.ctx, fn.interleaved = ctx, interleaved
+        fn.ctx, fn.interleaved, fn.learned = ctx, interleaved, _learned(freq=freq)
         keep = x if positions.requires_grad else None
         fn.save_for_backward(keep, positions, freq, axis)
         return rotary(ctx, x, positions, freq, axis, interleaved=interleaved)
@@ -533,13 +542,15 @@ class RotaryFn(torch.autograd.Function):
 
 
 class DiffAttentionFn(torch.autograd.Function):
-    """DiffAttentionFn.apply(ctx, q, k, v, lam, seqs, causal, scale, key_mask)."""
+    """DiffAttentionFn.apply(ctx, q, k, v, lam, seqs, causal, scale, key_mask),
+    with the gradients of q, k, v and lam."""
 
     @staticmethod
     def forward(fn, ctx, q, k, v, lam, seqs, causal=False, scale=None, key_mask=None):
         out, saved = diff_attention(ctx, q, k, v, lam, seqs, causal=causal, scale=scale,
                                     key_mask=key_mask, save=True)
         fn.ctx, fn.seqs, fn.causal, fn.scale = ctx, seqs, causal, scale
+        fn.learned = _learned(scale=scale)
         fn.save_for_backward(q, k, v, lam, out, *saved, key_mask)
         return out
 
@@ -555,12 +566,14 @@ class DiffAttentionFn(torch.autograd.Function):
 
 class NormBlockFn(torch.autograd.Function):
     """NormBlockFn.apply(ctx, x, y, gate, post_weight, pre_weight, options):
-    (s, n) of norm_block with the keyword arguments in the dict options."""
+    (s, n) of norm_block with the keyword arguments in the dict options, which
+    have no gradients."""
 
     @staticmethod
     def forward(fn, ctx, x, y, gate, post_weight, pre_weight, options):
         s, n, stats = norm_block(ctx, x, y, gate, post_weight, pre_weight, save=True, **options)
         fn.ctx, fn.options = ctx, {k: v for k, v in options.items() if k != "next_norm"}
+        fn.learned = _learned(**options)
         fn.save_for_backward(x, y, gate, post_weight, pre_weight, stats)
         fn.set_materialize_grads(False)
         return s, n

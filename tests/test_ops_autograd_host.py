@@ -110,3 +110,33 @@ def test_a_kept_graph_without_second_derivatives_is_not(calls, block):
     other, = torch.autograd.grad(r.pow(3).sum(), r, create_graph=True)
     second, = torch.autograd.grad(other.sum() + 0.0 * got.detach().sum(), r)
     assert torch.allclose(second, 6 * r)
+
+
+def test_a_learned_frequency_is_refused(calls):
+    """freq has no gradient; without one asked for it may be a parameter."""
+    freq = torch.nn.Parameter(_rand(2))
+    x, positions = _rand(5, 3, 4).requires_grad_(True), _rand(5, 2)
+    y = ops.RotaryFn.apply(None, x, positions, freq, AXIS)
+    with pytest.raises(capi.MtpxError, match="freq"):
+        y.sum().backward()
+    with torch.no_grad():
+        ops.RotaryFn.apply(None, x, positions, freq, AXIS)
+
+
+@pytest.mark.parametrize("name", ["residual_scale", "block_scale", "eps"])
+def test_a_learned_scale_of_the_norms_is_refused(calls, name):
+    t = _rand(5, 4).requires_grad_(True)
+    learned = torch.nn.Parameter(torch.tensor(0.5))
+    s, _ = ops.NormBlockFn.apply(None, t, t, t[0], t[1], t[2], {name: learned})
+    with pytest.raises(capi.MtpxError, match=name):
+        s.sum().backward()
+    s, _ = ops.NormBlockFn.apply(None, t, t, t[0], t[1], t[2], {name: learned.detach()})
+    s.sum().backward()
+
+
+def test_a_learned_scale_of_the_scores_is_refused(calls):
+    q, v = _rand(3, 2, 2, 4).requires_grad_(True), _rand(3, 2, 4)
+    learned = torch.nn.Parameter(torch.tensor(0.5))
+    out = ops.DiffAttentionFn.apply(None, q, q, v, _rand(2), None, False, learned)
+    with pytest.raises(capi.MtpxError, match="scale"):
+        out.sum().backward()
