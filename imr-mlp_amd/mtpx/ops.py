@@ -177,13 +177,15 @@ def _ptr(t):
 def _bytes(ctx, query, request, **sizes):
     """Workspace that a call of these sizes needs: asked for once per context."""
     key = (request, *sizes.values())
-    if key not in ctx.workspaces:
-        if len(ctx.workspaces) > 1000:
-            ctx.workspaces.clear()
+    size = ctx.workspaces.get(key)
+    if size is None:
         n = C.c_size_t()
         ctx._check(query(ctx.h, C.byref(request(**sizes)), C.byref(n)), "workspace")
-        ctx.workspaces[key] = n.value
-    return ctx.workspaces[key]
+        size = n.value
+        if len(ctx.workspaces) > 1000:  # (another thread may be reading them)
+            ctx.workspaces.clear()
+        ctx.workspaces[key] = size
+    return size
 
 
 def _workspace(ctx, size):

@@ -1,6 +1,8 @@
 """The autograd functions of mtpx.ops over stand-ins for the library's calls:
 what autograd does with them needs no GPU.  The stand-ins compute the real
 formulas and return tensors without a graph, as the kernels do."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -140,3 +142,41 @@ def test_a_learned_scale_of_the_scores_is_refused(calls):
     out = ops.DiffAttentionFn.apply(None, q, q, v, _rand(2), None, False, learned)
     with pytest.raises(capi.MtpxError, match="scale"):
         out.sum().backward()
+
+
+class _EmptiedByOthers(dict):
+    """A dictionary that another thread empties after each call of this one."""
+
+    def __contains__(self, key):
+        found = dict.__contains__(self, key)
+        self.clear()
+        return found
+
+    def get(self, key, default=None):
+        value = dict.get(self, key, default)
+        self.clear()
+        return value
+
+    def __setitem__(self, key, value):
+        dict.__setitem__(self, key, value)
+        self.clear()
+
+
+@pytest.mark.parametrize("known", [False, True])
+def test_workspace_sizes_while_another_thread_empties_them(known):
+    """Autograd's backward pass is another thread on the same context."""
+    class Ctx:
+        h, workspaces = None, _EmptiedByOthers()
+
+        @staticmethod
+        def _check(rc, what):
+            assert rc == 0
+
+    def query(h, request, size):
+        C.cast(size, C.POINTER(C.c_size_t))[0] = 4096
+        return 0
+
+    sizes = dict(dtype=0, rows=3, width=8)
+    if known:
+        dict.__setitem__(Ctx.workspaces, (ops.NormRequest, *sizes.values()), 4096)
+    assert ops._bytes(Ctx, query, ops.NormRequest, **sizes) == 4096
