@@ -415,7 +415,9 @@ def _norm(ctx, x, y, gate, post_weight, pre_weight, kind, gate_act, residual_sca
         if not one:
             gate_row = sg[0]
             if gate_row == 0:
-                _fail("a gate shared by all rows is [width]")
+                if rows > 1:
+                    _fail("a gate shared by all rows is [width]")
+                gate_row = width  # one row's stride is any
     if post_weight is not None:
         _strides(ctx, post_weight, "post_weight", (width,), of)
     if pre_weight is not None:
