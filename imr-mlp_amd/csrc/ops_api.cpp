@@ -49,6 +49,27 @@ int check_flat(mtpx_context *ctx, const void *p, size_t align, const char *name)
     return MTPX_OK;
 }
 
+// The context's device while a call queues its work, then the caller's again:
+// these calls run inside programs that keep a current device of their own.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device)
+    {
+        int d = -1;
+        if (hipGetDevice(&d) == hipSuccess && d == device)
+            return;
+        before = d;
+        (void)hipSetDevice(device);
+    }
+    ~OnDevice()
+    {
+        if (before >= 0)
+            (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
 bool whole_pieces(const mtpx_rows &r, size_t size)
 {
     return aligned(r.data, 16) && r.row * size % 16 == 0 && r.head * size % 16 == 0 &&
@@ -371,7 +392,7 @@ int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *req)
     a.lanes = 64;
     while (a.lanes > 4 && a.lanes / 2 >= pieces && half * (128 / a.lanes) <= 512)
         a.lanes /= 2;
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_rotary(r.dtype, a, (hipStream_t)r.stream), "launch rotary");
     return MTPX_OK;
 }
@@ -425,7 +446,7 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                 count[2 * side + j] = t.size();
                 all.insert(all.end(), t.begin(), t.end());
             }
-        (void)hipSetDevice(ctx->device);
+        OnDevice here(ctx->device);
         hipError_t e = upload(sq->tiles, all, ctx->stream);
         if (e == hipSuccess)
             e = hipStreamSynchronize(ctx->stream);
@@ -455,7 +476,7 @@ void mtpx_sequences_destroy(mtpx_sequences *seqs)
 {
     if (!seqs)
         return;
-    (void)hipSetDevice(seqs->device);
+    OnDevice here(seqs->device);
     delete seqs;
 }
 
@@ -467,7 +488,7 @@ int mtpx_diff_attention(mtpx_context *ctx, const mtpx_diff_attention_request *re
     MTPX_TRY(attn_args(ctx, *req, false, a));
     if (a.total_q == 0)
         return MTPX_OK;
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_attn_forward(req->dtype, a, (hipStream_t)req->stream), "launch attention");
     return MTPX_OK;
 }
@@ -496,7 +517,7 @@ int mtpx_diff_attention_backward(mtpx_context *ctx, const mtpx_diff_attention_re
     a.dlam_part = a.delta + w.delta / sizeof(float);
     a.kv_parts = key_parts(ctx, *req);
     a.kv_part = a.dlam_part + w.part / sizeof(float);
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_attn_backward(req->dtype, a, (hipStream_t)req->stream), "launch attention gradient");
     return MTPX_OK;
 }
@@ -539,7 +560,7 @@ int mtpx_diff_attention_cache(mtpx_context *ctx, const mtpx_diff_attention_cache
     CacheArgs a{r.sequences, r.heads, r.kv_heads, r.dim, cache_splits(ctx, r), r.capacity,
                 r.k_sequence, r.v_sequence, r.scale, r.q, r.k, r.v, r.out, r.lengths, r.lambda,
                 static_cast<float *>(r.workspace), vec};
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_attn_cache(r.dtype, a, (hipStream_t)r.stream), "launch cache attention");
     return MTPX_OK;
 }
@@ -550,7 +571,7 @@ int mtpx_norm_block(mtpx_context *ctx, const mtpx_norm_block_request *req)
         return set_error(ctx, MTPX_E_INVALID, "null argument");
     NormArgs a;
     MTPX_TRY(norm_args(ctx, *req, false, a));
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_norm_forward(req->dtype, a, (hipStream_t)req->stream), "launch norm block");
     return MTPX_OK;
 }
@@ -572,7 +593,7 @@ int mtpx_norm_block_backward(mtpx_context *ctx, const mtpx_norm_block_request *r
     MTPX_TRY(norm_args(ctx, *req, true, a));
     MTPX_TRY(check_workspace(ctx, req->workspace, req->workspace_bytes, norm_bytes(*req)));
     a.part = static_cast<float *>(req->workspace);
-    (void)hipSetDevice(ctx->device);
+    OnDevice here(ctx->device);
     HIP_TRY(launch_norm_backward(req->dtype, a, (hipStream_t)req->stream), "launch norm block gradient");
     return MTPX_OK;
 }

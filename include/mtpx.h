@@ -595,6 +595,7 @@ int mtpx_last_linear_timings(const mtpx_context *ctx, double out[4]);
  * waiting: no host memory is read after the return, nothing is allocated
  * (scratch memory is the caller's workspace), so a call can be recorded into
  * a HIP graph.  A tensor used on another stream is the caller's to order.
+ * The caller's current device is the same after a call as before.
  * `stream` is a hipStream_t; NULL is the device's default stream, not the
  * context's own.
  *
