@@ -1172,9 +1172,8 @@ hipError_t forward_rows(const AttnArgs &a, int table, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[table];
-    attn_forward_kernel<Type, D, 4, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s>>>(a, table, n);
-    return hipGetLastError();
+    return launch_kernel(attn_forward_kernel<Type, D, 4, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy>,
+                         dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s, a, table, n);
 }
 template <int D>
 hipError_t forward(const AttnArgs &a, hipStream_t s)
@@ -1189,9 +1188,8 @@ hipError_t dq_rows(const AttnArgs &a, int table, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[table];
-    attn_dq_kernel<Type, D, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy, FEW>
-        <<<dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s>>>(a, table, n);
-    return hipGetLastError();
+    return launch_kernel(attn_dq_kernel<Type, D, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy, FEW>,
+                         dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s, a, table, n);
 }
 template <int D>
 hipError_t backward(const AttnArgs &a, hipStream_t s)
@@ -1205,18 +1203,16 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
             return e;
     }
     const int nk = a.tiles.nk[kNarrow];
-    if (nk > 0) {
-        attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kKeyRows, S::kKeyBuffers, S::kKeyOccupancy>
-            <<<dim3((unsigned)((int64_t)nk * a.kv_heads * a.kv_parts)), dim3(S::kKeyWaves * kWave), S::kKeyLds,
-               s>>>(a, kNarrow, nk, a.tiles.nq[query_table<D>(a.tiles, a.heads)]);
-        if (a.kv_parts > 1) {
-            if (hipError_t e = hipGetLastError())
-                return e;
-            const int64_t n = a.kv_heads * a.total_k * 4 * a.dim;
-            attn_dkv_join<Type><<<dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s>>>(a);
-        }
-    }
-    return hipGetLastError();
+    if (nk == 0)
+        return hipSuccess;
+    const hipError_t e = launch_kernel(
+        attn_dkv_kernel<Type, D, S::kKeyWaves, S::kKeyWide, S::kKeyRows, S::kKeyBuffers, S::kKeyOccupancy>,
+        dim3((unsigned)((int64_t)nk * a.kv_heads * a.kv_parts)), dim3(S::kKeyWaves * kWave), S::kKeyLds, s, a, kNarrow,
+        nk, a.tiles.nq[query_table<D>(a.tiles, a.heads)]);
+    if (e != hipSuccess || a.kv_parts == 1)
+        return e;
+    const int64_t n = a.kv_heads * a.total_k * 4 * a.dim;
+    return launch_kernel(attn_dkv_join<Type>, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a);
 }
 
 template <int D, int W>
@@ -1227,9 +1223,8 @@ hipError_t cache_waves(const CacheArgs &a, hipStream_t s)
     static_assert(tiles <= 65536, "what loads into LDS address");
     constexpr size_t join = ((size_t)W * 16 * (2 + 2 * D) + 16 * 2 * D) * sizeof(float);
     constexpr int occ = D * sizeof(Type) < 256 ? 2 : 1;
-    attn_cache_kernel<Type, D, W, occ><<<dim3(a.splits, a.kv_heads * ((group + 15) / 16), a.sequences),
-                                         dim3(W * kWave), tiles > join ? tiles : join, s>>>(a);
-    return hipGetLastError();
+    return launch_kernel(attn_cache_kernel<Type, D, W, occ>, dim3(a.splits, a.kv_heads * ((group + 15) / 16), a.sequences),
+                         dim3(W * kWave), tiles > join ? tiles : join, s, a);
 }
 // Eight waves where one workgroup takes a whole cache, four where splits
 // share it, fewer where their tiles would not fit.
@@ -1242,8 +1237,7 @@ hipError_t cache(const CacheArgs &a, hipStream_t s)
     const hipError_t e = cache_waves<D, most < 4 ? most : 4>(a, s);
     if (e != hipSuccess)
         return e;
-    attn_cache_join<Type, D><<<dim3(a.heads, a.sequences), dim3(4 * D), 0, s>>>(a);
-    return hipGetLastError();
+    return launch_kernel(attn_cache_join<Type, D>, dim3(a.heads, a.sequences), dim3(4 * D), 0, s, a);
 }
 
 }  // namespace
@@ -1293,9 +1287,8 @@ hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s)
                          : dtype == MTPX_BF16 ? attn_backward_bf16(a, s) : attn_backward_f16(a, s);
     if (e != hipSuccess || a.tiles.nk[kNarrow] > 0)
         return e;
-    dlambda_kernel<<<dim3(a.heads), dim3(kThreads), 0, s>>>(a.dlam_part, a.dlambda,
-                                                            attn_backward_tiles(dtype, a.dim, a.heads, a.tiles));
-    return hipGetLastError();
+    return launch_kernel(dlambda_kernel, dim3(a.heads), dim3(kThreads), 0, s, a.dlam_part, a.dlambda,
+                         attn_backward_tiles(dtype, a.dim, a.heads, a.tiles));
 }
 hipError_t launch_attn_cache(int dtype, const CacheArgs &a, hipStream_t s)
 {

@@ -429,11 +429,7 @@ hipError_t run(const NormArgs &a, bool back, hipStream_t s)
     const int64_t need = (a.rows + R::kPerBlock - 1) / R::kPerBlock;
     const int64_t most = 256 * (16 * kWave / R::kBlock);
     const dim3 grid((unsigned)(back ? a.parts : need < most ? need : most)), block(R::kBlock);
-    if (back)
-        norm_backward_kernel<T, NT, E, V><<<grid, block, 0, s>>>(a);
-    else
-        norm_forward_kernel<T, NT, E, V><<<grid, block, 0, s>>>(a);
-    return hipGetLastError();
+    return launch_kernel(back ? norm_backward_kernel<T, NT, E, V> : norm_forward_kernel<T, NT, E, V>, grid, block, 0, s, a);
 }
 
 // The fewest threads that hold a row with 8 elements each (16 beyond 8,192
@@ -472,8 +468,7 @@ hipError_t by_vec(const NormArgs &a, bool back, hipStream_t s)
     const hipError_t e = a.vec ? by_width<T, 16 / sizeof(T)>(a, back, s) : by_width<T, 1>(a, back, s);
     if (e != hipSuccess || !back || !(a.dpost || a.dpre || (a.dgate && a.gate_row == 0)))
         return e;
-    norm_parts_kernel<T><<<dim3((a.width + kWave - 1) / kWave, 3), dim3(kMaxBlock), 0, s>>>(a);
-    return hipGetLastError();
+    return launch_kernel(norm_parts_kernel<T>, dim3((a.width + kWave - 1) / kWave, 3), dim3(kMaxBlock), 0, s, a);
 }
 
 hipError_t by_type(int dtype, const NormArgs &a, bool back, hipStream_t s)
@@ -504,13 +499,10 @@ hipError_t launch_norm_backward(int dtype, const NormArgs &a, hipStream_t s)
     if (a.rows > 0)
         return by_type(dtype, a, true, s);
     const dim3 grid((a.width + kWave - 1) / kWave, 3), block(kMaxBlock);
-    if (dtype == MTPX_F32)
-        norm_parts_kernel<float><<<grid, block, 0, s>>>(a);
-    else if (dtype == MTPX_BF16)
-        norm_parts_kernel<__bf16><<<grid, block, 0, s>>>(a);
-    else
-        norm_parts_kernel<_Float16><<<grid, block, 0, s>>>(a);
-    return hipGetLastError();
+    return launch_kernel(dtype == MTPX_F32    ? norm_parts_kernel<float>
+                         : dtype == MTPX_BF16 ? norm_parts_kernel<__bf16>
+                                              : norm_parts_kernel<_Float16>,
+                         grid, block, 0, s, a);
 }
 
 }  // namespace mtpx

@@ -18,7 +18,25 @@
 #include "mtpx_internal.hpp"
 #include "ops_internal.hpp"
 
+#include <tuple>
+#include <utility>
+
 namespace mtpx {
+
+// Launches a kernel and returns the launch's own error: the runtime's last
+// error may be an earlier call's, and is its caller's to read.
+template <class... P, size_t... I>
+hipError_t launch_with(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, std::tuple<P...> values,
+                       std::index_sequence<I...>)
+{
+    void *each[] = {&std::get<I>(values)...};
+    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, each, lds, s);
+}
+template <class... P, class... A>
+hipError_t launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, const A &...args)
+{
+    return launch_with(kernel, grid, block, lds, s, std::tuple<P...>(args...), std::index_sequence_for<P...>());
+}
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));

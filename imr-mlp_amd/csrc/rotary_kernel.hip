@@ -164,17 +164,9 @@ hipError_t launch(const RotaryArgs &a, hipStream_t s)
 {
     const int rows = kThreads / a.lanes;
     const dim3 grid((unsigned)((a.rows + rows - 1) / rows)), block(kThreads);
-    if (a.interleaved) {
-        if (a.dpositions)
-            rotary_kernel<T, W, false, true><<<grid, block, 0, s>>>(a);
-        else
-            rotary_kernel<T, W, false, false><<<grid, block, 0, s>>>(a);
-    } else if (a.dpositions) {
-        rotary_kernel<T, W, true, true><<<grid, block, 0, s>>>(a);
-    } else {
-        rotary_kernel<T, W, true, false><<<grid, block, 0, s>>>(a);
-    }
-    return hipGetLastError();
+    const auto kernel = a.interleaved ? (a.dpositions ? rotary_kernel<T, W, false, true> : rotary_kernel<T, W, false, false>)
+                                      : (a.dpositions ? rotary_kernel<T, W, true, true> : rotary_kernel<T, W, true, false>);
+    return launch_kernel(kernel, grid, block, 0, s, a);
 }
 
 template <class T>

@@ -1,5 +1,7 @@
 """The operators among a program's other calls: errors that are not theirs,
 handles that go away during a capture, broadcast inputs."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -7,6 +9,41 @@ from mtpx import ops
 from test_ops_gpu import rand
 
 pytestmark = pytest.mark.gpu
+
+
+def _hip():
+    """The HIP runtime that torch and the library share."""
+    for line in open("/proc/self/maps"):
+        if "libamdhip64" in line:
+            return C.CDLL(line.split()[-1])
+    raise AssertionError("no HIP runtime is loaded")
+
+
+def test_an_earlier_calls_error_is_not_this_calls(ctx):
+    """An allocation that another part of the program asked for and did not
+    get, without clearing the runtime's last error."""
+    hip, p = _hip(), C.c_void_p()
+    q = torch.ones(4, 2, 2, 8, device="cuda")
+    v, lam, seqs = torch.ones(4, 2, 16, device="cuda"), torch.ones(2, device="cuda"), ops.Sequences(ctx, [0, 4])
+    freq, axis = torch.ones(2, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    pos, x = torch.ones(4, 1, device="cuda"), torch.ones(4, 8, device="cuda")
+    lengths = torch.tensor([2, 3], dtype=torch.int32, device="cuda")
+    out, saved = ops.diff_attention(ctx, q, q, v, lam, seqs, save=True)
+    _, _, stats = ops.norm_block(ctx, x, x, save=True)
+    for call in (lambda: ops.rotary(ctx, q.flatten(1, 2), pos, freq, axis),
+                 lambda: ops.diff_attention(ctx, q, q, v, lam, seqs),
+                 lambda: ops.diff_attention_backward(ctx, v, q, q, v, lam, seqs, out, saved),
+                 lambda: ops.diff_attention_cache(ctx, q[:2], q[None].expand(2, -1, -1, -1, -1), v[None].expand(2, -1, -1, -1), lam, lengths),
+                 lambda: ops.norm_block(ctx, x, x),
+                 lambda: ops.norm_block_backward(ctx, x, x, x, x, None, None, None, stats)):
+        want = call()
+        assert hip.hipMalloc(C.byref(p), C.c_size_t(1 << 60)) != 0
+        try:
+            got = call()
+        finally:
+            hip.hipGetLastError()
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert a is None or torch.equal(a, b)
 
 
 def test_a_single_row_of_a_shared_gate(ctx):
