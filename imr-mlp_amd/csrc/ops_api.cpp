@@ -6,7 +6,9 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <mutex>
 #include <new>
+#include <utility>
 
 struct mtpx_sequences {
     int device = 0, n = 0;
@@ -18,6 +20,44 @@ struct mtpx_sequences {
 
 namespace mtpx {
 namespace {
+
+// Tables of destroyed handles, freed by the next creation: a handle may be
+// destroyed at any time (by a garbage collector, say), also while a graph is
+// recorded, which no free may happen in, and while queued work reads it.
+struct Retired {
+    std::mutex lock;
+    std::vector<std::pair<int, void *>> tables;  // by device
+
+    void add(int device, void *p)
+    {
+        std::lock_guard<std::mutex> held(lock);
+        tables.emplace_back(device, p);
+    }
+    // Those of the current device; waits for its work.
+    void free(int device)
+    {
+        std::vector<void *> mine;
+        {
+            std::lock_guard<std::mutex> held(lock);
+            mine.reserve(tables.size());
+            auto end = std::remove_if(tables.begin(), tables.end(), [&](const std::pair<int, void *> &t) {
+                if (t.first == device)
+                    mine.push_back(t.second);
+                return t.first == device;
+            });
+            tables.erase(end, tables.end());
+        }
+        if (!mine.empty())
+            (void)hipDeviceSynchronize();
+        for (void *p : mine)
+            (void)hipFree(p);
+    }
+};
+Retired &retired()
+{
+    static Retired *r = new Retired;  // kept: handles may be destroyed as the process ends
+    return *r;
+}
 
 constexpr int64_t kMaxLength = int64_t(1) << 30;  // rows of one sequence
 // a launch's threads are counted in 32 bits: workgroups of 512, rows of 64
@@ -447,6 +487,7 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                 all.insert(all.end(), t.begin(), t.end());
             }
         OnDevice here(ctx->device);
+        retired().free(ctx->device);
         hipError_t e = upload(sq->tiles, all, ctx->stream);
         if (e == hipSuccess)
             e = hipStreamSynchronize(ctx->stream);
@@ -476,7 +517,12 @@ void mtpx_sequences_destroy(mtpx_sequences *seqs)
 {
     if (!seqs)
         return;
-    OnDevice here(seqs->device);
+    try {
+        if (seqs->tiles.p)
+            retired().add(seqs->device, seqs->tiles.p);
+    } catch (const std::exception &) {  // no room to note it: left allocated
+    }
+    seqs->tiles.p = nullptr;
     delete seqs;
 }
 

@@ -248,7 +248,8 @@ def rotary_backward(ctx, dy, positions, freq, axis, *, interleaved=False, x=None
 class Sequences:
     """mtpx_sequences: the row ranges of a ragged batch.  q_offsets and
     k_offsets (default: the same) are n + 1 ascending row numbers on the
-    host."""
+    host.  Creation allocates and waits for its upload: once per batch, not
+    while a graph is recorded."""
 
     def __init__(self, ctx, q_offsets, k_offsets=None):
         self.h = None
@@ -263,7 +264,9 @@ class Sequences:
         self.h, self.q_rows, self.k_rows = h, int(q[-1]), int(k[-1])
 
     def close(self):
-        """Frees the tables, after the work queued on the device has ended."""
+        """Ends the use of the handle; work that is queued keeps its tables, a
+        recorded graph does not.  The next handle frees them, once the device
+        has ended its work."""
         if getattr(self, "h", None):
             _ops().mtpx_sequences_destroy(self.h)
             self.h = None

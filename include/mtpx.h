@@ -653,8 +653,11 @@ int mtpx_rotary(mtpx_context *ctx, const mtpx_rotary_request *request);
 /* Sequences of a ragged batch: sequence i holds the query rows
  * [q_offsets[i], q_offsets[i + 1]) and the key rows [k_offsets[i],
  * k_offsets[i + 1]) (host arrays of n + 1, ascending from 0; k_offsets NULL:
- * the same).  Empty sequences are allowed.  Built once per batch; waits for
- * its upload.  Destroy it after the work that uses it has finished. */
+ * the same).  Empty sequences are allowed.  Built once per batch: creation
+ * allocates and waits for its upload, and for the device where handles were
+ * destroyed before, whose tables it frees.  Destruction only ends the use of
+ * the handle: it may come while work that uses it is queued, and while a graph
+ * is recorded, but a graph that was recorded with it must not run any more. */
 typedef struct mtpx_sequences mtpx_sequences;
 int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                           const int64_t *k_offsets, mtpx_sequences **out);

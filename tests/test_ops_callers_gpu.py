@@ -1,6 +1,7 @@
 """The operators among a program's other calls: errors that are not theirs,
 handles that go away during a capture, broadcast inputs."""
 import ctypes as C
+import gc
 
 import pytest
 import torch
@@ -44,6 +45,30 @@ def test_an_earlier_calls_error_is_not_this_calls(ctx):
             hip.hipGetLastError()
         for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
             assert a is None or torch.equal(a, b)
+
+
+def test_sequences_may_go_away_during_a_capture(ctx):
+    """The collector frees a handle whenever it likes, also while a graph is
+    recorded; the graph and the next handle are whole."""
+    g = torch.Generator().manual_seed(3)
+    q, v, lam = rand(g, 90, 2, 2, 32, dtype=torch.bfloat16).cuda(), rand(g, 90, 2, 64, dtype=torch.bfloat16).cuda(), torch.rand(2).cuda()
+    seqs, gone = ops.Sequences(ctx, [0, 30, 90]), ops.Sequences(ctx, [0, 90])
+    want = ops.diff_attention(ctx, q, q, v, lam, seqs)
+    other = ops.diff_attention(ctx, q, q, v, lam, gone)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.diff_attention(ctx, q, q, v, lam, seqs)
+        del gone
+        gc.collect()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        again = ops.Sequences(ctx, [0, 90])
+        assert torch.equal(ops.diff_attention(ctx, q, q, v, lam, again), other)
+        again.close()
 
 
 def test_a_single_row_of_a_shared_gate(ctx):
