@@ -454,6 +454,15 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
         if (q_offsets[i + 1] - q_offsets[i] > kMaxLength || ko[i + 1] - ko[i] > kMaxLength)
             return set_error(ctx, MTPX_E_CAPACITY, "a sequence of more than 2^30 rows");
     }
+    // what a launch cannot take is refused before its tables are built
+    for (const int64_t *o : {q_offsets, ko})
+        for (int64_t rows : kTileRows) {
+            int64_t tiles = 0;
+            for (int i = 0; i < n; ++i)
+                tiles += (o[i + 1] - o[i] + rows - 1) / rows;
+            if (tiles > kMaxGroups)
+                return set_error(ctx, MTPX_E_CAPACITY, "too many rows for one launch");
+        }
     mtpx_sequences *sq = nullptr;
     try {
         sq = new mtpx_sequences;
@@ -478,10 +487,6 @@ int mtpx_sequences_create(mtpx_context *ctx, int n, const int64_t *q_offsets,
                     // with causal rows the last queries and the first keys have the most
                     return la != lb ? la > lb : side ? a.start < b.start : a.start > b.start;
                 });
-                if (t.size() > (size_t)kMaxGroups) {
-                    delete sq;
-                    return set_error(ctx, MTPX_E_CAPACITY, "too many rows for one launch");
-                }
                 first[2 * side + j] = all.size();
                 count[2 * side + j] = t.size();
                 all.insert(all.end(), t.begin(), t.end());

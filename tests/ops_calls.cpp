@@ -5,11 +5,17 @@
 //                      device 1 current: prints its name, its code, the device
 //                      its work was queued on (-1: none) and the one current
 //                      afterwards
+//   ops_calls sequences n rows megabytes
+//                      a handle of n sequences of so many rows, with so much
+//                      address space left to the process: prints its code
 #include "../imr-mlp_amd/csrc/ops_api.cpp"
 
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+
+#include <sys/resource.h>
+#include <unistd.h>
 
 static int current = 1, queued = -1;
 
@@ -108,8 +114,31 @@ static int devices()
     return 0;
 }
 
+static int sequences(int n, int64_t rows, size_t megabytes)
+{
+    mtpx_context ctx;
+    std::vector<int64_t> offsets(n + 1);
+    for (int i = 0; i <= n; ++i)
+        offsets[i] = i * rows;
+    long long pages = 0;
+    if (std::FILE *f = std::fopen("/proc/self/statm", "r")) {
+        if (std::fscanf(f, "%lld", &pages) != 1)
+            return 1;
+        std::fclose(f);
+    }
+    const rlim_t limit = (rlim_t)pages * sysconf(_SC_PAGESIZE) + ((rlim_t)megabytes << 20);
+    const rlimit space{limit, limit};
+    if (setrlimit(RLIMIT_AS, &space))
+        return 1;
+    mtpx_sequences *seqs = nullptr;
+    std::printf("%d\n", mtpx_sequences_create(&ctx, n, offsets.data(), nullptr, &seqs));
+    return 0;
+}
+
 int main(int argc, char **argv)
 {
+    if (argc > 4 && !std::strcmp(argv[1], "sequences"))
+        return sequences(std::atoi(argv[2]), std::atoll(argv[3]), std::atoi(argv[4]));
     if (argc > 1 && !std::strcmp(argv[1], "device"))
         return devices();
     return 2;

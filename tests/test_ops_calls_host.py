@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from mtpx import capi
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -33,3 +35,14 @@ def test_the_callers_device_stays_current(calls):
     for name, code, queued, after in seen:
         assert code == "0" and after == "1", (name, code, after)
         assert queued in ("0", "-1") and (queued == "0" or name == "sequences_destroy"), name
+
+
+@pytest.mark.parametrize("n,rows", [(1, 2 ** 30), (60, 2 ** 30), (2, 300_000_000)])
+def test_too_many_rows_are_refused_before_tables_are_built(calls, n, rows):
+    """A row of a table is 32 bytes per 64 rows and side: 60 sequences of 2^30
+    rows would take 97 GB of the host before they were found too many."""
+    assert calls("sequences", n, rows, 100) == [[str(capi.ERRORS_BY_NAME["MTPX_E_CAPACITY"])]]
+
+
+def test_many_rows_are_taken(calls):
+    assert calls("sequences", 200, 1_000_000, 2000) == [["0"]]
