@@ -80,6 +80,9 @@ __device__ inline void store_columns(T *row, int64_t map, int dim, int t, int la
 // has seen no key, is passed by every finite score.
 constexpr float kSlack = 8.f, kNoLevel = -3.0e38f;
 
+// Rows that see no more keys than this sum D from 32-bit products.
+constexpr int kFewKeys = 64;
+
 // Forward.  A workgroup takes kWaves * QT * 16 query rows of one head, each
 // wave QT * 16 of them; the keys and values come in tiles of KB rows straight
 // into LDS, the next tile while the present one is worked on (BUF 2).
@@ -303,17 +306,70 @@ __global__ __launch_bounds__(W * kWave, OCC) void attn_forward_kernel(AttnArgs a
     }
 }
 
+// S^T (both maps) and dP^T = V dO^T of 32 keys: those of block b of the tiles.
+template <class T, int D, int QT>
+__device__ inline void score_block(const Reader<T, D> &rd, const char *kt, const char *vt, int b,
+                                   const Frag<T> (&qf)[2][QT][D / 32], const Frag<T> (&df)[2][QT][D / 32],
+                                   f32x4 (&s)[2][2][QT], f32x4 (&dp)[2][QT])
+{
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r0 = b * 32 + u * 16;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+            s[0][u][t] = s[1][u][t] = dp[u][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk) {
+                const Frag<T> kf = rd.row_frag(kt, r0, m * D + kk * 32);
+                const Frag<T> vf = rd.row_frag(vt, r0, m * D + kk * 32);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    s[m][u][t] = mma(kf, qf[m][t][kk], s[m][u][t]);
+                    dp[u][t] = mma(vf, df[m][t][kk], dp[u][t]);
+                }
+            }
+    }
+}
+
+// Scores that a lane's row does not see become -inf.  seen: the bits of the
+// lane's first key and those after it; last: the last of them that its row of
+// group 0 sees.
+template <int QT>
+__device__ inline void hide(f32x4 (&s)[2][2][QT], unsigned seen, int last, bool causal)
+{
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool on = (seen >> (16 * u + r) & 1) && (!causal || 16 * u + r <= last + 16 * t);
+                s[0][u][t][r] = on ? s[0][u][t][r] : -INFINITY;
+                s[1][u][t][r] = on ? s[1][u][t][r] : -INFINITY;
+            }
+}
+
 // Gradient of the queries.  Work split, tiles and fragments as in the forward
 // pass: S^T and dP^T = V dO^T come out with a query per lane column, so
-// dS_m^T = P_m (dP - D_m) is operand B of dQ_m^T += K_m^T dS_m^T.  The rows'
-// D_m = dO . O_m are formed here from out and out1 (O_0 = out + lambda O_1)
-// and left for the key pass.  The roundings of 16-bit out and out1 reach the
-// gradients through them (q's is then off by 0.0027 of its size instead of
-// 0.0025; keeping what they leave off, a byte each, made a training step of
-// 1,000 structures 23% longer).  dlambda is -sum D_1; since the sum of
+// dS_m^T = P_m (dP - D_m) is operand B of dQ_m^T += K_m^T dS_m^T, rounded to T
+// for it.  The rows' D_m = dO . O_m are formed here from out and out1 (O_0 =
+// out + lambda O_1) and left for the key pass.  The roundings of 16-bit out and
+// out1 reach the gradients through them (q's is then off by 0.0027 of its size
+// instead of 0.0025; keeping what they leave off, a byte each, made a training
+// step of 1,000 structures 23% longer).  dlambda is -sum D_1; since the sum of
 // P_1 (dP - D_1) over a row is what the rounded out1 took from D_1, adding it
 // gives D_1 from 32-bit values.
-template <class T, int D, int QT, int KB, int BUF, int OCC, bool FEW>
+//
+// Where rows see few keys, dS is small beside D and those roundings are as
+// large as dS itself (bfloat16 rows of two to four keys: 0.0038 of q's gradient
+// where one rounding of dS and of the result leave 0.0032).  A workgroup whose
+// rows see few keys (kFewKeys, or the first rows of causal sequences)
+// therefore walks them once more first, and sums D from 32-bit products
+// (1,000 bfloat16 sequences of about 50 rows: a training step of 671 us, 654
+// us without).  D from 32-bit out and out1 is as good as that sum.
+template <class T, int D, int QT, int KB, int BUF, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int table, int ntiles)
 {
     using TL = Tile<T, D>;
@@ -335,9 +391,17 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
     Reader<T, D> rd;
     rd.init(lane);
 
+    // keys that the last row of the workgroup sees (a single one gives its
+    // row's scores no gradient)
+    constexpr int kRows = kWaves * QT * 16;
+    int nk = sq.nk > 1 ? sq.nk : 0;
+    if (a.causal)
+        nk = min(nk, min(sq.start + kRows, sq.nq) + shift);
+    const bool twice = sizeof(T) == 2 && nk > 0 && nk <= (a.causal ? max(kRows, kFewKeys) : kFewKeys);
+
     const int w0 = sq.start + wave * QT * 16;
     Frag<T> qf[2][QT][D / 32], df[2][QT][D / 32];
-    float base[2][QT], delta[2][QT], dlam = 0.f;
+    float base[2][QT], delta[2][QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int row = w0 + t * 16 + (lane & 15);
@@ -370,105 +434,35 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
             const float lse = live ? a.lse[at] : -INFINITY;
             // a row without a key: exp2(s c - inf) is 0
             base[m][t] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-            if (!FEW && live && g == 0)
-                a.delta[at] = delta[m][t];
         }
-        if (!FEW && g == 0)
-            dlam += delta[1][t];
     }
-    f32x4 acc[2][QT][D / 16];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                acc[m][t][i] = f32x4{0, 0, 0, 0};
 
-    int nk = sq.nk > 1 ? sq.nk : 0;
-    if (a.causal)
-        nk = min(nk, min(sq.start + kWaves * QT * 16, sq.nq) + shift);
-    bool first = FEW;  // of the walks over the keys, which sums D
-    float summed[2][QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-        summed[0][t] = summed[1][t] = 0.f;
     unsigned long long bits = 0;
     SeenKeys seen(mask, nk, lane);
-    if (nk > 0) {
-        bits = seen.at(0, KB) & kFull;
-        lk.load(smem, 0, bits, bits == kFull);
-        lv.load(smem, kTile, bits, bits == kFull);
-    }
-    int buf = 0;
-    for (int k0 = 0; k0 < nk;) {
-        wait_loads();
-        __syncthreads();
-        const unsigned long long now = bits;
-        const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
-        auto next = [&] {
-            const bool again = k0 + KB >= nk;
-            if (again && !first)
-                return;
-            buf = BUF - 1 - buf;
-            if (FEW && again) {
-                seen = SeenKeys(mask, nk, lane);
-                lk.move(-(int64_t)k0 * a.k.row);
-                lv.move(-(int64_t)k0 * a.v.row);
-            } else {
-                lk.next();
-                lv.next();
-            }
-            bits = seen.at(FEW && again ? 0 : k0 + KB, KB) & kFull;
-            lk.load(smem, buf * 2 * kTile, bits, bits == kFull);
-            lv.load(smem, buf * 2 * kTile + kTile, bits, bits == kFull);
-        };
-        if constexpr (BUF == 2)
-            next();
-        const bool idle = now == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift);
-        const bool partly = now != kFull || (a.causal && k0 + KB - 1 > w0 + shift);
-        if (!idle) {
+    auto load = [&](int k0, int to) {
+        bits = seen.at(k0, KB) & kFull;
+        lk.load(smem, to * 2 * kTile, bits, bits == kFull);
+        lv.load(smem, to * 2 * kTile + kTile, bits, bits == kFull);
+    };
+    auto idle = [&](int k0) { return bits == 0 || w0 >= sq.nq || (a.causal && k0 > w0 + QT * 16 - 1 + shift); };
+    auto last = [&](int k) { return w0 + (lane & 15) + shift - k - 4 * g; };
+    if (nk > 0)
+        load(0, 0);
+    if (twice) {
+        float summed[2][QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+            summed[0][t] = summed[1][t] = 0.f;
+        for (int k0 = 0;;) {
+            wait_loads();
+            __syncthreads();
 #pragma unroll 1
-        for (int b = 0; b < KB / 32; ++b) {
-            if (empty_block(now, b, a.causal, k0, w0 + QT * 16 - 1 + shift))
-                continue;
-            f32x4 s[2][2][QT], dp[2][QT];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r0 = b * 32 + u * 16;
-#pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    s[0][u][t] = s[1][u][t] = dp[u][t] = f32x4{0, 0, 0, 0};
-                }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int kk = 0; kk < D / 32; ++kk) {
-                        const Frag<T> kf = rd.row_frag(kt, r0, m * D + kk * 32);
-                        const Frag<T> vf = rd.row_frag(vt, r0, m * D + kk * 32);
-#pragma unroll
-                        for (int t = 0; t < QT; ++t) {
-                            s[m][u][t] = mma(kf, qf[m][t][kk], s[m][u][t]);
-                            dp[u][t] = mma(vf, df[m][t][kk], dp[u][t]);
-                        }
-                    }
-            }
-            if (partly) {
-                const unsigned mine = (unsigned)(now >> (32 * b + 4 * g));
-#pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    const int last = a.causal ? w0 + t * 16 + (lane & 15) + shift - k0 - 32 * b - 4 * g : 32;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const bool on = (mine >> (16 * u + r) & 1) && 16 * u + r <= last;
-                            s[0][u][t][r] = on ? s[0][u][t][r] : -INFINITY;
-                            s[1][u][t][r] = on ? s[1][u][t][r] : -INFINITY;
-                        }
-                }
-            }
-            if (FEW && first) {
+            for (int b = 0; b < KB / 32 && !idle(k0); ++b) {
+                if (empty_block(bits, b, a.causal, k0, w0 + QT * 16 - 1 + shift))
+                    continue;
+                f32x4 s[2][2][QT], dp[2][QT];
+                score_block<T, D, QT>(rd, smem, smem + kTile, b, qf, df, s, dp);
+                hide<QT>(s, (unsigned)(bits >> (32 * b + 4 * g)), last(k0 + 32 * b), a.causal);
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -477,10 +471,78 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                summed[m][t] = fmaf(exp2_fast(fmaf(s[m][u][t][r], c, -base[m][t])),
-                                                    dp[u][t][r], summed[m][t]);
-                continue;
+                                summed[m][t] = fmaf(exp2_fast(fmaf(s[m][u][t][r], c, -base[m][t])), dp[u][t][r],
+                                                    summed[m][t]);
             }
+            if (k0 + KB >= nk) {
+                if (k0 > 0) {  // back to the first tile; the only one stays
+                    __syncthreads();
+                    lk.move(-(int64_t)k0 * a.k.row);
+                    lv.move(-(int64_t)k0 * a.v.row);
+                    seen = SeenKeys(mask, nk, lane);
+                    load(0, 0);
+                }
+                break;
+            }
+            __syncthreads();
+            k0 += KB;
+            lk.next();
+            lv.next();
+            load(k0, 0);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+                delta[m][t] = column_sum(summed[m][t]);
+    }
+    float dlam = 0.f;
+    if (g == 0) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int row = w0 + t * 16 + lane;
+            dlam += delta[1][t];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+                if (row < sq.nq)
+                    a.delta[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] = delta[m][t];
+        }
+    }
+
+    f32x4 acc[2][QT][D / 16];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                acc[m][t][i] = f32x4{0, 0, 0, 0};
+    int buf = 0;
+    for (int k0 = 0; k0 < nk; k0 += KB) {
+        wait_loads();
+        __syncthreads();
+        const unsigned long long now = bits;
+        const bool rest = idle(k0);
+        const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
+        auto next = [&] {
+            if (k0 + KB < nk) {
+                buf = BUF - 1 - buf;
+                lk.next();
+                lv.next();
+                load(k0 + KB, buf);
+            }
+        };
+        if constexpr (BUF == 2)
+            next();
+        const bool partly = now != kFull || (a.causal && k0 + KB - 1 > w0 + shift);
+#pragma unroll 1
+        for (int b = 0; b < KB / 32 && !rest; ++b) {
+            if (empty_block(now, b, a.causal, k0, w0 + QT * 16 - 1 + shift))
+                continue;
+            f32x4 s[2][2][QT], dp[2][QT];
+            score_block<T, D, QT>(rd, kt, vt, b, qf, df, s, dp);
+            if (partly)
+                hide<QT>(s, (unsigned)(now >> (32 * b + 4 * g)), last(k0 + 32 * b), a.causal);
             Frag<T> sf[2][QT];
             float missing = 0.f;
 #pragma unroll
@@ -509,20 +571,9 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
                         acc[m][t][i] = mma(kf, sf[m][t], acc[m][t][i]);
                 }
         }
-        }
         if constexpr (BUF == 1) {
             __syncthreads();
             next();
-        }
-        k0 += KB;
-        if (FEW && first && k0 >= nk) {
-            k0 = 0;
-            first = false;
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int t = 0; t < QT; ++t)
-                    delta[m][t] = column_sum(summed[m][t]);
         }
     }
 
@@ -531,12 +582,6 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
         const int row = w0 + t * 16 + (lane & 15);
         if (row >= sq.nq)
             continue;
-        if (FEW && g == 0) {
-            dlam += delta[1][t];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                a.delta[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] = delta[m][t];
-        }
         T *qp = (T *)a.dq.data + head * a.dq.head + (sq.q0 + row) * a.dq.row;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -1150,15 +1195,11 @@ struct Shape {
 // Tables of 64 and 128 rows.
 constexpr int kNarrow = 0, kBroad = 1;
 
-// Batches of sequences up to this long walk over their keys twice in the query
-// pass (see there); in bfloat16 that takes the error of sequences of one to
-// three rows from 0.0048 to that of long ones, 0.0026.
-constexpr int kFewKeys = 64;
-
 // 32 rows a wave halve the reads from LDS per product and are right for work
 // that fills the device (32,000 rows of 8 heads, 64 wide: 5.8 ms, 6.9 ms with
 // 16 rows a wave); where tiles of 128 rows are fewer than two workgroups a CU,
 // tiles of 64 spread the work further (997 rows of 8 heads: 41 us and 26 us).
+// Sequences of few keys have as few rows where they attend to themselves.
 template <int D>
 int query_table(const TileTable &t, int heads)
 {
@@ -1183,12 +1224,12 @@ hipError_t forward(const AttnArgs &a, hipStream_t s)
     return forward_rows<D, 1>(a, kNarrow, s);
 }
 
-template <int D, int QT, bool FEW>
+template <int D, int QT>
 hipError_t dq_rows(const AttnArgs &a, int table, hipStream_t s)
 {
     using S = Shape<Type, D>;
     const int n = a.tiles.nq[table];
-    return launch_kernel(attn_dq_kernel<Type, D, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy, FEW>,
+    return launch_kernel(attn_dq_kernel<Type, D, QT, S::kRows, S::kQueryBuffers, S::kQueryOccupancy>,
                          dim3((unsigned)((int64_t)n * a.heads)), dim3(kThreads), S::kQueryBuffers * S::kLds, s, a, table, n);
 }
 template <int D>
@@ -1197,9 +1238,7 @@ hipError_t backward(const AttnArgs &a, hipStream_t s)
     using S = Shape<Type, D>;
     if (a.tiles.nq[kNarrow] > 0) {
         const bool broad = query_table<D>(a.tiles, a.heads) == kBroad;
-        if (hipError_t e = a.tiles.longest_k <= kFewKeys ? dq_rows<D, 1, true>(a, kNarrow, s)
-                           : broad                       ? dq_rows<D, S::kWide, false>(a, kBroad, s)
-                                                         : dq_rows<D, 1, false>(a, kNarrow, s))
+        if (hipError_t e = broad ? dq_rows<D, S::kWide>(a, kBroad, s) : dq_rows<D, 1>(a, kNarrow, s))
             return e;
     }
     const int nk = a.tiles.nk[kNarrow];
