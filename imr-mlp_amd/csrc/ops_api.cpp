@@ -160,7 +160,9 @@ AttnSizes attn_workspace(mtpx_context *ctx, const mtpx_diff_attention_request &r
     const int parts = key_parts(ctx, r);
     auto pad = [](size_t n) { return (n + 15) / 16 * 16; };
     AttnSizes s;
-    s.delta = pad(sizeof(float) * 2 * (size_t)r.heads * (size_t)q.total_q);
+    // D of both maps, and in float16 the largest of |dO|
+    const size_t planes = r.dtype == MTPX_F16 ? 3 : 2;
+    s.delta = pad(sizeof(float) * planes * (size_t)r.heads * (size_t)q.total_q);
     s.part = pad(sizeof(float) * (size_t)r.heads *
                  (size_t)attn_backward_tiles(r.dtype, r.dim, r.heads, q.table));
     s.kv = parts == 1 ? 0 : sizeof(float) * 4 * (size_t)r.dim * parts * r.kv_heads * (size_t)q.total_k;

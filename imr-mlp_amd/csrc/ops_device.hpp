@@ -392,6 +392,16 @@ __device__ inline float max3(float a, float b, float c)
     return r;
 }
 
+// The largest absolute value of three.
+__device__ inline float max3_abs(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// The exponent e of 2^(e-1) <= v < 2^e; 0 of 0, infinities and NaN.
+__device__ inline int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
+
 // Sum over 16 lanes or a wave, in a fixed order, in every lane: rotations or
 // shifts within rows of 16 lanes, then from row to row, by data-parallel moves
 // that need no LDS.
@@ -416,6 +426,18 @@ __device__ inline float wave_sum(float v)
     v += moved<0x118, 0xf>(v);
     v += moved<0x142, 0xa>(v);  // row_bcast:15
     v += moved<0x143, 0xc>(v);  // row_bcast:31
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// Maximum over a wave of values that are not negative, in every lane.
+__device__ inline float wave_max(float v)
+{
+    v = fmaxf(v, moved<0x111, 0xf>(v));
+    v = fmaxf(v, moved<0x112, 0xf>(v));
+    v = fmaxf(v, moved<0x114, 0xf>(v));
+    v = fmaxf(v, moved<0x118, 0xf>(v));
+    v = fmaxf(v, moved<0x142, 0xa>(v));
+    v = fmaxf(v, moved<0x143, 0xc>(v));
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
