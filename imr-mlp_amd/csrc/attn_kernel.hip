@@ -365,12 +365,12 @@ __device__ inline void hide(f32x4 (&s)[2][2][QT], unsigned seen, int last, bool 
 // pass: S^T and dP^T = V dO^T come out with a query per lane column, so
 // dS_m^T = P_m (dP - D_m) is operand B of dQ_m^T += K_m^T dS_m^T, rounded to T
 // for it.  The rows' D_m = dO . O_m are formed here from out and out1 (O_0 =
-// out + lambda O_1) and left for the key pass.  The roundings of 16-bit out and
-// out1 reach the gradients through them (q's is then off by 0.0027 of its size
-// instead of 0.0025; keeping what they leave off, a byte each, made a training
-// step of 1,000 structures 23% longer).  dlambda is -sum D_1; since the sum of
-// P_1 (dP - D_1) over a row is what the rounded out1 took from D_1, adding it
-// gives D_1 from 32-bit values.
+// out + lambda O_1).  The roundings of 16-bit out and out1 reach q's gradient
+// through them (in bfloat16 it is then off by 0.0027 of its size, where the
+// roundings of dS and of the result leave 0.0023; keeping what out and out1
+// leave off, a byte each, made a training step of 1,000 structures 23% longer).
+// The sum of P_m (dP - D_m) over a row is what they took from D_m: with it added,
+// D_m for the key pass and for dlambda = -sum D_1 comes from 32-bit values.
 //
 // Where rows see few keys, dS is small beside D and those roundings are as
 // large as dS itself (bfloat16 rows of two to four keys: 0.0038 of q's gradient
@@ -520,25 +520,15 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
             for (int t = 0; t < QT; ++t)
                 delta[m][t] = column_sum(summed[m][t]);
     }
-    float dlam = 0.f;
-    if (g == 0) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int row = w0 + t * 16 + lane;
-            dlam += delta[1][t];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                if (row < sq.nq)
-                    a.delta[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] = delta[m][t];
-        }
-    }
-
+    constexpr bool kRounded = sizeof(T) == 2;
+    float missing[2][QT];  // sums of the lane's P (dP - D)
     f32x4 acc[2][QT][D / 16];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         lift[t] = kScaled ? kMostLift : 0;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
+            missing[m][t] = 0.f;
             base[m][t] -= lift[t];
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
@@ -572,7 +562,6 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
             if (partly)
                 hide<QT>(s, (unsigned)(now >> (32 * b + 4 * g)), last(k0 + 32 * b), a.causal);
             Frag<T> sf[2][QT];
-            float missing = 0.f;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -583,8 +572,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
                         for (int r = 0; r < 4; ++r) {
                             const float p = exp2_fast(fmaf(s[m][u][t][r], c, -base[m][t]));
                             s[m][u][t][r] = p * (dp[u][t][r] - delta[m][t]);
-                            if (m == 1 && !kScaled)
-                                missing += s[m][u][t][r];
+                            if (!kScaled && (kRounded || m == 1))
+                                missing[m][t] += s[m][u][t][r];
                         }
                     if constexpr (!kScaled)
                         sf[m][t] = pack<T>(s[m][0][t], s[m][1][t]);
@@ -613,6 +602,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             base[m][t] -= down;
+                            missing[m][t] *= f;
                             s[m][0][t] *= f;
                             s[m][1][t] *= f;
 #pragma unroll
@@ -623,19 +613,17 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
                 }
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
-                    float part = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            part += s[1][u][t][r];
-                    missing += ldexpf(part, -lift[t]);
+                        for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
+                            for (int r = 0; r < 4; ++r)
+                                missing[m][t] += s[m][u][t][r];
                         sf[m][t] = pack<T>(s[m][0][t], s[m][1][t]);
+                    }
                 }
             }
-            dlam += missing;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -652,11 +640,22 @@ __global__ __launch_bounds__(kThreads, OCC) void attn_dq_kernel(AttnArgs a, int 
         }
     }
 
+    float dlam = 0.f;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int row = w0 + t * 16 + (lane & 15);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            if (kRounded || m == 1)
+                delta[m][t] += column_sum(ldexpf(missing[m][t], -lift[t]));
         if (row >= sq.nq)
             continue;
+        if (g == 0) {
+            dlam += delta[1][t];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+                a.delta[((int64_t)m * a.heads + head) * a.total_q + sq.q0 + row] = delta[m][t];
+        }
         T *qp = (T *)a.dq.data + head * a.dq.head + (sq.q0 + row) * a.dq.row;
 #pragma unroll
         for (int m = 0; m < 2; ++m)

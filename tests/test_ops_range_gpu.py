@@ -113,3 +113,16 @@ def test_an_infinite_gradient_is_not_hidden(ctx, dtype, bad):
     for name in ("dq", "dk", "dv"):
         assert not bool(torch.isfinite(got[name][:150]).all()), name
         assert bool(torch.isfinite(got[name][150:]).all()), name
+
+
+@dtypes
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_key_gradients_take_nothing_from_the_saved_results(ctx, dtype, dim):
+    """k's gradient: the roundings of dS and of the result alone, each u /
+    sqrt(3) of their own terms in the mean."""
+    c = attention_case(dim + 3, dtype, [160, 90, 230, 75], [160, 90, 230, 75], 8, 8, dim)
+    got, r = gradients(ctx, c), exact(c)
+    own = float((r["dk"].to(dtype).double() - r["dk"]).norm() / r["dk"].norm())
+    off = float((got["dk"] - r["dk"]).norm() / r["dk"].norm())
+    # one rounding measured, the other as large; 3 % for the spread of many thousand elements
+    assert off <= 1.03 * math.sqrt(2) * own + OO.F32 * (16 + 4 * dim + 4 * r["scores"]), off / own
