@@ -234,7 +234,8 @@ def rotary(ctx, x, positions, freq, axis, *, interleaved=False, inverse=False, o
 
 def rotary_backward(ctx, dy, positions, freq, axis, *, interleaved=False, x=None):
     """Gradient of x from that of the result: (dx, None), or (dx, dpositions)
-    with the forward pass's x given (positions float32 or float64)."""
+    with the forward pass's x given (positions float32 or float64; a 32-bit sum
+    for both)."""
     dpos = None
     if x is not None:
         dpos = torch.empty(positions.shape, dtype=positions.dtype, device=dy.device)

@@ -629,8 +629,8 @@ typedef struct mtpx_rows {
  * large positions keep their phase.  `inverse` turns by -theta: the backward
  * pass, x being the gradient of y and y the gradient of x.  With
  * dpositions (needs inverse, and `forward`, the x of the forward pass) the
- * gradient of the positions is written as well: f64 for f64 positions, f32
- * for f32 ones; integer positions have none.  y may be x itself (same
+ * gradient of the positions is written as well, in their type (a 32-bit sum
+ * also for f64 ones); integer positions have none.  y may be x itself (same
  * strides). */
 typedef struct mtpx_rotary_request {
     void *stream;
@@ -671,9 +671,11 @@ void mtpx_sequences_destroy(mtpx_sequences *seqs);
  * out 2 dim elements (two "maps" of dim, contiguous or not).  A key is seen
  * by a row if key_mask is NULL or nonzero for it, and, with `causal`, if it
  * is not after the row (the last row of a sequence sees its last key).  A
- * row without a key gives 0, its gradient is 0 and its lse -inf.  What q, k,
- * v hold at masked keys does not matter, NaN included; keys and values that
- * only later rows of a causal sequence see must be finite.
+ * row without a key gives 0, its gradient is 0 and its lse -inf.  What k and
+ * v hold at masked keys does not matter, NaN included.  A mask hides keys, not
+ * rows: what a masked atom's own row holds in q and dout counts, and so it does
+ * where it is not finite.  Keys and values that only later rows of a causal
+ * sequence see must be finite.
  *
  * Forward: out; with lse (f32 [2][heads][q rows], natural logarithm) and
  * out1 ([q rows][heads][2 dim], contiguous: P_1 v) what the backward pass
