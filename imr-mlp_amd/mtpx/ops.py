@@ -263,14 +263,15 @@ class Sequences:
         ctx._check(_ops().mtpx_sequences_create(ctx.h, q.size - 1, q.ctypes.data_as(ptr),
                                                 k.ctypes.data_as(ptr), C.byref(h)), "sequences")
         self.h, self.q_rows, self.k_rows = h, int(q[-1]), int(k[-1])
+        self._destroy = _ops().mtpx_sequences_destroy  # kept: this module's names may go first
 
     def close(self):
         """Ends the use of the handle; work that is queued keeps its tables, a
         recorded graph does not.  The next handle frees them, once the device
         has ended its work."""
         if getattr(self, "h", None):
-            _ops().mtpx_sequences_destroy(self.h)
-            self.h = None
+            h, self.h = self.h, None
+            self._destroy(h)
 
     def __del__(self):
         self.close()

@@ -180,3 +180,34 @@ def test_workspace_sizes_while_another_thread_empties_them(known):
     if known:
         dict.__setitem__(Ctx.workspaces, (ops.NormRequest, *sizes.values()), 4096)
     assert ops._bytes(Ctx, query, ops.NormRequest, **sizes) == 4096
+
+
+def test_a_handle_outlives_the_module(monkeypatch):
+    """At the end of a program the module's names may go before a handle that
+    a global holds: it is still destroyed, and without an error."""
+    destroyed = []
+
+    class Library:
+        @staticmethod
+        def mtpx_sequences_create(h, n, q, k, out):
+            C.cast(out, C.POINTER(C.c_void_p))[0] = 64
+            return 0
+
+        @staticmethod
+        def mtpx_sequences_destroy(h):
+            destroyed.append(h.value)
+
+    class Ctx:
+        h = None
+
+        @staticmethod
+        def _check(rc, what):
+            assert rc == 0
+
+    monkeypatch.setattr(ops, "_ops", lambda: Library)
+    handle = ops.Sequences(Ctx, [0, 4])
+    monkeypatch.setattr(ops, "_ops", None)
+    handle.__del__()
+    assert destroyed == [64]
+    handle.close()
+    assert destroyed == [64]
