@@ -101,7 +101,7 @@ constexpr int kFewKeys = 64;
 // maps keep their own maximum, sum and product, since their normalisers are
 // known only at the end; each V fragment read from LDS serves both.  P is
 // rounded to T for the product (its 32-bit sum is the normaliser), as V is in
-// T already.  32,000 rows of 8 heads, 64 wide, in 16 bits: 5.8 ms, 1,077
+// T already.  32,000 rows of 8 heads, 64 wide, in 16 bits: 5.9 ms, 1,070
 // TFLOP/s of the matrix units (a loop of nothing else reaches 1,200 at two
 // waves a SIMD), with the vector units issuing half of the time.
 template <class T, int D, int W, int QT, int KB, int BUF, int OCC>
@@ -377,8 +377,8 @@ __device__ inline void hide(f32x4 (&s)[2][2][QT], unsigned seen, int last, bool 
 // where one rounding of dS and of the result leave 0.0032).  A workgroup whose
 // rows see few keys (kFewKeys, or the first rows of causal sequences)
 // therefore walks them once more first and sums D from 32-bit products
-// (1,000 bfloat16 sequences of about 50 rows: a training step of 671 us, 654
-// us without).  D from 32-bit out and out1 is as good as that sum.
+// (18 us of a training step of 1,000 bfloat16 sequences of about 50 rows, which
+// takes 677 us).  D from 32-bit out and out1 is as good as that sum.
 //
 // float16: dS is scaled row by row (both maps alike).  The scale, 2^lift, sits
 // in the exponent of P and is lowered, and the row's products with it, when a
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(kThreads) void dlambda_kernel(const float *part, fl
 // half; the first then hands its dS to the second, which sums dK, and gets P
 // for the other rows, as it sums dV.  One wave alone would hold both sums and
 // could afford half as many keys, at twice the reads of the tiles from LDS
-// (8,192 causal rows of 16 heads, 64 wide: 1.75 ms; 1.54 ms so).  The query
+// (8,192 causal rows of 16 heads, 64 wide: 1.75 ms; 1.54 to 1.59 ms so).  The query
 // heads that share the key head follow one another, so their sum stays in
 // registers.  What bounds it now are the waits at its two barriers a tile.
 //
@@ -1317,7 +1317,7 @@ struct Shape {
     static constexpr int kOccupancy = kLds > 32768 ? 1 : D == 32 && sizeof(T) == 2 ? 3 : 2;
     // narrow 32-bit heads: three and four, to which one buffer leaves the LDS
     // (200 structures of 84 atoms: forward 103 us with two buffers and two
-    // waves, 92 us so; key pass 164 us with 64 rows twice, 122 us with 32 once)
+    // waves, 92 us so; key pass 164 us with 64 rows twice, 128 us with 32 once)
     static constexpr bool kMore = D == 32 && sizeof(T) == 4;
     static constexpr int kQueryBuffers = kMore ? 1 : kBuffers, kQueryOccupancy = kMore ? 3 : kOccupancy;
     static constexpr int kKeyRows = kMore ? 32 : kRows, kKeyBuffers = kMore ? 1 : kBuffers;
@@ -1330,9 +1330,9 @@ struct Shape {
 constexpr int kNarrow = 0, kBroad = 1;
 
 // 32 rows a wave halve the reads from LDS per product and are right for work
-// that fills the device (32,000 rows of 8 heads, 64 wide: 5.8 ms, 6.9 ms with
+// that fills the device (32,000 rows of 8 heads, 64 wide: 5.9 ms, 6.9 ms with
 // 16 rows a wave); where tiles of 128 rows are fewer than two workgroups a CU,
-// tiles of 64 spread the work further (997 rows of 8 heads: 41 us and 26 us).
+// tiles of 64 spread the work further (997 rows of 8 heads: 41 us and 31 us a call).
 // Sequences of few keys have as few rows where they attend to themselves.
 template <int D>
 int query_table(const TileTable &t, int heads)

@@ -35,7 +35,7 @@ struct alignas(sizeof(T) * A) Piece {
 // + lanes / units, ...  So a lane reads its cos and sin once, and in the
 // backward pass sums the pairs' gradients over heads in registers.  The work
 // is bound by the reads and writes of x and y (160,000 rows of 32 heads, 64
-// wide, 16 bits: 225 us, 5.8 TB/s).
+// wide, 16 bits: 233 us, 5.6 TB/s).
 template <class T, int W, bool PAIRS_APART, bool GRAD>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
 {
