@@ -16,7 +16,9 @@ learns, over a ragged batch of structures, an energy of long waves between two
 kinds of charge that no descriptor within the cutoff holds.  Afterwards the
 forces of the correction are taken through the rotation's gradient of the
 positions and compared with differences, and one atom is moved: its row alone
-is computed, against the keys and values kept for the others.
+is computed, against the keys and values kept for the others.  (The potential's
+energies per atom enter as fixed numbers, in the forces as in the differences:
+how they change with the positions is not part of either.)
 """
 import argparse
 import os

@@ -6,7 +6,7 @@ import gc
 import pytest
 import torch
 
-from mtpx import ops
+from mtpx import capi, ops
 from test_ops_gpu import rand
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,30 @@ def test_a_single_row_of_a_shared_gate(ctx):
     grads = [ops.norm_block_backward(ctx, x, x, x, x, t, None, None, want[2]) for t in (one, one.clone())]
     assert grads[0][2].shape == (1, 24)
     assert all(a is None or torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_a_loss_of_forces_is_refused(ctx):
+    """Through all three autograd functions on the device, whose backward pass
+    is another thread: the forces are there, a loss of them raises."""
+    g = torch.Generator().manual_seed(5)
+    w = rand(g, 24, 4 * 16, dtype=torch.float32).cuda().requires_grad_(True)
+    x, pos = rand(g, 20, 24, dtype=torch.float32).cuda(), torch.rand(20, 3, generator=g).cuda().requires_grad_(True)
+    freq, axis = torch.ones(4, device="cuda"), (torch.arange(4) % 3).int().cuda()
+    seqs, lam = ops.Sequences(ctx, [0, 8, 20]), torch.rand(1, generator=g).cuda()
+
+    def energy():
+        qk = ops.RotaryFn.apply(ctx, (x @ w)[:, :32].unflatten(1, (4, 8)), pos, freq, axis)
+        out = ops.DiffAttentionFn.apply(ctx, qk[:, None, :2], qk[:, None, 2:], (x @ w)[:, None, 32:48], lam, seqs)
+        return ops.NormBlockFn.apply(ctx, None, out.flatten(1), None, None, None, {})[1].square().sum()
+
+    want, = torch.autograd.grad(energy(), pos)
+    e = energy()
+    force, = torch.autograd.grad(e, pos, create_graph=True)
+    assert torch.equal(force, want) and float(force.detach().abs().max()) > 0.0
+    with pytest.raises(capi.MtpxError, match="second derivative"):
+        (e + force.square().sum()).backward()
+    with pytest.raises(capi.MtpxError, match="second derivative"):
+        torch.autograd.grad(force.square().sum(), w)
+    learned = freq.clone().requires_grad_(True)
+    with pytest.raises(capi.MtpxError, match="freq"):
+        ops.RotaryFn.apply(ctx, x[:, None, :8], pos, learned, axis).sum().backward()
