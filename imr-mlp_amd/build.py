@@ -51,7 +51,14 @@ SOURCES = [
     ("attn_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=2"], "attn_kernel_f16"),
     ("rotary_kernel.hip", ["-ffp-contract=fast"]),
     ("norm_kernel.hip", ["-ffp-contract=fast"]),
+    ("head_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=0"], "head_kernel_f32"),
+    ("head_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=1"], "head_kernel_bf16"),
+    ("head_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=2"], "head_kernel_f16"),
+    ("paged_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=0"], "paged_kernel_f32"),
+    ("paged_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=1"], "paged_kernel_bf16"),
+    ("paged_kernel.hip", ["-ffp-contract=fast", "-DMTPX_OPS_TYPE=2"], "paged_kernel_f16"),
     ("ops_api.cpp", ["-ffp-contract=off"]),
+    ("paged_api.cpp", ["-ffp-contract=off"]),
 ]
 
 

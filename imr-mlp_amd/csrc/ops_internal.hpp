@@ -87,6 +87,54 @@ struct NormArgs {
     int vec;
 };
 
+// Norms and rotation of heads: [0] is q, [1] is k; a vector is a head's map.
+struct HeadArgs {
+    int64_t rows;
+    int vectors[2], maps;
+    int dim, rotated, interleaved, kind, axes, position_dtype;
+    float eps;
+    mtpx_rows in[2], out[2];  // backward: out is the gradient of in
+    const void *weight[2];
+    const void *positions;
+    int64_t position_row, position_axis;
+    const float *freq;
+    const int *axis;
+    // append
+    mtpx_rows v;
+    mtpx_pages cache;
+    const int *offsets, *lengths;
+    int sequences;
+    // backward
+    mtpx_rows grad[2];
+    void *dweight[2], *dpositions;
+    float *part;  // [2][parts][dim]
+    int parts;
+    int width;  // elements of one access
+    int group;  // lanes of a vector: a power of two up to 64
+    int lanes;  // of a row: a power of two from group up to 256
+};
+
+struct PagedArgs {
+    int64_t rows;
+    int sequences, heads, kv_heads, dim, causal;
+    float scale;
+    mtpx_rows q, out;
+    mtpx_pages cache;
+    const int *offsets, *lengths;
+    const float *lambda;
+    int vec;
+    // key / page_rows is the upper half of 2 key page_magic, shifted
+    unsigned page_magic;
+    int page_shift;
+    // sequences of up to `deep` columns (a row's head of the group that shares
+    // a key head) go to the deep kernel, the others to the broad one; 0 columns
+    // or tiles: that kernel is not launched
+    int deep, deep_blocks, broad_tiles, broad_columns;
+    // the most workgroups that share a sequence's keys, and their results
+    int deep_splits, broad_splits;
+    float *deep_part, *broad_part;
+};
+
 // dtype is one of MTPX_F32, MTPX_BF16, MTPX_F16 (checked by the caller).
 hipError_t launch_attn_forward(int dtype, const AttnArgs &a, hipStream_t s);
 hipError_t launch_attn_backward(int dtype, const AttnArgs &a, hipStream_t s);
@@ -97,5 +145,9 @@ hipError_t launch_rotary(int dtype, const RotaryArgs &a, hipStream_t s);
 hipError_t launch_norm_forward(int dtype, const NormArgs &a, hipStream_t s);
 hipError_t launch_norm_backward(int dtype, const NormArgs &a, hipStream_t s);
 int norm_backward_parts(int64_t rows, int width);
+hipError_t launch_head_forward(int dtype, const HeadArgs &a, hipStream_t s);
+hipError_t launch_head_append(int dtype, const HeadArgs &a, hipStream_t s);
+hipError_t launch_head_backward(int dtype, const HeadArgs &a, hipStream_t s);
+hipError_t launch_paged(int dtype, const PagedArgs &a, hipStream_t s);
 
 }  // namespace mtpx

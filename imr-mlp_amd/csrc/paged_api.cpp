@@ -1,0 +1,442 @@
+// C ABI of the operators that serve a block from a paged cache, and of the
+// norms of queries and keys (include/mtpx.h): argument checks, workspaces,
+// launches on the caller's stream.
+#include "ops_checks.hpp"
+#include "ops_internal.hpp"
+
+#include <algorithm>
+#include <exception>
+
+namespace mtpx {
+namespace {
+
+constexpr int kMaxHeadDim = 256, kMaxAxes = 8, kMaxSequences = 1 << 24;
+constexpr int64_t kMaxRoom = int64_t(1) << 30;  // rows of one sequence
+
+// No exception leaves a C entry point: a message takes memory.
+template <class F>
+int guarded(const F &f) noexcept
+{
+    try {
+        return f();
+    } catch (const std::exception &) {
+        return MTPX_E_ALLOC;
+    }
+}
+
+// The rotation's arguments, which two requests name alike.
+template <class R>
+int check_turn(mtpx_context *ctx, const R &r)
+{
+    if (r.rotated < 0 || r.rotated > r.dim || r.rotated % 2 != 0)
+        return invalid(ctx, "rotated must be even and at most dim");
+    if (r.axes < 1 || r.axes > kMaxAxes)
+        return invalid(ctx, "axes must be 1 to 8");
+    if (r.position_dtype != MTPX_F32 && r.position_dtype != MTPX_F64 && r.position_dtype != MTPX_I32 &&
+        r.position_dtype != MTPX_I64)
+        return invalid(ctx, "unknown position_dtype");
+    if (r.position_row < 0 || r.position_axis < 0)
+        return invalid(ctx, "negative position stride");
+    if (r.rows == 0 || r.rotated == 0)
+        return MTPX_OK;
+    MTPX_TRY(check_flat(ctx, r.positions, r.position_dtype == MTPX_F32 || r.position_dtype == MTPX_I32 ? 4 : 8, "positions"));
+    MTPX_TRY(check_flat(ctx, r.freq, 4, "freq"));
+    return check_flat(ctx, r.axis, 4, "axis");
+}
+// And those of the norm, with the counts.
+template <class R>
+int check_norms(mtpx_context *ctx, const R &r, int last_kind)
+{
+    if (!is_dtype(r.dtype))
+        return invalid(ctx, "dtype must be MTPX_F32, MTPX_BF16 or MTPX_F16");
+    if (r.rows < 0 || r.dim < 1)
+        return invalid(ctx, "rows must not be negative and dim positive");
+    if (r.dim > kMaxHeadDim || r.rows > kMaxRows || r.heads > 65535 || r.kv_heads > 65535)
+        return set_error(ctx, MTPX_E_CAPACITY, "dim beyond 256, more than 65535 heads or too many rows");
+    if (r.kind < MTPX_NORM_RMS || r.kind > last_kind)
+        return invalid(ctx, "unknown norm kind");
+    if (!(r.eps >= 0.f) || !std::isfinite(r.eps))
+        return invalid(ctx, "eps must not be negative");
+    for (const void *w : {r.q_weight, r.k_weight})
+        if (!aligned(w, dtype_bytes(r.dtype)))
+            return invalid(ctx, "a weight is not aligned to its elements");
+    return check_turn(ctx, r);
+}
+int check_place(mtpx_context *ctx, const mtpx_rows &x, const mtpx_rows &y, int maps, const char *name)
+{
+    if (x.data == y.data && (x.row != y.row || x.head != y.head || (maps > 1 && x.map != y.map)))
+        return invalid(ctx, std::string(name) + " in the place of its input needs its strides");
+    return MTPX_OK;
+}
+
+template <class R>
+HeadArgs head_args(const R &r, int maps)
+{
+    HeadArgs a{};
+    a.rows = r.rows;
+    a.vectors[0] = r.heads * maps;
+    a.vectors[1] = r.kv_heads * maps;
+    a.maps = maps;
+    a.dim = r.dim;
+    a.rotated = r.rotated;
+    a.interleaved = r.interleaved != 0;
+    a.kind = r.kind;
+    a.axes = r.axes;
+    a.position_dtype = r.position_dtype;
+    a.eps = r.eps;
+    a.in[0] = r.q;
+    a.in[1] = r.k;
+    a.weight[0] = r.q_weight;
+    a.weight[1] = r.k_weight;
+    a.positions = r.positions;
+    a.position_row = r.position_row;
+    a.position_axis = r.position_axis;
+    a.freq = r.freq;
+    a.axis = r.axis;
+    return a;
+}
+
+// The widest access that every piece of a vector allows, and the lanes of a
+// vector and of a row.  `wide`: the tensors' addresses and strides.
+template <class Fits>
+void shape_heads(HeadArgs &a, int64_t size, int most_lanes, const Fits &fits)
+{
+    const int half = a.rotated / 2;
+    a.width = (int)(16 / size);
+    while (a.width > 1 && !((a.interleaved ? a.rotated : half) % a.width == 0 && (a.dim - a.rotated) % a.width == 0 &&
+                            aligned(a.weight[0], a.width * size) && aligned(a.weight[1], a.width * size) && fits(a.width)))
+        a.width /= 2;
+    const int unit = a.interleaved ? std::max(a.width / 2, 1) : a.width;
+    const int units = half / unit + (a.dim - a.rotated) / a.width;
+    a.group = 1;
+    while (a.group < 64 && a.group < units)
+        a.group *= 2;
+    const int64_t vectors = std::max(a.vectors[0], a.vectors[1]);
+    a.lanes = a.group;
+    while (a.lanes < most_lanes && a.lanes < vectors * a.group)
+        a.lanes *= 2;
+}
+bool fits_rows(const mtpx_rows &t, int width, int64_t size, int maps)
+{
+    return !t.data || (aligned(t.data, width * size) && t.row % width == 0 && t.head % width == 0 &&
+                       (maps == 1 || t.map % width == 0));
+}
+
+// Few rows: a whole workgroup each, which takes the fewest steps one after the
+// other; a wave otherwise.
+int row_lanes(mtpx_context *ctx, int64_t rows) { return rows <= 8 * (int64_t)ctx->num_cus ? 256 : 64; }
+
+// Workgroups of the backward pass.
+int head_parts(mtpx_context *ctx, const HeadArgs &a)
+{
+    const int64_t together = 256 / a.lanes;
+    return (int)std::min<int64_t>((a.rows + together - 1) / together, 4 * (int64_t)ctx->num_cus);
+}
+
+int check_head_sizes(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r)
+{
+    if (r.heads < 1 || r.kv_heads < 0)
+        return invalid(ctx, "heads must be positive and kv_heads not negative");
+    if (r.maps != 1 && r.maps != 2)
+        return invalid(ctx, "maps must be 1 or 2");
+    return MTPX_OK;
+}
+
+int head_request(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r, bool back, HeadArgs &a)
+{
+    MTPX_TRY(check_head_sizes(ctx, r));
+    MTPX_TRY(check_norms(ctx, r, MTPX_NORM_LAYER));
+    a = head_args(r, r.maps);
+    const size_t size = dtype_bytes(r.dtype);
+    if (back) {
+        if ((r.dq_weight && !r.q_weight) || (r.dk_weight && !r.k_weight))
+            return invalid(ctx, "a weight's gradient without the weight");
+        for (const void *p : {r.dq_weight, r.dk_weight})
+            if (!aligned(p, size))
+                return invalid(ctx, "a weight's gradient is not aligned to its elements");
+        if (r.dpositions && r.position_dtype != MTPX_F32 && r.position_dtype != MTPX_F64)
+            return invalid(ctx, "integer positions have no gradient");
+        if (r.dpositions && !aligned(r.dpositions, r.position_dtype == MTPX_F64 ? 8 : 4))
+            return invalid(ctx, "dpositions is not aligned to its elements");
+    }
+    a.out[0] = back ? r.dq : r.q_out;
+    a.out[1] = back ? r.dk : r.k_out;
+    if (back) {
+        a.grad[0] = r.dq_out;
+        a.grad[1] = r.dk_out;
+        a.dweight[0] = r.dq_weight;
+        a.dweight[1] = r.kv_heads ? r.dk_weight : nullptr;
+        a.dpositions = r.dpositions;
+    }
+    const char *const names[2][4] = {{"q", "q_out", "dq_out", "dq"}, {"k", "k_out", "dk_out", "dk"}};
+    for (int i = 0; i < 2 && r.rows > 0; ++i) {
+        if (a.vectors[i] == 0)
+            continue;
+        MTPX_TRY(check_rows(ctx, a.in[i], r.dtype, names[i][0]));
+        MTPX_TRY(check_rows(ctx, a.out[i], r.dtype, names[i][back ? 3 : 1]));
+        if (back)
+            MTPX_TRY(check_rows(ctx, a.grad[i], r.dtype, names[i][2]));
+        MTPX_TRY(check_place(ctx, back ? a.grad[i] : a.in[i], a.out[i], r.maps, names[i][back ? 3 : 1]));
+    }
+    shape_heads(a, size, back ? 64 : row_lanes(ctx, r.rows), [&](int width) {
+        for (int i = 0; i < 2; ++i)
+            if (a.vectors[i] && !(fits_rows(a.in[i], width, size, r.maps) && fits_rows(a.out[i], width, size, r.maps) &&
+                                  fits_rows(a.grad[i], width, size, r.maps)))
+                return false;
+        return true;
+    });
+    return MTPX_OK;
+}
+
+// Enough for any alignment of the tensors.
+size_t head_bytes(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r)
+{
+    const int64_t parts = std::min<int64_t>(r.rows, 4 * (int64_t)ctx->num_cus);
+    return std::max<size_t>(sizeof(float) * 2 * (size_t)parts * r.dim, 16);
+}
+
+// A cache's pages: what the host can see of them.
+int check_pages(mtpx_context *ctx, const mtpx_pages &c, int dtype)
+{
+    if (c.pages < 0 || c.page_rows < 1 || c.table_width < 0 || c.table_row < 0)
+        return invalid(ctx, "pages, table_width and table_row must not be negative and page_rows positive");
+    if (c.pages > INT32_MAX || c.page_rows > 1 << 20 || (int64_t)c.table_width * c.page_rows > kMaxRoom)
+        return set_error(ctx, MTPX_E_CAPACITY, "too many pages, rows of a page or rows of a sequence");
+    if (c.pages > 0) {
+        MTPX_TRY(check_rows(ctx, c.k, dtype, "cache.k"));
+        MTPX_TRY(check_rows(ctx, c.v, dtype, "cache.v"));
+        if (c.k_page < 0 || c.v_page < 0)
+            return invalid(ctx, "negative page stride");
+    }
+    return c.table_width > 0 ? check_flat(ctx, c.table, 4, "table") : MTPX_OK;
+}
+int check_batch(mtpx_context *ctx, int sequences, const int *offsets, const int *lengths)
+{
+    if (sequences < 0)
+        return invalid(ctx, "negative count of sequences");
+    if (sequences > kMaxSequences)
+        return set_error(ctx, MTPX_E_CAPACITY, "more than 2^24 sequences");
+    if (sequences == 0)
+        return MTPX_OK;
+    MTPX_TRY(check_flat(ctx, offsets, 4, "offsets"));
+    return check_flat(ctx, lengths, 4, "lengths");
+}
+bool pages_fit(const mtpx_pages &c, int width, int64_t size)
+{
+    return fits_rows(c.k, width, size, 2) && fits_rows(c.v, width, size, 2) && c.k_page % width == 0 && c.v_page % width == 0;
+}
+
+// How the work of a call is split, from what the host knows: rows, sequences,
+// the most new rows of one, and the room of the tables.
+struct PagedPlan {
+    int deep = 0, deep_blocks = 1, deep_splits = 1;
+    int broad_columns = 64, broad_tiles = 0, broad_splits = 1;
+    size_t deep_bytes = 0, broad_bytes = 0;
+    int64_t items = 0;
+};
+// Sequences of so many columns go to the deep part.
+constexpr int kDeepColumns = 32;
+
+PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
+{
+    PagedPlan p;
+    const int64_t group = r.heads / r.kv_heads, cus = ctx->num_cus;
+    const int64_t room = (int64_t)r.cache.table_width * r.cache.page_rows;
+    const int64_t most = r.max_rows > 0 ? std::min<int64_t>(r.max_rows, r.rows) : r.rows;
+    const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128;
+    const size_t part = sizeof(float) * 2 * (4 + 2 * width);
+    if (group <= kDeepColumns) {
+        p.deep = kDeepColumns;
+        p.deep_blocks = (int)(std::min<int64_t>(most * group, kDeepColumns) + 15) / 16;
+        const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * p.deep_blocks, 1);
+        if (room > 1024)
+            p.deep_splits = (int)std::min<int64_t>({(8 * cus + base - 1) / base, (room + 255) / 256, kMaxSplits});
+        if (p.deep_splits > 1)
+            p.deep_bytes = part * 16 * (size_t)base * p.deep_splits;
+        p.items += base * p.deep_splits;
+    }
+    if (p.deep == 0 || most * group > kDeepColumns) {
+        const int64_t columns = r.rows * group;
+        if (width <= 64 && r.dtype != MTPX_F32 && columns / 128 * r.kv_heads >= 2 * cus)
+            p.broad_columns = 128;
+        const int64_t base = std::max<int64_t>(columns / p.broad_columns, 1) * r.kv_heads;
+        p.broad_tiles = (int)std::min<int64_t>(columns / p.broad_columns + r.sequences, INT32_MAX);
+        if (base < 2 * cus && room > 1024)
+            p.broad_splits = (int)std::min<int64_t>({(2 * cus + base - 1) / base, (room + 1023) / 1024, kMaxSplits});
+        if (p.broad_splits > 1)
+            p.broad_bytes = part * p.broad_splits * (size_t)r.rows * r.heads;
+        p.items += (int64_t)p.broad_tiles * r.kv_heads * p.broad_splits;
+    }
+    return p;
+}
+
+int check_paged(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
+{
+    MTPX_TRY(check_heads(ctx, r.dtype, r.heads, r.kv_heads, r.dim, r.scale));
+    if (r.rows < 0 || r.max_rows < 0 || r.sequences < 0)
+        return invalid(ctx, "negative count");
+    if (r.cache.page_rows < 1 || r.cache.table_width < 0)
+        return invalid(ctx, "page_rows must be positive and table_width not negative");
+    if (r.rows > kMaxRows || r.sequences > kMaxSequences || r.heads > 65535 || r.cache.page_rows > 1 << 20 ||
+        (int64_t)r.cache.table_width * r.cache.page_rows > kMaxRoom)
+        return set_error(ctx, MTPX_E_CAPACITY, "too many rows, sequences, heads or rows of a sequence");
+    if (r.rows * r.heads > kMaxGroups || paged_plan(ctx, r).items > kMaxGroups)
+        return set_error(ctx, MTPX_E_CAPACITY, "too many rows and heads for one launch");
+    return MTPX_OK;
+}
+
+}  // namespace
+}  // namespace mtpx
+
+extern "C" {
+
+int mtpx_head_norm_rotary(mtpx_context *ctx, const mtpx_head_norm_rotary_request *req)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        HeadArgs a;
+        MTPX_TRY(head_request(ctx, *req, false, a));
+        if (a.rows == 0)
+            return MTPX_OK;
+        OnDevice here(ctx->device);
+        HIP_TRY(launch_head_forward(req->dtype, a, (hipStream_t)req->stream), "launch head norm");
+        return MTPX_OK;
+    });
+}
+
+int mtpx_head_norm_rotary_workspace(mtpx_context *ctx, const mtpx_head_norm_rotary_request *req, size_t *bytes)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req || !bytes)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        if (req->rows < 0 || req->dim < 1)
+            return invalid(ctx, "rows must not be negative and dim positive");
+        if (req->dim > kMaxHeadDim || req->rows > kMaxRows)
+            return set_error(ctx, MTPX_E_CAPACITY, "dim beyond 256 or too many rows");
+        *bytes = head_bytes(ctx, *req);
+        return MTPX_OK;
+    });
+}
+
+int mtpx_head_norm_rotary_backward(mtpx_context *ctx, const mtpx_head_norm_rotary_request *req)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        HeadArgs a;
+        MTPX_TRY(head_request(ctx, *req, true, a));
+        MTPX_TRY(check_workspace(ctx, req->workspace, req->workspace_bytes, head_bytes(ctx, *req)));
+        a.part = static_cast<float *>(req->workspace);
+        a.parts = head_parts(ctx, a);
+        OnDevice here(ctx->device);
+        HIP_TRY(launch_head_backward(req->dtype, a, (hipStream_t)req->stream), "launch head norm gradient");
+        return MTPX_OK;
+    });
+}
+
+int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *req)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        const mtpx_append_paged_request &r = *req;
+        if (r.heads < 0 || r.kv_heads < 1)
+            return invalid(ctx, "heads must not be negative and kv_heads positive");
+        MTPX_TRY(check_norms(ctx, r, MTPX_NORM_NONE));
+        MTPX_TRY(check_batch(ctx, r.sequences, r.offsets, r.lengths));
+        MTPX_TRY(check_pages(ctx, r.cache, r.dtype));
+        if (r.rows == 0 || r.sequences == 0)
+            return MTPX_OK;
+        MTPX_TRY(check_rows(ctx, r.k, r.dtype, "k"));
+        MTPX_TRY(check_rows(ctx, r.v, r.dtype, "v"));
+        HeadArgs a = head_args(r, 2);
+        a.cache = r.cache;
+        a.v = r.v;
+        a.offsets = r.offsets;
+        a.lengths = r.lengths;
+        a.sequences = r.sequences;
+        if (r.heads > 0) {
+            MTPX_TRY(check_rows(ctx, r.q, r.dtype, "q"));
+            MTPX_TRY(check_rows(ctx, r.q_out, r.dtype, "q_out"));
+            MTPX_TRY(check_place(ctx, r.q, r.q_out, 2, "q_out"));
+            a.out[0] = r.q_out;
+        }
+        const int64_t size = (int64_t)dtype_bytes(r.dtype);
+        shape_heads(a, size, row_lanes(ctx, r.rows), [&](int width) {
+            return fits_rows(a.in[1], width, size, 2) && fits_rows(a.v, width, size, 2) && pages_fit(r.cache, width, size) &&
+                   (r.heads == 0 || (fits_rows(a.in[0], width, size, 2) && fits_rows(a.out[0], width, size, 2)));
+        });
+        OnDevice here(ctx->device);
+        HIP_TRY(launch_head_append(r.dtype, a, (hipStream_t)r.stream), "launch append");
+        return MTPX_OK;
+    });
+}
+
+int mtpx_diff_attention_paged_workspace(mtpx_context *ctx, const mtpx_diff_attention_paged_request *req, size_t *bytes)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req || !bytes)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        mtpx_diff_attention_paged_request r = *req;
+        r.scale = 1.f;
+        MTPX_TRY(check_paged(ctx, r));
+        const PagedPlan p = paged_plan(ctx, r);
+        *bytes = p.deep_bytes + p.broad_bytes;
+        return MTPX_OK;
+    });
+}
+
+int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged_request *req)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !req)
+            return set_error(ctx, MTPX_E_INVALID, "null argument");
+        const mtpx_diff_attention_paged_request &r = *req;
+        MTPX_TRY(check_paged(ctx, r));
+        MTPX_TRY(check_pages(ctx, r.cache, r.dtype));
+        MTPX_TRY(check_batch(ctx, r.sequences, r.offsets, r.lengths));
+        if (r.rows == 0 || r.sequences == 0)
+            return MTPX_OK;
+        MTPX_TRY(check_rows(ctx, r.q, r.dtype, "q"));
+        MTPX_TRY(check_rows(ctx, r.out, r.dtype, "out"));
+        MTPX_TRY(check_flat(ctx, r.lambda, 4, "lambda"));
+        const PagedPlan p = paged_plan(ctx, r);
+        MTPX_TRY(check_workspace(ctx, r.workspace, r.workspace_bytes, p.deep_bytes + p.broad_bytes));
+        const int64_t size = (int64_t)dtype_bytes(r.dtype);
+        PagedArgs a{};
+        a.rows = r.rows;
+        a.sequences = r.sequences;
+        a.heads = r.heads;
+        a.kv_heads = r.kv_heads;
+        a.dim = r.dim;
+        a.causal = r.causal != 0;
+        a.scale = r.scale;
+        a.q = r.q;
+        a.out = r.out;
+        a.cache = r.cache;
+        a.offsets = r.offsets;
+        a.lengths = r.lengths;
+        a.lambda = r.lambda;
+        a.vec = r.dim * size % 16 == 0 && whole_pieces(r.q, size) && whole_pieces(r.out, size) &&
+                pages_fit(r.cache, (int)(16 / size), size);
+        int bits = 0;
+        while ((1 << bits) < r.cache.page_rows)
+            ++bits;
+        a.page_shift = bits;
+        a.page_magic = (unsigned)((uint64_t(1) << (31 + bits)) / (uint64_t)r.cache.page_rows + 1);
+        a.deep = p.deep;
+        a.deep_blocks = p.deep_blocks;
+        a.deep_splits = p.deep_splits;
+        a.broad_columns = p.broad_columns;
+        a.broad_tiles = p.broad_tiles;
+        a.broad_splits = p.broad_splits;
+        a.deep_part = static_cast<float *>(r.workspace);
+        a.broad_part = a.deep_part + p.deep_bytes / sizeof(float);
+        OnDevice here(ctx->device);
+        HIP_TRY(launch_paged(r.dtype, a, (hipStream_t)r.stream), "launch paged attention");
+        return MTPX_OK;
+    });
+}
+
+}  // extern "C"

@@ -1,13 +1,15 @@
 """Operators on device tensors (the last section of include/mtpx.h) for torch
 tensors: rotary positions with several axes, differential attention over
-ragged batches and over a cache, and the norms around a block with its gate
-and residual scale.
+ragged batches and over a cache, the norms around a block with its gate
+and residual scale, norms of queries and keys with the rotation in the same
+pass, and a cache in pages: rows appended to it, and differential attention
+of a chunk of new rows over it.
 
 Every function takes the Context first, queues its kernels on torch's current
 stream of the tensors' device and returns without waiting; workspaces and
 results come from torch's allocator, so a call can be captured into a graph.
 Functions with gradients come twice: as a pair (f, f_backward) on plain
-tensors, and as an autograd function (RotaryFn, DiffAttentionFn, NormBlockFn).
+tensors, and as an autograd function (RotaryFn, DiffAttentionFn, NormBlockFn, HeadNormRotaryFn).
 Gradients are first derivatives: differentiating one of them again (a loss of
 forces that were taken through a block) raises.
 Tensors are float32, bfloat16 or float16; their last dimension has to be
@@ -39,6 +41,7 @@ import torch  # noqa: E402
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POSITION_DTYPES = {torch.float32: 0, torch.float64: 3, torch.int32: 4, torch.int64: 5}
 NORMS = {"rms": 0, "layer": 1}
+APPEND_NORMS = {"rms": 0, "layer": 1, "none": 2}
 GATES = {"none": 0, "sigmoid": 1, "tanh": 2}
 
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -88,20 +91,59 @@ class NormRequest(C.Structure):
                 ("dgate_row", _l), ("workspace", _p), ("workspace_bytes", C.c_size_t)]
 
 
+class HeadNormRequest(C.Structure):
+    """mtpx_head_norm_rotary_request."""
+    _fields_ = [("stream", _p), ("dtype", _i), ("rows", _l), ("heads", _i), ("kv_heads", _i),
+                ("maps", _i), ("dim", _i), ("rotated", _i), ("kind", _i), ("interleaved", _i),
+                ("eps", _f), ("q", Rows), ("k", Rows), ("q_out", Rows), ("k_out", Rows),
+                ("q_weight", _p), ("k_weight", _p), ("positions", _p), ("position_dtype", _i),
+                ("position_row", _l), ("position_axis", _l), ("axes", _i), ("freq", _p),
+                ("axis", _p), ("dq_out", Rows), ("dk_out", Rows), ("dq", Rows), ("dk", Rows),
+                ("dq_weight", _p), ("dk_weight", _p), ("dpositions", _p), ("workspace", _p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Pages(C.Structure):
+    """mtpx_pages."""
+    _fields_ = [("k", Rows), ("v", Rows), ("k_page", _l), ("v_page", _l), ("pages", _l),
+                ("page_rows", _i), ("table", _p), ("table_row", _l), ("table_width", _i)]
+
+
+class AppendRequest(C.Structure):
+    """mtpx_append_paged_request."""
+    _fields_ = [("stream", _p), ("dtype", _i), ("rows", _l), ("sequences", _i), ("heads", _i),
+                ("kv_heads", _i), ("dim", _i), ("rotated", _i), ("kind", _i), ("interleaved", _i),
+                ("eps", _f), ("q", Rows), ("k", Rows), ("v", Rows), ("q_out", Rows),
+                ("q_weight", _p), ("k_weight", _p), ("positions", _p), ("position_dtype", _i),
+                ("position_row", _l), ("position_axis", _l), ("axes", _i), ("freq", _p),
+                ("axis", _p), ("cache", Pages), ("offsets", _p), ("lengths", _p)]
+
+
+class PagedRequest(C.Structure):
+    """mtpx_diff_attention_paged_request."""
+    _fields_ = [("stream", _p), ("dtype", _i), ("rows", _l), ("sequences", _i), ("max_rows", _i),
+                ("heads", _i), ("kv_heads", _i), ("dim", _i), ("causal", _i), ("scale", _f),
+                ("q", Rows), ("cache", Pages), ("offsets", _p), ("lengths", _p), ("lambda_", _p),
+                ("out", Rows), ("workspace", _p), ("workspace_bytes", C.c_size_t)]
+
+
 def _packer(cls):
     """The C layout of a request as one flat list of its fields: packing it
     takes a third of the time that filling the ctypes structure does, which
     counts in calls of a few microseconds."""
     codes = {_p: "P", _i: "i", _l: "q", _f: "f", C.c_size_t: "N"}
-    fmt = "".join("Pqqq" if f is Rows else codes[f] for _, f in cls._fields_)
+    # (the pages' structure ends with an int, padded to its strictest alignment)
+    codes[Rows], codes[Pages] = "Pqqq", "PqqqPqqqqqqiPqi0q"
+    fmt = "".join(codes[f] for _, f in cls._fields_)
     # (a structure's size is a multiple of its strictest alignment)
     s = struct.Struct("@" + fmt + "0P")
     assert s.size == C.sizeof(cls)
     return s.pack
 
 
-_pack_rotary, _pack_attention, _pack_cache, _pack_norm = (
-    _packer(c) for c in (RotaryRequest, AttentionRequest, CacheRequest, NormRequest))
+_pack_rotary, _pack_attention, _pack_cache, _pack_norm, _pack_heads, _pack_append, _pack_paged = (
+    _packer(c) for c in (RotaryRequest, AttentionRequest, CacheRequest, NormRequest,
+                         HeadNormRequest, AppendRequest, PagedRequest))
 
 _lib = None
 
@@ -117,11 +159,14 @@ def _ops():
         L.mtpx_sequences_destroy.argtypes = [_p]
         L.mtpx_sequences_destroy.restype = None
         for name, req in (("diff_attention", C.POINTER(AttentionRequest)),
-                          ("diff_attention_cache", _p), ("norm_block", _p)):
+                          ("diff_attention_cache", _p), ("norm_block", _p),
+                          ("head_norm_rotary", _p), ("diff_attention_paged", _p)):
             getattr(L, "mtpx_" + name).argtypes = [ctx, req]
             getattr(L, "mtpx_%s_workspace" % name).argtypes = [ctx, req, size]
         L.mtpx_diff_attention_backward.argtypes = [ctx, C.POINTER(AttentionRequest)]
         L.mtpx_norm_block_backward.argtypes = [ctx, _p]
+        L.mtpx_head_norm_rotary_backward.argtypes = [ctx, _p]
+        L.mtpx_append_paged.argtypes = [ctx, _p]
         _lib = L
     return _lib
 
@@ -480,6 +525,235 @@ def norm_block_backward(ctx, ds, dn, x, y, gate, post_weight, pre_weight, stats,
     return dx, dy, dgate, dpost, dpre
 
 
+# ---- norms of queries and keys, with their rotation ---------------------------------
+
+
+def _turns(ctx, positions, freq, axis, rows):
+    """The checked fields of a rotation, as a request has them, and how many
+    elements of a head it turns."""
+    sp = _tensor(ctx, positions, "positions", (rows, None)).stride()
+    ptype = POSITION_DTYPES.get(positions.dtype)
+    if ptype is None:
+        _fail("positions are %s, not float32, float64, int32 or int64" % positions.dtype)
+    pairs = (freq.numel(),) if isinstance(freq, torch.Tensor) else (None,)
+    _strides(ctx, freq, "freq", pairs, torch.float32)
+    _strides(ctx, axis, "axis", pairs, torch.int32)
+    return 2 * pairs[0], (positions.data_ptr(), ptype, sp[0], sp[1], positions.shape[1],
+                          freq.data_ptr(), axis.data_ptr())
+
+
+def _head_rows(ctx, t, name, shape, of):
+    """Heads [rows, heads, dim] or [rows, heads, maps, dim] as a request has them."""
+    s = _strides(ctx, t, name, shape, of)
+    return t.data_ptr(), s[0], s[1], s[2] if len(shape) == 4 else 0
+
+
+def _whole(t, shape):
+    """The same of a contiguous result."""
+    d = shape[-1]
+    return t.data_ptr(), t.numel() // max(1, len(t)), d * (shape[2] if len(shape) == 4 else 1), d
+
+
+def _heads_of(ctx, q, k):
+    """Checks what q and k share: the type's code, rows, heads, kv heads, maps and dim."""
+    dims = 4 if isinstance(q, torch.Tensor) and q.dim() == 4 else 3
+    dtype, shape = _typed(ctx, q, "q", dims), q.shape
+    if dims == 4 and shape[2] not in (1, 2):
+        _fail("q has %d maps, not 1 or 2" % shape[2])
+    kv = 0
+    if k is not None:
+        if not isinstance(k, torch.Tensor) or k.dim() != dims:
+            _fail("k has not as many dimensions as q")
+        kv = k.shape[1]
+        _tensor(ctx, k, "k", (shape[0], kv, *shape[2:]), q.dtype)
+        if kv == 0:
+            _fail("k has no heads")
+    return dtype, shape[0], shape[1], kv, shape[2] if dims == 4 else 1, shape[-1]
+
+
+def _weight(ctx, w, name, dim, of):
+    if w is None:
+        return 0
+    _strides(ctx, w, name, (dim,), of)
+    return w.data_ptr()
+
+
+def head_norm_rotary(ctx, q, k, q_weight, k_weight, positions, freq, axis, *, kind="rms",
+                     eps=1e-6, interleaved=False):
+    """Norms of queries and keys for each head, and their rotation: of q [rows,
+    heads, dim] or [rows, heads, maps, dim] and k (the same with its own heads;
+    None: q only) every head and map becomes norm(x) weight, turned as by
+    rotary; weights [dim] or None, positions, freq and axis as there.  Returns
+    (q, k)."""
+    dtype, rows, heads, kv, maps, dim = _heads_of(ctx, q, k)
+    of = q.dtype
+    if kind not in NORMS:
+        _fail("kind is one of %s" % (tuple(NORMS),))
+    rotated, turn = _turns(ctx, positions, freq, axis, rows)
+    qo = q.new_empty(q.shape)
+    ko, k_in, k_out = None, _NO_ROWS, _NO_ROWS
+    if k is not None:
+        ko = k.new_empty(k.shape)
+        k_in, k_out = _head_rows(ctx, k, "k", k.shape, of), _whole(ko, k.shape)
+    req = _pack_heads(
+        _stream(ctx), dtype, rows, heads, kv, maps, dim, rotated, NORMS[kind], interleaved, eps,
+        *_head_rows(ctx, q, "q", q.shape, of), *k_in, *_whole(qo, q.shape), *k_out,
+        _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of),
+        *turn, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, 0)
+    ctx._check(_ops().mtpx_head_norm_rotary(ctx.h, req), "head_norm_rotary")
+    return qo, ko
+
+
+def head_norm_rotary_backward(ctx, dq, dk, q, k, q_weight, k_weight, positions, freq, axis, *,
+                              kind="rms", eps=1e-6, interleaved=False, dpositions=False):
+    """(dq, dk, dq_weight, dk_weight, dpositions) from the gradients of the
+    results and the forward pass's inputs; None in the place of an input that
+    was not given, and of the positions' without dpositions (which needs
+    float32 or float64 ones; a 32-bit sum for both)."""
+    dtype, rows, heads, kv, maps, dim = _heads_of(ctx, q, k)
+    of = q.dtype
+    if kind not in NORMS:
+        _fail("kind is one of %s" % (tuple(NORMS),))
+    rotated, turn = _turns(ctx, positions, freq, axis, rows)
+    if (dk is None) != (k is None):
+        _fail("dk is given with k")
+    gq, gk, dpos = q.new_empty(q.shape), None, None
+    k_in, k_grad, k_out = _NO_ROWS, _NO_ROWS, _NO_ROWS
+    if k is not None:
+        gk = k.new_empty(k.shape)
+        k_in, k_grad = _head_rows(ctx, k, "k", k.shape, of), _head_rows(ctx, dk, "dk", k.shape, of)
+        k_out = _whole(gk, k.shape)
+    wq, wk = _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of)
+    dwq = None if q_weight is None else q.new_empty(dim)
+    dwk = None if k_weight is None else q.new_zeros(dim) if k is None else q.new_empty(dim)
+    if dpositions:
+        dpos = torch.empty(positions.shape, dtype=positions.dtype, device=q.device)
+    size = _bytes(ctx, _ops().mtpx_head_norm_rotary_workspace, HeadNormRequest, rows=rows, dim=dim)
+    w = _workspace(ctx, size)  # held until the kernels are queued
+    req = _pack_heads(
+        _stream(ctx), dtype, rows, heads, kv, maps, dim, rotated, NORMS[kind], interleaved, eps,
+        *_head_rows(ctx, q, "q", q.shape, of), *k_in, *_NO_ROWS, *_NO_ROWS, wq, wk, *turn,
+        *_head_rows(ctx, dq, "dq", q.shape, of), *k_grad, *_whole(gq, q.shape), *k_out,
+        _ptr(dwq), _ptr(dwk), _ptr(dpos), w.data_ptr(), size)
+    ctx._check(_ops().mtpx_head_norm_rotary_backward(ctx.h, req), "head_norm_rotary_backward")
+    return gq, gk, dwq, dwk, dpos
+
+
+# ---- a cache in pages ------------------------------------------------------------------
+
+
+def _pages(ctx, k_pages, v_pages, table, offsets, lengths, kv, dim, of):
+    """The checked fields of a cache and its batch: (mtpx_pages, offsets, lengths, sequences)."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 5:
+        _fail("k_pages is not [pages, page rows, kv heads, 2, dim]")
+    n, page = k_pages.shape[:2]
+    sk = _strides(ctx, k_pages, "k_pages", (n, page, kv, 2, dim), of)
+    sv = _strides(ctx, v_pages, "v_pages", (n, page, kv, 2 * dim), of)
+    if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
+        _fail("lengths are not [sequences]")
+    seqs = len(lengths)
+    _strides(ctx, lengths, "lengths", (seqs,), torch.int32)
+    _strides(ctx, offsets, "offsets", (seqs + 1,), torch.int32)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        _fail("table is not [sequences, pages of a sequence]")
+    width = table.shape[1]
+    st = _strides(ctx, table, "table", (seqs, width), torch.int32)
+    return (k_pages.data_ptr(), sk[1], sk[2], sk[3], v_pages.data_ptr(), sv[1], sv[2], dim, sk[0],
+            sv[0], n, page, table.data_ptr(), st[0], width), offsets.data_ptr(), lengths.data_ptr(), seqs
+
+
+def append_paged(ctx, k, v, k_pages, v_pages, table, offsets, lengths, positions, freq, axis, *,
+                 q=None, kind="none", q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                 out=None):
+    """Puts a batch's new rows into a cache: k [rows, kv heads, 2, dim], normed
+    (kind "rms" or "layer", weights [dim] or None; "none": as it is) and turned
+    by positions [rows, axes] as by head_norm_rotary, into k_pages [pages, page
+    rows, kv heads, 2, dim], and v [rows, kv heads, 2 dim] into v_pages [pages,
+    page rows, kv heads, 2 dim].  Sequence i has rows offsets[i] to offsets[i +
+    1] - 1 and lengths[i] rows with them; its row t lies in page table[i, t //
+    page rows].  offsets [sequences + 1], lengths [sequences] and table
+    [sequences, width] are int32 on the device and are not read on the host.
+    With q [rows, heads, 2, dim] its queries are normed and turned as well:
+    returns them (in out, which may be q), else None.  Rows of no sequence are
+    left as they are."""
+    dtype = _typed(ctx, k, "k", 4)
+    of = k.dtype
+    rows, kv, _, dim = k.shape
+    k_in = _head_rows(ctx, k, "k", (rows, kv, 2, dim), of)
+    sv = _strides(ctx, v, "v", (rows, kv, 2 * dim), of)
+    if kind not in APPEND_NORMS:
+        _fail("kind is one of %s" % (tuple(APPEND_NORMS),))
+    if kind == "none" and (q_weight is not None or k_weight is not None):
+        _fail("weights without a norm")
+    cache, off, length, seqs = _pages(ctx, k_pages, v_pages, table, offsets, lengths, kv, dim, of)
+    rotated, turn = _turns(ctx, positions, freq, axis, rows)
+    heads, q_in, q_out = 0, _NO_ROWS, _NO_ROWS
+    if q is not None:
+        _typed(ctx, q, "q", 4)
+        heads = q.shape[1]
+        shape = (rows, heads, 2, dim)
+        q_in = _head_rows(ctx, q, "q", shape, of)
+        if out is None:
+            out = q.new_empty(shape)
+            q_out = _whole(out, shape)
+        else:
+            q_out = _head_rows(ctx, out, "out", shape, of)
+    elif out is not None:
+        _fail("out without q")
+    req = _pack_append(
+        _stream(ctx), dtype, rows, seqs, heads, kv, dim, rotated, APPEND_NORMS[kind], interleaved,
+        eps, *q_in, *k_in, v.data_ptr(), sv[0], sv[1], dim, *q_out,
+        _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of),
+        *turn, *cache, off, length)
+    ctx._check(_ops().mtpx_append_paged(ctx.h, req), "append_paged")
+    return out
+
+
+def _paged_sizes(page, width, **sizes):
+    return PagedRequest(cache=Pages(page_rows=page, table_width=width), **sizes)
+
+
+def diff_attention_paged(ctx, q, k_pages, v_pages, lam, table, offsets, lengths, *, causal=True,
+                         scale=None, max_rows=None, out=None):
+    """Differential attention of each sequence's new rows over its pages, where
+    append_paged has put them already: q [rows, heads, 2, dim], the other
+    arguments as there, lam [heads] float32.  Row j of m new ones sees the
+    first lengths[i] - m + j + 1 rows of its sequence, without causal all of
+    them.  max_rows: the most new rows of a sequence, where the caller knows it
+    (1 in a plain decoding step), which saves work.  Returns [rows, heads, 2
+    dim]; rows of no sequence are left as they are."""
+    dtype = _typed(ctx, q, "q", 4)
+    of = q.dtype
+    rows, heads, _, dim = q.shape
+    sq = _strides(ctx, q, "q", (rows, heads, 2, dim), of)
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 5:
+        _fail("k_pages is not [pages, page rows, kv heads, 2, dim]")
+    kv = k_pages.shape[2]
+    cache, off, length, seqs = _pages(ctx, k_pages, v_pages, table, offsets, lengths, kv, dim, of)
+    _strides(ctx, lam, "lam", (heads,), torch.float32)
+    if max_rows is None:
+        max_rows = 0
+    elif max_rows < 1:
+        _fail("max_rows must be positive")
+    else:
+        max_rows = min(max_rows, max(rows, 1))
+    shape = (rows, heads, 2 * dim)
+    if out is None:
+        out, so = q.new_empty(shape), (heads * 2 * dim, 2 * dim)
+    else:
+        so = _strides(ctx, out, "out", shape, of)
+    size = _bytes(ctx, _ops().mtpx_diff_attention_paged_workspace, _paged_sizes, dtype=dtype,
+                  rows=rows, sequences=seqs, max_rows=max_rows, heads=heads, kv_heads=kv, dim=dim,
+                  page=cache[11], width=cache[14])
+    w = _workspace(ctx, size) if size else None  # held until the kernels are queued
+    req = _pack_paged(
+        _stream(ctx), dtype, rows, seqs, max_rows, heads, kv, dim, causal,
+        dim ** -0.5 if scale is None else scale, q.data_ptr(), sq[0], sq[1], sq[2], *cache, off,
+        length, lam.data_ptr(), out.data_ptr(), so[0], so[1], dim, _ptr(w), size)
+    ctx._check(_ops().mtpx_diff_attention_paged(ctx.h, req), "diff_attention_paged")
+    return out
+
+
 # ---- autograd ------------------------------------------------------------------------
 
 
@@ -594,3 +868,28 @@ class NormBlockFn(torch.autograd.Function):
         grads = norm_block_backward(fn.ctx, _last_contiguous(ds), _last_contiguous(dn), x, y,
                                     gate, post_weight, pre_weight, stats, **fn.options)
         return (None, *grads, None)
+
+
+class HeadNormRotaryFn(torch.autograd.Function):
+    """HeadNormRotaryFn.apply(ctx, q, k, q_weight, k_weight, positions, freq,
+    axis, options): (q, k) of head_norm_rotary with the keyword arguments in the
+    dict options, with the gradients of q, k, the weights and floating-point
+    positions.  freq and the options have none."""
+
+    @staticmethod
+    def forward(fn, ctx, q, k, q_weight, k_weight, positions, freq, axis, options):
+        fn.ctx, fn.options, fn.learned = ctx, dict(options), _learned(freq=freq, **options)
+        fn.save_for_backward(q, k, q_weight, k_weight, positions, freq, axis)
+        fn.set_materialize_grads(False)
+        return head_norm_rotary(ctx, q, k, q_weight, k_weight, positions, freq, axis, **options)
+
+    @staticmethod
+    @_first_only
+    def backward(fn, dq, dk):
+        q, k, q_weight, k_weight, positions, freq, axis = fn.saved_tensors
+        dq = torch.zeros_like(q) if dq is None else dq
+        dk = torch.zeros_like(k) if dk is None and k is not None else dk
+        grads = head_norm_rotary_backward(
+            fn.ctx, _last_contiguous(dq), _last_contiguous(dk), q, k, q_weight, k_weight, positions,
+            freq, axis, dpositions=positions.requires_grad, **fn.options)
+        return (None, *grads, None, None, None)

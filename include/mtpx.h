@@ -774,6 +774,135 @@ int mtpx_norm_block_backward(mtpx_context *ctx, const mtpx_norm_block_request *r
 int mtpx_norm_block_workspace(mtpx_context *ctx, const mtpx_norm_block_request *request,
                               size_t *bytes);
 
+/* Norms of queries and keys for each head with the rotary positions in the
+ * same pass.  For every head (and map) of row r, over its dim elements,
+ *   u = norm(x),  z = u weight,  y = z turned by the row's positions
+ * with norm as in mtpx_norm_block (MTPX_NORM_RMS or MTPX_NORM_LAYER), the
+ * weights [dim] of queries and of keys (NULL: 1) shared by all heads and maps,
+ * and the rotation of mtpx_rotary (rotated 0: none).  q_out may be q and
+ * k_out k (same strides) where no backward pass follows.
+ * Backward: reads q, k, the gradients dq_out and dk_out of the results and the
+ * weights; writes dq and dk, and each of dq_weight, dk_weight [dim] and
+ * dpositions ([rows][axes], contiguous, in the positions' type, a 32-bit sum
+ * over the heads of q and k) unless NULL.  The statistics are formed again
+ * from q and k: nothing is kept between the passes.  dq may be dq_out and dk
+ * dk_out (same strides). */
+typedef struct mtpx_head_norm_rotary_request {
+    void *stream;
+    int dtype;
+    int64_t rows;               /* below 2^26 */
+    int heads, kv_heads;        /* kv_heads 0: q only */
+    int maps;                   /* 1 or 2 */
+    int dim, rotated;           /* dim <= 256, rotated even and at most dim */
+    int kind, interleaved;
+    float eps;
+    mtpx_rows q, k, q_out, k_out;
+    const void *q_weight, *k_weight;
+    const void *positions;      /* [rows][axes]; MTPX_F32, F64, I32 or I64 */
+    int position_dtype;
+    int64_t position_row, position_axis;
+    int axes;                   /* 1 to 8 */
+    const float *freq;          /* [rotated / 2], radians per unit */
+    const int *axis;            /* [rotated / 2], each in [0, axes); others are read as axis 0 */
+    mtpx_rows dq_out, dk_out, dq, dk; /* backward only */
+    void *dq_weight, *dk_weight, *dpositions;
+    void *workspace;            /* backward only, 16-byte aligned */
+    size_t workspace_bytes;
+} mtpx_head_norm_rotary_request;
+int mtpx_head_norm_rotary(mtpx_context *ctx, const mtpx_head_norm_rotary_request *request);
+int mtpx_head_norm_rotary_backward(mtpx_context *ctx, const mtpx_head_norm_rotary_request *request);
+/* Workspace of mtpx_head_norm_rotary_backward. */
+int mtpx_head_norm_rotary_workspace(mtpx_context *ctx, const mtpx_head_norm_rotary_request *request,
+                                    size_t *bytes);
+
+/* A cache in pages of page_rows rows each.  Row t of sequence i is row
+ * t % page_rows of page table[i * table_row + t / page_rows] (device array):
+ * element e of map m of its head h is at
+ *   k.data[page * k_page + (t % page_rows) * k.row + h * k.head + m * k.map + e]
+ * and v in the same way (two "maps" of dim).  A sequence has room for
+ * table_width * page_rows rows.  A page may stand in several tables (a common
+ * prefix).  An entry outside [0, pages) names no page: what is appended there
+ * is dropped, and its keys are seen by no row. */
+typedef struct mtpx_pages {
+    mtpx_rows k, v;
+    int64_t k_page, v_page;
+    int64_t pages;              /* below 2^31 */
+    int page_rows;              /* 1 to 2^20 */
+    const int *table;
+    int64_t table_row;
+    int table_width;            /* table_width * page_rows at most 2^30 */
+} mtpx_pages;
+
+/* The new rows of a batch of sequences: sequence i has the rows offsets[i] to
+ * offsets[i + 1] - 1 of q, k and v (device array of sequences + 1, ascending;
+ * read as 0 below 0 and as `rows` beyond), and with them lengths[i] rows in
+ * all: row j of its m is row lengths[i] - m + j of its cache.  Rows that no
+ * sequence holds (padding before the first and behind the last) are neither
+ * read nor written.  Nothing of this is read on the host, so that a recorded
+ * graph serves any batch of the same shapes. */
+
+/* Puts a batch's new keys and values into their pages, the keys normed for
+ * each head (MTPX_NORM_NONE: as they are) and turned by their positions on the
+ * way, as mtpx_head_norm_rotary would; with q (heads 0: none) the queries too,
+ * into q_out, which may be q (same strides).  A row beyond its sequence's room,
+ * or before its start, is dropped; its query is not.  No two rows of a call may
+ * meet in one place of a page. */
+#define MTPX_NORM_NONE 2
+typedef struct mtpx_append_paged_request {
+    void *stream;
+    int dtype;
+    int64_t rows;               /* below 2^26 */
+    int sequences;              /* below 2^24 */
+    int heads, kv_heads, dim, rotated; /* dim <= 256 */
+    int kind, interleaved;
+    float eps;
+    mtpx_rows q, k, v, q_out;
+    const void *q_weight, *k_weight;
+    const void *positions;
+    int position_dtype;
+    int64_t position_row, position_axis;
+    int axes;
+    const float *freq;
+    const int *axis;
+    mtpx_pages cache;
+    const int *offsets, *lengths;
+} mtpx_append_paged_request;
+int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *request);
+
+/* Differential attention (mtpx_diff_attention) of each sequence's new rows
+ * over its pages, which hold the new rows already (mtpx_append_paged): row t of
+ * a cache sees its rows 0 to t (`causal`) or all lengths[i] of them.  What the
+ * pages hold beyond a length does not matter, NaN included; with `causal`, keys
+ * and values that only later rows see must be finite.  A length beyond the
+ * sequence's room counts what there is room for.  A row without a key gives 0.
+ * max_rows: no sequence has more new rows (0: unknown, any number).  It chooses
+ * how the work is split; rows of a sequence beyond it may be left unwritten.
+ * Keys are split over workgroups where there are few rows; the workspace holds
+ * their partial results. */
+typedef struct mtpx_diff_attention_paged_request {
+    void *stream;
+    int dtype;
+    int64_t rows;               /* below 2^26 */
+    int sequences;              /* below 2^24 */
+    int max_rows;
+    int heads, kv_heads, dim;   /* dim 1 to 128 */
+    int causal;
+    float scale;
+    mtpx_rows q;
+    mtpx_pages cache;
+    const int *offsets, *lengths;
+    const float *lambda;
+    mtpx_rows out;
+    void *workspace;
+    size_t workspace_bytes;
+} mtpx_diff_attention_paged_request;
+int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged_request *request);
+/* Workspace for these rows, sequences, max_rows, heads, dim and room (the
+ * cache's page_rows and table_width). */
+int mtpx_diff_attention_paged_workspace(mtpx_context *ctx,
+                                        const mtpx_diff_attention_paged_request *request,
+                                        size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif
