@@ -130,8 +130,9 @@ struct PagedArgs {
     // a key head) go to the deep kernel, the others to the broad one; 0 columns
     // or tiles: that kernel is not launched
     int deep, deep_blocks, broad_tiles, broad_columns;
-    // the most workgroups that share a sequence's keys, and their results
-    int deep_splits, broad_splits;
+    // the most workgroups that share a sequence's keys, the fewest keys of one of
+    // them (a multiple of 64), and their results
+    int deep_splits, broad_splits, deep_least, broad_least;
     float *deep_part, *broad_part;
 };
 

@@ -229,8 +229,8 @@ bool pages_fit(const mtpx_pages &c, int width, int64_t size)
 // How the work of a call is split, from what the host knows: rows, sequences,
 // the most new rows of one, and the room of the tables.
 struct PagedPlan {
-    int deep = 0, deep_blocks = 1, deep_splits = 1;
-    int broad_columns = 64, broad_tiles = 0, broad_splits = 1;
+    int deep = 0, deep_blocks = 1, deep_splits = 1, deep_least = 256;
+    int broad_columns = 64, broad_tiles = 0, broad_splits = 1, broad_least = 256;
     size_t deep_bytes = 0, broad_bytes = 0;
     int64_t items = 0;
 };
@@ -256,13 +256,17 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
         p.items += base * p.deep_splits;
     }
     if (p.deep == 0 || most * group > kDeepColumns) {
-        const int64_t columns = r.rows * group;
-        if (width <= 64 && r.dtype != MTPX_F32 && columns / 128 * r.kv_heads >= 2 * cus)
-            p.broad_columns = 128;
-        const int64_t base = std::max<int64_t>(columns / p.broad_columns, 1) * r.kv_heads;
+        // tiles of twice the columns read less from LDS for each product; narrow
+        // ones where those, with the keys of each in several runs, are too few to
+        // give each CU two workgroups
+        const int64_t columns = r.rows * group, full = 2 * cus, runs = std::min<int64_t>((room + 1023) / 1024, kMaxSplits);
+        const int narrow = width == 128 && r.dtype != MTPX_F32 ? 32 : 64, wide = r.dtype == MTPX_F32 ? narrow : 2 * narrow;
+        auto tiles = [&](int each) { return std::max<int64_t>(columns / each, 1) * r.kv_heads; };
+        p.broad_columns = tiles(wide) * runs >= full ? wide : narrow;
+        const int64_t base = tiles(p.broad_columns);
         p.broad_tiles = (int)std::min<int64_t>(columns / p.broad_columns + r.sequences, INT32_MAX);
-        if (base < 2 * cus && room > 1024)
-            p.broad_splits = (int)std::min<int64_t>({(2 * cus + base - 1) / base, (room + 1023) / 1024, kMaxSplits});
+        if (base < full)
+            p.broad_splits = (int)std::max<int64_t>(std::min((full + base - 1) / base, runs), 1);
         if (p.broad_splits > 1)
             p.broad_bytes = part * p.broad_splits * (size_t)r.rows * r.heads;
         p.items += (int64_t)p.broad_tiles * r.kv_heads * p.broad_splits;
@@ -431,6 +435,8 @@ int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged
         a.broad_columns = p.broad_columns;
         a.broad_tiles = p.broad_tiles;
         a.broad_splits = p.broad_splits;
+        a.deep_least = p.deep_least;
+        a.broad_least = p.broad_least;
         a.deep_part = static_cast<float *>(r.workspace);
         a.broad_part = a.deep_part + p.deep_bytes / sizeof(float);
         OnDevice here(ctx->device);
