@@ -114,6 +114,16 @@ struct HeadArgs {
     int lanes;  // of a row: a power of two from group up to 256
 };
 
+// How the tiles of one width are given to workgroups.
+struct RoleArgs {
+    int groups;     // workgroups (0: none)
+    int each_unit;  // one takes one tile; else they share all keys evenly,
+    int least;      // each with so many (as costs) at least, its partial results
+    float *part;    // here: [groups][2][columns][2][4 + 2 D] (NULL: one group)
+    int shift;      // costs are counted in units of 2^shift keys
+    int tiles;      // wide: the most of a key head
+};
+
 struct PagedArgs {
     int64_t rows;
     int sequences, heads, kv_heads, dim, causal;
@@ -123,17 +133,14 @@ struct PagedArgs {
     const int *offsets, *lengths;
     const float *lambda;
     int vec;
+    int alike;  // and keys and values have the same strides, within 32 bits a row
     // key / page_rows is the upper half of 2 key page_magic, shifted
     unsigned page_magic;
     int page_shift;
-    // sequences of up to `deep` columns (a row's head of the group that shares
-    // a key head) go to the deep kernel, the others to the broad one; 0 columns
-    // or tiles: that kernel is not launched
-    int deep, deep_blocks, broad_tiles, broad_columns;
-    // the most workgroups that share a sequence's keys, the fewest keys of one of
-    // them (a multiple of 64), and their results
-    int deep_splits, broad_splits, deep_least, broad_least;
-    float *deep_part, *broad_part;
+    // sequences of up to so many columns (a row's head of the group that shares
+    // a key head) have a narrow tile, the others wide ones
+    int narrow_columns;
+    RoleArgs narrow, wide;
 };
 
 // dtype is one of MTPX_F32, MTPX_BF16, MTPX_F16 (checked by the caller).

@@ -229,47 +229,46 @@ bool pages_fit(const mtpx_pages &c, int width, int64_t size)
 // How the work of a call is split, from what the host knows: rows, sequences,
 // the most new rows of one, and the room of the tables.
 struct PagedPlan {
-    int deep = 0, deep_blocks = 1, deep_splits = 1, deep_least = 256;
-    int broad_columns = 64, broad_tiles = 0, broad_splits = 1, broad_least = 256;
-    size_t deep_bytes = 0, broad_bytes = 0;
+    int narrow_columns = 0;
+    RoleArgs narrow{}, wide{};
+    size_t narrow_bytes = 0, wide_bytes = 0;
     int64_t items = 0;
 };
-// Sequences of so many columns go to the deep part.
-constexpr int kDeepColumns = 32;
+constexpr int kNarrowColumns = 32;
+constexpr int64_t kMaxShared = 4096;  // sequences whose keys workgroups share
 
 PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
 {
     PagedPlan p;
-    const int64_t group = r.heads / r.kv_heads, cus = ctx->num_cus;
-    const int64_t room = (int64_t)r.cache.table_width * r.cache.page_rows;
+    const int64_t group = r.heads / r.kv_heads, n = r.sequences;
+    const int64_t room = std::max<int64_t>((int64_t)r.cache.table_width * r.cache.page_rows, 1);
     const int64_t most = r.max_rows > 0 ? std::min<int64_t>(r.max_rows, r.rows) : r.rows;
     const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128;
-    const size_t part = sizeof(float) * 2 * (4 + 2 * width);
-    if (group <= kDeepColumns) {
-        p.deep = kDeepColumns;
-        p.deep_blocks = (int)(std::min<int64_t>(most * group, kDeepColumns) + 15) / 16;
-        const int64_t base = std::max<int64_t>((int64_t)r.sequences * r.kv_heads * p.deep_blocks, 1);
-        if (room > 1024)
-            p.deep_splits = (int)std::min<int64_t>({(8 * cus + base - 1) / base, (room + 255) / 256, kMaxSplits});
-        if (p.deep_splits > 1)
-            p.deep_bytes = part * 16 * (size_t)base * p.deep_splits;
-        p.items += base * p.deep_splits;
+    const bool half = r.dtype != MTPX_F32;
+    // workgroups that the device holds at once: by their 64 KiB of LDS, or 32
+    const int64_t slots = 2 * (int64_t)ctx->num_cus, least = 512;
+    auto role = [&](RoleArgs &a, size_t &bytes, int columns, int64_t units, bool each) {
+        a.each_unit = each || n > kMaxShared;
+        // all costs together stay below 2^30
+        const int64_t most_cost = units * (256 + room + r.rows);
+        while (most_cost >> a.shift >= int64_t(1) << 30)
+            ++a.shift;
+        a.least = (int)std::max<int64_t>(least >> a.shift, 1);
+        const int64_t groups = a.each_unit ? units : std::min(slots * (width == 32 && half ? 2 : 1), units * ((room + 255) / 256));
+        a.groups = (int)std::min<int64_t>(groups, INT32_MAX);
+        p.items += groups;
+        if (!a.each_unit && a.groups > 1)
+            bytes = sizeof(float) * 2 * (4 + 2 * width) * 2 * (size_t)columns * a.groups;
+    };
+    if (group <= kNarrowColumns) {
+        p.narrow_columns = kNarrowColumns;
+        role(p.narrow, p.narrow_bytes, kNarrowColumns, n * r.kv_heads, false);
     }
-    if (p.deep == 0 || most * group > kDeepColumns) {
-        // tiles of twice the columns read less from LDS for each product; narrow
-        // ones where those, with the keys of each in several runs, are too few to
-        // give each CU two workgroups
-        const int64_t columns = r.rows * group, full = 2 * cus, runs = std::min<int64_t>((room + 1023) / 1024, kMaxSplits);
-        const int narrow = width == 128 && r.dtype != MTPX_F32 ? 32 : 64, wide = r.dtype == MTPX_F32 ? narrow : 2 * narrow;
-        auto tiles = [&](int each) { return std::max<int64_t>(columns / each, 1) * r.kv_heads; };
-        p.broad_columns = tiles(wide) * runs >= full ? wide : narrow;
-        const int64_t base = tiles(p.broad_columns);
-        p.broad_tiles = (int)std::min<int64_t>(columns / p.broad_columns + r.sequences, INT32_MAX);
-        if (base < full)
-            p.broad_splits = (int)std::max<int64_t>(std::min((full + base - 1) / base, runs), 1);
-        if (p.broad_splits > 1)
-            p.broad_bytes = part * p.broad_splits * (size_t)r.rows * r.heads;
-        p.items += (int64_t)p.broad_tiles * r.kv_heads * p.broad_splits;
+    if (p.narrow_columns == 0 || most * group > kNarrowColumns) {
+        const int columns = half ? (width < 128 ? 128 : 64) : width < 128 ? 64 : 32;
+        const int64_t tiles = r.rows * group / columns + n;
+        p.wide.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+        role(p.wide, p.wide_bytes, columns, tiles * r.kv_heads, r.rows * group / columns * r.kv_heads >= 4 * slots);
     }
     return p;
 }
@@ -386,7 +385,7 @@ int mtpx_diff_attention_paged_workspace(mtpx_context *ctx, const mtpx_diff_atten
         r.scale = 1.f;
         MTPX_TRY(check_paged(ctx, r));
         const PagedPlan p = paged_plan(ctx, r);
-        *bytes = p.deep_bytes + p.broad_bytes;
+        *bytes = p.narrow_bytes + p.wide_bytes;
         return MTPX_OK;
     });
 }
@@ -406,7 +405,7 @@ int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged
         MTPX_TRY(check_rows(ctx, r.out, r.dtype, "out"));
         MTPX_TRY(check_flat(ctx, r.lambda, 4, "lambda"));
         const PagedPlan p = paged_plan(ctx, r);
-        MTPX_TRY(check_workspace(ctx, r.workspace, r.workspace_bytes, p.deep_bytes + p.broad_bytes));
+        MTPX_TRY(check_workspace(ctx, r.workspace, r.workspace_bytes, p.narrow_bytes + p.wide_bytes));
         const int64_t size = (int64_t)dtype_bytes(r.dtype);
         PagedArgs a{};
         a.rows = r.rows;
@@ -424,21 +423,22 @@ int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged
         a.lambda = r.lambda;
         a.vec = r.dim * size % 16 == 0 && whole_pieces(r.q, size) && whole_pieces(r.out, size) &&
                 pages_fit(r.cache, (int)(16 / size), size);
+        const mtpx_pages &c = r.cache;
+        const int64_t limit = int64_t(1) << 26;  // elements: eight rows and two maps stay within 32 bits of bytes
+        a.alike = a.vec && c.k.row == c.v.row && c.k.map == c.v.map && c.k_page == c.v_page && c.k.row < limit && c.k.map < limit;
         int bits = 0;
         while ((1 << bits) < r.cache.page_rows)
             ++bits;
         a.page_shift = bits;
         a.page_magic = (unsigned)((uint64_t(1) << (31 + bits)) / (uint64_t)r.cache.page_rows + 1);
-        a.deep = p.deep;
-        a.deep_blocks = p.deep_blocks;
-        a.deep_splits = p.deep_splits;
-        a.broad_columns = p.broad_columns;
-        a.broad_tiles = p.broad_tiles;
-        a.broad_splits = p.broad_splits;
-        a.deep_least = p.deep_least;
-        a.broad_least = p.broad_least;
-        a.deep_part = static_cast<float *>(r.workspace);
-        a.broad_part = a.deep_part + p.deep_bytes / sizeof(float);
+        a.narrow_columns = p.narrow_columns;
+        a.narrow = p.narrow;
+        a.wide = p.wide;
+        float *part = static_cast<float *>(r.workspace);
+        if (p.narrow_bytes)
+            a.narrow.part = part;
+        if (p.wide_bytes)
+            a.wide.part = part + p.narrow_bytes / sizeof(float);
         OnDevice here(ctx->device);
         HIP_TRY(launch_paged(r.dtype, a, (hipStream_t)r.stream), "launch paged attention");
         return MTPX_OK;

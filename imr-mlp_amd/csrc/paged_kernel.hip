@@ -5,9 +5,13 @@
 //
 // The heads of a group read the same keys, so a sequence's m rows and the g
 // heads of a group are m g columns of one product: column x is row x / g, head
-// x % g.  A sequence of few columns goes to the deep part (its keys over waves
-// and workgroups), one of many to the broad part (its columns over them);
-// paged_join joins what workgroups that share a sequence's keys have left.
+// x % g.  A unit of the work is a tile of columns of one sequence and group,
+// with the keys that they see.  A few columns (a decoding step) are bound by the
+// reads of the cache, many (a prompt's chunk) by the matrix units: there are
+// narrow and wide tiles.  Where units are many, a workgroup takes one; where they
+// are few or unlike, the workgroups that the device holds at once share all
+// units' keys evenly (Shares), and paged_join joins the runs of a unit that
+// several of them have.
 //
 // Compiled once per element type (MTPX_OPS_TYPE).
 #include "paged_device.hpp"
@@ -55,113 +59,237 @@ struct Sequence {
     }
 };
 
-// The run of keys of one of the workgroups that share a sequence's keys:
-// whole units, as even as they go, no fewer than `least` of them.
-struct Run {
-    int begin, end, used;
-    __device__ inline Run(int keys, int split, int splits, int unit, int least)
+// Floats of a partial result of one column and map: level, sum, -, -, product.
+template <int D>
+constexpr int kPart = 4 + 2 * D;
+
+// What kernels of one width of tiles are told apart by: sequences of up to
+// a.narrow columns have one narrow tile, the others wide ones.
+template <int COLS>
+struct Role {
+    const RoleArgs &r;
+    bool narrow;
+    __device__ inline int tiles(const PagedArgs &a, const Sequence &sq) const
     {
-        const int units = (keys + unit - 1) / unit, each = max(least, (units + splits - 1) / splits);
-        used = max(1, (units + each - 1) / each);
-        begin = min(keys, split * each * unit);
-        end = min(keys, begin + each * unit);
+        const int64_t columns = (int64_t)sq.rows * (a.heads / a.kv_heads);
+        return columns > 0 && (columns <= a.narrow_columns) == narrow ? (int)((columns + COLS - 1) / COLS) : 0;
+    }
+    // What the first t tiles of a sequence cost: the keys that they see and
+    // kStart for each, in units of 2^shift.  (Keys of causal tiles as a mean over
+    // their rows: a cost need not be exact, only the same in every workgroup.)
+    __device__ inline int cost(const PagedArgs &a, const Sequence &sq, int t) const
+    {
+        const int before = a.causal ? max(0, sq.length - sq.rows) : sq.length;
+        const int64_t slope = a.causal ? (int64_t)t * (t + 1) * COLS / (2 * (a.heads / a.kv_heads)) : 0;
+        return t * (start() + (before >> r.shift)) + (int)(slope >> r.shift);
+    }
+    __device__ inline int start() const { return max(1, 256 >> r.shift); }
+};
+
+// Inclusive sums over a wave: shifts within rows of 16 lanes, then from row to row.
+__device__ inline int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+}
+
+// The units of one key head lie one after the other on a line of costs, tile by
+// tile and sequence by sequence, the key heads behind one another; workgroup w
+// takes what lies from w `each` on.  Built by a whole workgroup, for up to 64 runs
+// of 64 sequences.
+struct Line {
+    int before[kWave];  // cost of the sequences before each run of 64
+};
+template <int COLS>
+struct Shares {
+    const PagedArgs &a;
+    Role<COLS> role;
+    Line &line;
+    int head, total, each;  // of a key head, of all, of a workgroup
+
+    __device__ inline int sequence_cost(int i) const
+    {
+        if (i >= a.sequences)
+            return 0;
+        const Sequence sq(a, i);
+        return role.cost(a, sq, role.tiles(a, sq));
+    }
+    __device__ inline int runs() const { return (a.sequences + kWave - 1) / kWave; }
+    __device__ inline Shares(const PagedArgs &args, const Role<COLS> &r, Line &l) : a(args), role(r), line(l)
+    {
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+        if (runs() == 1) {
+            head = __builtin_amdgcn_readlane(wave_scan(sequence_cost(lane)), kWave - 1);
+        } else {
+            for (int i = wave; i < runs(); i += waves) {
+                const int sum = wave_scan(sequence_cost(i * kWave + lane));
+                if (lane == kWave - 1)
+                    line.before[i] = sum;
+            }
+            __syncthreads();
+            const int own = lane < runs() ? line.before[lane] : 0, upto = wave_scan(own);
+            __syncthreads();
+            if (wave == 0)
+                line.before[lane] = upto - own;  // (runs beyond the last begin where it ends)
+            __syncthreads();
+            head = __builtin_amdgcn_readlane(upto, kWave - 1);
+        }
+        total = head * a.kv_heads;
+        each = max((total + role.r.groups - 1) / role.r.groups, role.r.least);
+    }
+    // The sequence at cost p (below head) of a key head, and the cost of those before it.
+    __device__ inline int find(int p, int &start) const
+    {
+        const int lane = threadIdx.x & (kWave - 1);
+        const int run = runs() == 1 ? 0 : __popcll(__ballot(line.before[lane] <= p)) - 1;
+        const int own = sequence_cost(run * kWave + lane);
+        const int upto = wave_scan(own) + (runs() == 1 ? 0 : line.before[run]);
+        const int l = __popcll(__ballot(upto <= p));
+        start = __builtin_amdgcn_readlane(upto - own, l);
+        return run * kWave + l;
+    }
+    // The cost of the sequences before i.
+    __device__ inline int start(int i) const
+    {
+        const int lane = threadIdx.x & (kWave - 1), run = i / kWave;
+        const int own = sequence_cost(run * kWave + lane);
+        return __builtin_amdgcn_readlane(wave_scan(own) - own, i % kWave) + (runs() == 1 ? 0 : line.before[run]);
     }
 };
 
-// Floats of a partial result of one row, head and map: level, sum, -, -, product.
-template <int D>
-constexpr int kPart = 4 + 2 * D;
-template <int D>
-__device__ inline float *deep_result(const PagedArgs &a, int seq, int kv, int x, int m, int split)
+// Where cost p falls into the n steps of a unit whose costs begin at a0, its keys'
+// at `keys`, and end at a1.  (In 64-bit floats, whose quotient is the same
+// wherever it is formed, and does not fall as p grows.)
+__device__ inline int step_at(int p, int keys, int a1, int n)
 {
-    return a.deep_part + (((((int64_t)seq * a.kv_heads + kv) * a.deep_blocks * 16 + x) * 2 + m) * a.deep_splits + split) * kPart<D>;
-}
-template <int D>
-__device__ inline float *broad_result(const PagedArgs &a, int64_t row, int head, int m, int split)
-{
-    return a.broad_part + (((row * a.heads + head) * 2 + m) * a.broad_splits + split) * kPart<D>;
+    return p >= a1 ? n : p <= keys ? 0 : min(n, (int)((double)(p - keys) * n / (a1 - keys)));
 }
 
-// The page of the lane's key of a tile (lane l: key l of it), -1 where there is
-// none: read a tile ahead of its use.
 __device__ inline int page_of(const PagedArgs &a, int key)
 {
     return (int)(__umulhi(2u * (unsigned)key, a.page_magic) >> a.page_shift);
 }
-__device__ inline int look_up(const PagedArgs &a, const Sequence &sq, int key, int end)
-{
-    return key < end ? sq.table[page_of(a, key)] : -1;
-}
 __device__ inline bool there(const PagedArgs &a, int page) { return page >= 0 && page < a.cache.pages; }
-// Bytes from a pool's start to the row of the lane's key, whose page this is.
-template <class T>
-__device__ inline int64_t row_bytes(const PagedArgs &a, const mtpx_rows &s, int64_t stride, int page, int key)
-{
-    const int slot = key - page_of(a, key) * a.cache.page_rows;
-    return there(a, page) ? (page * stride + slot * s.row) * (int64_t)sizeof(T) : 0;
-}
-// The same number in all lanes: lane `from`'s.
-__device__ inline int64_t of_lane(int64_t v, int from)
-{
-    const unsigned lo = __builtin_amdgcn_readlane((int)v, from), hi = __builtin_amdgcn_readlane((int)(v >> 32), from);
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
 
-// A tile's way from the pages straight into LDS, by W waves (wave `wave` of
-// them): a wave's instruction fills kGroup rows of the tile.  FAST: rows are
-// whole 16-byte pieces, and a page holds whole groups, so that a group's place
-// is the same in all lanes.
+// The way of a tile of keys and values from the pages straight into LDS, by W
+// waves.  look_up() reads the table for a tile, one tile ahead of fetch().
+// Any pages: lane l looks up key l of the tile, and every wave's instruction fills
+// kGroup rows of it from where those lanes say.
 template <class T, int D, int ROWS, int W, bool FAST>
-struct PageLoader {
+struct TileLoader {
     using TL = Tile<T, D>;
     static constexpr int kGroup = 1024 / TL::kRowBytes;
     static constexpr int N = ROWS / (kGroup * W);
     static_assert(N * kGroup * W == ROWS, "rows of a tile");
-    static constexpr bool kSame = W * kGroup % 8 == 0;
-    const char *at;  // FAST: the lane's place in a group at the pool's start
-    int64_t map;
-    int lane, wave;
+    const PagedArgs &a;
+    const int *table;
+    int kv, lane, wave, page = -1, first = 0;
+
+    __device__ inline TileLoader(const PagedArgs &args, const int *t, int head, int l, int w)
+        : a(args), table(t), kv(head), lane(l), wave(w)
+    {
+    }
+    __device__ inline void look_up(int k0, int end)
+    {
+        first = k0;
+        page = k0 + lane < end ? table[page_of(a, k0 + lane)] : -1;
+    }
+    // Returns which of the tile's keys are there; the others become zeros.
+    __device__ inline unsigned long long fetch(char *smem, int k_tile, int v_tile)
+    {
+        const unsigned long long seen = __ballot(there(a, page)) & ~0ull >> (64 - ROWS);
+        const int slot = first + lane - page_of(a, first + lane) * a.cache.page_rows;
+        auto half = [&](const mtpx_rows &s, int64_t stride, int tile) {
+            const int64_t mine = there(a, page) ? (int64_t)(unsigned)page * stride + (int64_t)(unsigned)slot * s.row : 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r0 = (i * W + wave) * kGroup, r = r0 + lane / TL::kPieces;
+                const int col = ((lane % TL::kPieces) ^ (r & 7)) * TL::E, c = col % D, to = tile + r0 * TL::kRowBytes;
+                const T *p = (const T *)s.data + kv * s.head + (int64_t)__shfl((long long)mine, r) + col / D * s.map + c;
+                const bool on = (seen >> r & 1) && c < a.dim;
+                if (a.vec)
+                    load_to_lds(on ? (const void *)p : (const void *)&kZeroPiece, to);
+                else
+                    *reinterpret_cast<u32x4 *>(smem + to + lane * 16) = load16(p, on ? a.dim - c : 0, 0);
+            }
+        };
+        half(a.cache.k, a.cache.k_page, k_tile);
+        half(a.cache.v, a.cache.v_page, v_tile);
+        return seen;
+    }
+};
+
+// 16 bytes per lane straight into LDS as load_to_lds(), from the same address in
+// all lanes and an offset of each.
+__device__ inline void load_lanes_to_lds(const void *p, unsigned lane_offset, unsigned offset)
+{
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_offset), "s"(p), "{m0}"(offset) : "memory");
+}
+
+// FAST: rows of whole 16-byte pieces, keys and values laid out alike, pages of
+// whole runs of ROWS / W rows.  A wave's rows of a tile are one run, in one page,
+// so that all addresses and the table are the scalar unit's work and the lanes
+// keep their offsets (1,000 structures of 160 ... see launch): the vector unit has
+// the softmax to do.
+template <class T, int D, int ROWS, int W>
+struct TileLoader<T, D, ROWS, W, true> {
+    using TL = Tile<T, D>;
+    static constexpr int kGroup = 1024 / TL::kRowBytes, kRun = ROWS / W, N = kRun / kGroup;
+    static_assert(N * kGroup == kRun && kRun % 8 == 0, "rows of a wave");
+    static constexpr int kColumns = kGroup >= 8 ? 1 : 8 / kGroup < N ? 8 / kGroup : N;  // the permutation's phases
+    const PagedArgs &a;
+    const int *table;
+    const char *k, *v;
+    int lane, wave, first = 0, page = -1;
+    unsigned offset[kColumns];
 
     __device__ inline int column(int i) const
     {
-        const int r = (kSame ? 0 : i * W * kGroup) + wave * kGroup + lane / TL::kPieces;
-        return ((lane % TL::kPieces) ^ (r & 7)) * TL::E;
+        return ((lane % TL::kPieces) ^ ((i * kGroup + lane / TL::kPieces) & 7)) * TL::E;
     }
-    __device__ inline int64_t column_bytes(int i) const
+    __device__ inline TileLoader(const PagedArgs &args, const int *t, int kv, int l, int w) : a(args), table(t), lane(l), wave(w)
     {
-        return (column(i) / D * map + column(i) % D) * (int64_t)sizeof(T);
-    }
-    __device__ inline void init(const mtpx_rows &s, int head, int l, int w)
-    {
-        map = s.map;
-        lane = l;
-        wave = w;
-        at = (const char *)((const T *)s.data + head * s.head);
-        if constexpr (FAST)
-            at += lane / TL::kPieces * s.row * (int64_t)sizeof(T);
-        if constexpr (kSame)
-            at += column_bytes(0);
-    }
-    // bytes: of the lane's key; seen: the tile's rows that are there (all: every one).
-    __device__ inline void load(const PagedArgs &a, char *smem, int tile, int64_t bytes, unsigned long long seen, bool all) const
-    {
+        k = (const char *)((const T *)a.cache.k.data + kv * a.cache.k.head);
+        v = (const char *)((const T *)a.cache.v.data + kv * a.cache.v.head);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int r0 = (i * W + wave) * kGroup, r = r0 + lane / TL::kPieces, to = tile + (i * W + wave) * 1024;
-            const char *p = at + (FAST ? of_lane(bytes, r0) : (int64_t)__shfl((long long)bytes, r));
-            if constexpr (!kSame)
-                p += column_bytes(i);
-            if (FAST && all && a.dim == D) {
-                load_to_lds(p, to);
-                continue;
+        for (int i = 0; i < kColumns; ++i)
+            offset[i] = (unsigned)(lane / TL::kPieces * (int)a.cache.k.row + column(i) / D * (int)a.cache.k.map + column(i) % D) *
+                        (unsigned)sizeof(T);
+    }
+    __device__ inline void look_up(int k0, int end)
+    {
+        first = k0;
+        page = k0 + lane < end ? table[page_of(a, k0 + lane)] : -1;
+    }
+    __device__ inline unsigned long long fetch(char *, int k_tile, int v_tile)
+    {
+        const unsigned long long seen = __ballot(there(a, page)) & ~0ull >> (64 - ROWS);
+        const int of_run = __builtin_amdgcn_readlane(page, wave * kRun);
+        const int key = first + wave * kRun, slot = key - page_of(a, key) * a.cache.page_rows;
+        const unsigned row = (unsigned)a.cache.k.row * (unsigned)sizeof(T);
+        const uint64_t at = (uint64_t)(unsigned)of_run * (uint64_t)(a.cache.k_page * (int64_t)sizeof(T)) + (uint64_t)(unsigned)slot * row;
+        const unsigned mine = (unsigned)(seen >> (wave * kRun)) & ~0u >> (32 - kRun);
+        const bool all = mine == ~0u >> (32 - kRun) && a.dim == D;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const char *from = (half ? v : k) + at;
+            const int to = (half ? v_tile : k_tile) + wave * kRun * TL::kRowBytes;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const char *p = from + (uint64_t)(i * kGroup) * row;
+                if (all) {
+                    load_lanes_to_lds(p, offset[i % kColumns], to + i * 1024);
+                    continue;
+                }
+                const bool on = (mine >> (i * kGroup + lane / TL::kPieces) & 1) && column(i % kColumns) % D < a.dim;
+                load_to_lds(on ? (const void *)(p + offset[i % kColumns]) : (const void *)&kZeroPiece, to + i * 1024);
             }
-            const int c = column(i) % D;
-            const bool on = (seen >> r & 1) && c < a.dim;
-            if (FAST || a.vec)
-                load_to_lds(on ? (const void *)p : (const void *)&kZeroPiece, to);
-            else
-                *reinterpret_cast<u32x4 *>(smem + to + lane * 16) = load16((const T *)p, on ? a.dim - c : 0, 0);
         }
+        return seen;
     }
 };
 
@@ -174,18 +302,26 @@ __device__ inline void store_columns(T *row, int64_t map, int dim, int t, int la
     store4(row + m * map, c, dim, v, vec);
 }
 
-// The broad part.  A workgroup takes columns of one sequence and group; keys and
-// values come in tiles of KB rows, the next one while the present one is worked
-// on (BUF 2).  S^T = K Q^T leaves a column of the product per lane column: its
-// running level and sum are per lane, and exp(S^T), rounded to T, is operand B of
-// O^T += V^T P^T as it stands.  The two maps keep their own level, sum and product.
+// A run of a unit's keys: tiles of KB keys [begin, end) of `steps`; all of them
+// give the result, others a partial one.
+struct Segment {
+    int kv, begin, end, steps;
+    int64_t x0;  // first column of the tile
+    float *part;
+};
+
+// Keys and values come in tiles of KB rows, the next one while the present one is
+// worked on (BUF 2).  S^T = K Q^T leaves a column of the product per lane column:
+// its running level and sum are per lane, and exp(S^T), rounded to T, is operand B
+// of O^T += V^T P^T as it stands.  The two maps keep their own level, sum and
+// product.
 //
 // A wave has QT 16 columns and both maps, which share each fragment of V read
 // from LDS (M 2); or two waves share the columns, a map each (M 1).  A wave of
 // wide heads has registers for 16 columns of two maps or 32 of one: those read
 // 24 KiB of LDS for what takes the former 32 KiB (D 128, 32 keys).
 template <class T, int D, int W, int M, int QT, int KB, int BUF, bool FAST>
-__device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
+__device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segment &sg, char *smem)
 {
     using TL = Tile<T, D>;
     constexpr int kTile = KB * TL::kRowBytes, kCols = W * M / 2 * QT * 16;
@@ -193,30 +329,16 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m0 = M == 2 ? 0 : wave & 1, part = M == 2 ? wave : wave >> 1;
-    const int group = a.heads / a.kv_heads;
-    const Work wk = work_item(item, a.broad_tiles, a.kv_heads * a.broad_splits);
-    const int kv = wk.head % a.kv_heads, split = wk.head / a.kv_heads;
-    // the last rows of a causal sequence have the most keys: they go first
-    const int tile = a.broad_tiles - 1 - wk.tile;
-    auto start = [&](int i) { return (int64_t)row_offset(a.offsets, i, a.rows) * group / kCols + i; };
-    const int seq = __builtin_amdgcn_readfirstlane(last_true([&](int i) { return start(i) <= tile; }, a.sequences, kWave));
-    if (seq < 0)
-        return;
-    const Sequence sq(a, seq);
-    const int64_t columns = (int64_t)sq.rows * group, x0 = (tile - start(seq)) * kCols;
-    if (x0 >= columns || columns <= a.deep)
-        return;
+    const int group = a.heads / a.kv_heads, kv = sg.kv;
+    const int64_t columns = (int64_t)sq.rows * group, x0 = sg.x0;
     const int nk = sq.keys(a, (int)((min(x0 + kCols, columns) - 1) / group));
-    const Run run(nk, split, a.broad_splits, KB, a.broad_least / KB);
-    if (split >= run.used)
-        return;
+    const int run_begin = sg.begin * KB, run_end = min(nk, sg.end * KB);
 
+    TileLoader<T, D, KB, W, FAST> tiles(a, sq.table, kv, lane, wave);
+    tiles.look_up(run_begin, run_end);
     const float c = a.scale * kLog2e;
     Reader<T, D> rd;
     rd.init(lane);
-    PageLoader<T, D, KB, W, FAST> lk, lv;
-    lk.init(a.cache.k, kv, lane, wave);
-    lv.init(a.cache.v, kv, lane, wave);
 
     const int64_t w0 = x0 + part * QT * 16;  // first column of the wave
     Frag<T> qf[M][QT][D / 32];
@@ -251,27 +373,20 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
         }
 
     unsigned long long bits = 0;
-    int page = -1;
     auto load = [&](int k0, int to) {
-        bits = __ballot(there(a, page)) & kFull;
-        const int64_t kb = row_bytes<T>(a, a.cache.k, a.cache.k_page, page, k0 + lane);
-        const int64_t vb = row_bytes<T>(a, a.cache.v, a.cache.v_page, page, k0 + lane);
-        lk.load(a, smem, to * 2 * kTile, kb, bits, bits == kFull);
-        lv.load(a, smem, to * 2 * kTile + kTile, vb, bits, bits == kFull);
-        page = look_up(a, sq, k0 + KB + lane, run.end);
+        bits = tiles.fetch(smem, to * 2 * kTile, to * 2 * kTile + kTile);
+        tiles.look_up(k0 + KB, run_end);
     };
-    if (run.begin < run.end) {
-        page = look_up(a, sq, run.begin + lane, run.end);
-        load(run.begin, 0);
-    }
+    if (run_begin < run_end)
+        load(run_begin, 0);
     int buf = 0;
-    for (int k0 = run.begin; k0 < run.end; k0 += KB) {
+    for (int k0 = run_begin; k0 < run_end; k0 += KB) {
         wait_loads();
         __syncthreads();
         const unsigned long long now = bits;
         const char *kt = smem + buf * 2 * kTile, *vt = kt + kTile;
         auto next = [&] {
-            if (k0 + KB < run.end) {
+            if (k0 + KB < run_end) {
                 buf = BUF - 1 - buf;
                 load(k0 + KB, buf);
             }
@@ -290,9 +405,13 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
                     // u, then map, then columns: one K fragment ahead
                     constexpr int kEach = M * (D / 32), kSteps = 2 * kEach;
                     auto key_frag = [&](int x) {
-                        const int column = x / (D / 32) % M * D + x % (D / 32) * 32;
-                        const char *of = M == 2 ? kt : kt + m0 * (2 * D * sizeof(T) / 2);
-                        return rd.row_frag(of, b * 32 + x / kEach * 16, column);
+                        const int r0 = b * 32 + x / kEach * 16, column = x / (D / 32) % M * D + x % (D / 32) * 32;
+                        if constexpr (M == 2)
+                            return rd.row_frag(kt, r0, column);
+                        else if constexpr (D * sizeof(T) % 128 == 0)  // whole runs of 8 pieces
+                            return rd.row_frag(kt + m0 * (D * sizeof(T)), r0, column);
+                        else
+                            return m0 ? rd.row_frag(kt, r0, D + column) : rd.row_frag(kt, r0, column);
                     };
                     Frag<T> kf = key_frag(0);
 #pragma unroll
@@ -390,8 +509,8 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
         }
     }
 
-    if constexpr (M == 1)
-        __syncthreads();  // the last tile's reads, before its place takes results
+    const bool whole = sg.begin == 0 && sg.end == sg.steps;
+    __syncthreads();  // the last tile's reads, before its place takes results or another tile
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int64_t x = w0 + t * 16 + (lane & 15);
@@ -401,12 +520,12 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
 #pragma unroll
         for (int m = 0; m < M; ++m)
             total[m] = column_sum(sum[m][t]);
-        if (run.used > 1) {
+        if (!whole) {
             if (x >= columns)
                 continue;
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                float *p = broad_result<D>(a, row, head, m0 + m, split);
+                float *p = sg.part + ((x - x0) * 2 + m0 + m) * kPart<D>;
                 if (g == 0) {
                     p[0] = level[m][t];
                     p[1] = total[m];
@@ -449,379 +568,230 @@ __device__ inline void broad_part(const PagedArgs &a, int item, char *smem)
     }
 }
 
-// Waits until no more than N of the loads that this wave has queued are under way.
-template <int N>
-__device__ inline void wait_all_but()
+// The work of workgroup `item` of a role: one unit, or the runs of units that lie
+// in its share.
+template <class T, int D, int W, int M, int QT, int KB, int BUF, bool FAST, bool NARROW>
+__device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line)
 {
-    static_assert(N < 64, "what the counter holds");
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
-    asm volatile("" ::: "memory");
+    constexpr int kCols = W * M / 2 * QT * 16;
+    const Role<kCols> role{NARROW ? a.narrow : a.wide, NARROW};
+    const int group = a.heads / a.kv_heads, n = role.r.groups;
+    // neighbours on one XCD, whose L2 holds the keys that they share
+    const int w = n % 8 ? item : item % 8 * (n / 8) + item / 8;
+    int p = 0, p0 = 0, p1 = 0;  // on the line: the next unit's, the share's
+    for (bool begun = false;; begun = true) {
+        int seq, kv, tile, a0 = 0, a1 = 0;
+        if (!role.r.each_unit) {
+            const Shares<kCols> shares(a, role, line);
+            if (!begun) {
+                p0 = p = w * shares.each;
+                p1 = min(p0 + shares.each, shares.total);
+            }
+            if (p >= p1)
+                return;
+            kv = (int)((unsigned)p / (unsigned)shares.head);
+            int at;
+            seq = __builtin_amdgcn_readfirstlane(shares.find(p - kv * shares.head, at));
+            at += kv * shares.head;
+            const Sequence sq(a, seq);
+            tile = __builtin_amdgcn_readfirstlane(
+                last_true([&](int t) { return at + role.cost(a, sq, t) <= p; }, role.tiles(a, sq), kWave));
+            a0 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile));
+            a1 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile + 1));
+        } else if (NARROW) {
+            seq = item / a.kv_heads;
+            kv = item % a.kv_heads;
+            tile = 0;
+        } else {
+            const Work wk = work_item(item, role.r.tiles, a.kv_heads);
+            // the last rows of a causal sequence have the most keys: they go first
+            const int at = role.r.tiles - 1 - wk.tile;
+            // (tile t of sequence i is number offsets[i] g / columns + i + t)
+            auto start = [&](int i) { return (int64_t)row_offset(a.offsets, i, a.rows) * group / kCols + i; };
+            seq = __builtin_amdgcn_readfirstlane(last_true([&](int i) { return start(i) <= at; }, a.sequences, kWave));
+            if (seq < 0)
+                return;
+            kv = wk.head;
+            tile = (int)(at - start(seq));
+        }
+        const Sequence sq(a, seq);
+        if (tile >= role.tiles(a, sq))
+            return;
+        const int64_t columns = (int64_t)sq.rows * group, x0 = (int64_t)tile * kCols;
+        const int nk = sq.keys(a, (int)((min(x0 + kCols, columns) - 1) / group)), steps = (nk + KB - 1) / KB;
+        Segment sg{kv, 0, steps, steps, x0, nullptr};
+        bool any = true;
+        if (!role.r.each_unit) {
+            sg.begin = __builtin_amdgcn_readfirstlane(step_at(p0, a0 + role.start(), a1, steps));
+            sg.end = __builtin_amdgcn_readfirstlane(step_at(p1, a0 + role.start(), a1, steps));
+            // a run that begins a unit and does not end it, or another
+            sg.part = role.r.part + ((int64_t)w * 2 + (sg.begin == 0)) * kCols * 2 * kPart<D>;
+            // a unit without keys has its zeros written where it begins
+            any = sg.begin < sg.end || (steps == 0 && p0 <= a0);
+        }
+        if (any)
+            attend<T, D, W, M, QT, KB, BUF, FAST>(a, sq, sg, smem);
+        if (role.r.each_unit)
+            return;
+        p = a1;
+    }
 }
 
-// The deep part.  A workgroup takes 16 columns of one sequence and group (fewer
-// leave columns of the product empty, which costs nothing, as the reads of the
-// cache bound it) and one of the runs of their keys; its waves take steps of 32
-// keys in turn, each with its own maxima and sums, and are joined through LDS at
-// the end.  Keys and values go into LDS of the wave's own: those of the next step
-// are queued as soon as the present one's have been read, so that a wave has a
-// step's keys or values under way at any time.  FAST: nothing else is loaded in
-// the loop (64 entries of the table lie in a register), so that a wait can leave
-// the later loads under way.
-template <class T, int D, int W, bool FAST>
-__device__ inline void deep_part(const PagedArgs &a, int item, char *smem)
+// Four columns from y on of a column x of a unit from the runs of both maps.
+template <class T, int D, int COLS, int KB>
+__device__ inline void join_unit(const PagedArgs &a, const Role<COLS> &role, const Sequence &sq, int kv, int tile, int a0, int a1,
+                                 int each, int total, int piece, int pieces)
 {
-    using TL = Tile<T, D>;
-    using PL = PageLoader<T, D, 32, 1, FAST>;
-    constexpr int kTile = 32 * TL::kRowBytes;
-    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = a.heads / a.kv_heads;
-    const int block = item % a.deep_blocks, split = item / a.deep_blocks % a.deep_splits;
-    const int kv = item / (a.deep_blocks * a.deep_splits) % a.kv_heads;
-    const int seq = item / (a.deep_blocks * a.deep_splits) / a.kv_heads;
-    const Sequence sq(a, seq);
-    const int64_t columns = (int64_t)sq.rows * group;
-    const int x0 = block * 16;
-    if (columns > a.deep || x0 >= columns)
-        return;
-    const int count = min(16, (int)columns - x0);
-    const int nk = sq.keys(a, (x0 + count - 1) / group);
-    const Run run(nk, split, a.deep_splits, 32, a.deep_least / 32);
-    if (split >= run.used)
-        return;
-
-    const float c = a.scale * kLog2e;
-    const int kt = wave * 2 * kTile, vt = kt + kTile;
-    Reader<T, D> rd;
-    rd.init(lane);
-    PL lk, lv;
-    lk.init(a.cache.k, kv, lane, 0);
-    lv.init(a.cache.v, kv, lane, 0);
-    // entries of the table from `base` on
-    int entries = -1, base = -64;
-    const int pages = run.end > 0 ? page_of(a, run.end - 1) + 1 : 0;
-    // the step's keys: whether they are there and where
-    unsigned next_bits = 0;
-    int64_t key_bytes = 0, value_bytes = 0;
-    auto find = [&](int k0) {
-        const int key = k0 + (lane & 31);
-        int page;
-        if constexpr (FAST) {
-            const int first = page_of(a, k0), end = page_of(a, min(k0 + 32, run.end) - 1) + 1;
-            if (end > base + 64) {
-                base = first;
-                entries = base + lane < pages ? sq.table[base + lane] : -1;
-                wait_loads();
-            }
-            page = __shfl(entries, min(page_of(a, key) - base, 63));
-            page = key < run.end ? page : -1;
-        } else {
-            page = look_up(a, sq, key, run.end);
-        }
-        next_bits = (unsigned)__ballot(there(a, page));
-        key_bytes = row_bytes<T>(a, a.cache.k, a.cache.k_page, page, key);
-        value_bytes = row_bytes<T>(a, a.cache.v, a.cache.v_page, page, key);
-    };
-    const int begin = run.begin + 32 * wave;
-    if (begin < run.end) {
-        find(begin);
-        lk.load(a, smem, kt, key_bytes, next_bits, next_bits == ~0u);
-        lv.load(a, smem, vt, value_bytes, next_bits, next_bits == ~0u);
+    const int64_t columns = (int64_t)sq.rows * group, x0 = (int64_t)tile * COLS;
+    const int nk = sq.keys(a, (int)((min(x0 + COLS, columns) - 1) / group)), steps = (nk + KB - 1) / KB;
+    const int first = a0 / each, last = (a1 - 1) / each;
+    auto part_at = [&](int w) { return step_at(min(w * each, total), a0 + role.start(), a1, steps); };
+    // the workgroups that have a run of the unit: the first has its begin
+    int from = -1, upto = -1;
+    for (int w = first; w <= last; ++w) {
+        const int b = part_at(w), e = part_at(w + 1);
+        if (b == e)
+            continue;
+        if (b == 0 && e == steps)
+            return;  // it has written the result
+        from = from < 0 ? w : from;
+        upto = w;
     }
-    const int x = x0 + col, j = x / group, head = kv * group + x % group;
-    const int last = a.causal ? sq.shift + j : nk;
-    const T *qp = (const T *)a.q.data + head * a.q.head + (int64_t)(sq.first + j) * a.q.row;
-    Frag<T> qf[2][D / 32];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk)
-            qf[m][kk] = load_frag(qp + m * a.q.map, kk * 32 + 8 * g, a.dim, col < count, FAST || a.vec);
-
-    f32x4 acc[2][D / 8];
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-        acc[0][i] = acc[1][i] = f32x4{0, 0, 0, 0};
-
-    wait_loads();
-    for (int k0 = begin; k0 < run.end; k0 += 32 * W) {
-        const bool more = k0 + 32 * W < run.end;
-        const unsigned bits = next_bits;
-        if constexpr (FAST)
-            wait_all_but<PL::N>();
-        else
-            wait_loads();
-        f32x4 s[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                s[m][u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int kk = 0; kk < D / 32; ++kk)
-                    s[m][u] = mma(rd.row_frag(smem + kt, 16 * u, m * D + kk * 32), qf[m][kk], s[m][u]);
-            }
-        wait_reads();
-        if (more) {
-            find(k0 + 32 * W);
-            lk.load(a, smem, kt, key_bytes, next_bits, next_bits == ~0u);
-        }
-        if (bits != ~0u || k0 + 31 > last) {
-            const unsigned mine = bits >> (4 * g);
-            const int most = last - k0 - 4 * g;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool on = (mine >> (16 * u + r) & 1) && 16 * u + r <= most;
-                    s[0][u][r] = on ? s[0][u][r] : -INFINITY;
-                    s[1][u][r] = on ? s[1][u][r] : -INFINITY;
-                }
-        }
-        Frag<T> pf[2];
+    if (from < 0)
+        return;
+    const int count = (int)min((int64_t)COLS, columns - x0);
+    for (int e = piece * blockDim.x + threadIdx.x; e < count * (D / 2); e += pieces * blockDim.x) {
+        const int x = e / (D / 2), y = e % (D / 2) * 4;
+        auto run = [&](int w, int m) {
+            return role.r.part + (((int64_t)w * 2 + (w == from)) * COLS * 2 + x * 2 + m) * kPart<D>;
+        };
+        f32x4 v[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            float hi = s[m][0][0];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    hi = fmaxf(hi, s[m][u][r]);
-            hi = fmaxf(top[m], column_max(hi) * c);
-            if (__any(hi > top[m])) {
-                const float f = top[m] == -INFINITY ? 0.f : exp2_fast(top[m] - hi);
-                top[m] = hi;
-                sum[m] *= f;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    acc[m][i] *= f;
-            }
-            const float level = hi == -INFINITY ? 0.f : hi;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = exp2_fast(fmaf(s[m][u][r], c, -level));
-                    s[m][u][r] = p;
-                    sum[m] += p;
-                }
-            pf[m] = pack<T>(s[m][0], s[m][1]);
-        }
-        if (FAST && more)
-            wait_all_but<PL::N>();
-        else
-            wait_loads();
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            const Frag<T> vf = rd.column_frag(smem + vt, 0, i * 16);
-            acc[0][i] = mma(vf, pf[0], acc[0][i]);
-            acc[1][i] = mma(vf, pf[1], acc[1][i]);
-        }
-        wait_reads();
-        if (more)
-            lv.load(a, smem, vt, value_bytes, next_bits, next_bits == ~0u);
-    }
-
-    // Join the waves, one map at a time: column-major products in LDS, and the
-    // first map's result beside them while the second's are joined.
-    float *red = reinterpret_cast<float *>(smem);  // [W][16][kPart], [16][2 D]
-    float *first = red + W * 16 * kPart<D>;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const float total = column_sum(sum[m]);
-        __syncthreads();
-        float *mine = red + (wave * 16 + col) * kPart<D>;
-        if (g == 0) {
-            mine[0] = top[m];
-            mine[1] = total;
-        }
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<f32x4 *>(mine + 4 + i * 16 + 4 * g) = acc[m][i];
-        __syncthreads();
-        for (int e = tid; e < count * 2 * D; e += W * kWave) {
-            const int h = e / (2 * D), y = e % (2 * D);
-            float hi = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-                hi = fmaxf(hi, red[(w * 16 + h) * kPart<D>]);
-            float v = 0.f, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float *o = red + (w * 16 + h) * kPart<D>;
-                const float f = o[0] == -INFINITY ? 0.f : exp2_fast(o[0] - hi);
-                v = fmaf(f, o[4 + y], v);
-                l = fmaf(f, o[1], l);
-            }
-            if (run.used > 1) {
-                float *p = deep_result<D>(a, seq, kv, x0 + h, m, split);
-                if (y == 0) {
-                    p[0] = hi;
-                    p[1] = l;
-                }
-                p[4 + y] = v;
-                continue;
-            }
-            v = l == 0.f ? 0.f : v / l;
-            if (m == 0) {
-                first[e] = v;
-            } else if (y % D < a.dim) {
-                const int hd = kv * group + (x0 + h) % group, row = sq.first + (x0 + h) / group;
-                ((T *)a.out.data)[(int64_t)row * a.out.row + hd * a.out.head + y / D * a.out.map + y % D] =
-                    (T)(first[e] - a.lambda[hd] * v);
-            }
-        }
-    }
-}
-
-template <class T, int D, int W, int M, int QT, int KB, int BUF, int OCC, bool FAST>
-__global__ __launch_bounds__(W * kWave, OCC) void paged_broad_kernel(PagedArgs a)
-{
-    extern __shared__ __align__(16) char smem[];
-    broad_part<T, D, W, M, QT, KB, BUF, FAST>(a, blockIdx.x, smem);
-}
-template <class T, int D, int W, int OCC, bool FAST>
-__global__ __launch_bounds__(W * kWave, OCC) void paged_deep_kernel(PagedArgs a)
-{
-    extern __shared__ __align__(16) char smem[];
-    deep_part<T, D, W, FAST>(a, blockIdx.x, smem);
-}
-
-// Four columns from y on of a row and head from the runs of both maps.
-template <class T, int D>
-__device__ inline void join_runs(const PagedArgs &a, const float *p0, const float *p1, int used, int64_t row, int head, int y)
-{
-    const float *from[2] = {p0, p1};
-    f32x4 v[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const float *p = from[m];
-        float hi = kNoLevel;
+            float hi = kNoLevel, total = 0.f;
 #pragma unroll 4
-        for (int i = 0; i < used; ++i)
-            hi = fmaxf(hi, p[i * kPart<D>]);
-        float total = 0.f;
-        v[m] = f32x4{0, 0, 0, 0};
+            for (int w = from; w <= upto; ++w)
+                if (part_at(w) != part_at(w + 1))
+                    hi = fmaxf(hi, run(w, m)[0]);
+            v[m] = f32x4{0, 0, 0, 0};
 #pragma unroll 4
-        for (int i = 0; i < used; ++i) {
-            const float f = exp2_fast(p[i * kPart<D>] - hi);  // 0 of an empty run
-            total = fmaf(f, p[i * kPart<D> + 1], total);
-            v[m] += f * *reinterpret_cast<const f32x4 *>(p + i * kPart<D> + 4 + y);
+            for (int w = from; w <= upto; ++w) {
+                if (part_at(w) == part_at(w + 1))
+                    continue;
+                const float *p = run(w, m);
+                const float f = exp2_fast(p[0] - hi);  // 0 of an empty run
+                total = fmaf(f, p[1], total);
+                v[m] += f * *reinterpret_cast<const f32x4 *>(p + 4 + y);
+            }
+            v[m] *= total == 0.f ? 0.f : 1.f / total;
         }
-        v[m] *= total == 0.f ? 0.f : 1.f / total;
+        const int64_t row = sq.first + (x0 + x) / group;
+        const int head = kv * group + (int)((x0 + x) % group);
+        T *out = (T *)a.out.data + row * a.out.row + head * a.out.head + y / D * a.out.map;
+        store4(out, y % D, a.dim, v[0] - a.lambda[head] * v[1], a.vec);
     }
-    T *out = (T *)a.out.data + row * a.out.row + head * a.out.head + y / D * a.out.map;
-    store4(out, y % D, a.dim, v[0] - a.lambda[head] * v[1], a.vec);
-}
-constexpr int kJoin = 256;
-
-// A workgroup per sequence, group and block of 16 columns.
-template <class T, int D>
-__global__ __launch_bounds__(kJoin) void paged_join_deep(PagedArgs a)
-{
-    const int block = blockIdx.x % a.deep_blocks, kv = blockIdx.x / a.deep_blocks % a.kv_heads;
-    const int seq = blockIdx.x / a.deep_blocks / a.kv_heads, group = a.heads / a.kv_heads;
-    const Sequence sq(a, seq);
-    const int64_t columns = (int64_t)sq.rows * group;
-    const int x0 = block * 16;
-    if (columns > a.deep || x0 >= columns)
-        return;
-    const int count = min(16, (int)columns - x0);
-    const int used = Run(sq.keys(a, (x0 + count - 1) / group), 0, a.deep_splits, 32, a.deep_least / 32).used;
-    if (used <= 1)
-        return;
-    for (int e = threadIdx.x; e < count * (D / 2); e += kJoin) {
-        const int x = x0 + e / (D / 2), y = e % (D / 2) * 4;
-        join_runs<T, D>(a, deep_result<D>(a, seq, kv, x, 0, 0), deep_result<D>(a, seq, kv, x, 1, 0), used,
-                        sq.first + x / group, kv * group + x % group, y);
-    }
-}
-
-// D / 2 lanes per row and head.
-template <class T, int D>
-__global__ __launch_bounds__(kJoin) void paged_join_broad(PagedArgs a, int unit)
-{
-    constexpr int kLanes = D / 2;
-    const int64_t item = (int64_t)blockIdx.x * (kJoin / kLanes) + threadIdx.x / kLanes;
-    const int64_t row = item / a.heads;
-    const int head = item % a.heads, group = a.heads / a.kv_heads;
-    const int seq = last_true([&](int i) { return row_offset(a.offsets, i, a.rows) <= row; }, a.sequences + 1, kLanes);
-    if (row >= a.rows || seq < 0 || seq >= a.sequences)
-        return;
-    const Sequence sq(a, seq);
-    const int64_t columns = (int64_t)sq.rows * group, x = (row - sq.first) * group + head % group;
-    if (columns <= a.deep)
-        return;
-    const int64_t end = min(columns, x / a.broad_columns * a.broad_columns + a.broad_columns);
-    const int used = Run(sq.keys(a, (int)((end - 1) / group)), 0, a.broad_splits, unit, a.broad_least / unit).used;
-    if (used > 1)
-        join_runs<T, D>(a, broad_result<D>(a, row, head, 0, 0), broad_result<D>(a, row, head, 1, 0), used, row, head,
-                        threadIdx.x % kLanes * 4);
 }
 
 // Tile shapes by head width.
 template <class T, int D>
 struct Shape {
+    static constexpr int kWaves = 4;
     static constexpr int kRows = 2 * D * (int)sizeof(T) <= 256 ? 64 : 32;
-    // maps of a wave, and groups of 16 columns in broad tiles: two share the
-    // reads from LDS that bound 16-bit products; 32-bit products take so long
-    // that more waves serve them better
-    static constexpr int kMaps = D == 128 && sizeof(T) == 2 ? 1 : 2;
-    static constexpr int kWide = sizeof(T) == 2 ? 2 : 1;
-    static constexpr size_t kLds = 2 * (size_t)kRows * 2 * D * sizeof(T);
+    static constexpr size_t kTiles = 2 * (size_t)kRows * 2 * D * sizeof(T);
     // two buffers of both tiles within the 64 KiB that loads into LDS address
-    static constexpr int kBuffers = kLds <= 32768 ? 2 : 1;
-    static constexpr int kOccupancy = kLds > 32768 ? 1 : 2;
-    // waves whose keys and values of a step fit into that
-    static constexpr int kDeepWaves = 512 / (D * (int)sizeof(T)) > 8 ? 8 : 512 / (D * (int)sizeof(T));
-    static constexpr int kGroup = 32 / (D * (int)sizeof(T) / 16);  // rows of 1 KiB
+    static constexpr int kBuffers = kTiles <= 32768 ? 2 : 1;
+    static constexpr size_t kLds = kBuffers * kTiles;
+    // maps of a wave and groups of 16 columns: narrow tiles have two waves that
+    // work on 16 columns, which keeps them behind the reads of the cache
+    static constexpr int kMaps = sizeof(T) == 2 && D <= 64 ? 2 : 1, kGroups = sizeof(T) == 4 && D == 128 ? 1 : 2;
+    static constexpr int kNarrow = kWaves / 2 * 16, kWide = kWaves * kMaps / 2 * kGroups * 16;
+    static constexpr int kPage = kRows / kWaves;  // rows of a wave
 };
-constexpr int kWaves = 4;  // of the broad part
 
-template <int D, bool FAST>
-hipError_t deep(const PagedArgs &a, hipStream_t s)
+template <class T, int D, bool FAST>
+__global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_narrow_kernel(PagedArgs a)
 {
-    constexpr int W = Shape<Type, D>::kDeepWaves;
-    constexpr size_t tiles = (size_t)W * 2 * 32 * 2 * D * sizeof(Type);
-    static_assert(tiles <= 65536, "what loads into LDS address");
-    constexpr size_t join = ((size_t)W * 16 * kPart<D> + 16 * 2 * D) * sizeof(float);
-    constexpr int occ = W < 4 ? 1 : 2;  // waves per SIMD that LDS lets in
-    const int64_t items = (int64_t)a.sequences * a.kv_heads * a.deep_blocks;
-    const hipError_t e = launch_kernel(paged_deep_kernel<Type, D, W, occ, FAST>, dim3((unsigned)(items * a.deep_splits)),
-                                       dim3(W * kWave), tiles > join ? tiles : join, s, a);
-    if (e != hipSuccess || a.deep_splits == 1)
-        return e;
-    return launch_kernel(paged_join_deep<Type, D>, dim3((unsigned)items), dim3(kJoin), 0, s, a);
+    using S = Shape<T, D>;
+    // (behind the tiles: loads into LDS count from its start)
+    extern __shared__ __align__(16) char smem[];
+    Line &line = *reinterpret_cast<Line *>(smem + S::kLds);
+    work<T, D, S::kWaves, 1, 1, S::kRows, S::kBuffers, FAST, true>(a, blockIdx.x, smem, line);
 }
-template <int D, int QT, bool FAST>
-hipError_t broad(const PagedArgs &a, hipStream_t s)
+template <class T, int D, bool FAST>
+__global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_wide_kernel(PagedArgs a)
 {
-    using S = Shape<Type, D>;
-    const hipError_t e = launch_kernel(
-        paged_broad_kernel<Type, D, kWaves, S::kMaps, QT, S::kRows, S::kBuffers, S::kOccupancy, FAST>,
-        dim3((unsigned)((int64_t)a.broad_tiles * a.kv_heads * a.broad_splits)), dim3(kWaves * kWave), S::kBuffers * S::kLds, s, a);
-    if (e != hipSuccess || a.broad_splits == 1)
-        return e;
-    constexpr int items = kJoin / (D / 2);
-    return launch_kernel(paged_join_broad<Type, D>, dim3((unsigned)((a.rows * a.heads + items - 1) / items)), dim3(kJoin), 0, s, a,
-                         S::kRows);
+    using S = Shape<T, D>;
+    // (behind the tiles: loads into LDS count from its start)
+    extern __shared__ __align__(16) char smem[];
+    Line &line = *reinterpret_cast<Line *>(smem + S::kLds);
+    work<T, D, S::kWaves, S::kMaps, S::kGroups, S::kRows, S::kBuffers, FAST, false>(a, blockIdx.x, smem, line);
+}
+
+constexpr int kJoin = 256;
+template <class T, int D>
+__global__ __launch_bounds__(kJoin) void paged_narrow_join(PagedArgs a)
+{
+    using S = Shape<T, D>;
+    __shared__ Line line;
+    const Role<S::kNarrow> role{a.narrow, true};
+    const Shares<S::kNarrow> shares(a, role, line);
+    const int kv = blockIdx.x % a.kv_heads, seq = blockIdx.x / a.kv_heads;
+    const Sequence sq(a, seq);
+    if (role.tiles(a, sq) == 0)
+        return;
+    const int at = kv * shares.head + shares.start(seq);
+    join_unit<T, D, S::kNarrow, S::kRows>(a, role, sq, kv, 0, at, at + role.cost(a, sq, 1), shares.each, shares.total, 0, 1);
+}
+template <class T, int D>
+__global__ __launch_bounds__(kJoin) void paged_wide_join(PagedArgs a, int pieces)
+{
+    using S = Shape<T, D>;
+    __shared__ Line line;
+    const Role<S::kWide> role{a.wide, false};
+    const Shares<S::kWide> shares(a, role, line);
+    const int piece = blockIdx.x % pieces, kv = blockIdx.x / pieces % a.kv_heads, at = blockIdx.x / pieces / a.kv_heads;
+    const int group = a.heads / a.kv_heads;
+    auto start = [&](int i) { return (int64_t)row_offset(a.offsets, i, a.rows) * group / S::kWide + i; };
+    const int seq = last_true([&](int i) { return start(i) <= at; }, a.sequences, kWave);
+    if (seq < 0)
+        return;
+    const Sequence sq(a, seq);
+    const int tile = (int)(at - start(seq));
+    if (tile >= role.tiles(a, sq))
+        return;
+    const int from = kv * shares.head + shares.start(seq);
+    join_unit<T, D, S::kWide, S::kRows>(a, role, sq, kv, tile, from + role.cost(a, sq, tile), from + role.cost(a, sq, tile + 1),
+                                        shares.each, shares.total, piece,
+                                        pieces);
 }
 
 template <int D, bool FAST>
 hipError_t run(const PagedArgs &a, hipStream_t s)
 {
     using S = Shape<Type, D>;
-    if (a.broad_tiles > 0)
-        if (hipError_t e = a.broad_columns == kWaves * S::kMaps / 2 * 16 ? broad<D, 1, FAST>(a, s) : broad<D, S::kWide, FAST>(a, s))
+    const dim3 block(S::kWaves * kWave);
+    if (a.wide.groups > 0) {
+        hipError_t e = launch_kernel(paged_wide_kernel<Type, D, FAST>, dim3((unsigned)a.wide.groups), block, S::kLds + sizeof(Line), s, a);
+        if (e == hipSuccess && a.wide.part) {
+            constexpr int pieces = S::kWide * (D / 2) / kJoin;
+            e = launch_kernel(paged_wide_join<Type, D>, dim3((unsigned)((int64_t)a.wide.tiles * a.kv_heads * pieces)), dim3(kJoin), 0,
+                              s, a, pieces);
+        }
+        if (e != hipSuccess)
             return e;
-    return a.deep > 0 ? deep<D, FAST>(a, s) : hipSuccess;
+    }
+    if (a.narrow.groups == 0)
+        return hipSuccess;
+    const hipError_t e = launch_kernel(paged_narrow_kernel<Type, D, FAST>, dim3((unsigned)a.narrow.groups), block, S::kLds + sizeof(Line), s, a);
+    if (e != hipSuccess || !a.narrow.part)
+        return e;
+    return launch_kernel(paged_narrow_join<Type, D>, dim3((unsigned)((int64_t)a.sequences * a.kv_heads)), dim3(kJoin), 0, s, a);
 }
 template <int D>
 hipError_t by_pages(const PagedArgs &a, hipStream_t s)
 {
-    return a.vec && a.cache.page_rows % Shape<Type, D>::kGroup == 0 ? run<D, true>(a, s) : run<D, false>(a, s);
+    return a.alike && a.cache.page_rows % Shape<Type, D>::kPage == 0 ? run<D, true>(a, s) : run<D, false>(a, s);
 }
 
 }  // namespace
