@@ -114,14 +114,21 @@ struct HeadArgs {
     int lanes;  // of a row: a power of two from group up to 256
 };
 
+// n / d for n below 2^31: the upper half of 2 n magic, shifted.
+struct Divisor {
+    unsigned magic;
+    int shift;
+};
+
 // How the tiles of one width are given to workgroups.
 struct RoleArgs {
     int groups;     // workgroups (0: none)
     int each_unit;  // one takes one tile; else they share all keys evenly,
-    int least;      // each with so many (as costs) at least, its partial results
+    int least;      // each with so many steps at least, its partial results
     float *part;    // here: [groups][2][columns][2][4 + 2 D] (NULL: one group)
-    int shift;      // costs are counted in units of 2^shift keys
-    int tiles;      // wide: the most of a key head
+    // wide: the most tiles of a key head, and of four times the columns (0: every
+    // tile in its turn)
+    int tiles, quarters;
 };
 
 struct PagedArgs {
@@ -134,9 +141,8 @@ struct PagedArgs {
     const float *lambda;
     int vec;
     int alike;  // and keys and values have the same strides, within 32 bits a row
-    // key / page_rows is the upper half of 2 key page_magic, shifted
-    unsigned page_magic;
-    int page_shift;
+    int heads_each;       // of a group
+    Divisor page, group;  // by page_rows and heads_each
     // sequences of up to so many columns (a row's head of the group that shares
     // a key head) have a narrow tile, the others wide ones
     int narrow_columns;

@@ -235,7 +235,7 @@ struct PagedPlan {
     int64_t items = 0;
 };
 constexpr int kNarrowColumns = 32;
-constexpr int64_t kMaxShared = 4096;  // sequences whose keys workgroups share
+constexpr int64_t kMaxShared = 4096, kMaxUnits = 1 << 18;  // sequences and tiles whose keys workgroups share
 
 PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
 {
@@ -246,15 +246,12 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     const int width = r.dim <= 32 ? 32 : r.dim <= 64 ? 64 : 128;
     const bool half = r.dtype != MTPX_F32;
     // workgroups that the device holds at once: by their 64 KiB of LDS, or 32
-    const int64_t slots = 2 * (int64_t)ctx->num_cus, least = 512;
+    const int64_t slots = 2 * (int64_t)ctx->num_cus;
     auto role = [&](RoleArgs &a, size_t &bytes, int columns, int64_t units, bool each) {
-        a.each_unit = each || n > kMaxShared;
-        // all costs together stay below 2^30
-        const int64_t most_cost = units * (256 + room + r.rows);
-        while (most_cost >> a.shift >= int64_t(1) << 30)
-            ++a.shift;
-        a.least = (int)std::max<int64_t>(least >> a.shift, 1);
-        const int64_t groups = a.each_unit ? units : std::min(slots * (width == 32 && half ? 2 : 1), units * ((room + 255) / 256));
+        // (costs are counted in 32 bits)
+        a.each_unit = each || n > kMaxShared || units > kMaxUnits || units * ((room + r.rows) / 32 + 16) > INT32_MAX / 2;
+        a.least = 2;
+        const int64_t groups = a.each_unit ? units : std::min(slots * (width == 32 && half ? 2 : 1), units * ((room + 63) / 64));
         a.groups = (int)std::min<int64_t>(groups, INT32_MAX);
         p.items += groups;
         if (!a.each_unit && a.groups > 1)
@@ -267,10 +264,22 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     if (p.narrow_columns == 0 || most * group > kNarrowColumns) {
         const int columns = half ? (width < 128 ? 128 : 64) : width < 128 ? 64 : 32;
         const int64_t tiles = r.rows * group / columns + n;
+        const bool each = r.rows * group / columns * r.kv_heads >= 4 * slots;
         p.wide.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
-        role(p.wide, p.wide_bytes, columns, tiles * r.kv_heads, r.rows * group / columns * r.kv_heads >= 4 * slots);
+        p.wide.quarters = each && r.causal ? (int)std::min<int64_t>(r.rows * group / (4 * columns) + n, INT32_MAX) : 0;
+        role(p.wide, p.wide_bytes, columns, (tiles + p.wide.quarters) * r.kv_heads, each);
     }
     return p;
+}
+
+// magic = floor(2^(31 + shift) / d) + 1 with 2^shift >= d: n magic / 2^(31 + shift)
+// is above n / d by less than n / 2^31 of 1 / d.
+Divisor divisor(int d)
+{
+    int shift = 0;
+    while ((1 << shift) < d)
+        ++shift;
+    return {(unsigned)((uint64_t(1) << (31 + shift)) / (uint64_t)d + 1), shift};
 }
 
 int check_paged(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
@@ -426,11 +435,9 @@ int mtpx_diff_attention_paged(mtpx_context *ctx, const mtpx_diff_attention_paged
         const mtpx_pages &c = r.cache;
         const int64_t limit = int64_t(1) << 26;  // elements: eight rows and two maps stay within 32 bits of bytes
         a.alike = a.vec && c.k.row == c.v.row && c.k.map == c.v.map && c.k_page == c.v_page && c.k.row < limit && c.k.map < limit;
-        int bits = 0;
-        while ((1 << bits) < r.cache.page_rows)
-            ++bits;
-        a.page_shift = bits;
-        a.page_magic = (unsigned)((uint64_t(1) << (31 + bits)) / (uint64_t)r.cache.page_rows + 1);
+        a.heads_each = r.heads / r.kv_heads;
+        a.page = divisor(c.page_rows);
+        a.group = divisor(a.heads_each);
         a.narrow_columns = p.narrow_columns;
         a.narrow = p.narrow;
         a.wide = p.wide;

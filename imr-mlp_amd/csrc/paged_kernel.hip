@@ -37,12 +37,15 @@ typedef _Float16 Type;
 // the level of a row that has seen no key, is passed by every finite score.
 constexpr float kSlack = 8.f, kNoLevel = -3.0e38f;
 
+// n / d for n below 2^31, by what the host has made of d.
+__device__ inline int quotient(int n, const Divisor &d) { return (int)(__umulhi(2u * (unsigned)n, d.magic) >> d.shift); }
+
 // One sequence's place in the batch and in the cache.
 struct Sequence {
-    int first, rows;   // of the batch
-    int length, shift; // keys; row j sees those up to shift + j (causal)
-    const int *table;
+    int first, rows;    // of the batch
+    int length, shift;  // keys; row j sees those up to shift + j (causal)
 
+    __device__ inline Sequence() : first(0), rows(0), length(0), shift(0) {}
     __device__ inline Sequence(const PagedArgs &a, int i)
     {
         first = row_offset(a.offsets, i, a.rows);
@@ -50,12 +53,21 @@ struct Sequence {
         const int given = max(0, a.lengths[i]);
         length = min(given, a.cache.table_width * a.cache.page_rows);
         shift = given - rows;
-        table = a.cache.table + i * a.cache.table_row;
     }
-    // Keys that rows up to `last` see.
+    // Lane `lane`'s, in all lanes.
+    __device__ inline Sequence of_lane(int lane) const
+    {
+        Sequence s;
+        s.first = __builtin_amdgcn_readlane(first, lane);
+        s.rows = __builtin_amdgcn_readlane(rows, lane);
+        s.length = __builtin_amdgcn_readlane(length, lane);
+        s.shift = __builtin_amdgcn_readlane(shift, lane);
+        return s;
+    }
+    // Keys that columns up to `last` see.
     __device__ inline int keys(const PagedArgs &a, int last) const
     {
-        return a.causal ? max(0, min(length, shift + last + 1)) : length;
+        return a.causal ? max(0, min(length, shift + quotient(last, a.group) + 1)) : length;
     }
 };
 
@@ -64,26 +76,36 @@ template <int D>
 constexpr int kPart = 4 + 2 * D;
 
 // What kernels of one width of tiles are told apart by: sequences of up to
-// a.narrow columns have one narrow tile, the others wide ones.
-template <int COLS>
+// a.narrow_columns columns have one narrow tile, the others wide ones.  (Columns:
+// below 2^23, as rows and heads are.)
+template <int COLS, int KB>
 struct Role {
+    // what a unit takes to begin, in steps of KB keys
+    static constexpr int kStart = 128 / KB;
     const RoleArgs &r;
     bool narrow;
+
     __device__ inline int tiles(const PagedArgs &a, const Sequence &sq) const
     {
-        const int64_t columns = (int64_t)sq.rows * (a.heads / a.kv_heads);
-        return columns > 0 && (columns <= a.narrow_columns) == narrow ? (int)((columns + COLS - 1) / COLS) : 0;
+        const int columns = sq.rows * a.heads_each;
+        return columns > 0 && (columns <= a.narrow_columns) == narrow ? (columns + COLS - 1) / COLS : 0;
     }
-    // What the first t tiles of a sequence cost: the keys that they see and
-    // kStart for each, in units of 2^shift.  (Keys of causal tiles as a mean over
-    // their rows: a cost need not be exact, only the same in every workgroup.)
+    // The steps of tile t.
+    __device__ inline int steps(const PagedArgs &a, const Sequence &sq, int t) const
+    {
+        return (sq.keys(a, min((t + 1) * COLS, sq.rows * a.heads_each) - 1) + KB - 1) / KB;
+    }
+    // What the first t tiles of a sequence cost: kStart and no less than its steps
+    // each.  Where the new rows are a small part, every tile as much as the last.
+    // Else tile t has before + (t + 1) COLS / g keys, rounded up, whose sum's
+    // rounding may leave a step off and the keys' two more: four are added.
     __device__ inline int cost(const PagedArgs &a, const Sequence &sq, int t) const
     {
-        const int before = a.causal ? max(0, sq.length - sq.rows) : sq.length;
-        const int64_t slope = a.causal ? (int64_t)t * (t + 1) * COLS / (2 * (a.heads / a.kv_heads)) : 0;
-        return t * (start() + (before >> r.shift)) + (int)(slope >> r.shift);
+        if (!a.causal || sq.rows <= sq.length / 8)
+            return t * (kStart + (sq.length + KB - 1) / KB);
+        const int before = max(0, min(sq.shift, sq.length)) / KB + 4;
+        return t * (kStart + before) + (int)((int64_t)t * (t + 1) / 2 * COLS / (a.heads_each * KB));
     }
-    __device__ inline int start() const { return max(1, 256 >> r.shift); }
 };
 
 // Inclusive sums over a wave: shifts within rows of 16 lanes, then from row to row.
@@ -100,79 +122,98 @@ __device__ inline int wave_scan(int v)
 // The units of one key head lie one after the other on a line of costs, tile by
 // tile and sequence by sequence, the key heads behind one another; workgroup w
 // takes what lies from w `each` on.  Built by a whole workgroup, for up to 64 runs
-// of 64 sequences.
+// of 64 sequences (of more than one run, the sums before each lie in LDS).
 struct Line {
-    int before[kWave];  // cost of the sequences before each run of 64
+    int before[kWave];
 };
-template <int COLS>
+struct Costs {
+    int head, total, each;  // of a key head, of all, of a workgroup
+};
+template <class R>
 struct Shares {
     const PagedArgs &a;
-    Role<COLS> role;
+    const R &role;
     Line &line;
-    int head, total, each;  // of a key head, of all, of a workgroup
+    Costs costs;
+    int lane;
+    // the lane's sequence of a run of 64, and the costs up to its end and before the run
+    int run = -1, upto = 0, own = 0;
+    Sequence sq;
 
-    __device__ inline int sequence_cost(int i) const
+    __device__ inline bool single() const { return a.sequences <= kWave; }
+    __device__ inline void read(int i)
     {
-        if (i >= a.sequences)
-            return 0;
-        const Sequence sq(a, i);
-        return role.cost(a, sq, role.tiles(a, sq));
+        if (i == run)
+            return;
+        run = i;
+        const int at = i * kWave + lane;
+        sq = Sequence();
+        if (at < a.sequences)
+            sq = Sequence(a, at);
+        own = role.cost(a, sq, role.tiles(a, sq));
+        upto = wave_scan(own) + (single() ? 0 : line.before[i]);
     }
-    __device__ inline int runs() const { return (a.sequences + kWave - 1) / kWave; }
-    __device__ inline Shares(const PagedArgs &args, const Role<COLS> &r, Line &l) : a(args), role(r), line(l)
+    // Where the line is there.
+    __device__ inline Shares(const PagedArgs &args, const R &r, Line &l, const Costs &c)
+        : a(args), role(r), line(l), costs(c), lane(threadIdx.x & (kWave - 1))
     {
-        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
-        if (runs() == 1) {
-            head = __builtin_amdgcn_readlane(wave_scan(sequence_cost(lane)), kWave - 1);
+    }
+    __device__ inline Shares(const PagedArgs &args, const R &r, Line &l)
+        : a(args), role(r), line(l), lane(threadIdx.x & (kWave - 1))
+    {
+        const int wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+        int groups = role.r.groups;
+        if (single()) {
+            read(0);
+            costs.head = __builtin_amdgcn_readlane(upto, kWave - 1);
+            // one sequence whose tiles cost the same: whole parts of a tile, which
+            // begin at the same keys and so read them together
+            if (a.sequences == 1) {
+                const int units = role.tiles(a, sq.of_lane(0)) * a.kv_heads, parts = units > 0 ? groups / units : 0;
+                if (parts * units >= groups / 8 * 7)
+                    groups = parts * units;
+            }
         } else {
-            for (int i = wave; i < runs(); i += waves) {
-                const int sum = wave_scan(sequence_cost(i * kWave + lane));
+            const int n = (a.sequences + kWave - 1) / kWave;
+            for (int i = wave; i < n; i += waves) {
+                const int at = i * kWave + lane;
+                Sequence s;
+                if (at < a.sequences)
+                    s = Sequence(a, at);
+                const int sum = wave_scan(role.cost(a, s, role.tiles(a, s)));
                 if (lane == kWave - 1)
                     line.before[i] = sum;
             }
             __syncthreads();
-            const int own = lane < runs() ? line.before[lane] : 0, upto = wave_scan(own);
+            const int mine = lane < n ? line.before[lane] : 0, all = wave_scan(mine);
             __syncthreads();
             if (wave == 0)
-                line.before[lane] = upto - own;  // (runs beyond the last begin where it ends)
+                line.before[lane] = all - mine;  // (runs beyond the last begin where it ends)
             __syncthreads();
-            head = __builtin_amdgcn_readlane(upto, kWave - 1);
+            costs.head = __builtin_amdgcn_readlane(all, kWave - 1);
         }
-        total = head * a.kv_heads;
-        each = max((total + role.r.groups - 1) / role.r.groups, role.r.least);
+        costs.total = costs.head * a.kv_heads;
+        costs.each = max((costs.total + groups - 1) / groups, role.r.least);
     }
-    // The sequence at cost p (below head) of a key head, and the cost of those before it.
-    __device__ inline int find(int p, int &start) const
+    // The sequence at cost p (below costs.head) of a key head, and the cost of those before it.
+    __device__ inline int find(int p, Sequence &s, int &start)
     {
-        const int lane = threadIdx.x & (kWave - 1);
-        const int run = runs() == 1 ? 0 : __popcll(__ballot(line.before[lane] <= p)) - 1;
-        const int own = sequence_cost(run * kWave + lane);
-        const int upto = wave_scan(own) + (runs() == 1 ? 0 : line.before[run]);
+        read(single() ? 0 : __popcll(__ballot(line.before[lane] <= p)) - 1);
         const int l = __popcll(__ballot(upto <= p));
         start = __builtin_amdgcn_readlane(upto - own, l);
+        s = sq.of_lane(l);
         return run * kWave + l;
     }
-    // The cost of the sequences before i.
-    __device__ inline int start(int i) const
+    // Sequence i, and the cost of those before it.
+    __device__ inline void at(int i, Sequence &s, int &start)
     {
-        const int lane = threadIdx.x & (kWave - 1), run = i / kWave;
-        const int own = sequence_cost(run * kWave + lane);
-        return __builtin_amdgcn_readlane(wave_scan(own) - own, i % kWave) + (runs() == 1 ? 0 : line.before[run]);
+        read(i / kWave);
+        start = __builtin_amdgcn_readlane(upto - own, i % kWave);
+        s = sq.of_lane(i % kWave);
     }
 };
 
-// Where cost p falls into the n steps of a unit whose costs begin at a0, its keys'
-// at `keys`, and end at a1.  (In 64-bit floats, whose quotient is the same
-// wherever it is formed, and does not fall as p grows.)
-__device__ inline int step_at(int p, int keys, int a1, int n)
-{
-    return p >= a1 ? n : p <= keys ? 0 : min(n, (int)((double)(p - keys) * n / (a1 - keys)));
-}
-
-__device__ inline int page_of(const PagedArgs &a, int key)
-{
-    return (int)(__umulhi(2u * (unsigned)key, a.page_magic) >> a.page_shift);
-}
+__device__ inline int page_of(const PagedArgs &a, int key) { return quotient(key, a.page); }
 __device__ inline bool there(const PagedArgs &a, int page) { return page >= 0 && page < a.cache.pages; }
 
 // The way of a tile of keys and values from the pages straight into LDS, by W
@@ -302,12 +343,13 @@ __device__ inline void store_columns(T *row, int64_t map, int dim, int t, int la
     store4(row + m * map, c, dim, v, vec);
 }
 
-// A run of a unit's keys: tiles of KB keys [begin, end) of `steps`; all of them
-// give the result, others a partial one.
+// A run of a unit's keys: steps [begin, end) of `steps` of KB keys each; all of
+// them give the result, others a partial one.
 struct Segment {
     int kv, begin, end, steps;
-    int64_t x0;  // first column of the tile
+    int x0;  // first column of the tile
     float *part;
+    const int *table;
 };
 
 // Keys and values come in tiles of KB rows, the next one while the present one is
@@ -329,26 +371,24 @@ __device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segm
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m0 = M == 2 ? 0 : wave & 1, part = M == 2 ? wave : wave >> 1;
-    const int group = a.heads / a.kv_heads, kv = sg.kv;
-    const int64_t columns = (int64_t)sq.rows * group, x0 = sg.x0;
-    const int nk = sq.keys(a, (int)((min(x0 + kCols, columns) - 1) / group));
+    const int group = a.heads_each, kv = sg.kv, columns = sq.rows * group, x0 = sg.x0;
+    const int nk = sq.keys(a, min(x0 + kCols, columns) - 1);
     const int run_begin = sg.begin * KB, run_end = min(nk, sg.end * KB);
 
-    TileLoader<T, D, KB, W, FAST> tiles(a, sq.table, kv, lane, wave);
+    TileLoader<T, D, KB, W, FAST> tiles(a, sg.table, kv, lane, wave);
     tiles.look_up(run_begin, run_end);
     const float c = a.scale * kLog2e;
     Reader<T, D> rd;
     rd.init(lane);
 
-    const int64_t w0 = x0 + part * QT * 16;  // first column of the wave
+    const int w0 = x0 + part * QT * 16;  // first column of the wave
     Frag<T> qf[M][QT][D / 32];
     int last[QT];  // key that the lane's column sees
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t x = w0 + t * 16 + (lane & 15);
-        const int j = (int)(x / group);
+        const int x = w0 + t * 16 + (lane & 15), j = quotient(x, a.group);
         last[t] = a.causal ? sq.shift + j : nk;
-        const T *qp = (const T *)a.q.data + (kv * group + x % group) * a.q.head + (int64_t)(sq.first + j) * a.q.row;
+        const T *qp = (const T *)a.q.data + (kv * group + x - j * group) * a.q.head + (int64_t)(sq.first + j) * a.q.row;
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -357,8 +397,8 @@ __device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segm
     }
     // keys that the wave's first and last columns see last
     const bool none = w0 >= columns;
-    const int low = a.causal ? sq.shift + (int)(w0 / group) : nk;
-    const int high = a.causal ? sq.shift + (int)((min(w0 + QT * 16, columns) - 1) / group) : nk;
+    const int low = a.causal ? sq.shift + quotient(w0, a.group) : nk;
+    const int high = a.causal ? sq.shift + quotient(max(min(w0 + QT * 16, columns) - 1, 0), a.group) : nk;
     f32x4 acc[M][QT][D / 8];
     float level[M][QT], sum[M][QT];
 #pragma unroll
@@ -513,9 +553,8 @@ __device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segm
     __syncthreads();  // the last tile's reads, before its place takes results or another tile
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t x = w0 + t * 16 + (lane & 15);
-        const int head = kv * group + (int)(x % group);
-        const int64_t row = sq.first + x / group;
+        const int x = w0 + t * 16 + (lane & 15), j = quotient(x, a.group), head = kv * group + x - j * group;
+        const int64_t row = sq.first + j;
         float total[M];
 #pragma unroll
         for (int m = 0; m < M; ++m)
@@ -568,127 +607,125 @@ __device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segm
     }
 }
 
+// The number of the first tile of sequence i among all wide ones: tiles of
+// different sequences have different numbers, some none.
+template <int COLS>
+__device__ inline int tile_number(const PagedArgs &a, int i)
+{
+    return row_offset(a.offsets, i, a.rows) * a.heads_each / COLS + i;
+}
+
 // The work of workgroup `item` of a role: one unit, or the runs of units that lie
 // in its share.
 template <class T, int D, int W, int M, int QT, int KB, int BUF, bool FAST, bool NARROW>
 __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line)
 {
     constexpr int kCols = W * M / 2 * QT * 16;
-    const Role<kCols> role{NARROW ? a.narrow : a.wide, NARROW};
-    const int group = a.heads / a.kv_heads, n = role.r.groups;
+    const Role<kCols, KB> role{NARROW ? a.narrow : a.wide, NARROW};
     // neighbours on one XCD, whose L2 holds the keys that they share
-    const int w = n % 8 ? item : item % 8 * (n / 8) + item / 8;
-    int p = 0, p0 = 0, p1 = 0;  // on the line: the next unit's, the share's
-    for (bool begun = false;; begun = true) {
-        int seq, kv, tile, a0 = 0, a1 = 0;
+    const int n = role.r.groups, w = n % 8 ? item : item % 8 * (n / 8) + item / 8;
+    Costs costs{0, 0, 0};
+    if (!role.r.each_unit)
+        costs = Shares<Role<kCols, KB>>(a, role, line).costs;
+    const int p0 = w * costs.each, p1 = min(p0 + costs.each, costs.total);
+    // (one place that works on a unit: a second would cost the first its registers)
+    for (int p = p0;;) {
+        Segment sg;
+        Sequence sq;
+        int seq, tile = 0;
+        bool any = true, late = false;
         if (!role.r.each_unit) {
-            const Shares<kCols> shares(a, role, line);
-            if (!begun) {
-                p0 = p = w * shares.each;
-                p1 = min(p0 + shares.each, shares.total);
-            }
             if (p >= p1)
                 return;
-            kv = (int)((unsigned)p / (unsigned)shares.head);
+            sg.kv = (int)((unsigned)p / (unsigned)costs.head);
+            Shares<Role<kCols, KB>> shares(a, role, line, costs);
             int at;
-            seq = __builtin_amdgcn_readfirstlane(shares.find(p - kv * shares.head, at));
-            at += kv * shares.head;
-            const Sequence sq(a, seq);
-            tile = __builtin_amdgcn_readfirstlane(
-                last_true([&](int t) { return at + role.cost(a, sq, t) <= p; }, role.tiles(a, sq), kWave));
-            a0 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile));
-            a1 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile + 1));
-        } else if (NARROW) {
-            seq = item / a.kv_heads;
-            kv = item % a.kv_heads;
-            tile = 0;
-        } else {
-            const Work wk = work_item(item, role.r.tiles, a.kv_heads);
-            // the last rows of a causal sequence have the most keys: they go first
-            const int at = role.r.tiles - 1 - wk.tile;
-            // (tile t of sequence i is number offsets[i] g / columns + i + t)
-            auto start = [&](int i) { return (int64_t)row_offset(a.offsets, i, a.rows) * group / kCols + i; };
-            seq = __builtin_amdgcn_readfirstlane(last_true([&](int i) { return start(i) <= at; }, a.sequences, kWave));
-            if (seq < 0)
-                return;
-            kv = wk.head;
-            tile = (int)(at - start(seq));
-        }
-        const Sequence sq(a, seq);
-        if (tile >= role.tiles(a, sq))
-            return;
-        const int64_t columns = (int64_t)sq.rows * group, x0 = (int64_t)tile * kCols;
-        const int nk = sq.keys(a, (int)((min(x0 + kCols, columns) - 1) / group)), steps = (nk + KB - 1) / KB;
-        Segment sg{kv, 0, steps, steps, x0, nullptr};
-        bool any = true;
-        if (!role.r.each_unit) {
-            sg.begin = __builtin_amdgcn_readfirstlane(step_at(p0, a0 + role.start(), a1, steps));
-            sg.end = __builtin_amdgcn_readfirstlane(step_at(p1, a0 + role.start(), a1, steps));
-            // a run that begins a unit and does not end it, or another
+            seq = shares.find(p - sg.kv * costs.head, sq, at);
+            at += sg.kv * costs.head;
+            if constexpr (!NARROW)
+                tile = __builtin_amdgcn_readfirstlane(
+                    last_true([&](int t) { return at + role.cost(a, sq, t) <= p; }, role.tiles(a, sq), kWave));
+            const int a0 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile)), keys = a0 + role.kStart;
+            sg.steps = role.steps(a, sq, tile);
+            sg.begin = max(0, min(sg.steps, p0 - keys));
+            sg.end = max(0, min(sg.steps, p1 - keys));
+            // a run that begins a unit lies behind one that does not
             sg.part = role.r.part + ((int64_t)w * 2 + (sg.begin == 0)) * kCols * 2 * kPart<D>;
             // a unit without keys has its zeros written where it begins
-            any = sg.begin < sg.end || (steps == 0 && p0 <= a0);
+            any = sg.begin < sg.end || (sg.steps == 0 && p0 <= a0);
+            p = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile + 1));
+        } else {
+            if constexpr (NARROW) {
+                seq = item / a.kv_heads;
+                sg.kv = item % a.kv_heads;
+            } else {
+                // sequence by sequence, whose workgroups then share what L2 holds of
+                // its keys, the last rows first; a causal sequence's first quarter,
+                // which sees the fewest keys, behind all others, to fill the end
+                const Work wk = work_item(item, role.r.tiles + role.r.quarters, a.kv_heads);
+                sg.kv = wk.head;
+                late = wk.tile >= role.r.tiles;
+                const int at = role.r.tiles - 1 - wk.tile + (late ? role.r.quarters : 0);
+                seq = __builtin_amdgcn_readfirstlane(last_true(
+                    [&](int i) { return (late ? tile_number<4 * kCols>(a, i) : tile_number<kCols>(a, i)) <= at; }, a.sequences, kWave));
+                if (seq < 0)
+                    return;
+                tile = at - (late ? tile_number<4 * kCols>(a, seq) : tile_number<kCols>(a, seq));
+            }
+            sq = Sequence(a, seq);
+            const int tiles = role.tiles(a, sq), quarter = NARROW || role.r.quarters == 0 ? 0 : (tiles + 3) / 4;
+            if (tile >= tiles || (!NARROW && role.r.quarters > 0 && (tile < quarter) != late))
+                return;
+            sg.begin = 0;
+            sg.end = sg.steps = role.steps(a, sq, tile);
+            sg.part = nullptr;
         }
+        sg.x0 = tile * kCols;
+        sg.table = a.cache.table + seq * a.cache.table_row;
         if (any)
             attend<T, D, W, M, QT, KB, BUF, FAST>(a, sq, sg, smem);
         if (role.r.each_unit)
             return;
-        p = a1;
     }
 }
 
-// Four columns from y on of a column x of a unit from the runs of both maps.
-template <class T, int D, int COLS, int KB>
-__device__ inline void join_unit(const PagedArgs &a, const Role<COLS> &role, const Sequence &sq, int kv, int tile, int a0, int a1,
-                                 int each, int total, int piece, int pieces)
+// Joins what several workgroups have left of a unit that begins at cost a0: those
+// in whose shares its steps lie.  `pieces` workgroups join a unit.
+constexpr int kJoin = 256;
+template <class T, int D, class R, int COLS>
+__device__ inline void join_unit(const PagedArgs &a, const R &role, const Shares<R> &shares, const Sequence &sq, int kv, int tile,
+                                 int a0, int piece, int pieces)
 {
-    const int group = a.heads / a.kv_heads;
-    const int64_t columns = (int64_t)sq.rows * group, x0 = (int64_t)tile * COLS;
-    const int nk = sq.keys(a, (int)((min(x0 + COLS, columns) - 1) / group)), steps = (nk + KB - 1) / KB;
-    const int first = a0 / each, last = (a1 - 1) / each;
-    auto part_at = [&](int w) { return step_at(min(w * each, total), a0 + role.start(), a1, steps); };
-    // the workgroups that have a run of the unit: the first has its begin
-    int from = -1, upto = -1;
-    for (int w = first; w <= last; ++w) {
-        const int b = part_at(w), e = part_at(w + 1);
-        if (b == e)
-            continue;
-        if (b == 0 && e == steps)
-            return;  // it has written the result
-        from = from < 0 ? w : from;
-        upto = w;
-    }
-    if (from < 0)
-        return;
-    const int count = (int)min((int64_t)COLS, columns - x0);
-    for (int e = piece * blockDim.x + threadIdx.x; e < count * (D / 2); e += pieces * blockDim.x) {
+    const int steps = role.steps(a, sq, tile), keys = a0 + role.kStart;
+    const int from = keys / shares.costs.each, upto = (keys + steps - 1) / shares.costs.each;
+    if (steps == 0 || from == upto)
+        return;  // written already
+    const int group = a.heads_each, x0 = tile * COLS, count = min(COLS, sq.rows * group - x0);
+    constexpr int kColumn = 2 * kPart<D>;
+    constexpr int64_t kSlot = (int64_t)COLS * kColumn;
+    for (int e = piece * kJoin + threadIdx.x; e < count * (D / 2); e += pieces * kJoin) {
         const int x = e / (D / 2), y = e % (D / 2) * 4;
-        auto run = [&](int w, int m) {
-            return role.r.part + (((int64_t)w * 2 + (w == from)) * COLS * 2 + x * 2 + m) * kPart<D>;
-        };
-        f32x4 v[2];
+        const float *p = role.r.part + from * 2 * kSlot + x * kColumn;
+        float hi[2] = {kNoLevel, kNoLevel}, total[2] = {0.f, 0.f};
+        f32x4 v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll 4
+        for (int i = 0; i <= upto - from; ++i) {
+            const float *q = p + (2 * i + (i == 0)) * kSlot;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float hi = kNoLevel, total = 0.f;
-#pragma unroll 4
-            for (int w = from; w <= upto; ++w)
-                if (part_at(w) != part_at(w + 1))
-                    hi = fmaxf(hi, run(w, m)[0]);
-            v[m] = f32x4{0, 0, 0, 0};
-#pragma unroll 4
-            for (int w = from; w <= upto; ++w) {
-                if (part_at(w) == part_at(w + 1))
-                    continue;
-                const float *p = run(w, m);
-                const float f = exp2_fast(p[0] - hi);  // 0 of an empty run
-                total = fmaf(f, p[1], total);
-                v[m] += f * *reinterpret_cast<const f32x4 *>(p + 4 + y);
+            for (int m = 0; m < 2; ++m, q += kPart<D>) {
+                const float level = q[0], up = fmaxf(hi[m], level);
+                // (0 for what has seen no key)
+                const float f = exp2_fast(hi[m] - up), g = exp2_fast(level - up);
+                hi[m] = up;
+                total[m] = fmaf(f, total[m], g * q[1]);
+                v[m] = f * v[m] + g * *reinterpret_cast<const f32x4 *>(q + 4 + y);
             }
-            v[m] *= total == 0.f ? 0.f : 1.f / total;
         }
-        const int64_t row = sq.first + (x0 + x) / group;
-        const int head = kv * group + (int)((x0 + x) % group);
-        T *out = (T *)a.out.data + row * a.out.row + head * a.out.head + y / D * a.out.map;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            v[m] *= total[m] == 0.f ? 0.f : 1.f / total[m];
+        const int j = quotient(x0 + x, a.group), head = kv * group + x0 + x - j * group;
+        T *out = (T *)a.out.data + (int64_t)(sq.first + j) * a.out.row + head * a.out.head + y / D * a.out.map;
         store4(out, y % D, a.dim, v[0] - a.lambda[head] * v[1], a.vec);
     }
 }
@@ -709,84 +746,81 @@ struct Shape {
     static constexpr int kPage = kRows / kWaves;  // rows of a wave
 };
 
-template <class T, int D, bool FAST>
-__global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_narrow_kernel(PagedArgs a)
+// Both roles in one launch, the wide tiles first, which take the longest.  (Eight
+// workgroups of each in turn, for the reads of one and the products of the other to
+// share the CUs, are slower: 48 sequences, two of them with chunks of 727 rows,
+// 388 us; 330 us so.)
+constexpr int kNarrowOnly = 1, kWideOnly = 2, kBoth = 3;
+template <class T, int D, bool FAST, int ROLES>
+__global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_kernel(PagedArgs a)
 {
     using S = Shape<T, D>;
-    // (behind the tiles: loads into LDS count from its start)
+    // (the line behind the tiles: loads into LDS count from its start)
     extern __shared__ __align__(16) char smem[];
     Line &line = *reinterpret_cast<Line *>(smem + S::kLds);
-    work<T, D, S::kWaves, 1, 1, S::kRows, S::kBuffers, FAST, true>(a, blockIdx.x, smem, line);
-}
-template <class T, int D, bool FAST>
-__global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_wide_kernel(PagedArgs a)
-{
-    using S = Shape<T, D>;
-    // (behind the tiles: loads into LDS count from its start)
-    extern __shared__ __align__(16) char smem[];
-    Line &line = *reinterpret_cast<Line *>(smem + S::kLds);
-    work<T, D, S::kWaves, S::kMaps, S::kGroups, S::kRows, S::kBuffers, FAST, false>(a, blockIdx.x, smem, line);
+    int item = blockIdx.x;
+    bool narrow = ROLES == kNarrowOnly;
+    if constexpr (ROLES == kBoth) {
+        narrow = item >= a.wide.groups;
+        if (narrow)
+            item -= a.wide.groups;
+    }
+    if (ROLES != kNarrowOnly && !narrow)
+        work<T, D, S::kWaves, S::kMaps, S::kGroups, S::kRows, S::kBuffers, FAST, false>(a, item, smem, line);
+    if (ROLES != kWideOnly && narrow)
+        work<T, D, S::kWaves, 1, 1, S::kRows, S::kBuffers, FAST, true>(a, item, smem, line);
 }
 
-constexpr int kJoin = 256;
+// A workgroup per key head and sequence (narrow), or so many per wide tile.
 template <class T, int D>
-__global__ __launch_bounds__(kJoin) void paged_narrow_join(PagedArgs a)
+__global__ __launch_bounds__(kJoin) void paged_join(PagedArgs a, int narrow_items, int pieces)
 {
     using S = Shape<T, D>;
     __shared__ Line line;
-    const Role<S::kNarrow> role{a.narrow, true};
-    const Shares<S::kNarrow> shares(a, role, line);
-    const int kv = blockIdx.x % a.kv_heads, seq = blockIdx.x / a.kv_heads;
-    const Sequence sq(a, seq);
-    if (role.tiles(a, sq) == 0)
+    int item = blockIdx.x, start;
+    Sequence sq;
+    if (item < narrow_items) {
+        using R = Role<S::kNarrow, S::kRows>;
+        const R role{a.narrow, true};
+        Shares<R> shares(a, role, line);
+        const int kv = item % a.kv_heads;
+        shares.at(item / a.kv_heads, sq, start);
+        if (role.tiles(a, sq) > 0)
+            join_unit<T, D, R, S::kNarrow>(a, role, shares, sq, kv, 0, kv * shares.costs.head + start, 0, 1);
         return;
-    const int at = kv * shares.head + shares.start(seq);
-    join_unit<T, D, S::kNarrow, S::kRows>(a, role, sq, kv, 0, at, at + role.cost(a, sq, 1), shares.each, shares.total, 0, 1);
-}
-template <class T, int D>
-__global__ __launch_bounds__(kJoin) void paged_wide_join(PagedArgs a, int pieces)
-{
-    using S = Shape<T, D>;
-    __shared__ Line line;
-    const Role<S::kWide> role{a.wide, false};
-    const Shares<S::kWide> shares(a, role, line);
-    const int piece = blockIdx.x % pieces, kv = blockIdx.x / pieces % a.kv_heads, at = blockIdx.x / pieces / a.kv_heads;
-    const int group = a.heads / a.kv_heads;
-    auto start = [&](int i) { return (int64_t)row_offset(a.offsets, i, a.rows) * group / S::kWide + i; };
-    const int seq = last_true([&](int i) { return start(i) <= at; }, a.sequences, kWave);
+    }
+    item -= narrow_items;
+    using R = Role<S::kWide, S::kRows>;
+    const R role{a.wide, false};
+    const int piece = item % pieces, kv = item / pieces % a.kv_heads, at = item / pieces / a.kv_heads;
+    const int seq = __builtin_amdgcn_readfirstlane(
+        last_true([&](int i) { return tile_number<S::kWide>(a, i) <= at; }, a.sequences, kWave));
     if (seq < 0)
         return;
-    const Sequence sq(a, seq);
-    const int tile = (int)(at - start(seq));
-    if (tile >= role.tiles(a, sq))
+    const int tile = at - tile_number<S::kWide>(a, seq);
+    if (tile >= role.tiles(a, Sequence(a, seq)))
         return;
-    const int from = kv * shares.head + shares.start(seq);
-    join_unit<T, D, S::kWide, S::kRows>(a, role, sq, kv, tile, from + role.cost(a, sq, tile), from + role.cost(a, sq, tile + 1),
-                                        shares.each, shares.total, piece,
-                                        pieces);
+    Shares<R> shares(a, role, line);
+    shares.at(seq, sq, start);
+    join_unit<T, D, R, S::kWide>(a, role, shares, sq, kv, tile, kv * shares.costs.head + start + role.cost(a, sq, tile), piece, pieces);
 }
 
 template <int D, bool FAST>
 hipError_t run(const PagedArgs &a, hipStream_t s)
 {
     using S = Shape<Type, D>;
-    const dim3 block(S::kWaves * kWave);
-    if (a.wide.groups > 0) {
-        hipError_t e = launch_kernel(paged_wide_kernel<Type, D, FAST>, dim3((unsigned)a.wide.groups), block, S::kLds + sizeof(Line), s, a);
-        if (e == hipSuccess && a.wide.part) {
-            constexpr int pieces = S::kWide * (D / 2) / kJoin;
-            e = launch_kernel(paged_wide_join<Type, D>, dim3((unsigned)((int64_t)a.wide.tiles * a.kv_heads * pieces)), dim3(kJoin), 0,
-                              s, a, pieces);
-        }
-        if (e != hipSuccess)
-            return e;
-    }
-    if (a.narrow.groups == 0)
-        return hipSuccess;
-    const hipError_t e = launch_kernel(paged_narrow_kernel<Type, D, FAST>, dim3((unsigned)a.narrow.groups), block, S::kLds + sizeof(Line), s, a);
-    if (e != hipSuccess || !a.narrow.part)
+    const auto kernel = a.wide.groups == 0     ? paged_kernel<Type, D, FAST, kNarrowOnly>
+                        : a.narrow.groups == 0 ? paged_kernel<Type, D, FAST, kWideOnly>
+                                               : paged_kernel<Type, D, FAST, kBoth>;
+    const hipError_t e = launch_kernel(kernel, dim3((unsigned)(a.narrow.groups + a.wide.groups)), dim3(S::kWaves * kWave),
+                                       S::kLds + sizeof(Line), s, a);
+    if (e != hipSuccess || (!a.narrow.part && !a.wide.part))
         return e;
-    return launch_kernel(paged_narrow_join<Type, D>, dim3((unsigned)((int64_t)a.sequences * a.kv_heads)), dim3(kJoin), 0, s, a);
+    // a join's thread takes four columns of four results of a wide tile
+    constexpr int all = S::kWide * (D / 2) / (4 * kJoin), pieces = all > 0 ? all : 1;
+    const int narrow_items = a.narrow.part ? a.sequences * a.kv_heads : 0;
+    const int64_t wide_items = a.wide.part ? (int64_t)a.wide.tiles * a.kv_heads * pieces : 0;
+    return launch_kernel(paged_join<Type, D>, dim3((unsigned)(narrow_items + wide_items)), dim3(kJoin), 0, s, a, narrow_items, pieces);
 }
 template <int D>
 hipError_t by_pages(const PagedArgs &a, hipStream_t s)

@@ -209,7 +209,7 @@ static int page_sizes()
         r.cache.page_rows = n, r.cache.table_width = 0;
         if (mtpx_diff_attention_paged(&ctx, &r))
             return 1;
-        std::printf("%d %u %d\n", n, seen.page_magic, seen.page_shift);
+        std::printf("%d %u %d\n", n, seen.page.magic, seen.page.shift);
     }
     return 0;
 }
@@ -223,8 +223,8 @@ static int plan(char **v)
     const mtpx::PagedPlan p = mtpx::paged_plan(&ctx, r);
     size_t bytes = 0;
     const int code = mtpx_diff_attention_paged_workspace(&ctx, &r, &bytes);
-    std::printf("%d %d %d %d %d %d %d %zu\n", code, p.deep, p.deep_blocks, p.deep_splits, p.broad_columns, p.broad_tiles,
-                p.broad_splits, bytes);
+    std::printf("%d %d %d %d %d %d %d %d %zu\n", code, p.narrow_columns, p.narrow.groups, p.narrow.each_unit, p.wide.groups,
+                p.wide.each_unit, p.wide.tiles, ctx.num_cus, bytes);
     return 0;
 }
 
