@@ -120,6 +120,19 @@ struct Divisor {
     int shift;
 };
 
+// What the first t tiles of a sequence's columns cost, in steps of `step` keys:
+// `start` and no less than its steps each.  Where the new rows are a small part,
+// every tile as much as the last.  Else tile t sees `before` + (t + 1) columns /
+// heads keys, rounded up; the sum's rounding may leave a step off and the keys'
+// two more, so four are added.
+__host__ __device__ inline int tile_costs(bool causal, int length, int rows, int shift, int heads, int columns, int step, int start, int t)
+{
+    if (!causal || rows <= length / 8)
+        return t * (start + (length + step - 1) / step);
+    const int before = (shift < 0 ? 0 : shift < length ? shift : length) / step + 4;
+    return t * (start + before) + (int)((int64_t)t * (t + 1) / 2 * columns / (heads * step));
+}
+
 // How the tiles of one width are given to workgroups.
 struct RoleArgs {
     int groups;     // workgroups (0: none)

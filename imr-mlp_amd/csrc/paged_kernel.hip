@@ -95,16 +95,9 @@ struct Role {
     {
         return (sq.keys(a, min((t + 1) * COLS, sq.rows * a.heads_each) - 1) + KB - 1) / KB;
     }
-    // What the first t tiles of a sequence cost: kStart and no less than its steps
-    // each.  Where the new rows are a small part, every tile as much as the last.
-    // Else tile t has before + (t + 1) COLS / g keys, rounded up, whose sum's
-    // rounding may leave a step off and the keys' two more: four are added.
     __device__ inline int cost(const PagedArgs &a, const Sequence &sq, int t) const
     {
-        if (!a.causal || sq.rows <= sq.length / 8)
-            return t * (kStart + (sq.length + KB - 1) / KB);
-        const int before = max(0, min(sq.shift, sq.length)) / KB + 4;
-        return t * (kStart + before) + (int)((int64_t)t * (t + 1) / 2 * COLS / (a.heads_each * KB));
+        return tile_costs(a.causal, sq.length, sq.rows, sq.shift, a.heads_each, COLS, KB, kStart, t);
     }
 };
 

@@ -190,13 +190,15 @@ def _tensor(ctx, t, name, shape=None, dtype=None):
 def _strides(ctx, t, name, shape, dtype):
     """Strides of a tensor of this shape and type on the context's device whose
     last dimension is contiguous."""
-    if (not isinstance(t, torch.Tensor) or t.get_device() != ctx.device or t.dtype is not dtype or
-            t.shape != shape):
-        _tensor(ctx, t, name, shape, dtype)  # says which
-    s = t.stride()
-    if s[-1] != 1 and t.shape[-1] > 1:
-        _fail("the last dimension of %s is not contiguous" % name)
-    return s
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == ctx.device:
+            s = t.stride()
+            if s[-1] == 1 or shape[-1] <= 1:
+                return s
+    except AttributeError:
+        pass
+    _tensor(ctx, t, name, shape, dtype)  # says which
+    _fail("the last dimension of %s is not contiguous" % name)
 
 
 def _typed(ctx, t, name, dims):
@@ -531,44 +533,53 @@ def norm_block_backward(ctx, ds, dn, x, y, gate, post_weight, pre_weight, stats,
 def _turns(ctx, positions, freq, axis, rows):
     """The checked fields of a rotation, as a request has them, and how many
     elements of a head it turns."""
-    sp = _tensor(ctx, positions, "positions", (rows, None)).stride()
+    shape = _tensor(ctx, positions, "positions", (rows, None)).shape
+    sp = positions.stride()
     ptype = POSITION_DTYPES.get(positions.dtype)
     if ptype is None:
         _fail("positions are %s, not float32, float64, int32 or int64" % positions.dtype)
-    pairs = (freq.numel(),) if isinstance(freq, torch.Tensor) else (None,)
+    pairs = (freq.numel(),) if isinstance(freq, torch.Tensor) else (0,)
     _strides(ctx, freq, "freq", pairs, torch.float32)
     _strides(ctx, axis, "axis", pairs, torch.int32)
-    return 2 * pairs[0], (positions.data_ptr(), ptype, sp[0], sp[1], positions.shape[1],
+    return 2 * pairs[0], (positions.data_ptr(), ptype, sp[0], sp[1], shape[1],
                           freq.data_ptr(), axis.data_ptr())
 
 
 def _head_rows(ctx, t, name, shape, of):
     """Heads [rows, heads, dim] or [rows, heads, maps, dim] as a request has them."""
     s = _strides(ctx, t, name, shape, of)
-    return t.data_ptr(), s[0], s[1], s[2] if len(shape) == 4 else 0
+    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), s[0], s[1], 0)
 
 
-def _whole(t, shape):
+def _like(t):
+    """An unwritten contiguous tensor of the same shape."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _whole(t, heads, maps, dim):
     """The same of a contiguous result."""
-    d = shape[-1]
-    return t.data_ptr(), t.numel() // max(1, len(t)), d * (shape[2] if len(shape) == 4 else 1), d
+    return t.data_ptr(), heads * maps * dim, maps * dim, dim
 
 
 def _heads_of(ctx, q, k):
-    """Checks what q and k share: the type's code, rows, heads, kv heads, maps and dim."""
+    """Checks what q and k share: the type's code, rows, heads, kv heads, maps and
+    dim, and k's shape."""
     dims = 4 if isinstance(q, torch.Tensor) and q.dim() == 4 else 3
     dtype, shape = _typed(ctx, q, "q", dims), q.shape
-    if dims == 4 and shape[2] not in (1, 2):
-        _fail("q has %d maps, not 1 or 2" % shape[2])
-    kv = 0
-    if k is not None:
-        if not isinstance(k, torch.Tensor) or k.dim() != dims:
-            _fail("k has not as many dimensions as q")
-        kv = k.shape[1]
-        _tensor(ctx, k, "k", (shape[0], kv, *shape[2:]), q.dtype)
-        if kv == 0:
-            _fail("k has no heads")
-    return dtype, shape[0], shape[1], kv, shape[2] if dims == 4 else 1, shape[-1]
+    if dims == 4:
+        rows, heads, maps, dim = shape
+        if maps not in (1, 2):
+            _fail("q has %d maps, not 1 or 2" % maps)
+    else:
+        (rows, heads, dim), maps = shape, 1
+    if k is None:
+        return dtype, rows, heads, 0, maps, dim, None
+    if not isinstance(k, torch.Tensor) or k.dim() != dims:
+        _fail("k has not as many dimensions as q")
+    kv = k.shape[1]
+    if kv == 0:
+        _fail("k has no heads")
+    return dtype, rows, heads, kv, maps, dim, (rows, kv, maps, dim) if dims == 4 else (rows, kv, dim)
 
 
 def _weight(ctx, w, name, dim, of):
@@ -585,19 +596,19 @@ def head_norm_rotary(ctx, q, k, q_weight, k_weight, positions, freq, axis, *, ki
     None: q only) every head and map becomes norm(x) weight, turned as by
     rotary; weights [dim] or None, positions, freq and axis as there.  Returns
     (q, k)."""
-    dtype, rows, heads, kv, maps, dim = _heads_of(ctx, q, k)
-    of = q.dtype
+    dtype, rows, heads, kv, maps, dim, k_shape = _heads_of(ctx, q, k)
+    shape, of = q.shape, q.dtype
     if kind not in NORMS:
         _fail("kind is one of %s" % (tuple(NORMS),))
     rotated, turn = _turns(ctx, positions, freq, axis, rows)
-    qo = q.new_empty(q.shape)
+    q_in, qo = _head_rows(ctx, q, "q", shape, of), _like(q)
     ko, k_in, k_out = None, _NO_ROWS, _NO_ROWS
     if k is not None:
-        ko = k.new_empty(k.shape)
-        k_in, k_out = _head_rows(ctx, k, "k", k.shape, of), _whole(ko, k.shape)
+        k_in, ko = _head_rows(ctx, k, "k", k_shape, of), _like(k)
+        k_out = _whole(ko, kv, maps, dim)
     req = _pack_heads(
         _stream(ctx), dtype, rows, heads, kv, maps, dim, rotated, NORMS[kind], interleaved, eps,
-        *_head_rows(ctx, q, "q", q.shape, of), *k_in, *_whole(qo, q.shape), *k_out,
+        *q_in, *k_in, *_whole(qo, heads, maps, dim), *k_out,
         _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of),
         *turn, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, 0)
     ctx._check(_ops().mtpx_head_norm_rotary(ctx.h, req), "head_norm_rotary")
@@ -610,30 +621,30 @@ def head_norm_rotary_backward(ctx, dq, dk, q, k, q_weight, k_weight, positions, 
     results and the forward pass's inputs; None in the place of an input that
     was not given, and of the positions' without dpositions (which needs
     float32 or float64 ones; a 32-bit sum for both)."""
-    dtype, rows, heads, kv, maps, dim = _heads_of(ctx, q, k)
-    of = q.dtype
+    dtype, rows, heads, kv, maps, dim, k_shape = _heads_of(ctx, q, k)
+    shape, of = q.shape, q.dtype
     if kind not in NORMS:
         _fail("kind is one of %s" % (tuple(NORMS),))
     rotated, turn = _turns(ctx, positions, freq, axis, rows)
     if (dk is None) != (k is None):
         _fail("dk is given with k")
-    gq, gk, dpos = q.new_empty(q.shape), None, None
+    gq, gk, dpos = _like(q), None, None
     k_in, k_grad, k_out = _NO_ROWS, _NO_ROWS, _NO_ROWS
     if k is not None:
-        gk = k.new_empty(k.shape)
-        k_in, k_grad = _head_rows(ctx, k, "k", k.shape, of), _head_rows(ctx, dk, "dk", k.shape, of)
-        k_out = _whole(gk, k.shape)
+        gk = _like(k)
+        k_in, k_grad = _head_rows(ctx, k, "k", k_shape, of), _head_rows(ctx, dk, "dk", k_shape, of)
+        k_out = _whole(gk, kv, maps, dim)
     wq, wk = _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of)
     dwq = None if q_weight is None else q.new_empty(dim)
     dwk = None if k_weight is None else q.new_zeros(dim) if k is None else q.new_empty(dim)
     if dpositions:
         dpos = torch.empty(positions.shape, dtype=positions.dtype, device=q.device)
     size = _bytes(ctx, _ops().mtpx_head_norm_rotary_workspace, HeadNormRequest, rows=rows, dim=dim)
-    w = _workspace(ctx, size)  # held until the kernels are queued
+    w = q.new_empty(size, dtype=torch.uint8)  # held until the kernels are queued
     req = _pack_heads(
         _stream(ctx), dtype, rows, heads, kv, maps, dim, rotated, NORMS[kind], interleaved, eps,
-        *_head_rows(ctx, q, "q", q.shape, of), *k_in, *_NO_ROWS, *_NO_ROWS, wq, wk, *turn,
-        *_head_rows(ctx, dq, "dq", q.shape, of), *k_grad, *_whole(gq, q.shape), *k_out,
+        *_head_rows(ctx, q, "q", shape, of), *k_in, *_NO_ROWS, *_NO_ROWS, wq, wk, *turn,
+        *_head_rows(ctx, dq, "dq", shape, of), *k_grad, *_whole(gq, heads, maps, dim), *k_out,
         _ptr(dwq), _ptr(dwk), _ptr(dpos), w.data_ptr(), size)
     ctx._check(_ops().mtpx_head_norm_rotary_backward(ctx.h, req), "head_norm_rotary_backward")
     return gq, gk, dwq, dwk, dpos
@@ -646,12 +657,12 @@ def _pages(ctx, k_pages, v_pages, table, offsets, lengths, kv, dim, of):
     """The checked fields of a cache and its batch: (mtpx_pages, offsets, lengths, sequences)."""
     if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 5:
         _fail("k_pages is not [pages, page rows, kv heads, 2, dim]")
-    n, page = k_pages.shape[:2]
+    n, page, *_ = k_pages.shape
     sk = _strides(ctx, k_pages, "k_pages", (n, page, kv, 2, dim), of)
     sv = _strides(ctx, v_pages, "v_pages", (n, page, kv, 2 * dim), of)
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         _fail("lengths are not [sequences]")
-    seqs = len(lengths)
+    seqs = lengths.shape[0]
     _strides(ctx, lengths, "lengths", (seqs,), torch.int32)
     _strides(ctx, offsets, "offsets", (seqs + 1,), torch.int32)
     if not isinstance(table, torch.Tensor) or table.dim() != 2:
@@ -694,8 +705,8 @@ def append_paged(ctx, k, v, k_pages, v_pages, table, offsets, lengths, positions
         shape = (rows, heads, 2, dim)
         q_in = _head_rows(ctx, q, "q", shape, of)
         if out is None:
-            out = q.new_empty(shape)
-            q_out = _whole(out, shape)
+            out = _like(q)
+            q_out = _whole(out, heads, 2, dim)
         else:
             q_out = _head_rows(ctx, out, "out", shape, of)
     elif out is not None:
@@ -742,10 +753,14 @@ def diff_attention_paged(ctx, q, k_pages, v_pages, lam, table, offsets, lengths,
         out, so = q.new_empty(shape), (heads * 2 * dim, 2 * dim)
     else:
         so = _strides(ctx, out, "out", shape, of)
-    size = _bytes(ctx, _ops().mtpx_diff_attention_paged_workspace, _paged_sizes, dtype=dtype,
-                  rows=rows, sequences=seqs, max_rows=max_rows, heads=heads, kv_heads=kv, dim=dim,
-                  page=cache[11], width=cache[14])
-    w = _workspace(ctx, size) if size else None  # held until the kernels are queued
+    key = (PagedRequest, dtype, rows, seqs, max_rows, heads, kv, dim, cache[11], cache[14])
+    size = ctx.workspaces.get(key)
+    if size is None:
+        size = _bytes(ctx, _ops().mtpx_diff_attention_paged_workspace, _paged_sizes, dtype=dtype,
+                      rows=rows, sequences=seqs, max_rows=max_rows, heads=heads, kv_heads=kv,
+                      dim=dim, page=cache[11], width=cache[14])
+        ctx.workspaces[key] = size
+    w = q.new_empty(size, dtype=torch.uint8) if size else None  # held until the kernels are queued
     req = _pack_paged(
         _stream(ctx), dtype, rows, seqs, max_rows, heads, kv, dim, causal,
         dim ** -0.5 if scale is None else scale, q.data_ptr(), sq[0], sq[1], sq[2], *cache, off,

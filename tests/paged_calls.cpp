@@ -8,6 +8,8 @@
 //   paged_calls refuse   one line per refused request: its name, its code, and
 //                        whether anything was queued
 //   paged_calls pages    page_rows, magic and shift of every page size up to 4100
+//   paged_calls costs n  n sequences and tiles at random: how many tiles were looked
+//                        at, and how many cost less than they take
 //   paged_calls plan rows sequences max_rows heads kv_heads dim dtype page width
 //                        how a call's work is split, and its workspace
 #include "../imr-mlp_amd/csrc/paged_api.cpp"
@@ -214,6 +216,39 @@ static int page_sizes()
     return 0;
 }
 
+static int costs(int n)
+{
+    unsigned long long state = 88172645463325252ull;
+    auto random = [&](int most) {  // 1 to most, spread over its logarithm
+        state ^= state << 13, state ^= state >> 7, state ^= state << 17;
+        int bits = 1;
+        while (bits < 30 && (1 << bits) < most)
+            ++bits;
+        const int top = 1 << (state >> 40) % (bits + 1), v = 1 + (int)((state >> 8) % (unsigned)top);
+        return v < most ? v : most;
+    };
+    long looked = 0, wrong = 0;
+    const int shapes[][2] = {{32, 64}, {32, 32}, {128, 64}, {64, 32}, {64, 64}};
+    for (int i = 0; i < n; ++i) {
+        const int *s = shapes[i % 5], heads = random(80), rows = random(100000 / heads + 1), given = random(200000) - 1;
+        const int room = i % 3 ? given : random(200000), length = given < room ? given : room, shift = given - rows, start = 128 / s[1];
+        const int columns = rows * heads, tiles = (columns + s[0] - 1) / s[0], first = random(tiles) - 1;
+        for (int t = first; t < tiles && t < first + 50; ++t) {
+            const int last = ((t + 1) * s[0] < columns ? (t + 1) * s[0] : columns) - 1;
+            int keys = shift + last / heads + 1;
+            keys = keys < 0 ? 0 : keys < length ? keys : length;
+            for (bool causal : {false, true}) {
+                const int steps = ((causal ? keys : length) + s[1] - 1) / s[1];
+                auto cost = [&](int at) { return mtpx::tile_costs(causal, length, rows, shift, heads, s[0], s[1], start, at); };
+                wrong += cost(t + 1) - cost(t) < start + steps;
+                ++looked;
+            }
+        }
+    }
+    std::printf("%ld %ld\n", looked, wrong);
+    return 0;
+}
+
 static int plan(char **v)
 {
     mtpx_diff_attention_paged_request r{};
@@ -224,7 +259,7 @@ static int plan(char **v)
     size_t bytes = 0;
     const int code = mtpx_diff_attention_paged_workspace(&ctx, &r, &bytes);
     std::printf("%d %d %d %d %d %d %d %d %zu\n", code, p.narrow_columns, p.narrow.groups, p.narrow.each_unit, p.wide.groups,
-                p.wide.each_unit, p.wide.tiles, ctx.num_cus, bytes);
+                p.wide.each_unit, p.wide.tiles, p.wide.quarters, bytes);
     return 0;
 }
 
@@ -236,6 +271,8 @@ int main(int argc, char **argv)
         return refusals();
     if (argc > 1 && !std::strcmp(argv[1], "pages"))
         return page_sizes();
+    if (argc > 2 && !std::strcmp(argv[1], "costs"))
+        return costs(std::atoi(argv[2]));
     if (argc > 10 && !std::strcmp(argv[1], "plan"))
         return plan(argv + 2);
     return 2;

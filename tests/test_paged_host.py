@@ -103,27 +103,43 @@ def test_a_keys_page_by_multiplication(calls):
             assert ((2 * k * magic) >> 32) >> shift == k // n, (n, k)
 
 
-@pytest.mark.parametrize("seed", range(40))
+def test_a_tile_costs_what_it_takes(calls):
+    """Workgroups share keys by costs: a tile whose cost were below its steps would lose the last of them."""
+    looked, wrong = (int(v) for v in calls("costs", 200000)[0])
+    assert looked > 1000000 and wrong == 0
+
+
+@pytest.mark.parametrize("seed", range(60))
 def test_plans_cover_the_work(calls, seed):
-    """Every sequence's columns lie in the deep part's blocks or in a broad tile,
-    a tile's number names one place, and the workspace holds all partial results."""
+    """Every sequence's columns lie in a narrow tile or in wide ones, a tile's
+    number names one place, and the workspace holds all partial results."""
     rng = random.Random(seed)
-    n, kv = rng.choice([1, 3, 64, 500]), rng.choice([1, 2, 8])
+    n, kv = rng.choice([1, 3, 64, 500, 5000]), rng.choice([1, 2, 8])
     group, dim, dtype = rng.choice([1, 3, 4, 17, 33, 64]), rng.choice([16, 64, 128]), rng.choice([0, 1])
-    new = [rng.choice([0, 1, 1, 2, 40, 700]) if rng.random() < 0.5 else 1 for _ in range(n)]
-    rows, first = sum(new) + 5, 2
+    new = [rng.choice([0, 1, 1, 2, 40, 700]) if rng.random() < 0.5 and n < 5000 else 1 for _ in range(n)]
+    first = 2
+    rows = sum(new) + 5
     most = rng.choice([0, max(1, max(new))])
     page, width = rng.choice([16, 100]), rng.choice([3, 300])
-    code, deep, blocks, splits, columns, tiles, broad_splits, size = (int(v) for v in calls("plan", rows, n, most, group * kv, kv, dim, dtype, page, width)[0])
+    out = calls("plan", rows, n, most, group * kv, kv, dim, dtype, page, width)[0]
+    code, limit, narrow, narrow_each, wide, wide_each, tiles, quarters, size = (int(v) for v in out)
+    if rows * group * kv > (2 ** 32 - 1) // 512:
+        return
     assert code == 0
-    at, place, off = first, {}, [first]
+    # columns of the tiles, as the kernels have them
+    columns = {(0, 16): 64, (0, 64): 64, (0, 128): 32, (1, 16): 128, (1, 64): 128, (1, 128): 64}[dtype, dim]
+    at, off = first, [first]
     for m in new:
         at += m
         off.append(at)
+    place = {}
     for i, m in enumerate(new):
-        if m * group <= deep:
-            assert blocks * 16 >= m * group
+        if m == 0:
             continue
+        if m * group <= limit:
+            assert narrow > 0 and m * group <= 32 and (not narrow_each or narrow == n * kv)
+            continue
+        assert wide > 0
         start = off[i] * group // columns + i
         for t in range(-(-m * group // columns)):
             assert start + t < tiles and start + t not in place
@@ -132,13 +148,11 @@ def test_plans_cover_the_work(calls, seed):
     starts = [off[i] * group // columns + i for i in range(n)]
     for t, i in place.items():
         assert max(j for j in range(n) if starts[j] <= t) == i
-    wide = 32 if dim <= 32 else 64 if dim <= 64 else 128
-    part = 2 * 4 * (4 + 2 * wide)
-    want = 0
-    if deep and splits > 1:
-        want += n * kv * blocks * 16 * splits * part
-    if broad_splits > 1:
-        want += rows * group * kv * broad_splits * part
+    if wide and wide_each:
+        assert wide == (tiles + quarters) * kv
+    wide_part = 2 * 4 * (4 + 2 * (32 if dim <= 32 else 64 if dim <= 64 else 128))
+    want = 0 if narrow_each or narrow < 2 else narrow * 2 * 32 * wide_part
+    want += 0 if wide_each or wide < 2 else wide * 2 * columns * wide_part
     assert size == want
 
 
