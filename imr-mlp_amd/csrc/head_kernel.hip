@@ -47,6 +47,14 @@ struct alignas(sizeof(T) * A) Piece {
     T e[N];
 };
 
+// 1 / sqrt(v), a unit in the last place off; the instruction takes numbers below
+// the smallest normal one for 0.
+__device__ inline float inverse_root(float v)
+{
+    const bool small = v < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v) * (small ? 0x1p32f : 1.f);
+}
+
 // A vector's elements over the lanes of its group: U units each.  A unit is W
 // elements of both halves of the pairs, or the pairs of W elements side by side
 // (one pair where W is 1); units beyond the turning ones are W elements that
@@ -208,7 +216,7 @@ struct Layout {
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 q = fmaf(v[i][e], v[i][e], q);
-        const float inv = 1.f / sqrtf(fmaf(sum(q), scale, a.eps));
+        const float inv = inverse_root(fmaf(sum(q), scale, a.eps));
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void head_forward_kernel(HeadArgs a)
 // rotation leaves as it is.  u is formed again from x.  A row's lanes lie in one
 // wave; a workgroup takes rows part, part + groups, ... and keeps its share of
 // the weights' gradients in registers until the end: a.parts partial rows.
-template <class T, int W, bool APART, int U>
+template <class T, int W, bool APART, int U, bool MOVED>
 __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
 {
     using L = Layout<T, W, APART, U>;
@@ -392,18 +400,19 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
             T *dx = (T *)to.data + row * to.row;
             float w[U][L::E];
             at.weights(a.weight[job], w);
-            typename L::Raw next, next_dy;
-            at.load(x + (first >> bits) * fx.head + (first & bits) * fx.map, next);
-            at.load(dy + (first >> bits) * fy.head + (first & bits) * fy.map, next_dy);
+            auto read = [&](int v, typename L::Raw &rx, typename L::Raw &ry) {
+                if (v < n) {
+                    at.load(x + (v >> bits) * fx.head + (v & bits) * fx.map, rx);
+                    at.load(dy + (v >> bits) * fy.head + (v & bits) * fy.map, ry);
+                }
+            };
+            typename L::Raw rx, ry;
+            read(first, rx, ry);
             for (int v = first; v < n; v += step) {
                 float u[U][L::E], g[U][L::E];
-                at.widen(next, u);
-                at.widen(next_dy, g);
-                const int ahead = v + step;
-                if (ahead < n) {
-                    at.load(x + (ahead >> bits) * fx.head + (ahead & bits) * fx.map, next);
-                    at.load(dy + (ahead >> bits) * fy.head + (ahead & bits) * fy.map, next_dy);
-                }
+                at.widen(rx, u);
+                at.widen(ry, g);
+                read(v + step, rx, ry);
                 const float inv = at.normalise(a, u);
                 float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -414,30 +423,36 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
                         const float d1 = g[i][k], d2 = g[i][l];
                         g[i][k] = d1 * c[i][j] + d2 * s[i][j];
                         g[i][l] = d2 * c[i][j] - d1 * s[i][j];
-                        if (a.dpositions)
+                        if constexpr (MOVED)
                             d[i][j] += g[i][l] * (u[i][k] * w[i][k]) - g[i][k] * (u[i][l] * w[i][l]);
                     }
 #pragma unroll
                     for (int e = 0; e < L::E; ++e) {
                         dw[job][i][e] = fmaf(g[i][e], u[i][e], dw[job][i][e]);
                         g[i][e] *= w[i][e];
-                        s0 += g[i][e];
                         s1 = fmaf(g[i][e], u[i][e], s1);
                     }
                 }
-                s0 = a.kind == MTPX_NORM_LAYER ? at.sum(s0) * scale : 0.f;
-                s1 = at.sum(s1) * scale;
+                if (a.kind == MTPX_NORM_LAYER) {
+#pragma unroll
+                    for (int i = 0; i < U; ++i)
+#pragma unroll
+                        for (int e = 0; e < L::E; ++e)
+                            s0 += g[i][e];
+                    s0 = at.sum(s0) * scale * inv;
+                }
+                s1 = at.sum(s1) * scale * inv;
 #pragma unroll
                 for (int i = 0; i < U; ++i)
 #pragma unroll
                     for (int e = 0; e < L::E; ++e)
-                        g[i][e] = inv * (g[i][e] - s0 - u[i][e] * s1);
+                        g[i][e] = fmaf(-u[i][e], s1, fmaf(g[i][e], inv, -s0));
                 typename L::Raw r;
                 at.round(g, r);
                 at.store(dx + (v >> bits) * to.head + (v & bits) * to.map, r);
             }
         }
-        if (a.dpositions) {
+        if constexpr (MOVED) {
             float sums[kMaxAxes] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < U; ++i)
@@ -523,9 +538,10 @@ hipError_t launch(const HeadArgs &a, Pass pass, hipStream_t s)
 {
     const int rows = kThreads / a.lanes;
     const dim3 grid((unsigned)(pass == kBackward ? a.parts : (a.rows + rows - 1) / rows)), block(kThreads);
-    const auto kernel = pass == kForward  ? head_forward_kernel<Type, W, APART, U, false>
-                        : pass == kAppend ? head_forward_kernel<Type, W, APART, U, true>
-                                          : head_backward_kernel<Type, W, APART, U>;
+    const auto kernel = pass == kForward   ? head_forward_kernel<Type, W, APART, U, false>
+                        : pass == kAppend  ? head_forward_kernel<Type, W, APART, U, true>
+                        : a.dpositions     ? head_backward_kernel<Type, W, APART, U, true>
+                                           : head_backward_kernel<Type, W, APART, U, false>;
     return launch_kernel(kernel, grid, block, 0, s, a);
 }
 template <int W, int U>

@@ -99,7 +99,7 @@ HeadArgs head_args(const R &r, int maps)
 // The widest access that every piece of a vector allows, and the lanes of a
 // vector and of a row.  `wide`: the tensors' addresses and strides.
 template <class Fits>
-void shape_heads(HeadArgs &a, int64_t size, int most_lanes, const Fits &fits)
+void shape_heads(HeadArgs &a, int64_t size, int most_lanes, int64_t threads, const Fits &fits)
 {
     const int half = a.rotated / 2;
     a.width = (int)(16 / size);
@@ -113,7 +113,7 @@ void shape_heads(HeadArgs &a, int64_t size, int most_lanes, const Fits &fits)
         a.group *= 2;
     const int64_t vectors = std::max(a.vectors[0], a.vectors[1]);
     a.lanes = a.group;
-    while (a.lanes < most_lanes && a.lanes < vectors * a.group)
+    while (a.lanes < most_lanes && a.lanes < vectors * a.group && a.rows * a.lanes < threads)
         a.lanes *= 2;
 }
 bool fits_rows(const mtpx_rows &t, int width, int64_t size, int maps)
@@ -122,9 +122,13 @@ bool fits_rows(const mtpx_rows &t, int width, int64_t size, int maps)
                        (maps == 1 || t.map % width == 0));
 }
 
-// Few rows: a whole workgroup each, which takes the fewest steps one after the
-// other; a wave otherwise.
+// Lanes of a row: a whole workgroup where there are few rows, as that takes the
+// fewest steps one after the other; else up to a wave, as few as leave the device
+// full, since a row's cos and sin are formed by as many lanes and its vectors read
+// ahead (160,000 rows of 16 and 16 vectors of 64 in 16 bits: forward 303 us with 64
+// lanes, 230 us with 16; backward 695 us with 64, 422 us with 8).
 int row_lanes(mtpx_context *ctx, int64_t rows) { return rows <= 8 * (int64_t)ctx->num_cus ? 256 : 64; }
+constexpr int64_t kForwardThreads = int64_t(1) << 21, kBackwardThreads = int64_t(1) << 20;
 
 // Workgroups of the backward pass.
 int head_parts(mtpx_context *ctx, const HeadArgs &a)
@@ -178,7 +182,7 @@ int head_request(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r, bool
             MTPX_TRY(check_rows(ctx, a.grad[i], r.dtype, names[i][2]));
         MTPX_TRY(check_place(ctx, back ? a.grad[i] : a.in[i], a.out[i], r.maps, names[i][back ? 3 : 1]));
     }
-    shape_heads(a, size, back ? 64 : row_lanes(ctx, r.rows), [&](int width) {
+    shape_heads(a, size, back ? 64 : row_lanes(ctx, r.rows), back ? kBackwardThreads : kForwardThreads, [&](int width) {
         for (int i = 0; i < 2; ++i)
             if (a.vectors[i] && !(fits_rows(a.in[i], width, size, r.maps) && fits_rows(a.out[i], width, size, r.maps) &&
                                   fits_rows(a.grad[i], width, size, r.maps)))
@@ -375,7 +379,7 @@ int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *req)
             a.out[0] = r.q_out;
         }
         const int64_t size = (int64_t)dtype_bytes(r.dtype);
-        shape_heads(a, size, row_lanes(ctx, r.rows), [&](int width) {
+        shape_heads(a, size, row_lanes(ctx, r.rows), kForwardThreads, [&](int width) {
             return fits_rows(a.in[1], width, size, 2) && fits_rows(a.v, width, size, 2) && pages_fit(r.cache, width, size) &&
                    (r.heads == 0 || (fits_rows(a.in[0], width, size, 2) && fits_rows(a.out[0], width, size, 2)));
         });
