@@ -11,7 +11,9 @@ results come from torch's allocator, so a call can be captured into a graph.
 Functions with gradients come twice: as a pair (f, f_backward) on plain
 tensors, and as an autograd function (RotaryFn, DiffAttentionFn, NormBlockFn, HeadNormRotaryFn).
 Gradients are first derivatives: differentiating one of them again (a loss of
-forces that were taken through a block) raises.
+forces that were taken through a block) raises.  A backward pass can be recorded
+into a graph if no graph of the same leaves that was made on another stream lives
+any more, and raises otherwise.
 Tensors are float32, bfloat16 or float16; their last dimension has to be
 contiguous, other strides are free.  There is no fallback: a missing library
 or a refused argument raises.  torch and the library share one HIP runtime if
@@ -795,6 +797,33 @@ def _learned(**values):
     return [n for n, t in values.items() if isinstance(t, torch.Tensor) and t.requires_grad]
 
 
+_STREAM = "mtpx.ops: stream"
+
+
+def _mark_leaves(fn):
+    """Notes, in a forward pass, on which stream the graph's ends at its leaves
+    have come to be: autograd hands gradients over on that stream."""
+    for node, _ in fn.next_functions:
+        if type(node) is _Leaf and node.variable.is_cuda:
+            node.metadata.setdefault(_STREAM, _stream(fn.ctx))
+
+
+def _same_streams(fn):
+    """Refuses a backward pass that is being recorded into a graph while another
+    graph of the same leaves, made on another stream (an eager one, as a rule),
+    lives: autograd would hand the gradients over on that stream, which the
+    recording does not hold, and ending it would end the process."""
+    marks = [node.metadata.get(_STREAM) for node, _ in fn.next_functions if type(node) is _Leaf]
+    if any(m is not None for m in marks) and torch.cuda.is_current_stream_capturing():
+        now = _stream(fn.ctx)
+        if any(m not in (None, now) for m in marks):
+            _fail("a backward pass recorded while an earlier graph of the same leaves lives: "
+                  "drop what still refers to that one first")
+
+
+_Leaf = type(torch.zeros(1, requires_grad=True).expand(1).grad_fn.next_functions[0][0])
+
+
 def _first_only(backward):
     """The kernels' gradients carry no graph.  Where autograd keeps one
     (create_graph), it would take them for constants, and a loss of them, as of
@@ -805,6 +834,7 @@ def _first_only(backward):
     def once(fn, *grads):
         if fn.learned:
             _fail("%s requires a gradient and has none" % " and ".join(fn.learned))
+        _same_streams(fn)
         with torch.no_grad():
             out = backward(fn, *grads)
         if not torch.is_grad_enabled():
@@ -826,6 +856,7 @@ class RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(fn, ctx, x, positions, freq, axis, interleaved=False):
         fn.ctx, fn.interleaved, fn.learned = ctx, interleaved, _learned(freq=freq)
+        _mark_leaves(fn)
         keep = x if positions.requires_grad else None
         fn.save_for_backward(keep, positions, freq, axis)
         return rotary(ctx, x, positions, freq, axis, interleaved=interleaved)
@@ -849,6 +880,7 @@ class DiffAttentionFn(torch.autograd.Function):
                                     key_mask=key_mask, save=True)
         fn.ctx, fn.seqs, fn.causal, fn.scale = ctx, seqs, causal, scale
         fn.learned = _learned(scale=scale)
+        _mark_leaves(fn)
         fn.save_for_backward(q, k, v, lam, out, *saved, key_mask)
         return out
 
@@ -872,6 +904,7 @@ class NormBlockFn(torch.autograd.Function):
         s, n, stats = norm_block(ctx, x, y, gate, post_weight, pre_weight, save=True, **options)
         fn.ctx, fn.options = ctx, {k: v for k, v in options.items() if k != "next_norm"}
         fn.learned = _learned(**options)
+        _mark_leaves(fn)
         fn.save_for_backward(x, y, gate, post_weight, pre_weight, stats)
         fn.set_materialize_grads(False)
         return s, n
@@ -894,6 +927,7 @@ class HeadNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(fn, ctx, q, k, q_weight, k_weight, positions, freq, axis, options):
         fn.ctx, fn.options, fn.learned = ctx, dict(options), _learned(freq=freq, **options)
+        _mark_leaves(fn)
         fn.save_for_backward(q, k, q_weight, k_weight, positions, freq, axis)
         fn.set_materialize_grads(False)
         return head_norm_rotary(ctx, q, k, q_weight, k_weight, positions, freq, axis, **options)

@@ -301,3 +301,45 @@ def test_oracle_gradients_against_differences(kind, interleaved):
         # central differences: h^2 third derivatives (about 1e-8 here), cancellation 1e-16 / h
         assert abs((loss(*up) - loss(*down)) / (2 * h) - float((grads[i][0] * d).sum())) < 1e-6
         assert bool((grads[i][0].abs() <= grads[i][1] * (1 + 1e-12) + 1e-12).all())
+
+
+class _OnStream(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, x, note):
+        fn.ctx = None
+        ops._mark_leaves(fn)
+        note.append(fn.next_functions[0][0].metadata)
+        return x * 2
+
+    @staticmethod
+    def backward(fn, g):
+        ops._same_streams(fn)
+        return g * 2, None
+
+
+class _Node:
+    def __init__(self, is_cuda=True, **metadata):
+        self.metadata, self.next_functions = dict(metadata), ()
+        self.variable = type("V", (), dict(is_cuda=is_cuda))
+
+
+def test_leaves_are_marked_by_the_first_graph(monkeypatch):
+    """The mark lives as long as the leaf's end of a graph; recording beside another stream's raises."""
+    x, note = torch.ones(2, requires_grad=True), []
+    _OnStream.apply(x, note).sum().backward()
+    assert ops._STREAM not in note[0]  # a host tensor has no stream
+    monkeypatch.setattr(ops, "_Leaf", _Node)
+    monkeypatch.setattr(ops, "_stream", lambda ctx: stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    fn = type("F", (), dict(ctx=None, next_functions=((_Node(), 0), (None, 0), (_Node(is_cuda=False), 0))))
+    stream, capturing = 7, False
+    ops._mark_leaves(fn)
+    stream = 9
+    ops._mark_leaves(fn)
+    assert [n.metadata for n, _ in fn.next_functions if n is not None] == [{ops._STREAM: 7}, {}]
+    ops._same_streams(fn)
+    capturing = True
+    with pytest.raises(capi.MtpxError, match="earlier graph"):
+        ops._same_streams(fn)
+    stream = 7
+    ops._same_streams(fn)
