@@ -139,9 +139,9 @@ struct RoleArgs {
     int each_unit;  // one takes one tile; else they share all keys evenly,
     int least;      // each with so many steps at least, its partial results
     float *part;    // here: [groups][2][columns][2][4 + 2 D] (NULL: one group)
-    // wide: the most tiles of a key head, and of four times the columns (0: every
-    // tile in its turn)
-    int tiles, quarters;
+    // wide: the most tiles of a key head, as many of every sequence (`level`) or
+    // by number; and of four times the columns (0: every tile in its turn)
+    int tiles, level, quarters;
 };
 
 struct PagedArgs {

@@ -626,7 +626,7 @@ __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line
         Segment sg;
         Sequence sq;
         int seq, tile = 0;
-        bool any = true, late = false;
+        bool any = true, wrong = false;
         if (!role.r.each_unit) {
             if (p >= p1)
                 return;
@@ -652,22 +652,29 @@ __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line
                 seq = item / a.kv_heads;
                 sg.kv = item % a.kv_heads;
             } else {
+                // the last rows of a causal sequence have the most keys: they go
+                // first, of all sequences where those are alike (`level`); else
                 // sequence by sequence, whose workgroups then share what L2 holds of
-                // its keys, the last rows first; a causal sequence's first quarter,
-                // which sees the fewest keys, behind all others, to fill the end
+                // its keys, and the first quarter of each behind all others, to
+                // fill the end
                 const Work wk = work_item(item, role.r.tiles + role.r.quarters, a.kv_heads);
                 sg.kv = wk.head;
-                late = wk.tile >= role.r.tiles;
+                const bool late = wk.tile >= role.r.tiles;
                 const int at = role.r.tiles - 1 - wk.tile + (late ? role.r.quarters : 0);
-                seq = __builtin_amdgcn_readfirstlane(last_true(
-                    [&](int i) { return (late ? tile_number<4 * kCols>(a, i) : tile_number<kCols>(a, i)) <= at; }, a.sequences, kWave));
-                if (seq < 0)
-                    return;
-                tile = at - (late ? tile_number<4 * kCols>(a, seq) : tile_number<kCols>(a, seq));
+                if (role.r.level) {
+                    seq = at % a.sequences;
+                    tile = at / a.sequences;
+                } else {
+                    auto number = [&](int i) { return late ? tile_number<4 * kCols>(a, i) : tile_number<kCols>(a, i); };
+                    seq = __builtin_amdgcn_readfirstlane(last_true([&](int i) { return number(i) <= at; }, a.sequences, kWave));
+                    if (seq < 0)
+                        return;
+                    tile = at - number(seq);
+                    wrong = role.r.quarters > 0 && (tile < (role.tiles(a, Sequence(a, seq)) + 3) / 4) != late;
+                }
             }
             sq = Sequence(a, seq);
-            const int tiles = role.tiles(a, sq), quarter = NARROW || role.r.quarters == 0 ? 0 : (tiles + 3) / 4;
-            if (tile >= tiles || (!NARROW && role.r.quarters > 0 && (tile < quarter) != late))
+            if (wrong || tile >= role.tiles(a, sq))
                 return;
             sg.begin = 0;
             sg.end = sg.steps = role.steps(a, sq, tile);
@@ -775,11 +782,12 @@ __global__ __launch_bounds__(kJoin) void paged_join(PagedArgs a, int narrow_item
     if (item < narrow_items) {
         using R = Role<S::kNarrow, S::kRows>;
         const R role{a.narrow, true};
+        if (role.tiles(a, Sequence(a, item / a.kv_heads)) == 0)
+            return;
         Shares<R> shares(a, role, line);
         const int kv = item % a.kv_heads;
         shares.at(item / a.kv_heads, sq, start);
-        if (role.tiles(a, sq) > 0)
-            join_unit<T, D, R, S::kNarrow>(a, role, shares, sq, kv, 0, kv * shares.costs.head + start, 0, 1);
+        join_unit<T, D, R, S::kNarrow>(a, role, shares, sq, kv, 0, kv * shares.costs.head + start, 0, 1);
         return;
     }
     item -= narrow_items;

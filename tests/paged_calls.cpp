@@ -258,8 +258,8 @@ static int plan(char **v)
     const mtpx::PagedPlan p = mtpx::paged_plan(&ctx, r);
     size_t bytes = 0;
     const int code = mtpx_diff_attention_paged_workspace(&ctx, &r, &bytes);
-    std::printf("%d %d %d %d %d %d %d %d %zu\n", code, p.narrow_columns, p.narrow.groups, p.narrow.each_unit, p.wide.groups,
-                p.wide.each_unit, p.wide.tiles, p.wide.quarters, bytes);
+    std::printf("%d %d %d %d %d %d %d %d %d %zu\n", code, p.narrow_columns, p.narrow.groups, p.narrow.each_unit, p.wide.groups,
+                p.wide.each_unit, p.wide.tiles, p.wide.level, p.wide.quarters, bytes);
     return 0;
 }
 

@@ -215,6 +215,14 @@ def test_paged_broad_tiles(ctx, dtype):
 
 
 @dtypes
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new", [[520] * 8, [1500, 90, 700, 1, 5, 1900]])
+def test_paged_a_tile_a_workgroup(ctx, dtype, causal, new):
+    """So many tiles that each is a workgroup's: of sequences alike, and of others."""
+    check_paged(ctx, dtype, new, [n + i for i, n in enumerate(new)], 48, 72, 72, 16, causal, behind=3, max_rows=max(new))
+
+
+@dtypes
 def test_paged_large_scores(ctx, dtype):
     check_paged(ctx, dtype, [1, 60], [2000, 300], 16, 4, 2, 32, scale=12.0)
 

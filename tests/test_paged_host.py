@@ -122,7 +122,7 @@ def test_plans_cover_the_work(calls, seed):
     most = rng.choice([0, max(1, max(new))])
     page, width = rng.choice([16, 100]), rng.choice([3, 300])
     out = calls("plan", rows, n, most, group * kv, kv, dim, dtype, page, width)[0]
-    code, limit, narrow, narrow_each, wide, wide_each, tiles, quarters, size = (int(v) for v in out)
+    code, limit, narrow, narrow_each, wide, wide_each, tiles, level, quarters, size = (int(v) for v in out)
     if rows * group * kv > (2 ** 32 - 1) // 512:
         return
     assert code == 0
@@ -142,7 +142,8 @@ def test_plans_cover_the_work(calls, seed):
         assert wide > 0
         start = off[i] * group // columns + i
         for t in range(-(-m * group // columns)):
-            assert start + t < tiles and start + t not in place
+            assert (level and t * n + i < tiles) or start + t < tiles
+            assert start + t not in place
             place[start + t] = i
     # the number of a tile leads back to its sequence
     starts = [off[i] * group // columns + i for i in range(n)]
@@ -150,6 +151,7 @@ def test_plans_cover_the_work(calls, seed):
         assert max(j for j in range(n) if starts[j] <= t) == i
     if wide and wide_each:
         assert wide == (tiles + quarters) * kv
+    assert not level or wide_each
     wide_part = 2 * 4 * (4 + 2 * (32 if dim <= 32 else 64 if dim <= 64 else 128))
     want = 0 if narrow_each or narrow < 2 else narrow * 2 * 32 * wide_part
     want += 0 if wide_each or wide < 2 else wide * 2 * columns * wide_part
