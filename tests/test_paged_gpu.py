@@ -235,6 +235,41 @@ def test_paged_many_sequences(ctx):
     check_paged(ctx, torch.bfloat16, new.tolist(), (new + g.randint(0, 40, 500)).tolist(), 8, 2, 1, 32)
 
 
+def test_paged_thousands_of_sequences(ctx):
+    """More than workgroups share: a tile of each is one workgroup's."""
+    g = np.random.RandomState(6)
+    new = g.randint(0, 2, 4200)
+    new[7], new[4000] = 50, 9
+    check_paged(ctx, torch.bfloat16, new.tolist(), (new + g.randint(0, 30, 4200)).tolist(), 8, 2, 1, 32)
+
+
+@dtypes
+def test_paged_layouts(ctx, dtype):
+    """Keys and values in pools of different strides, one behind the other in one
+    tensor, at any alignment, heads outside slots: the result of contiguous ones."""
+    g = torch.Generator().manual_seed(12)
+    lengths, new, page, kv, d = [500, 3, 90], [40, 1, 1], 32, 2, 64
+    c = PO.pool(g, lengths, page, kv, d, dtype, fill=0.0)
+    q, lam = rand(g, 42, 6, 2, d, dtype=dtype).cuda(), torch.rand(6, generator=g).cuda()
+    k, v = c["k_pages"].cuda(), c["v_pages"].cuda()
+    rest = (lam, c["table"].cuda(), offsets(new).cuda(), i32(lengths).cuda())
+    want = ops.diff_attention_paged(ctx, q, k, v, *rest)
+    n = len(k)
+    apart = torch.zeros(n, page + 3, kv, 2 * d + 16, dtype=dtype).cuda()
+    apart[:, :page, :, :2 * d] = v
+    both = torch.stack([k.flatten(3), v], 1)  # pages, keys or values, slots, heads, elements
+    heads_out = torch.stack([k.flatten(3).transpose(1, 2), v.transpose(1, 2)])
+    odd = torch.zeros(k.numel() + 1, dtype=dtype).cuda()[1:].view(k.shape).copy_(k)
+    for kp, vp in ((k, apart[:, :page, :, :2 * d]), (both[:, 0].unflatten(3, (2, d)), both[:, 1]),
+                   (heads_out[0].transpose(1, 2).unflatten(3, (2, d)), heads_out[1].transpose(1, 2)), (odd, v)):
+        assert torch.equal(ops.diff_attention_paged(ctx, q, kp, vp, *rest), want)
+    wide = torch.zeros(3, c["table"].shape[1] + 5, dtype=torch.int32).cuda()
+    wide[:, 2:2 + c["table"].shape[1]] = rest[1]
+    part = wide[:, 2:2 + c["table"].shape[1]]
+    assert part.stride(0) != part.shape[1]
+    assert torch.equal(ops.diff_attention_paged(ctx, q, k, v, lam, part, *rest[2:]), want)
+
+
 def test_lengths_beyond_the_room_and_below_zero(ctx):
     """A length counts what its table has room for, its rows' places those it says; below zero it is 0."""
     g = torch.Generator().manual_seed(1)
