@@ -9,9 +9,11 @@ reference), the E/F/S and training kernels with -ffp-contract=fast (FMA).
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +22,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libmtpx.so")
 CALC_EFS = os.path.join(LIB_DIR, "mtpx_calc_efs")
+CALLS = os.path.join(HERE, "mtpx", "_calls.so")
 CXX = os.environ.get("CXX", "g++")
 OBJ_DIR = os.path.join(HERE, "_build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -120,9 +123,29 @@ def build(verbose: bool = False, changed_only: bool = False) -> str:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, CALC_EFS)
+    build_calls(verbose)
     if verbose:
         print("built %s in %.1fs" % (LIB, time.time() - t0), flush=True)
     return LIB
+
+
+def build_calls(verbose: bool = False) -> None:
+    """mtpx/_calls.so, the calls of mtpx.ops on torch's tensors (host code; its
+    library's entries are handed to it).  Without torch there is no mtpx.ops."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return
+    torch = spec.submodule_search_locations[0]
+    tmp = CALLS + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           "-I", os.path.join(ROOT, "include"), "-I", os.path.join(torch, "include"),
+           "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp,
+           "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, CALLS)
 
 
 if __name__ == "__main__":

@@ -173,6 +173,33 @@ def _ops():
     return _lib
 
 
+_native = None
+
+
+def _calls():
+    """The serving calls as native steps (csrc/torch_calls.cpp).  They take a call
+    that is plainly right, which is nearly all of them, and return None for any
+    other: the checks here then say what is wrong with it, or take it if nothing
+    is (a max_rows of numpy's type, say)."""
+    global _native
+    if _native is None:
+        L = capi.lib()
+        try:
+            from . import _calls as native
+        except ImportError as e:
+            raise RuntimeError("mtpx/_calls.so does not fit this torch or is not built "
+                               "(run imr-mlp_amd/build.py)") from e
+        native.setup(*(C.cast(getattr(L, "mtpx_" + f), _p).value for f in
+                       ("head_norm_rotary", "append_paged", "diff_attention_paged",
+                        "diff_attention_paged_workspace")))
+        _native = native
+    return _native
+
+
+def _handle(ctx):
+    return getattr(ctx.h, "value", None)
+
+
 def _fail(what):
     raise MtpxError(capi.ERRORS_BY_NAME["MTPX_E_INVALID"], what)
 
@@ -215,8 +242,11 @@ def _typed(ctx, t, name, dims):
     return code
 
 
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (not there: no device either)
+
+
 def _stream(ctx):
-    return torch._C._cuda_getCurrentRawStream(ctx.device)
+    return _stream_of(ctx.device)
 
 
 def _ptr(t):
@@ -598,6 +628,12 @@ def head_norm_rotary(ctx, q, k, q_weight, k_weight, positions, freq, axis, *, ki
     None: q only) every head and map becomes norm(x) weight, turned as by
     rotary; weights [dim] or None, positions, freq and axis as there.  Returns
     (q, k)."""
+    done = _calls().head_norm_rotary(_handle(ctx), ctx.device, _stream_of, q, k, q_weight, k_weight,
+                                     positions, freq, axis, NORMS.get(kind), eps, interleaved)
+    if done is not None:
+        if type(done) is int:
+            ctx._check(done, "head_norm_rotary")
+        return done
     dtype, rows, heads, kv, maps, dim, k_shape = _heads_of(ctx, q, k)
     shape, of = q.shape, q.dtype
     if kind not in NORMS:
@@ -689,6 +725,13 @@ def append_paged(ctx, k, v, k_pages, v_pages, table, offsets, lengths, positions
     With q [rows, heads, 2, dim] its queries are normed and turned as well:
     returns them (in out, which may be q), else None.  Rows of no sequence are
     left as they are."""
+    done = _calls().append_paged(_handle(ctx), ctx.device, _stream_of, k, v, k_pages, v_pages, table,
+                                 offsets, lengths, positions, freq, axis, q, APPEND_NORMS.get(kind),
+                                 q_weight, k_weight, eps, interleaved, out)
+    if done is not None:
+        if type(done) is int:
+            ctx._check(done, "append_paged")
+        return done if q is not None else None
     dtype = _typed(ctx, k, "k", 4)
     of = k.dtype
     rows, kv, _, dim = k.shape
@@ -735,6 +778,12 @@ def diff_attention_paged(ctx, q, k_pages, v_pages, lam, table, offsets, lengths,
     them.  max_rows: the most new rows of a sequence, where the caller knows it
     (1 in a plain decoding step), which saves work.  Returns [rows, heads, 2
     dim]; rows of no sequence are left as they are."""
+    done = _calls().diff_attention_paged(_handle(ctx), ctx.device, _stream_of, q, k_pages, v_pages,
+                                         lam, table, offsets, lengths, causal, scale, max_rows, out)
+    if done is not None:
+        if type(done) is int:
+            ctx._check(done, "diff_attention_paged")
+        return done
     dtype = _typed(ctx, q, "q", 4)
     of = q.dtype
     rows, heads, _, dim = q.shape
