@@ -169,7 +169,7 @@ int head_request(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r, bool
         a.grad[0] = r.dq_out;
         a.grad[1] = r.dk_out;
         a.dweight[0] = r.dq_weight;
-        a.dweight[1] = r.kv_heads ? r.dk_weight : nullptr;
+        a.dweight[1] = r.dk_weight;
         a.dpositions = r.dpositions;
     }
     const char *const names[2][4] = {{"q", "q_out", "dq_out", "dq"}, {"k", "k_out", "dk_out", "dk"}};

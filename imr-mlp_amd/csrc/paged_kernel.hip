@@ -42,14 +42,14 @@ __device__ inline int quotient(int n, const Divisor &d) { return (int)(__umulhi(
 
 // One sequence's place in the batch and in the cache.
 struct Sequence {
-    int first, rows;    // of the batch
+    int first, rows;    // of the batch (below 0: the offsets do not ascend here)
     int length, shift;  // keys; row j sees those up to shift + j (causal)
 
     __device__ inline Sequence() : first(0), rows(0), length(0), shift(0) {}
     __device__ inline Sequence(const PagedArgs &a, int i)
     {
         first = row_offset(a.offsets, i, a.rows);
-        rows = max(0, row_offset(a.offsets, i + 1, a.rows) - first);
+        rows = row_offset(a.offsets, i + 1, a.rows) - first;
         const int given = max(0, a.lengths[i]);
         length = min(given, a.cache.table_width * a.cache.page_rows);
         shift = given - rows;
@@ -115,7 +115,9 @@ __device__ inline int wave_scan(int v)
 // The units of one key head lie one after the other on a line of costs, tile by
 // tile and sequence by sequence, the key heads behind one another; workgroup w
 // takes what lies from w `each` on.  Built by a whole workgroup, for up to 64 runs
-// of 64 sequences (of more than one run, the sums before each lie in LDS).
+// of 64 sequences (of more than one run, the sums before each lie in LDS).  Costs
+// are 32-bit numbers, which the host has made sure of for offsets that ascend: of
+// others the line is empty.
 struct Line {
     int before[kWave];
 };
@@ -158,7 +160,7 @@ struct Shares {
         int groups = role.r.groups;
         if (single()) {
             read(0);
-            costs.head = __builtin_amdgcn_readlane(upto, kWave - 1);
+            costs.head = __any(sq.rows < 0) ? 0 : __builtin_amdgcn_readlane(upto, kWave - 1);
             // one sequence whose tiles cost the same: whole parts of a tile, which
             // begin at the same keys and so read them together
             if (a.sequences == 1) {
@@ -174,8 +176,9 @@ struct Shares {
                 if (at < a.sequences)
                     s = Sequence(a, at);
                 const int sum = wave_scan(role.cost(a, s, role.tiles(a, s)));
+                const bool astray = __any(s.rows < 0);
                 if (lane == kWave - 1)
-                    line.before[i] = sum;
+                    line.before[i] = astray ? -1 : sum;
             }
             __syncthreads();
             const int mine = lane < n ? line.before[lane] : 0, all = wave_scan(mine);
@@ -183,7 +186,7 @@ struct Shares {
             if (wave == 0)
                 line.before[lane] = all - mine;  // (runs beyond the last begin where it ends)
             __syncthreads();
-            costs.head = __builtin_amdgcn_readlane(all, kWave - 1);
+            costs.head = __any(mine < 0) ? 0 : __builtin_amdgcn_readlane(all, kWave - 1);
         }
         costs.total = costs.head * a.kv_heads;
         costs.each = max((costs.total + groups - 1) / groups, role.r.least);
@@ -696,6 +699,8 @@ template <class T, int D, class R, int COLS>
 __device__ inline void join_unit(const PagedArgs &a, const R &role, const Shares<R> &shares, const Sequence &sq, int kv, int tile,
                                  int a0, int piece, int pieces)
 {
+    if (shares.costs.total == 0)
+        return;
     const int steps = role.steps(a, sq, tile), keys = a0 + role.kStart;
     const int from = keys / shares.costs.each, upto = (keys + steps - 1) / shares.costs.each;
     if (steps == 0 || from == upto)

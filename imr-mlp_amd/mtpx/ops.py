@@ -674,7 +674,7 @@ def head_norm_rotary_backward(ctx, dq, dk, q, k, q_weight, k_weight, positions, 
         k_out = _whole(gk, kv, maps, dim)
     wq, wk = _weight(ctx, q_weight, "q_weight", dim, of), _weight(ctx, k_weight, "k_weight", dim, of)
     dwq = None if q_weight is None else q.new_empty(dim)
-    dwk = None if k_weight is None else q.new_zeros(dim) if k is None else q.new_empty(dim)
+    dwk = None if k_weight is None else q.new_empty(dim)
     if dpositions:
         dpos = torch.empty(positions.shape, dtype=positions.dtype, device=q.device)
     size = _bytes(ctx, _ops().mtpx_head_norm_rotary_workspace, HeadNormRequest, rows=rows, dim=dim)

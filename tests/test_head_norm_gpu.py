@@ -180,3 +180,13 @@ def test_large_positions_keep_their_phase(ctx):
     want, _ = OO.turned(x.double(), pos.double() * freq.double(), False)
     # turns of 2^38: their fraction in 64 bits is good to 2^-14
     assert float((y.double().cpu() - want).abs().max()) < 2 * math.pi * 2 ** -13
+
+
+@pytest.mark.parametrize("rows", [0, 37])
+def test_a_weight_without_keys(ctx, rows):
+    """Its gradient is zero, whatever lay in its place."""
+    q, w = torch.randn(rows, 2, 16).cuda(), torch.ones(16).cuda()
+    pos, freq, axis = torch.rand(rows, 1).cuda(), torch.rand(8).cuda(), torch.zeros(8, dtype=torch.int32).cuda()
+    torch.full((16,), float("nan")).cuda()
+    got = ops.head_norm_rotary_backward(ctx, q, None, q, None, w, w, pos, freq, axis)
+    assert got[1] is None and float(got[3].abs().max()) == 0.0

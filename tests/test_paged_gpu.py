@@ -287,6 +287,19 @@ def test_lengths_beyond_the_room_and_below_zero(ctx):
         assert float(got[6:].abs().max()) == 0.0
 
 
+@pytest.mark.parametrize("n,rows", [(5, 1), (5, 90), (70, 7), (70, 90), (300, 90)])
+def test_offsets_that_do_not_ascend(ctx, n, rows):
+    """The same rows again and again, more of them than there are: no row is written, and the call ends."""
+    g = torch.Generator().manual_seed(2)
+    c = PO.pool(g, [128], 16, 2, 32, torch.bfloat16)
+    table, lengths = c["table"].repeat(n, 1).cuda(), i32([128] * n).cuda()
+    q, lam = rand(g, rows, 4, 2, 32, dtype=torch.bfloat16).cuda(), torch.rand(4, generator=g).cuda()
+    out = torch.full((rows, 4, 64), 7.0, dtype=torch.bfloat16).cuda()
+    for off in (i32([0, rows] * n)[:n + 1], i32([rows, 0] + [rows] * n)[:n + 1]):
+        ops.diff_attention_paged(ctx, q, c["k_pages"].cuda(), c["v_pages"].cuda(), lam, table, off.cuda(), lengths, out=out)
+        assert bool((out == 7.0).all())
+
+
 def test_common_prefix_and_the_contiguous_cache(ctx):
     """Pages that several tables name; a row per sequence is diff_attention_cache's, up to the order of sums."""
     g = torch.Generator().manual_seed(7)
