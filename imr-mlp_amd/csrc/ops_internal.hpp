@@ -142,6 +142,7 @@ struct RoleArgs {
     // wide: the most tiles of a key head, as many of every sequence (`level`) or
     // by number; and of four times the columns (0: every tile in its turn)
     int tiles, level, quarters;
+    int split;  // steps that writing and joining a partial result are worth
 };
 
 struct PagedArgs {

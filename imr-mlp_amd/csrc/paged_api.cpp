@@ -259,7 +259,7 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
         // (small calls of both widths share the slots, so that neither waits for the
         // other: 12 sequences of up to 700 rows in 32 bits, 52 us and 41 us a call)
         const bool small = both && units * ((room + 63) / 64) <= 8 * slots;
-        const int64_t mine = small ? slots / 2 : slots * (width == 32 && half ? 2 : 1);
+        const int64_t mine = small ? slots / 2 : slots;
         const int64_t groups = a.each_unit ? units : std::min(mine, units * ((room + 63) / 64));
         a.groups = (int)std::min<int64_t>(groups, INT32_MAX);
         p.items += groups;
@@ -276,7 +276,15 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
         // sequences of 4,096 rows, 16 heads of 64: 960 us, 980 us sequence by
         // sequence; of 2,500 to 6,000 rows: 1,015 and 937 us)
         const int64_t all = r.rows * group / columns, level = (most * group + columns - 1) / columns * n;
-        const bool each = all * r.kv_heads >= 4 * slots;
+        // A tile a workgroup, of more tiles than slots: about as long as the longest
+        // tile over the even share, with tiles half as long as there is room on
+        // average.  Shared, a slot and a tile have `split` steps' time of partial
+        // results each (3 prompts of 1,024 rows, 32 heads of 64: 59 us and 89 us
+        // shared; one of 8,192, 16 heads: 446 and 464 us; a chunk of 2,048 rows of
+        // 32,000: 1,066 and 778 us).
+        p.wide.split = half ? 8 : 3;
+        const int64_t steps = (room - 1) / (2 * width * (half ? 2 : 4) <= 256 ? 64 : 32) + 1, units = all * r.kv_heads;
+        const bool each = units >= 4 * slots || (units > slots && steps * slots <= 2 * p.wide.split * (units + slots));
         p.wide.level = each && level * 10 <= all * 11;
         const int64_t tiles = p.wide.level ? level : all + n;
         p.wide.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);

@@ -101,15 +101,21 @@ struct Role {
     }
 };
 
-// Inclusive sums over a wave: shifts within rows of 16 lanes, then from row to row.
+// Inclusive sums, or the like, over a wave: shifts within rows of 16 lanes, then
+// from row to row (0 comes in).
+template <class Op>
+__device__ inline int wave_scan(int v, const Op &op)
+{
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+    return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+}
 __device__ inline int wave_scan(int v)
 {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
-    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return wave_scan(v, [](int x, int y) { return x + y; });
 }
 
 // The units of one key head lie one after the other on a line of costs, tile by
@@ -121,15 +127,19 @@ __device__ inline int wave_scan(int v)
 struct Line {
     int before[kWave];
 };
+// Where the tiles are no more than the workgroups and the longest takes no more
+// than an even share with its part of writing and joining partial results, a
+// workgroup takes a tile: a tile costs 1 then.
 struct Costs {
     int head, total, each;  // of a key head, of all, of a workgroup
+    bool whole;             // tiles
 };
 template <class R>
 struct Shares {
     const PagedArgs &a;
     const R &role;
     Line &line;
-    Costs costs;
+    Costs costs{0, 0, 0, false};
     int lane;
     // the lane's sequence of a run of 64, and the costs up to its end and before the run
     int run = -1, upto = 0, own = 0;
@@ -145,7 +155,8 @@ struct Shares {
         sq = Sequence();
         if (at < a.sequences)
             sq = Sequence(a, at);
-        own = role.cost(a, sq, role.tiles(a, sq));
+        const int tiles = role.tiles(a, sq);
+        own = costs.whole ? tiles : role.cost(a, sq, tiles);
         upto = wave_scan(own) + (single() ? 0 : line.before[i]);
     }
     // Where the line is there.
@@ -161,6 +172,16 @@ struct Shares {
         if (single()) {
             read(0);
             costs.head = __any(sq.rows < 0) ? 0 : __builtin_amdgcn_readlane(upto, kWave - 1);
+            if (!role.narrow) {
+                const int n = role.tiles(a, sq);
+                const int units = __builtin_amdgcn_readlane(wave_scan(n), kWave - 1) * a.kv_heads;
+                const int longest = wave_scan(n > 0 ? role.steps(a, sq, n - 1) : 0, [](int x, int y) { return max(x, y); });
+                const int even = (costs.head * a.kv_heads + role.r.split * (units + groups)) / groups;
+                if (costs.head > 0 && units <= groups && __builtin_amdgcn_readlane(longest, kWave - 1) + role.kStart <= even) {
+                    costs = {units / a.kv_heads, units, 1, true};
+                    return;
+                }
+            }
             // one sequence whose tiles cost the same: whole parts of a tile, which
             // begin at the same keys and so read them together
             if (a.sequences == 1) {
@@ -620,7 +641,7 @@ __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line
     const Role<kCols, KB> role{NARROW ? a.narrow : a.wide, NARROW};
     // neighbours on one XCD, whose L2 holds the keys that they share
     const int n = role.r.groups, w = n % 8 ? item : item % 8 * (n / 8) + item / 8;
-    Costs costs{0, 0, 0};
+    Costs costs{0, 0, 0, false};
     if (!role.r.each_unit)
         costs = Shares<Role<kCols, KB>>(a, role, line).costs;
     const int p0 = w * costs.each, p1 = min(p0 + costs.each, costs.total);
@@ -639,8 +660,9 @@ __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line
             seq = shares.find(p - sg.kv * costs.head, sq, at);
             at += sg.kv * costs.head;
             if constexpr (!NARROW)
-                tile = __builtin_amdgcn_readfirstlane(
-                    last_true([&](int t) { return at + role.cost(a, sq, t) <= p; }, role.tiles(a, sq), kWave));
+                tile = costs.whole ? p - at
+                                   : __builtin_amdgcn_readfirstlane(last_true(
+                                         [&](int t) { return at + role.cost(a, sq, t) <= p; }, role.tiles(a, sq), kWave));
             const int a0 = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile)), keys = a0 + role.kStart;
             sg.steps = role.steps(a, sq, tile);
             sg.begin = max(0, min(sg.steps, p0 - keys));
@@ -650,6 +672,12 @@ __device__ inline void work(const PagedArgs &a, int item, char *smem, Line &line
             // a unit without keys has its zeros written where it begins
             any = sg.begin < sg.end || (sg.steps == 0 && p0 <= a0);
             p = __builtin_amdgcn_readfirstlane(at + role.cost(a, sq, tile + 1));
+            if (costs.whole) {
+                sg.begin = 0;
+                sg.end = sg.steps;
+                any = true;
+                p = p1;
+            }
         } else {
             if constexpr (NARROW) {
                 seq = item / a.kv_heads;
@@ -699,7 +727,7 @@ template <class T, int D, class R, int COLS>
 __device__ inline void join_unit(const PagedArgs &a, const R &role, const Shares<R> &shares, const Sequence &sq, int kv, int tile,
                                  int a0, int piece, int pieces)
 {
-    if (shares.costs.total == 0)
+    if (shares.costs.total == 0 || shares.costs.whole)
         return;
     const int steps = role.steps(a, sq, tile), keys = a0 + role.kStart;
     const int from = keys / shares.costs.each, upto = (keys + steps - 1) / shares.costs.each;
