@@ -252,30 +252,38 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     // workgroups that the device holds at once: by their 64 KiB of LDS, or 32
     const int64_t slots = 2 * (int64_t)ctx->num_cus;
     const bool both = group <= kNarrowColumns && most * group > kNarrowColumns;
-    auto role = [&](RoleArgs &a, size_t &bytes, int columns, int64_t units, bool each) {
+    const int columns = half ? (width < 128 ? 128 : 64) : width < 128 ? 64 : 32;
+    const int64_t all = r.rows * group / columns;  // whole wide tiles of a key head
+    // A few long sequences among many short ones (by the average's share of the
+    // longest): shares of both widths run beside each other, on less than all slots
+    // each, as the ones read while the others multiply (46 single rows and chunks
+    // of 727, heads of 128: 287 us, 330 us with all slots each, 388 us with half;
+    // 30 rows and two chunks of 512, heads of 64: 161 us, 175 us).  Many wide tiles
+    // of up to 64 need all (46 rows and a chunk of 2,048: 392 us, 464 us with half).
+    const bool beside = both && half && r.rows * 4 <= n * most && (all + n) * r.kv_heads < (width == 128 ? 4 : 1) * slots;
+    auto role = [&](RoleArgs &a, size_t &bytes, int tile, int64_t units, bool each) {
         // (costs are counted in 32 bits)
         a.each_unit = each || n > kMaxShared || units > kMaxUnits || units * ((room + r.rows) / 32 + 16) > INT32_MAX / 2;
         a.least = 2;
         // (small calls of both widths share the slots, so that neither waits for the
         // other: 12 sequences of up to 700 rows in 32 bits, 52 us and 41 us a call)
         const bool small = both && units * ((room + 63) / 64) <= 8 * slots;
-        const int64_t mine = small ? slots / 2 : slots;
+        const int64_t mine = small || (beside && (&a == &p.narrow || width < 128)) ? slots / 2 : beside ? slots / 4 * 3 : slots;
         const int64_t groups = a.each_unit ? units : std::min(mine, units * ((room + 63) / 64));
         a.groups = (int)std::min<int64_t>(groups, INT32_MAX);
         p.items += groups;
         if (!a.each_unit && a.groups > 1)
-            bytes = sizeof(float) * 2 * (4 + 2 * width) * 2 * (size_t)columns * a.groups;
+            bytes = sizeof(float) * 2 * (4 + 2 * width) * 2 * (size_t)tile * a.groups;
     };
     if (group <= kNarrowColumns) {
         p.narrow_columns = kNarrowColumns;
         role(p.narrow, p.narrow_bytes, kNarrowColumns, n * r.kv_heads, false);
     }
     if (p.narrow_columns == 0 || both) {
-        const int columns = half ? (width < 128 ? 128 : 64) : width < 128 ? 64 : 32;
         // every sequence's tiles in one order where that leaves few without rows (8
         // sequences of 4,096 rows, 16 heads of 64: 960 us, 980 us sequence by
         // sequence; of 2,500 to 6,000 rows: 1,015 and 937 us)
-        const int64_t all = r.rows * group / columns, level = (most * group + columns - 1) / columns * n;
+        const int64_t level = (most * group + columns - 1) / columns * n;
         // A tile a workgroup, of more tiles than slots: about as long as the longest
         // tile over the even share, with tiles half as long as there is room on
         // average.  Shared, a slot and a tile have `split` steps' time of partial
