@@ -264,7 +264,6 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     auto role = [&](RoleArgs &a, size_t &bytes, int tile, int64_t units, bool each) {
         // (costs are counted in 32 bits)
         a.each_unit = each || n > kMaxShared || units > kMaxUnits || units * ((room + r.rows) / 32 + 16) > INT32_MAX / 2;
-        a.least = 2;
         // (small calls of both widths share the slots, so that neither waits for the
         // other: 12 sequences of up to 700 rows in 32 bits, 52 us and 41 us a call)
         const bool small = both && units * ((room + 63) / 64) <= 8 * slots;

@@ -168,7 +168,7 @@ struct Shares {
         : a(args), role(r), line(l), lane(threadIdx.x & (kWave - 1))
     {
         const int wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
-        int groups = role.r.groups;
+        const int groups = role.r.groups;
         if (single()) {
             read(0);
             costs.head = __any(sq.rows < 0) ? 0 : __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -181,13 +181,6 @@ struct Shares {
                     costs = {units / a.kv_heads, units, 1, true};
                     return;
                 }
-            }
-            // one sequence whose tiles cost the same: whole parts of a tile, which
-            // begin at the same keys and so read them together
-            if (a.sequences == 1) {
-                const int units = role.tiles(a, sq.of_lane(0)) * a.kv_heads, parts = units > 0 ? groups / units : 0;
-                if (parts * units >= groups / 8 * 7)
-                    groups = parts * units;
             }
         } else {
             const int n = (a.sequences + kWave - 1) / kWave;
@@ -210,7 +203,7 @@ struct Shares {
             costs.head = __any(mine < 0) ? 0 : __builtin_amdgcn_readlane(all, kWave - 1);
         }
         costs.total = costs.head * a.kv_heads;
-        costs.each = max((costs.total + groups - 1) / groups, role.r.least);
+        costs.each = (costs.total + groups - 1) / groups;
     }
     // The sequence at cost p (below costs.head) of a key head, and the cost of those before it.
     __device__ inline int find(int p, Sequence &s, int &start)
