@@ -96,8 +96,9 @@ HeadArgs head_args(const R &r, int maps)
     return a;
 }
 
-// The widest access that every piece of a vector allows, and the lanes of a
-// vector and of a row.  `wide`: the tensors' addresses and strides.
+// The widest access that every piece of a vector allows (`fits`: the tensors'
+// addresses and strides), the lanes of a vector, and those of a row: up to
+// most_lanes, while all rows' lanes are fewer than `threads`.
 template <class Fits>
 void shape_heads(HeadArgs &a, int64_t size, int most_lanes, int64_t threads, const Fits &fits)
 {
@@ -123,18 +124,24 @@ bool fits_rows(const mtpx_rows &t, int width, int64_t size, int maps)
 }
 
 // Lanes of a row: a whole workgroup where there are few rows, as that takes the
-// fewest steps one after the other; else up to a wave, as few as leave the device
-// full, since a row's cos and sin are formed by as many lanes and its vectors read
-// ahead (160,000 rows of 16 and 16 vectors of 64 in 16 bits: forward 303 us with 64
-// lanes, 230 us with 16; backward 695 us with 64, 422 us with 8).
+// fewest steps one after the other (36 heads of two vectors of 64 in 16 bits: 64
+// rows 5.1 us, 7.3 us with a wave each; 4,001 rows 21 us, 16 us with a wave each);
+// else up to a wave, as few as leave the device full, since a row's cos and sin are
+// formed by as many lanes and its vectors read ahead (160,000 rows of 16 and 16
+// vectors of 64 in 16 bits: forward 303 us with 64 lanes, 235 us with 16; backward
+// 479 us with 64, 382 us with 8).
 int row_lanes(mtpx_context *ctx, int64_t rows) { return rows <= 8 * (int64_t)ctx->num_cus ? 256 : 64; }
 constexpr int64_t kForwardThreads = int64_t(1) << 21, kBackwardThreads = int64_t(1) << 20;
 
-// Workgroups of the backward pass.
+// Workgroups of the backward pass: as many as the device holds of it, by the
+// registers that a lane's elements take (160,000 rows of 8 and 8 heads of two
+// vectors of 64 in 16 bits, pairs side by side: 389 us with 3 a compute unit, 441
+// with 2 and 459 with 4; 4,001 rows with the halves apart: 22 us with 2, 28 with 3
+// or 4; 160,000 rows of 10 and 5 heads of 40 in 32 bits: 560 us with 4, 623 with 3).
 int head_parts(mtpx_context *ctx, const HeadArgs &a)
 {
-    const int64_t together = 256 / a.lanes;
-    return (int)std::min<int64_t>((a.rows + together - 1) / together, 4 * (int64_t)ctx->num_cus);
+    const int64_t together = 256 / a.lanes, each = a.width < 8 ? 4 : a.interleaved ? 3 : 2;
+    return (int)std::min<int64_t>((a.rows + together - 1) / together, each * (int64_t)ctx->num_cus);
 }
 
 int check_head_sizes(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r)
@@ -238,8 +245,14 @@ struct PagedPlan {
     size_t narrow_bytes = 0, wide_bytes = 0;
     int64_t items = 0;
 };
+// Columns of a narrow tile (64 sequences of one row, 32 heads of 64 on 4: 152 us,
+// 163 us on wide tiles; 8 heads of 32: 165 and 180 us).
 constexpr int kNarrowColumns = 32;
-constexpr int64_t kMaxShared = 4096, kMaxUnits = 1 << 18;  // sequences and tiles whose keys workgroups share
+// Sequences and tiles whose keys workgroups share.  Of so many a tile each is a
+// little faster if they are alike (4,096 rows of 50 to 1,500 keys: 1,233 us, 1,346
+// us shared), and a long one among them does not keep the device waiting (one of
+// 32,000: 454 us, 31 us shared).
+constexpr int64_t kMaxShared = 4096, kMaxUnits = 1 << 18;
 
 PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
 {
