@@ -838,7 +838,8 @@ typedef struct mtpx_pages {
  * read as 0 below 0 and as `rows` beyond), and with them lengths[i] rows in
  * all: row j of its m is row lengths[i] - m + j of its cache.  Rows that no
  * sequence holds (padding before the first and behind the last) are neither
- * read nor written.  Nothing of this is read on the host, so that a recorded
+ * read nor written.  Offsets that do not ascend name no batch: nothing outside
+ * the tensors is read or written for them, and rows may be left unwritten.  Nothing of this is read on the host, so that a recorded
  * graph serves any batch of the same shapes. */
 
 /* Puts a batch's new keys and values into their pages, the keys normed for
