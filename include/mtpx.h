@@ -883,7 +883,7 @@ int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *reques
 typedef struct mtpx_diff_attention_paged_request {
     void *stream;
     int dtype;
-    int64_t rows;               /* below 2^26 */
+    int64_t rows;               /* below 2^26, rows * heads below 2^23 */
     int sequences;              /* below 2^24 */
     int max_rows;
     int heads, kv_heads, dim;   /* dim 1 to 128 */

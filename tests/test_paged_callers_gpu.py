@@ -2,6 +2,7 @@
 that are not theirs, gradients in place, captured steps, autograd through a block
 and the serving of what it has learned."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -203,3 +204,56 @@ def test_refused_on_the_device(ctx):
     with pytest.raises(capi.MtpxError, match="dim beyond 128"):
         ops.diff_attention_paged(ctx, torch.zeros(2, 1, 2, 132, device="cuda"), kp, vp, torch.zeros(1, device="cuda"),
                                  i32(0)[None], i32(0, 2), i32(2))
+
+
+def test_threads_of_their_own(ctx):
+    """Two threads at once, each with its context and stream: a call leaves the interpreter while it queues its work."""
+    g = torch.Generator().manual_seed(11)
+    c = PO.pool(g, [300, 40, 77], 16, 2, 32, torch.bfloat16)
+    q, k, v = (rand(g, *s, dtype=torch.bfloat16).cuda() for s in ((20, 4, 2, 32), (20, 2, 2, 32), (20, 2, 64)))
+    w, lam, pos = rand(g, 32, dtype=torch.bfloat16).cuda(), torch.rand(4, generator=g).cuda(), torch.rand(20, 2, generator=g).cuda()
+    freq, axis = torch.rand(16, generator=g).cuda(), (torch.arange(16) % 2).int().cuda()
+    table, off, n = c["table"].cuda(), i32(0, 12, 13, 20), i32(300, 40, 77)
+
+    def step(own):
+        kp, vp = c["k_pages"].cuda(), c["v_pages"].cuda()
+        qt = ops.append_paged(own, k, v, kp, vp, table, off, n, pos, freq, axis, q=q, kind="rms", q_weight=w)
+        return (*ops.head_norm_rotary(own, q, k, w, w, pos, freq, axis), ops.diff_attention_paged(own, qt, kp, vp, lam, table, off, n))
+
+    want = step(ctx)
+    torch.cuda.synchronize()
+    wrong, failed = [], []
+
+    def work():
+        try:
+            own, stream = capi.Context(0), torch.cuda.Stream()
+            for _ in range(40):
+                with torch.cuda.stream(stream):
+                    got = step(own)
+                stream.synchronize()
+                wrong.extend(1 for a, b in zip(got, want) if not torch.equal(a, b))
+            own.close()
+        except Exception as e:  # noqa: BLE001 -- a thread's failure is the test's
+            failed.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and not wrong
+
+
+@dtypes
+def test_a_cache_without_room(ctx, dtype):
+    """Tables of no pages and pools of none: nothing is put anywhere, no row sees a key."""
+    q, k, v = torch.ones(3, 2, 2, 16, dtype=dtype).cuda(), torch.ones(3, 1, 2, 16, dtype=dtype).cuda(), torch.ones(3, 1, 32, dtype=dtype).cuda()
+    pos, freq, axis, lam = torch.ones(3, 1).cuda(), torch.ones(4).cuda(), torch.zeros(4, dtype=torch.int32).cuda(), torch.ones(2).cuda()
+    off, n = i32(0, 1, 3), i32(5, 2)
+    for pages, table in ((3, torch.zeros(2, 0, dtype=torch.int32).cuda()), (0, torch.zeros(2, 2, dtype=torch.int32).cuda())):
+        kp, vp = torch.full((pages, 4, 1, 2, 16), 7.0, dtype=dtype).cuda(), torch.full((pages, 4, 1, 32), 7.0, dtype=dtype).cuda()
+        ops.append_paged(ctx, k, v, kp, vp, table, off, n, pos, freq, axis)
+        assert bool((kp == 7.0).all()) and bool((vp == 7.0).all())
+        for causal in (True, False):
+            out = ops.diff_attention_paged(ctx, q, kp, vp, lam, table, off, n, causal=causal)
+            assert float(out.abs().max()) == 0.0

@@ -223,6 +223,14 @@ def test_paged_a_tile_a_workgroup(ctx, dtype, causal, new):
 
 
 @dtypes
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_paged_long_among_short(ctx, dtype, dim):
+    """Shares of both widths beside each other, of fewer workgroups each; a tile a workgroup and parts of tiles."""
+    check_paged(ctx, dtype, [1] * 12 + [90], [700 + 200 * i for i in range(12)] + [3000], 16, 4, 2, dim, max_rows=90)
+    check_paged(ctx, dtype, [1] * 9 + [70, 40], [100 * i for i in range(1, 12)], 32, 2, 1, dim, max_rows=70)
+
+
+@dtypes
 def test_paged_large_scores(ctx, dtype):
     check_paged(ctx, dtype, [1, 60], [2000, 300], 16, 4, 2, 32, scale=12.0)
 
