@@ -855,8 +855,10 @@ hipError_t run(const PagedArgs &a, hipStream_t s)
                                        S::kLds + sizeof(Line), s, a);
     if (e != hipSuccess || (!a.narrow.part && !a.wide.part))
         return e;
-    // a join's thread takes four columns of four results of a wide tile
-    constexpr int all = S::kWide * (D / 2) / (4 * kJoin), pieces = all > 0 ? all : 1;
+    // a thread of a wide tile's join takes four columns of a result, or of two (12
+    // sequences of up to 700 rows in 32 bits: 38 us, 41 us of four; of one: a chunk of
+    // 128 rows of 4,000 of each of 16 sequences, 32 heads of 64, 218 us, 209 us so)
+    constexpr int all = S::kWide * (D / 2) / kJoin, pieces = all < 8 ? all : 8;
     const int narrow_items = a.narrow.part ? a.sequences * a.kv_heads : 0;
     const int64_t wide_items = a.wide.part ? (int64_t)a.wide.tiles * a.kv_heads * pieces : 0;
     return launch_kernel(paged_join<Type, D>, dim3((unsigned)(narrow_items + wide_items)), dim3(kJoin), 0, s, a, narrow_items, pieces);
