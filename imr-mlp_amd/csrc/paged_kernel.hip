@@ -283,11 +283,14 @@ __device__ inline void load_lanes_to_lds(const void *p, unsigned lane_offset, un
 }
 
 // FAST: rows of whole 16-byte pieces, keys and values laid out alike, pages of
-// whole runs of ROWS / W rows.  A wave's rows of a tile are one run, in one page,
-// so that all addresses and the table are the scalar unit's work and the lanes
-// keep their offsets: the vector unit has the softmax to do (a chunk of 2,048 rows
-// of 32,000, 16 heads of 64: 790 us, 930 us through the other loader; 46 single
-// rows and two chunks of 727, heads of 128: 286 and 398 us).
+// whole runs of kGroup rows, which one load of a wave brings.  Lane l forms the
+// address of key l once for keys and values, a load begins where the first of its
+// rows lies, and the lanes keep their offsets from there: the vector unit has the
+// softmax to do (a chunk of 2,048 rows of 32,000, 16 heads of 64: 780 us, 930 us
+// through the other loader; 46 single rows and two chunks of 727, heads of 128: 290
+// and 398 us; a chunk of 1,024 rows of 8,192 in pages of 24, 32 heads of 64: 221 and
+// 263 us.  Addresses of whole runs of a wave by the scalar unit alone take 1 to 2 %
+// less, and leave such pages to the other loader).
 template <class T, int D, int ROWS, int W>
 struct TileLoader<T, D, ROWS, W, true> {
     using TL = Tile<T, D>;
@@ -321,19 +324,25 @@ struct TileLoader<T, D, ROWS, W, true> {
     __device__ inline unsigned long long fetch(char *, int k_tile, int v_tile)
     {
         const unsigned long long seen = __ballot(there(a, page)) & ~0ull >> (64 - ROWS);
-        const int of_run = __builtin_amdgcn_readlane(page, wave * kRun);
-        const int key = first + wave * kRun, slot = key - page_of(a, key) * a.cache.page_rows;
-        const unsigned row = (unsigned)a.cache.k.row * (unsigned)sizeof(T);
-        const uint64_t at = (uint64_t)(unsigned)of_run * (uint64_t)(a.cache.k_page * (int64_t)sizeof(T)) + (uint64_t)(unsigned)slot * row;
+        const int slot = first + lane - page_of(a, first + lane) * a.cache.page_rows;
+        const uint64_t at = (uint64_t)(unsigned)page * (uint64_t)(a.cache.k_page * (int64_t)sizeof(T)) +
+                            (uint64_t)(unsigned)slot * ((unsigned)a.cache.k.row * (unsigned)sizeof(T));
+        uint64_t begins[N];  // of a load's rows
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int l = wave * kRun + i * kGroup;
+            begins[i] = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(at >> 32), l) << 32 |
+                        (unsigned)__builtin_amdgcn_readlane((int)at, l);
+        }
         const unsigned mine = (unsigned)(seen >> (wave * kRun)) & ~0u >> (32 - kRun);
         const bool all = mine == ~0u >> (32 - kRun) && a.dim == D;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const char *from = (half ? v : k) + at;
+            const char *from = half ? v : k;
             const int to = (half ? v_tile : k_tile) + wave * kRun * TL::kRowBytes;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const char *p = from + (uint64_t)(i * kGroup) * row;
+                const char *p = from + begins[i];
                 if (all) {
                     load_lanes_to_lds(p, offset[i % kColumns], to + i * 1024);
                     continue;
@@ -781,7 +790,7 @@ struct Shape {
     // work on 16 columns, which keeps them behind the reads of the cache
     static constexpr int kMaps = sizeof(T) == 2 && D <= 64 ? 2 : 1, kGroups = sizeof(T) == 4 && D == 128 ? 1 : 2;
     static constexpr int kNarrow = kWaves / 2 * 16, kWide = kWaves * kMaps / 2 * kGroups * 16;
-    static constexpr int kPage = kRows / kWaves;  // rows of a wave
+    static constexpr int kPage = 1024 / (2 * D * (int)sizeof(T));  // rows of a wave's load
 };
 
 // Both roles in one launch, the wide tiles first, which take the longest.  (Eight

@@ -224,6 +224,14 @@ def test_paged_a_tile_a_workgroup(ctx, dtype, causal, new):
 
 @dtypes
 @pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("page", [2, 4, 8, 24, 100])
+def test_paged_pages_of_runs(ctx, dtype, dim, page):
+    """Pages that end inside a wave's rows of a tile, at the end of one of its loads or within one."""
+    check_paged(ctx, dtype, [1, 70, 1], [500, 333, 77], page, 4, 2, dim, hidden=0.1)
+
+
+@dtypes
+@pytest.mark.parametrize("dim", [32, 64, 128])
 def test_paged_long_among_short(ctx, dtype, dim):
     """Shares of both widths beside each other, of fewer workgroups each; a tile a workgroup and parts of tiles."""
     check_paged(ctx, dtype, [1] * 12 + [90], [700 + 200 * i for i in range(12)] + [3000], 16, 4, 2, dim, max_rows=90)
