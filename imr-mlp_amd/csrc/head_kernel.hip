@@ -266,6 +266,15 @@ __device__ inline void wave_order()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The same for all lanes of a row: one wave's, or a workgroup's.
+__device__ inline void row_order(const HeadArgs &a)
+{
+    if (a.lanes > kWave)
+        __syncthreads();
+    else
+        wave_order();
+}
+
 // `lanes` lanes per row (several rows a wave where a row has little work, a
 // whole workgroup where there are few rows), `group` of them per vector.  A lane
 // keeps its unit's place in every vector, and so its cos, sin and weights, and
@@ -306,10 +315,7 @@ __global__ __launch_bounds__(kThreads) void head_forward_kernel(HeadArgs a)
     float2 *table = tables + mine * at.pairs;
     if (there)
         fill_table(a, row, lane, table);
-    if (a.lanes > kWave)
-        __syncthreads();
-    else
-        wave_order();
+    row_order(a);
     if (!there)
         return;
     float c[U][L::P], s[U][L::P];
@@ -365,8 +371,8 @@ __global__ __launch_bounds__(kThreads) void head_forward_kernel(HeadArgs a)
 
 // With g = dz w:  dx = (g - [mean g] - u mean(g u)) / size,  dw = sum dz u, and
 // a pair's share of the positions' gradient freq (dz2 z1 - dz1 z2), which the
-// rotation leaves as it is.  u is formed again from x.  A row's lanes lie in one
-// wave; a workgroup takes rows part, part + groups, ... and keeps its share of
+// rotation leaves as it is.  u is formed again from x.  A row's lanes are a part of
+// a wave or a workgroup; a workgroup takes rows part, part + groups, ... and keeps its share of
 // the weights' gradients in registers until the end: a.parts partial rows.
 template <class T, int W, bool APART, int U, bool MOVED>
 __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
@@ -374,6 +380,7 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
     using L = Layout<T, W, APART, U>;
     // the tables of the rows, and at the end the lanes' sums
     __shared__ float shared[kThreads * L::E * U];
+    __shared__ float moved[MOVED ? kMaxAxes : 1][kThreads / kWave];  // the waves' sums
     const int lane = threadIdx.x & (a.lanes - 1), mine = threadIdx.x / a.lanes;
     const L at(a, lane);
     float2 *table = (float2 *)shared + mine * at.pairs;
@@ -396,9 +403,9 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
                 at.load((const T *)x.data + row * x.row + (first >> bits) * x.head + (first & bits) * x.map, early[job][0]);
                 at.load((const T *)y.data + row * y.row + (first >> bits) * y.head + (first & bits) * y.map, early[job][1]);
             }
-        wave_order();  // the last row's reads of the table
+        row_order(a);  // the last row's reads of the table
         fill_table(a, row, lane, table);
-        wave_order();
+        row_order(a);
         float c[U][L::P], s[U][L::P], d[U][L::P];
         read_table<L, U, L::P>(at, table, c, s);
 #pragma unroll
@@ -485,8 +492,16 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
                 if (k >= a.axes)
                     break;
                 float v = sums[k];
-                for (int o = a.lanes / 2; o > 0; o >>= 1)
+                for (int o = min(a.lanes, kWave) / 2; o > 0; o >>= 1)
                     v += __shfl_xor(v, o);
+                if (a.lanes > kWave) {
+                    if (lane % kWave == 0)
+                        moved[k][lane / kWave] = v;
+                    __syncthreads();
+                    v = moved[k][0];
+                    for (int w = 1; w < kThreads / kWave; ++w)
+                        v += moved[k][w];
+                }
                 if (lane == 0) {
                     if (a.position_dtype == MTPX_F64)
                         ((double *)a.dpositions)[row * a.axes + k] = v;
@@ -497,7 +512,11 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
         }
     }
 
-    // the lanes of a workgroup that hold the same elements, in their order
+    // the lanes of a workgroup that hold the same elements, in a fixed order: an
+    // element a thread, of short vectors, which many lanes hold, a part of one's (one
+    // row of vectors of 16: 13.6 us, 17.6 us an element a thread; 4,001 rows of 40:
+    // 25.8 and 24.9 us)
+    const int runs = a.dim <= 32 ? kThreads / a.dim : 1;
 #pragma unroll
     for (int job = 0; job < 2; ++job) {
         if (!a.dweight[job])
@@ -506,15 +525,34 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
-            for (int e = 0; e < L::E; ++e)
-                if (at.inside(at.unit(i), e))
-                    shared[threadIdx.x / a.group * a.dim + at.element(at.unit(i), e)] = dw[job][i][e];
+            for (int x = 0; x < L::E; ++x)
+                if (at.inside(at.unit(i), x))
+                    shared[threadIdx.x / a.group * a.dim + at.element(at.unit(i), x)] = dw[job][i][x];
         __syncthreads();
-        for (int e = threadIdx.x; e < a.dim; e += kThreads) {
-            float v = 0.f;
-            for (int k = 0; k < kThreads / a.group; ++k)
+        float *const part = a.part + ((int64_t)job * a.parts + blockIdx.x) * a.dim;
+        if (runs == 1) {
+            for (int e = threadIdx.x; e < a.dim; e += kThreads) {
+                float v = 0.f;
+                for (int k = 0; k < kThreads / a.group; ++k)
+                    v += shared[k * a.dim + e];
+                part[e] = v;
+            }
+            continue;
+        }
+        const int e = threadIdx.x % a.dim, run = threadIdx.x / a.dim;
+        float v = 0.f;
+        if (run < runs)
+#pragma unroll 4
+            for (int k = run; k < kThreads / a.group; k += runs)
                 v += shared[k * a.dim + e];
-            a.part[((int64_t)job * a.parts + blockIdx.x) * a.dim + e] = v;
+        __syncthreads();
+        shared[threadIdx.x] = v;
+        __syncthreads();
+        if (run == 0) {
+#pragma unroll 4
+            for (int k = 1; k < runs; ++k)
+                v += shared[k * a.dim + e];
+            part[e] = v;
         }
     }
 }

@@ -111,7 +111,7 @@ struct HeadArgs {
     int parts;
     int width;  // elements of one access
     int group;  // lanes of a vector: a power of two up to 64
-    int lanes;  // of a row: a power of two from group up to 256
+    int lanes;  // of a row: a power of two from group up to 256 (backward: not 128)
 };
 
 // n / d for n below 2^31: the upper half of 2 n magic, shifted.

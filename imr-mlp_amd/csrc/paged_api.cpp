@@ -96,11 +96,32 @@ HeadArgs head_args(const R &r, int maps)
     return a;
 }
 
+// Lanes of a row: a whole workgroup where there are few rows, as that takes the
+// fewest steps one after the other (36 heads of two vectors of 64 in 16 bits: 64
+// rows 5.1 us, 7.3 us with a wave each; 4,001 rows 21 us, 16 us with a wave each);
+// else up to a wave, as few as leave the device full, since a row's cos and sin are
+// formed by as many lanes and its vectors read ahead (160,000 rows of 16 and 16
+// vectors of 64 in 16 bits: forward 303 us with 64 lanes, 235 us with 16; backward
+// 479 us with 64, 382 us with 8).  The backward pass's workgroups have more to end
+// with, which many rows pay for if they take few steps (those heads: 1 row 13.7 us
+// with a wave, 11.1 us with a workgroup; 2,048 rows 21 and 28 us; 32 vectors of 128
+// with a wave each: 1,024 rows 40 and 23 us).
+constexpr int64_t kForwardThreads = int64_t(1) << 21, kBackwardThreads = int64_t(1) << 20;
+void row_lanes(mtpx_context *ctx, HeadArgs &a, bool back)
+{
+    const int64_t wanted = (int64_t)std::max(a.vectors[0], a.vectors[1]) * a.group, few = 2 * (int64_t)ctx->num_cus;
+    const int most = a.rows <= few || (a.rows <= 4 * few && (!back || wanted >= 16 * 64)) ? 256 : 64;
+    a.lanes = a.group;
+    while (a.lanes < most && a.lanes < wanted && a.rows * a.lanes < (back ? kBackwardThreads : kForwardThreads))
+        a.lanes *= 2;
+    if (back && a.lanes == 128)
+        a.lanes = 64;  // the backward pass's workgroups have one row of more than a wave, or none
+}
+
 // The widest access that every piece of a vector allows (`fits`: the tensors'
-// addresses and strides), the lanes of a vector, and those of a row: up to
-// most_lanes, while all rows' lanes are fewer than `threads`.
+// addresses and strides), and the lanes of a vector and of a row.
 template <class Fits>
-void shape_heads(HeadArgs &a, int64_t size, int most_lanes, int64_t threads, const Fits &fits)
+void shape_heads(mtpx_context *ctx, HeadArgs &a, int64_t size, bool back, const Fits &fits)
 {
     const int half = a.rotated / 2;
     a.width = (int)(16 / size);
@@ -112,26 +133,13 @@ void shape_heads(HeadArgs &a, int64_t size, int most_lanes, int64_t threads, con
     a.group = 1;
     while (a.group < 64 && a.group < units)
         a.group *= 2;
-    const int64_t vectors = std::max(a.vectors[0], a.vectors[1]);
-    a.lanes = a.group;
-    while (a.lanes < most_lanes && a.lanes < vectors * a.group && a.rows * a.lanes < threads)
-        a.lanes *= 2;
+    row_lanes(ctx, a, back);
 }
 bool fits_rows(const mtpx_rows &t, int width, int64_t size, int maps)
 {
     return !t.data || (aligned(t.data, width * size) && t.row % width == 0 && t.head % width == 0 &&
                        (maps == 1 || t.map % width == 0));
 }
-
-// Lanes of a row: a whole workgroup where there are few rows, as that takes the
-// fewest steps one after the other (36 heads of two vectors of 64 in 16 bits: 64
-// rows 5.1 us, 7.3 us with a wave each; 4,001 rows 21 us, 16 us with a wave each);
-// else up to a wave, as few as leave the device full, since a row's cos and sin are
-// formed by as many lanes and its vectors read ahead (160,000 rows of 16 and 16
-// vectors of 64 in 16 bits: forward 303 us with 64 lanes, 235 us with 16; backward
-// 479 us with 64, 382 us with 8).
-int row_lanes(mtpx_context *ctx, int64_t rows) { return rows <= 8 * (int64_t)ctx->num_cus ? 256 : 64; }
-constexpr int64_t kForwardThreads = int64_t(1) << 21, kBackwardThreads = int64_t(1) << 20;
 
 // Workgroups of the backward pass: as many as the device holds of it, by the
 // registers that a lane's elements take (160,000 rows of 8 and 8 heads of two
@@ -189,7 +197,7 @@ int head_request(mtpx_context *ctx, const mtpx_head_norm_rotary_request &r, bool
             MTPX_TRY(check_rows(ctx, a.grad[i], r.dtype, names[i][2]));
         MTPX_TRY(check_place(ctx, back ? a.grad[i] : a.in[i], a.out[i], r.maps, names[i][back ? 3 : 1]));
     }
-    shape_heads(a, size, back ? 64 : row_lanes(ctx, r.rows), back ? kBackwardThreads : kForwardThreads, [&](int width) {
+    shape_heads(ctx, a, size, back, [&](int width) {
         for (int i = 0; i < 2; ++i)
             if (a.vectors[i] && !(fits_rows(a.in[i], width, size, r.maps) && fits_rows(a.out[i], width, size, r.maps) &&
                                   fits_rows(a.grad[i], width, size, r.maps)))
@@ -418,7 +426,7 @@ int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *req)
             a.out[0] = r.q_out;
         }
         const int64_t size = (int64_t)dtype_bytes(r.dtype);
-        shape_heads(a, size, row_lanes(ctx, r.rows), kForwardThreads, [&](int width) {
+        shape_heads(ctx, a, size, false, [&](int width) {
             return fits_rows(a.in[1], width, size, 2) && fits_rows(a.v, width, size, 2) && pages_fit(r.cache, width, size) &&
                    (r.heads == 0 || (fits_rows(a.in[0], width, size, 2) && fits_rows(a.out[0], width, size, 2)));
         });
