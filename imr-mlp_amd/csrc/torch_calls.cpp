@@ -1,8 +1,9 @@
-// The serving calls of mtpx.ops as one native step each (module mtpx._calls):
+// Calls of mtpx.ops as one native step each (module mtpx._calls):
 // tensors are looked at, a request filled and the library called without
 // Python's steps between, which take longer than the kernels of small calls do
 // (one row's queries and keys: 11.3 us a call through the checks in Python, 4.8 us
-// so; appended: 13.0 and 4.1; attended: 13.7 and 7.2, its two kernels' own time).
+// so; its gradients: 19.8 and 9.7; appended: 13.0 and 4.1; attended: 13.7 and 7.2, its
+// two kernels' own time).
 //
 // A call that is not plainly right -- another type, shape, device or kind of
 // object -- returns None, and mtpx.ops goes through its own checks, which say
@@ -20,11 +21,13 @@
 #include <cfloat>
 #include <cmath>
 #include <exception>
+#include <type_traits>
 
 namespace {
 
 struct Entries {
-    decltype(&mtpx_head_norm_rotary) head_norm_rotary;
+    decltype(&mtpx_head_norm_rotary) head_norm_rotary, head_norm_rotary_backward;
+    decltype(&mtpx_head_norm_rotary_workspace) head_norm_rotary_workspace;
     decltype(&mtpx_append_paged) append_paged;
     decltype(&mtpx_diff_attention_paged) diff_attention_paged;
     decltype(&mtpx_diff_attention_paged_workspace) diff_attention_paged_workspace;
@@ -206,41 +209,55 @@ PyObject *guarded(PyObject *const *args, Py_ssize_t given, Py_ssize_t wanted, co
 
 bool is_type(const at::Tensor &t) { return type_code(t.scalar_type()) >= 0 && type_code(t.scalar_type()) <= MTPX_F16; }
 
-// (context, device, stream, q, k, q_weight, k_weight, positions, freq, axis, kind, eps, interleaved)
+// q and k from argument i on, weights and rotation behind them, kind, eps and
+// interleaved from argument j on
+bool heads(Call &c, int i, int j, mtpx_head_norm_rotary_request &r, const at::Tensor *&q, const at::Tensor *&k)
+{
+    const int64_t dims = THPVariable_Check(c.args[i]) && THPVariable_Unpack(c.args[i]).dim() == 4 ? 4 : 3;
+    q = c.tensor(i, dims);
+    if (!q || !is_type(*q) || !c.rows(i, dims, q->scalar_type()))
+        return false;
+    const auto type = q->scalar_type();
+    r.dtype = type_code(type);
+    r.rows = q->size(0);
+    r.maps = dims == 4 ? (int)q->size(2) : 1;
+    r.dim = (int)q->size(dims - 1);
+    r.heads = (int)q->size(1);
+    c.need(q->size(1) <= INT32_MAX && q->size(dims - 1) <= INT32_MAX && (r.maps == 1 || r.maps == 2));
+    r.q = rows_of(*q);
+    if (!c.absent(i + 1)) {
+        k = c.rows(i + 1, dims, type);
+        if (!k)
+            return false;
+        c.need(k->size(0) == r.rows && k->size(1) > 0 && k->size(1) <= INT32_MAX && k->size(dims - 1) == r.dim);
+        c.need(dims == 3 || k->size(2) == r.maps);
+        r.kv_heads = (int)k->size(1);
+        r.k = rows_of(*k);
+    }
+    turn(c, i + 4, r);
+    r.q_weight = weight(c, i + 2, r.dim, type);
+    r.k_weight = weight(c, i + 3, r.dim, type);
+    r.kind = (int)c.integer(j);
+    r.eps = c.real(j + 1);
+    r.interleaved = c.truth(j + 2);
+    r.stream = c.stream();
+    return c.good;
+}
+PyObject *wrapped(const at::Tensor &t)
+{
+    if (t.defined())
+        return THPVariable_Wrap(t);
+    Py_RETURN_NONE;
+}
+
+// (context, device, stream, q, k, q_weight, k_weight, positions, freq, axis, kind, eps, interleaved): (q, k)
 PyObject *head_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     return guarded(args, n, 13, [&](mtpx_context *context, Call &c) -> PyObject * {
-        const int64_t dims = THPVariable_Check(args[3]) && THPVariable_Unpack(args[3]).dim() == 4 ? 4 : 3;
-        const at::Tensor *q = c.tensor(3, dims), *k = nullptr;
-        if (!q || !is_type(*q) || !c.rows(3, dims, q->scalar_type()))
-            Py_RETURN_NONE;
-        const auto type = q->scalar_type();
+        const at::Tensor *q = nullptr, *k = nullptr;
         mtpx_head_norm_rotary_request r{};
-        r.dtype = type_code(type);
-        r.rows = q->size(0);
-        r.maps = dims == 4 ? (int)q->size(2) : 1;
-        r.dim = (int)q->size(dims - 1);
-        r.heads = (int)q->size(1);
-        c.need(q->size(1) <= INT32_MAX && q->size(dims - 1) <= INT32_MAX && (r.maps == 1 || r.maps == 2));
-        if (!c.absent(4)) {
-            k = c.rows(4, dims, type);
-            if (!k)
-                Py_RETURN_NONE;
-            c.need(k->size(0) == r.rows && k->size(1) > 0 && k->size(1) <= INT32_MAX && k->size(dims - 1) == r.dim);
-            c.need(dims == 3 || k->size(2) == r.maps);
-            r.kv_heads = (int)k->size(1);
-            r.k = rows_of(*k);
-        }
-        turn(c, 7, r);
-        r.q_weight = weight(c, 5, r.dim, type);
-        r.k_weight = weight(c, 6, r.dim, type);
-        r.kind = (int)c.integer(10);
-        r.eps = c.real(11);
-        r.interleaved = c.truth(12);
-        r.stream = c.stream();
-        if (!c.good)
+        if (!heads(c, 3, 10, r, q, k))
             Py_RETURN_NONE;
-        r.q = rows_of(*q);
         const at::Tensor qo = like(*q);
         r.q_out = rows_of(qo);
         at::Tensor ko;
@@ -249,11 +266,55 @@ PyObject *head_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t n)
             r.k_out = rows_of(ko);
         }
         const int rc = enter(entries.head_norm_rotary, context, r);
+        return rc ? PyLong_FromLong(rc) : Py_BuildValue("NN", wrapped(qo), wrapped(ko));
+    });
+}
+
+// (context, device, stream, dq, dk, q, k, q_weight, k_weight, positions, freq, axis, kind, eps, interleaved,
+//  dpositions): (dq, dk, dq_weight, dk_weight, dpositions)
+PyObject *head_norm_rotary_backward(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    return guarded(args, n, 16, [&](mtpx_context *context, Call &c) -> PyObject * {
+        const at::Tensor *q = nullptr, *k = nullptr;
+        mtpx_head_norm_rotary_request r{};
+        const bool moved = c.truth(15);
+        if (!heads(c, 5, 12, r, q, k) || c.absent(4) != !k)
+            Py_RETURN_NONE;
+        const at::Tensor *dy = c.rows(3, q->dim(), q->scalar_type());
+        if (!dy || dy->sizes() != q->sizes())
+            Py_RETURN_NONE;
+        r.dq_out = rows_of(*dy);
+        const at::Tensor gq = like(*q);
+        r.dq = rows_of(gq);
+        at::Tensor gk, wq, wk, dpos;
+        if (k) {
+            const at::Tensor *dz = c.rows(4, k->dim(), k->scalar_type());
+            if (!dz || dz->sizes() != k->sizes())
+                Py_RETURN_NONE;
+            r.dk_out = rows_of(*dz);
+            gk = like(*k);
+            r.dk = rows_of(gk);
+        }
+        if (r.q_weight) {
+            wq = at::empty({r.dim}, q->options());
+            r.dq_weight = wq.data_ptr();
+        }
+        if (r.k_weight) {
+            wk = at::empty({r.dim}, q->options());
+            r.dk_weight = wk.data_ptr();
+        }
+        if (moved) {
+            dpos = like(THPVariable_Unpack(args[9]));
+            r.dpositions = dpos.data_ptr();
+        }
+        int rc = entries.head_norm_rotary_workspace(context, &r, &r.workspace_bytes);
         if (rc)
             return PyLong_FromLong(rc);
-        if (k)
-            return Py_BuildValue("NN", THPVariable_Wrap(qo), THPVariable_Wrap(ko));
-        return Py_BuildValue("NO", THPVariable_Wrap(qo), Py_None);
+        const at::Tensor work = at::empty({(int64_t)r.workspace_bytes}, q->options().dtype(at::kByte));
+        r.workspace = work.data_ptr();  // held until the kernels are queued
+        rc = enter(entries.head_norm_rotary_backward, context, r);
+        return rc ? PyLong_FromLong(rc)
+                  : Py_BuildValue("NNNNN", wrapped(gq), wrapped(gk), wrapped(wq), wrapped(wk), wrapped(dpos));
     });
 }
 
@@ -370,21 +431,27 @@ PyObject *diff_attention_paged(PyObject *, PyObject *const *args, Py_ssize_t n)
 // The addresses of the library's entries, in the order of Entries.
 PyObject *setup(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
-    if (n != 4)
-        return PyErr_Format(PyExc_TypeError, "four addresses");
-    void *p[4];
-    for (int i = 0; i < 4; ++i)
+    constexpr int kEntries = 6;
+    if (n != kEntries)
+        return PyErr_Format(PyExc_TypeError, "%d addresses", kEntries);
+    void *p[kEntries];
+    for (int i = 0; i < kEntries; ++i)
         if (!(p[i] = PyLong_AsVoidPtr(args[i])))
             return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "a null address");
-    entries = {reinterpret_cast<decltype(entries.head_norm_rotary)>(p[0]), reinterpret_cast<decltype(entries.append_paged)>(p[1]),
-               reinterpret_cast<decltype(entries.diff_attention_paged)>(p[2]),
-               reinterpret_cast<decltype(entries.diff_attention_paged_workspace)>(p[3])};
+    int i = 0;
+    auto take = [&](auto &entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(p[i++]); };
+    take(entries.head_norm_rotary);
+    take(entries.head_norm_rotary_backward);
+    take(entries.head_norm_rotary_workspace);
+    take(entries.append_paged);
+    take(entries.diff_attention_paged);
+    take(entries.diff_attention_paged_workspace);
     Py_RETURN_NONE;
 }
 
 #define MTPX_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {MTPX_METHOD(setup), MTPX_METHOD(head_norm_rotary), MTPX_METHOD(append_paged),
-                         MTPX_METHOD(diff_attention_paged), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {MTPX_METHOD(setup), MTPX_METHOD(head_norm_rotary), MTPX_METHOD(head_norm_rotary_backward),
+                         MTPX_METHOD(append_paged), MTPX_METHOD(diff_attention_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mtpx._calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

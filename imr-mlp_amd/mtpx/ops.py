@@ -177,7 +177,7 @@ _native = None
 
 
 def _calls():
-    """The serving calls as native steps (csrc/torch_calls.cpp).  They take a call
+    """Norms of heads and the serving calls as native steps (csrc/torch_calls.cpp).  They take a call
     that is plainly right, which is nearly all of them, and return None for any
     other: the checks here then say what is wrong with it, or take it if nothing
     is (a max_rows of numpy's type, say)."""
@@ -190,8 +190,8 @@ def _calls():
             raise RuntimeError("mtpx/_calls.so does not fit this torch or is not built "
                                "(run imr-mlp_amd/build.py)") from e
         native.setup(*(C.cast(getattr(L, "mtpx_" + f), _p).value for f in
-                       ("head_norm_rotary", "append_paged", "diff_attention_paged",
-                        "diff_attention_paged_workspace")))
+                       ("head_norm_rotary", "head_norm_rotary_backward", "head_norm_rotary_workspace",
+                        "append_paged", "diff_attention_paged", "diff_attention_paged_workspace")))
         _native = native
     return _native
 
@@ -659,6 +659,13 @@ def head_norm_rotary_backward(ctx, dq, dk, q, k, q_weight, k_weight, positions, 
     results and the forward pass's inputs; None in the place of an input that
     was not given, and of the positions' without dpositions (which needs
     float32 or float64 ones; a 32-bit sum for both)."""
+    done = _calls().head_norm_rotary_backward(
+        _handle(ctx), ctx.device, _stream_of, dq, dk, q, k, q_weight, k_weight, positions, freq, axis,
+        NORMS.get(kind), eps, interleaved, dpositions)
+    if done is not None:
+        if type(done) is int:
+            ctx._check(done, "head_norm_rotary_backward")
+        return done
     dtype, rows, heads, kv, maps, dim, k_shape = _heads_of(ctx, q, k)
     shape, of = q.shape, q.dtype
     if kind not in NORMS:

@@ -7,7 +7,7 @@ import torch
 from mtpx import capi, ops
 from test_ops_gpu import dtypes, rand
 
-CALLS = (("head_norm_rotary", 13), ("append_paged", 20), ("diff_attention_paged", 14))
+CALLS = (("head_norm_rotary", 13), ("head_norm_rotary_backward", 16), ("append_paged", 20), ("diff_attention_paged", 14))
 
 
 @pytest.mark.parametrize("name,n", CALLS)
@@ -26,9 +26,9 @@ def test_a_library_that_is_not_there():
     with pytest.raises(TypeError):
         ops._calls().setup(1, 2, 3)
     with pytest.raises(TypeError):
-        ops._calls().setup("a", "b", "c", "d")
+        ops._calls().setup("a", "b", "c", "d", "e", "f")
     with pytest.raises(ValueError):
-        ops._calls().setup(0, 0, 0, 0)
+        ops._calls().setup(0, 0, 0, 0, 0, 0)
 
 
 class _NoneOfThem:
@@ -73,6 +73,9 @@ def test_the_same_results(ctx, monkeypatch, dtype, positions):
         for kw in ({}, dict(kind="layer", eps=1e-3, interleaved=True), dict(eps=1)):
             for wq, wk in ((w, u), (None, u), (w, None)):
                 _both(monkeypatch, lambda: ops.head_norm_rotary(ctx, x, y, wq, wk, p, freq, axis, **kw))
+                for moved in (False, True)[:1 + positions.is_floating_point]:
+                    _both(monkeypatch, lambda: ops.head_norm_rotary_backward(ctx, x * 0.5, None if y is None else _wide(y), x, y, wq, wk, p, freq, axis,
+                                                                             dpositions=moved, **kw))
     _both(monkeypatch, lambda: ops.head_norm_rotary(ctx, q, k, w, u, pos.t().contiguous().t(), freq[:0], axis[:0]))
 
     def filled(kt, vt, **kw):
@@ -108,7 +111,10 @@ def test_refused_either_way(ctx, monkeypatch):
     put = lambda k=k, v=v, kp=kp, vp=vp, table=table, off=off, n=n, **kw: ops.append_paged(ctx, k, v, kp, vp, table, off, n, pos, freq, axis, **kw)  # noqa: E731
     attend = lambda q=q, kp=kp, vp=vp, lam=lam, table=table, off=off, n=n, **kw: ops.diff_attention_paged(ctx, q, kp, vp, lam, table, off, n, **kw)  # noqa: E731
     odd, far = torch.zeros(3, 2, 2, 7).cuda(), torch.zeros(3, 1, dtype=torch.int16).cuda()
-    for call in (lambda: head(eps=-1.0), lambda: head(eps=float("nan")), lambda: head(kind="none"), lambda: head(pos=far), lambda: head(q=q.double()),
+    back = lambda dq=q, dk=k, q=q, k=k, w=w, pos=pos, **kw: ops.head_norm_rotary_backward(ctx, dq, dk, q, k, w, w, pos, freq, axis, **kw)  # noqa: E731
+    for call in (lambda: back(dk=None), lambda: back(k=None), lambda: back(dq=q[:2]), lambda: back(dq=q.half()), lambda: back(dk=k[..., :4]),
+                 lambda: back(pos=pos.int(), dpositions=True), lambda: back(eps=-1.0), lambda: back(kind="none"), lambda: back(w=w.half()),
+                 lambda: head(eps=-1.0), lambda: head(eps=float("nan")), lambda: head(kind="none"), lambda: head(pos=far), lambda: head(q=q.double()),
                  lambda: head(q=q[:2]), lambda: head(q=odd, k=None), lambda: head(q=q[:, :0]), lambda: head(w=w.half()), lambda: head(w=torch.ones(8)),
                  lambda: head(axis=axis.long()), lambda: head(freq=torch.ones(5).cuda(), axis=torch.zeros(5, dtype=torch.int32).cuda()),
                  lambda: put(k=k[..., ::2], v=v), lambda: put(q=q, kind="other"), lambda: put(q=q, out=q[:2]), lambda: put(out=q), lambda: put(k_weight=w),
