@@ -1,4 +1,5 @@
-"""Build libmtpx.so for gfx950 with hipcc (in-tree, no JIT cache).
+"""Build libmtpx.so for gfx950 with hipcc, and with the host's compiler
+mtpx/_calls.so for the torch that is installed (in-tree, no JIT cache).
 
     python imr-mlp_amd/build.py [-v] [--changed]
 
