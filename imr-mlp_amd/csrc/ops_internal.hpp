@@ -120,6 +120,32 @@ struct Divisor {
     int shift;
 };
 
+// A search by `lanes` places at a time (a power of two) for the first place below
+// n at which something no longer holds that holds at all places before.  Every
+// round leaves fewer places, by one lane too, which bisects them: of 4,096 places
+// 64 lanes find one in two rounds, one lane in at most 13.
+struct Search {
+    int from = 0, to;  // it holds below `from`, and no longer from `to` on
+    int lanes, shift, step = 0;
+
+    __host__ __device__ inline Search(int n, int by) : to(n), lanes(by), shift(by > 1 ? 31 - __builtin_clz(by) : 1) {}
+    // Whether places are left; where lane l looks: at no place if that is not below `to`.
+    __host__ __device__ inline bool next()
+    {
+        step = (int)(((int64_t)to - from + (1 << shift) - 1) >> shift);
+        return from < to;
+    }
+    __host__ __device__ inline int64_t place(int l) const { return from + (int64_t)(l + 1) * step - 1; }
+    // The first `count` of the lanes' places hold.
+    __host__ __device__ inline void narrow(int count)
+    {
+        const int64_t end = place(count);
+        if (count < lanes && end < to)
+            to = (int)end;
+        from += count * step;
+    }
+};
+
 // What the first t tiles of a sequence's columns cost, in steps of `step` keys:
 // `start` and no less than its steps each.  Where the new rows are a small part,
 // every tile as much as the last.  Else tile t sees `before` + (t + 1) columns /

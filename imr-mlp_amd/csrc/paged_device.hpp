@@ -8,28 +8,19 @@ namespace mtpx {
 
 // The largest i < n for which pred(i) holds, -1 if none: pred holds up to some
 // i and not beyond.  `lanes` neighbouring lanes (a power of two up to a wave)
-// search together, as many places at a time: 64 lanes find one of 4,096 in two
-// dependent reads.
+// search together, as many places at a time.
 template <class P>
 __device__ inline int last_true(const P &pred, int n, int lanes)
 {
-    const int l = threadIdx.x & (lanes - 1), shift = 31 - __clz(lanes);
-    const int base = (threadIdx.x & (kWave - 1)) & ~(lanes - 1);
+    const int l = threadIdx.x & (lanes - 1), base = (threadIdx.x & (kWave - 1)) & ~(lanes - 1);
     const unsigned long long all = ~0ull >> (kWave - lanes);
-    int first = 0, span = n;
-    while (span > 0) {
-        const int step = (int)(((int64_t)span + lanes - 1) >> shift);
-        const int64_t at = (int64_t)l * step;
-        const unsigned long long holds = __ballot(at < span && pred(first + (int)at)) >> base & all;
-        const int count = holds == all ? lanes : __ffsll(~holds) - 1;
-        if (count == 0)
-            break;
-        first += (count - 1) * step;
-        if (step == 1)
-            return first;
-        span = min(step, span - (count - 1) * step);
+    Search s(n, lanes);
+    while (s.next()) {
+        const int64_t at = s.place(l);
+        const unsigned long long holds = __ballot(at < s.to && pred((int)at)) >> base & all;
+        s.narrow(holds == all ? lanes : __ffsll(~holds) - 1);
     }
-    return first - 1;
+    return s.from - 1;
 }
 
 // The first row of sequence i (of sequence n: the end of the last one).
