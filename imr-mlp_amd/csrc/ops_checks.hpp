@@ -9,8 +9,9 @@
 
 namespace mtpx {
 
-// a launch's threads are counted in 32 bits: workgroups of 512, rows of 64
-constexpr int64_t kMaxGroups = UINT32_MAX / 512, kMaxRows = UINT32_MAX / 64;
+// a launch's threads are counted in 32 bits: workgroups of 512, rows of 64 in
+// workgroups of 256, the last one whole
+constexpr int64_t kMaxGroups = UINT32_MAX / 512, kMaxRows = (UINT32_MAX - 255) / 64;
 
 inline int invalid(mtpx_context *ctx, const std::string &msg) { return set_error(ctx, MTPX_E_INVALID, msg); }
 

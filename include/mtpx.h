@@ -635,7 +635,7 @@ typedef struct mtpx_rows {
 typedef struct mtpx_rotary_request {
     void *stream;
     int dtype;
-    int64_t rows;            /* below 2^26 */
+    int64_t rows;            /* at most 2^26 - 4 */
     int heads, dim, rotated; /* rotated even, at most dim; dim <= 1024 */
     int interleaved, inverse;
     mtpx_rows x, y;          /* map unused */
@@ -752,7 +752,7 @@ int mtpx_diff_attention_cache_workspace(mtpx_context *ctx,
 typedef struct mtpx_norm_block_request {
     void *stream;
     int dtype;
-    int64_t rows;             /* below 2^26 */
+    int64_t rows;             /* at most 2^26 - 4 */
     int width;                /* 1 to 16384 */
     int kind, gate_act;
     float residual_scale, block_scale, eps;
@@ -790,7 +790,7 @@ int mtpx_norm_block_workspace(mtpx_context *ctx, const mtpx_norm_block_request *
 typedef struct mtpx_head_norm_rotary_request {
     void *stream;
     int dtype;
-    int64_t rows;               /* below 2^26 */
+    int64_t rows;               /* at most 2^26 - 4 */
     int heads, kv_heads;        /* kv_heads 0: q only */
     int maps;                   /* 1 or 2 */
     int dim, rotated;           /* dim <= 256, rotated even and at most dim */
@@ -852,7 +852,7 @@ typedef struct mtpx_pages {
 typedef struct mtpx_append_paged_request {
     void *stream;
     int dtype;
-    int64_t rows;               /* below 2^26 */
+    int64_t rows;               /* at most 2^26 - 4 */
     int sequences;              /* below 2^24 */
     int heads, kv_heads, dim, rotated; /* dim <= 256 */
     int kind, interleaved;
@@ -883,7 +883,7 @@ int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *reques
 typedef struct mtpx_diff_attention_paged_request {
     void *stream;
     int dtype;
-    int64_t rows;               /* below 2^26, rows * heads below 2^23 */
+    int64_t rows;               /* rows * heads below 2^23 */
     int sequences;              /* below 2^24 */
     int max_rows;
     int heads, kv_heads, dim;   /* dim 1 to 128 */

@@ -93,9 +93,9 @@ static int lanes(char **v)
     r.cache.k = r.cache.v = r.k;
     r.cache.k_page = r.cache.v_page = row * 16;
     r.cache.pages = 4, r.cache.page_rows = 16, r.cache.table = numbers, r.cache.table_row = 2, r.cache.table_width = 2;
-    for (int bit = 0; bit <= 26; ++bit)
-        for (int64_t rows : {(int64_t(1) << bit) - 1, int64_t(1) << bit, (int64_t(1) << bit) + 1}) {
-            if (rows < 1 || rows > mtpx::kMaxRows)
+    for (int bit = 1; bit <= 26; ++bit)
+        for (int64_t rows : {(int64_t(1) << bit) - 4, (int64_t(1) << bit) - 1, int64_t(1) << bit, (int64_t(1) << bit) + 1}) {
+            if (rows < 1)
                 continue;
             r.rows = rows;
             if (const int code = mtpx_append_paged(&ctx, &r)) {

@@ -6,6 +6,8 @@ import subprocess
 
 import pytest
 
+from mtpx import capi
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -35,10 +37,17 @@ def test_a_search_ends_where_it_should(calls):
     (1, 16, 16, 0, 1), (1, 8, 8, 1, 1), (0, 8, 8, 0, 2), (0, 2, 2, 0, 1), (1, 8, 0, 0, 1), (2, 64, 64, 0, 8), (0, 255, 2, 1, 3)])
 def test_lanes_of_a_row(calls, dtype, dim, rotated, interleaved, heads):
     """A row's lanes are a power of two from a vector's up to a workgroup, one among
-    them where vectors are short and rows many."""
+    them where vectors are short and rows many.  A launch's threads, whole workgroups
+    of them, are a 32-bit number up to the most rows, and more are refused."""
     seen = set()
-    for line in calls("lanes", dtype, dim, rotated, interleaved, heads):
-        rows, group, lanes = (int(v) for v in line)
+    for rows, *line in calls("lanes", dtype, dim, rotated, interleaved, heads):
+        rows = int(rows)
+        assert (line[0] == "refused") == (rows > 2 ** 26 - 4), rows
+        if line[0] == "refused":
+            assert int(line[1]) == capi.ERRORS_BY_NAME["MTPX_E_CAPACITY"]
+            continue
+        group, lanes = (int(v) for v in line)
+        assert -(-rows * lanes // 256) * 256 < 2 ** 32
         assert lanes & (lanes - 1) == 0 and group <= lanes <= 256
         seen.add((group, lanes))
     assert ((1, 1) in seen) == (min(g for g, _ in seen) == 1)
