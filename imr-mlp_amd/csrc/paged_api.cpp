@@ -407,6 +407,8 @@ int mtpx_append_paged(mtpx_context *ctx, const mtpx_append_paged_request *req)
         if (r.heads < 0 || r.kv_heads < 1)
             return invalid(ctx, "heads must not be negative and kv_heads positive");
         MTPX_TRY(check_norms(ctx, r, MTPX_NORM_NONE));
+        if (r.kind == MTPX_NORM_NONE && (r.q_weight || r.k_weight))
+            return invalid(ctx, "weights without a norm");
         MTPX_TRY(check_batch(ctx, r.sequences, r.offsets, r.lengths));
         MTPX_TRY(check_pages(ctx, r.cache, r.dtype));
         if (r.rows == 0 || r.sequences == 0)

@@ -843,9 +843,9 @@ typedef struct mtpx_pages {
  * graph serves any batch of the same shapes. */
 
 /* Puts a batch's new keys and values into their pages, the keys normed for
- * each head (MTPX_NORM_NONE: as they are) and turned by their positions on the
- * way, as mtpx_head_norm_rotary would; with q (heads 0: none) the queries too,
- * into q_out, which may be q (same strides).  A row beyond its sequence's room,
+ * each head (MTPX_NORM_NONE: as they are, without weights) and turned by their
+ * positions on the way, as mtpx_head_norm_rotary would; with q (heads 0: none)
+ * the queries too, into q_out, which may be q (same strides).  A row beyond its sequence's room,
  * or before its start, is dropped; its query is not.  No two rows of a call may
  * meet in one place of a page. */
 #define MTPX_NORM_NONE 2

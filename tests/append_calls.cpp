@@ -6,6 +6,8 @@
 //   append_calls lanes DTYPE DIM ROTATED INTERLEAVED HEADS
 //                               lanes of a vector and of a row for rows from 1 up to
 //                               the most, one line each
+//   append_calls weights        the code of an append with a weight for each norm, and
+//                               whether its work was queued
 #include "../imr-mlp_amd/csrc/paged_api.cpp"
 
 #include <cstdio>
@@ -13,6 +15,7 @@
 #include <cstring>
 
 static mtpx::HeadArgs seen;
+static bool queued = false;
 
 extern "C" {
 hipError_t hipSetDevice(int) { return hipSuccess; }
@@ -31,6 +34,7 @@ hipError_t launch_head_forward(int, const HeadArgs &, hipStream_t) { return hipS
 hipError_t launch_head_append(int, const HeadArgs &a, hipStream_t)
 {
     seen = a;
+    queued = true;
     return hipSuccess;
 }
 hipError_t launch_head_backward(int, const HeadArgs &, hipStream_t) { return hipSuccess; }
@@ -82,17 +86,24 @@ alignas(16) static float room[4096];
 static int numbers[16] = {0};
 static mtpx_context ctx;
 
-static int lanes(char **v)
+static mtpx_append_paged_request append(int dtype, int dim, int rotated, int kv_heads)
 {
     mtpx_append_paged_request r{};
-    r.dtype = std::atoi(v[0]), r.dim = std::atoi(v[1]), r.rotated = std::atoi(v[2]), r.interleaved = std::atoi(v[3]);
-    r.kv_heads = std::atoi(v[4]), r.sequences = 1, r.axes = 1, r.kind = MTPX_NORM_NONE;
+    r.dtype = dtype, r.dim = dim, r.rotated = rotated, r.kv_heads = kv_heads;
+    r.rows = r.sequences = 1, r.axes = 1, r.kind = MTPX_NORM_NONE;
     const int64_t map = r.dim, head = 2 * map, row = head * r.kv_heads;
     r.k = r.v = mtpx_rows{room, row, head, map};
     r.positions = room, r.freq = room, r.axis = numbers, r.offsets = r.lengths = numbers;
     r.cache.k = r.cache.v = r.k;
     r.cache.k_page = r.cache.v_page = row * 16;
     r.cache.pages = 4, r.cache.page_rows = 16, r.cache.table = numbers, r.cache.table_row = 2, r.cache.table_width = 2;
+    return r;
+}
+
+static int lanes(char **v)
+{
+    auto r = append(std::atoi(v[0]), std::atoi(v[1]), std::atoi(v[2]), std::atoi(v[4]));
+    r.interleaved = std::atoi(v[3]);
     for (int bit = 1; bit <= 26; ++bit)
         for (int64_t rows : {(int64_t(1) << bit) - 4, (int64_t(1) << bit) - 1, int64_t(1) << bit, (int64_t(1) << bit) + 1}) {
             if (rows < 1)
@@ -107,11 +118,27 @@ static int lanes(char **v)
     return 0;
 }
 
+static int weights()
+{
+    for (int kind : {MTPX_NORM_RMS, MTPX_NORM_LAYER, MTPX_NORM_NONE})
+        for (int given = 0; given < 4; ++given) {
+            auto r = append(MTPX_F32, 8, 8, 1);
+            r.kind = kind, r.heads = 1, r.q = r.k, r.q_out = r.k;
+            r.q_weight = given & 1 ? room : nullptr, r.k_weight = given & 2 ? room : nullptr;
+            queued = false;
+            const int code = mtpx_append_paged(&ctx, &r);
+            std::printf("%d %d %d %d\n", kind, given, code, queued);
+        }
+    return 0;
+}
+
 int main(int argc, char **argv)
 {
     if (argc > 1 && !std::strcmp(argv[1], "search"))
         return search();
     if (argc > 6 && !std::strcmp(argv[1], "lanes"))
         return lanes(argv + 2);
+    if (argc > 1 && !std::strcmp(argv[1], "weights"))
+        return weights();
     return 2;
 }

@@ -1,12 +1,12 @@
-"""How an append's rows find their sequences, on the CPU: the search ends at the
-right place for every number of lanes that the plan of a call gives a row."""
+"""The C entry of appends and how rows find their sequences, on the CPU: the search
+ends at the right place for every number of lanes that the plan of a call gives a row."""
 import os
 import shutil
 import subprocess
 
 import pytest
 
-from mtpx import capi
+from mtpx import capi, ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -51,3 +51,10 @@ def test_lanes_of_a_row(calls, dtype, dim, rotated, interleaved, heads):
         assert lanes & (lanes - 1) == 0 and group <= lanes <= 256
         seen.add((group, lanes))
     assert ((1, 1) in seen) == (min(g for g, _ in seen) == 1)
+
+
+def test_weights_without_a_norm(calls):
+    """Keys go into their pages as they are: a weight is refused, nothing is queued."""
+    for kind, given, code, queued in ([int(v) for v in line] for line in calls("weights")):
+        wrong = kind == ops.APPEND_NORMS["none"] and given > 0
+        assert (code, queued) == ((capi.ERRORS_BY_NAME["MTPX_E_INVALID"], 0) if wrong else (0, 1)), (kind, given)
