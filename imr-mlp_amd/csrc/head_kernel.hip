@@ -74,6 +74,10 @@ struct Layout {
     {
     }
     __device__ inline int unit(int i) const { return first + i * group; }
+    // Whether the lane's unit i turns: elements that are copied, two of which would
+    // make a pair of it, leave each other alone (0 times an infinity is none).  With
+    // the halves apart a copied element's partner is none and stays 0.
+    __device__ inline bool turns(int i) const { return APART || unit(i) < turning; }
     // Whether element e of unit u exists.
     __device__ inline bool inside(int u, int e) const { return u < turning || (u < units && e < W); }
     __device__ inline int element(int u, int e) const
@@ -345,6 +349,8 @@ __global__ __launch_bounds__(kThreads) void head_forward_kernel(HeadArgs a)
 #pragma unroll
                 for (int e = 0; e < L::E; ++e)
                     z[i][e] *= w[i][e];
+                if (!at.turns(i))
+                    continue;
 #pragma unroll
                 for (int j = 0; j < L::P; ++j) {
                     const float z1 = z[i][L::one(j)], z2 = z[i][L::two(j)];
@@ -443,8 +449,10 @@ __global__ __launch_bounds__(kThreads) void head_backward_kernel(HeadArgs a)
                     for (int j = 0; j < L::P; ++j) {
                         const int k = L::one(j), l = L::two(j);
                         const float d1 = g[i][k], d2 = g[i][l];
-                        g[i][k] = d1 * c[i][j] + d2 * s[i][j];
-                        g[i][l] = d2 * c[i][j] - d1 * s[i][j];
+                        // (a choice of the partner, not a branch: a step of 4,001 rows of 10 and 5
+                        // heads of 40 in 32 bits, 36 turning, takes 40.8 us, 41.4 us with one)
+                        g[i][k] = d1 * c[i][j] + (at.turns(i) ? d2 : 0.f) * s[i][j];
+                        g[i][l] = d2 * c[i][j] - (at.turns(i) ? d1 : 0.f) * s[i][j];
                         if constexpr (MOVED)
                             d[i][j] += g[i][l] * (u[i][k] * w[i][k]) - g[i][k] * (u[i][l] * w[i][l]);
                     }
