@@ -13,6 +13,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "mtpx.h"
@@ -428,6 +430,21 @@ PyObject *diff_attention_paged(PyObject *, PyObject *const *args, Py_ssize_t n)
     });
 }
 
+// The stream that was current when a graph's end at a leaf was made: (id, index and
+// type of its device), None of anything else.
+PyObject *stream_of(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 1)
+        return PyErr_Format(PyExc_TypeError, "%zd arguments, not 1", n);
+    try {
+        if (torch::autograd::THPCppFunction_Check(args[0]))
+            if (const auto s = reinterpret_cast<torch::autograd::THPCppFunction *>(args[0])->cdata->stream())
+                return Py_BuildValue("Lii", (long long)s->id(), (int)s->device_index(), (int)s->device_type());
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
 // The addresses of the library's entries, in the order of Entries.
 PyObject *setup(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
@@ -451,7 +468,7 @@ PyObject *setup(PyObject *, PyObject *const *args, Py_ssize_t n)
 
 #define MTPX_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MTPX_METHOD(setup), MTPX_METHOD(head_norm_rotary), MTPX_METHOD(head_norm_rotary_backward),
-                         MTPX_METHOD(append_paged), MTPX_METHOD(diff_attention_paged), {nullptr, nullptr, 0, nullptr}};
+                         MTPX_METHOD(append_paged), MTPX_METHOD(diff_attention_paged), MTPX_METHOD(stream_of), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mtpx._calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
