@@ -132,16 +132,23 @@ def build(verbose: bool = False, changed_only: bool = False) -> str:
 
 def build_calls(verbose: bool = False) -> None:
     """mtpx/_calls.so, the calls of mtpx.ops on torch's tensors (host code; its
-    library's entries are handed to it).  Without torch there is no mtpx.ops."""
+    library's entries are handed to it).  Without torch there is no mtpx.ops;
+    without headers to build against, the library is whole and the operators of
+    mtpx.ops that need these calls say that they are not built."""
     spec = importlib.util.find_spec("torch")
     if spec is None:
         return
     torch = spec.submodule_search_locations[0]
+    python, headers = sysconfig.get_paths()["include"], os.path.join(torch, "include")
+    missing = [h for h in (os.path.join(python, "Python.h"), os.path.join(headers, "ATen", "ATen.h")) if not os.path.exists(h)]
+    if missing:
+        print("%s is not built: no %s" % (CALLS, ", no ".join(missing)), flush=True)
+        return
     tmp = CALLS + ".tmp"
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-           "-I", os.path.join(ROOT, "include"), "-I", os.path.join(torch, "include"),
-           "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
-           "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp,
+           "-I", os.path.join(ROOT, "include"), "-I", headers,
+           "-I", os.path.join(headers, "torch", "csrc", "api", "include"),
+           "-I", python, os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp,
            "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -868,7 +868,10 @@ def _recording():
 def _made_on(fn, node):
     """The stream that was current when an end of the graph at a leaf was made,
     on which autograd hands that leaf's gradient over."""
-    at = _calls().stream_of(node)
+    try:
+        at = _calls().stream_of(node)
+    except RuntimeError:  # the native calls are not built: not known
+        at = None
     if at is None:
         return _stream(fn.ctx)
     return torch.cuda.Stream(stream_id=at[0], device_index=at[1], device_type=at[2]).cuda_stream
