@@ -6,6 +6,9 @@
 //   append_calls lanes DTYPE DIM ROTATED INTERLEAVED HEADS
 //                               lanes of a vector and of a row for rows from 1 up to
 //                               the most, one line each
+//   append_calls backward ROWS HEADS MAPS DIM ROTATED INTERLEAVED DTYPE
+//                               lanes of a row and workgroups of the backward pass of
+//                               head norms on a device of 256 compute units
 //   append_calls weights        the code of an append with a weight for each norm, and
 //                               whether its work was queued
 #include "../imr-mlp_amd/csrc/paged_api.cpp"
@@ -37,7 +40,11 @@ hipError_t launch_head_append(int, const HeadArgs &a, hipStream_t)
     queued = true;
     return hipSuccess;
 }
-hipError_t launch_head_backward(int, const HeadArgs &, hipStream_t) { return hipSuccess; }
+hipError_t launch_head_backward(int, const HeadArgs &a, hipStream_t)
+{
+    seen = a;
+    return hipSuccess;
+}
 hipError_t launch_paged(int, const PagedArgs &, hipStream_t) { return hipSuccess; }
 }  // namespace mtpx
 
@@ -118,6 +125,22 @@ static int lanes(char **v)
     return 0;
 }
 
+static int backward(char **v)
+{
+    mtpx_head_norm_rotary_request r{};
+    r.rows = std::atoll(v[0]), r.heads = std::atoi(v[1]), r.maps = std::atoi(v[2]), r.dim = std::atoi(v[3]);
+    r.rotated = std::atoi(v[4]), r.interleaved = std::atoi(v[5]), r.dtype = std::atoi(v[6]);
+    r.axes = 1, r.positions = r.freq = room, r.axis = numbers;
+    const int64_t map = r.dim, head = r.maps * map;
+    r.q = r.dq_out = r.dq = mtpx_rows{room, head * r.heads, head, map};
+    r.workspace = room, r.workspace_bytes = size_t(1) << 40;
+    ctx.num_cus = 256;
+    if (const int code = mtpx_head_norm_rotary_backward(&ctx, &r))
+        return code;
+    std::printf("%d %d\n", seen.lanes, seen.parts);
+    return 0;
+}
+
 static int weights()
 {
     for (int kind : {MTPX_NORM_RMS, MTPX_NORM_LAYER, MTPX_NORM_NONE})
@@ -138,6 +161,8 @@ int main(int argc, char **argv)
         return search();
     if (argc > 6 && !std::strcmp(argv[1], "lanes"))
         return lanes(argv + 2);
+    if (argc > 8 && !std::strcmp(argv[1], "backward"))
+        return backward(argv + 2);
     if (argc > 1 && !std::strcmp(argv[1], "weights"))
         return weights();
     return 2;

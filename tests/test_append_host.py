@@ -7,6 +7,7 @@ import subprocess
 import pytest
 
 from mtpx import capi, ops
+from test_head_norm_rows_gpu import WORKGROUP_ROWS
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -51,6 +52,13 @@ def test_lanes_of_a_row(calls, dtype, dim, rotated, interleaved, heads):
         assert lanes & (lanes - 1) == 0 and group <= lanes <= 256
         seen.add((group, lanes))
     assert ((1, 1) in seen) == (min(g for g, _ in seen) == 1)
+
+
+@pytest.mark.parametrize("rows,heads,maps,dim,rotated,dtype,interleaved", WORKGROUP_ROWS)
+def test_a_workgroup_has_rows_one_after_the_other(calls, rows, heads, maps, dim, rotated, dtype, interleaved):
+    """The shapes that the device's test of such rows takes have a workgroup a row, and fewer workgroups than rows."""
+    lanes, parts = (int(v) for v in calls("backward", rows, heads, maps, dim, rotated, int(interleaved), ops.DTYPES[dtype])[0])
+    assert lanes == 256 and parts < rows
 
 
 def test_weights_without_a_norm(calls):
