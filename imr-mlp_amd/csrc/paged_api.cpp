@@ -278,7 +278,7 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     // A few long sequences among many short ones (by the average's share of the
     // longest): shares of both widths run beside each other, on less than all slots
     // each, as the ones read while the others multiply (46 single rows and chunks
-    // of 727, heads of 128: 287 us, 330 us with all slots each, 388 us with half;
+    // of 727, heads of 128: 294 us, 334 us with all slots each, 398 us with half;
     // 30 rows and two chunks of 512, heads of 64: 161 us, 175 us).  Many wide tiles
     // of up to 64 need all (46 rows and a chunk of 2,048: 392 us, 464 us with half).
     const bool beside = both && half && r.rows * 4 <= n * most && (all + n) * r.kv_heads < (width == 128 ? 4 : 1) * slots;
@@ -301,15 +301,15 @@ PagedPlan paged_plan(mtpx_context *ctx, const mtpx_diff_attention_paged_request 
     }
     if (p.narrow_columns == 0 || both) {
         // every sequence's tiles in one order where that leaves few without rows (8
-        // sequences of 4,096 rows, 16 heads of 64: 960 us, 980 us sequence by
-        // sequence; of 2,500 to 6,000 rows: 1,015 and 937 us)
+        // sequences of 4,096 rows, 16 heads of 64: 926 us, 942 us sequence by
+        // sequence; of 2,500 to 6,000 rows: 1,060 and 981 us)
         const int64_t level = (most * group + columns - 1) / columns * n;
         // A tile a workgroup, of more tiles than slots: about as long as the longest
         // tile over the even share, with tiles half as long as there is room on
         // average.  Shared, a slot and a tile have `split` steps' time of partial
         // results each (3 prompts of 1,024 rows, 32 heads of 64: 59 us and 89 us
         // shared; one of 8,192, 16 heads: 446 and 464 us; a chunk of 2,048 rows of
-        // 32,000: 1,066 and 778 us).
+        // 32,000: 1,094 and 795 us).
         p.wide.split = half ? 8 : 3;
         const int64_t steps = (room - 1) / (2 * width * (half ? 2 : 4) <= 256 ? 64 : 32) + 1, units = all * r.kv_heads;
         const bool each = units >= 4 * slots || (units > slots && steps * slots <= 2 * p.wide.split * (units + slots));
@@ -343,8 +343,10 @@ int check_paged(mtpx_context *ctx, const mtpx_diff_attention_paged_request &r)
     if (r.rows > kMaxRows || r.sequences > kMaxSequences || r.heads > 65535 || r.cache.page_rows > 1 << 20 ||
         (int64_t)r.cache.table_width * r.cache.page_rows > kMaxRoom)
         return set_error(ctx, MTPX_E_CAPACITY, "too many rows, sequences, heads or rows of a sequence");
+    // (columns, of which there are rows times heads, and the costs of their tiles are
+    // counted in 32 bits)
     if (r.rows * r.heads > kMaxGroups || paged_plan(ctx, r).items > kMaxGroups)
-        return set_error(ctx, MTPX_E_CAPACITY, "too many rows and heads for one launch");
+        return set_error(ctx, MTPX_E_CAPACITY, "too many rows and heads for one call");
     return MTPX_OK;
 }
 

@@ -286,9 +286,9 @@ __device__ inline void load_lanes_to_lds(const void *p, unsigned lane_offset, un
 // whole runs of kGroup rows, which one load of a wave brings.  Lane l forms the
 // address of key l once for keys and values, a load begins where the first of its
 // rows lies, and the lanes keep their offsets from there: the vector unit has the
-// softmax to do (a chunk of 2,048 rows of 32,000, 16 heads of 64: 780 us, 930 us
-// through the other loader; 46 single rows and two chunks of 727, heads of 128: 290
-// and 398 us; a chunk of 1,024 rows of 8,192 in pages of 24, 32 heads of 64: 221 and
+// softmax to do (a chunk of 2,048 rows of 32,000, 16 heads of 64: 795 us, 920 us
+// through the other loader; 46 single rows and two chunks of 727, heads of 128: 294
+// and 391 us; a chunk of 1,024 rows of 8,192 in pages of 24, 32 heads of 64: 221 and
 // 263 us.  Addresses of whole runs of a wave by the scalar unit alone take 1 to 2 %
 // less, and leave such pages to the other loader).
 template <class T, int D, int ROWS, int W>
@@ -389,9 +389,9 @@ struct Segment {
 // Wide tiles are bound by the matrix units and what their waves wait for between
 // products.  A pair of row and key takes 8 D operations by the formula, 12 D here,
 // where each map has its own product with V, as its sum is known at the end only: 8
-// prompts of 4,096 rows, 16 heads of 64, take 950 us, 600 TFLOP/s of the former and
-// 900 of the latter; a chunk of 2,048 rows of 32,000 takes 780 us, 670 and 1,000
-// TFLOP/s.  (A plain product of two large matrices reaches 1,140 TFLOP/s.)  Narrow tiles are bound by the reads of the cache: 64 rows
+// prompts of 2,500 to 6,000 rows, 16 heads of 64, take 985 us (960 us on another
+// card), 580 TFLOP/s of the former and 865 of the latter; a chunk of 2,048 rows of
+// 32,000 takes 795 us, 655 and 980 TFLOP/s.  (A plain product of two large matrices reaches 1,140 TFLOP/s.)  Narrow tiles are bound by the reads of the cache: 64 rows
 // against up to 8,192 keys each, 32 heads of 64 on 4, take 150 us, 5.2 TB/s.
 template <class T, int D, int W, int M, int QT, int KB, int BUF, bool FAST>
 __device__ inline void attend(const PagedArgs &a, const Sequence &sq, const Segment &sg, char *smem)
@@ -796,7 +796,7 @@ struct Shape {
 // Both roles in one launch, the wide tiles first, which take the longest.  (Eight
 // workgroups of each in turn, for the reads of one and the products of the other to
 // share the CUs, are slower: 48 sequences, two of them with chunks of 727 rows,
-// 388 us; 330 us so.)
+// 501 us; 294 us so.)
 constexpr int kNarrowOnly = 1, kWideOnly = 2, kBoth = 3;
 template <class T, int D, bool FAST, int ROLES>
 __global__ __launch_bounds__((Shape<T, D>::kWaves * kWave), 2) void paged_kernel(PagedArgs a)
