@@ -784,8 +784,9 @@ def diff_attention_paged(ctx, q, k_pages, v_pages, lam, table, offsets, lengths,
     arguments as there, lam [heads] float32.  Row j of m new ones sees the
     first lengths[i] - m + j + 1 rows of its sequence, without causal all of
     them.  max_rows: the most new rows of a sequence, where the caller knows it
-    (1 in a plain decoding step), which saves work.  Returns [rows, heads, 2
-    dim]; rows of no sequence are left as they are."""
+    (1 in a plain decoding step), which saves work; rows of a sequence beyond it
+    may be left unwritten.  Returns [rows, heads, 2 dim]; rows of no sequence are
+    left as they are."""
     done = _calls().diff_attention_paged(_handle(ctx), ctx.device, _stream_of, q, k_pages, v_pages,
                                          lam, table, offsets, lengths, causal, scale, max_rows, out)
     if done is not None:
